@@ -6,6 +6,7 @@ The library is loaded after torch so that its HIP runtime dependency
 fallback: if the library is missing or fails to load, every operator raises.
 """
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -169,6 +170,34 @@ SIGNATURES = {
         _c_p, _c_i64,                             # out, so
         _c_i64, _c_i64, _c_i64, _c_p,             # M, N, K, stream
     ],
+    "evo2_gated_linear_workspace_bytes": [_c_i64, _c_i64, _c_i64],
+    "evo2_gated_linear": [
+        _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i32,  # x, sx, w1, w2, sw, gelu
+        _c_p, _c_i64, _c_p, _c_p,                 # h, sh, z1, z2
+        _c_i64, _c_i64, _c_i64, _c_p,             # M, I, H, stream
+    ],
+    "evo2_gated_linear_backward": [
+        _c_p, _c_i64, _c_p, _c_i64,               # dh, sdh, x, sx
+        _c_p, _c_p, _c_i64, _c_i32,               # w1, w2, sw, gelu
+        _c_p, _c_p, _c_p, _c_p, _c_p,             # z1, z2, dx, dw1, dw2
+        _c_p, _c_i64,                             # workspace, bytes
+        _c_i64, _c_i64, _c_i64, _c_p,             # M, I, H, stream
+    ],
+    "evo2_linear_loss_workspace_bytes": [_c_i64, _c_i64, _c_i64, _c_i32],
+    "evo2_linear_loss": [
+        _c_p, _c_i64, _c_p, _c_i64,               # h, sh, w, sw
+        _c_p, _c_i64, _c_i32,                     # targets, ignore, reduction
+        _c_p, _c_p, _c_p, _c_p,                   # nll, lse, loss, count
+        _c_p, _c_i64,                             # workspace, bytes
+        _c_i64, _c_i64, _c_i64, _c_p,             # T, V, H, stream
+    ],
+    "evo2_linear_loss_backward": [
+        _c_p, _c_i64, _c_p, _c_i64,               # h, sh, w, sw
+        _c_p, _c_i64, _c_p,                       # targets, ignore, lse
+        _c_p, _c_i64, _c_p,                       # grad, sgrad, count
+        _c_p, _c_p, _c_p, _c_i64,                 # dh, dw, workspace, bytes
+        _c_i64, _c_i64, _c_i64, _c_p,             # T, V, H, stream
+    ],
     "evo2_rotary_prefill": [
         _c_p, _c_i64, _c_p, _c_f,                 # qkv, sqkv, inv_freq, factor
         _c_p, _c_p, _c_p, _c_i64,                 # q, k, vt, Lv
@@ -293,7 +322,9 @@ SIGNATURES = {
 
 RESTYPES = {"evo2_last_error": ctypes.c_char_p, "evo2_hcl_workspace_bytes": ctypes.c_int64,
             "evo2_decode_attention_workspace_bytes": ctypes.c_int64,
-            "evo2_fp8_gemm_persist_order": ctypes.c_int64}
+            "evo2_fp8_gemm_persist_order": ctypes.c_int64,
+            "evo2_gated_linear_workspace_bytes": ctypes.c_int64,
+            "evo2_linear_loss_workspace_bytes": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib = None
@@ -373,6 +404,22 @@ def overlap(a, b):
         return False
     (a0, a1), (b0, b1) = span(a), span(b)
     return a0 < b1 and b0 < a1
+
+
+def on_device(t):
+    """A context in which t's device is the current one (launches go there)."""
+    if t.get_device() == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def rows16(t):
+    """t (rows, n of a multiple of 8, 16-bit) with rows of unit stride that start
+    on 16 bytes and do not overlap: itself, or a copy."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] \
+            and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def require_device(*tensors):

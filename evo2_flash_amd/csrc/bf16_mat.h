@@ -1,0 +1,553 @@
+// bf16 matrix products on v_mfma_f32_32x32x16_bf16 with fp32 sums, in the three
+// orientations a linear layer and its gradients need, and with the epilogues of
+// the gated product and of the head's cross entropy:
+//   MAT_NT  out[m, n] = sum_k x[m, k] w[n, k]   (x (M, K), w (N, K))
+//   MAT_NN  out[m, n] = sum_k x[m, k] w[k, n]   (x (M, K), w (K, N))
+//   MAT_TN  out[m, n] = sum_k x[k, m] w[k, n]   (x (K, M), w (K, N))
+//
+// A workgroup of four waves owns 256 columns by 64 TM rows of the output, a wave
+// 128 by 32 TM of them, with w as MFMA operand A so that a lane ends up with
+// four consecutive columns of one row.  K moves in slices of 64: 32 KB of w and
+// 8 TM KB of x per stage, HBM -> LDS by direct-to-LDS loads; slice k + NST is
+// loaded into the stage of slice k as soon as every wave has read it, and the
+// workgroup meets at one barrier per slice.  Workgroups are persistent (one per
+// CU walks its tiles) and the loads run on across tile boundaries, so a tile's
+// first slices land while the one before finishes.
+//
+// An operand whose rows run along K ("K-contiguous") is staged as rows of 128
+// bytes, 16-byte chunk c of row r at c ^ ((r >> 1) & 7), and read 16 bytes a
+// lane.  One whose rows run along M or N is staged as 64 rows of the tile's
+// width as they lie in memory and transposed on the way out of LDS
+// (ds_read_b64_tr_b16: a group of 16 lanes reads 4 rows of 16 columns and each
+// lane receives one column's four values), so no operand is ever transposed in
+// memory.  Its 32-byte pairs of chunks are XORed with the row's low bits, so
+// that the four rows a group reads lie on distinct banks.
+//
+// Loads go through buffer descriptors rebased to the wave's first row of each
+// slice, so that operands may pass 4 GB; rows and columns outside the operand read
+// zeros.
+#pragma once
+
+#include <algorithm>
+#include <climits>
+
+#include "attn_common.h"
+
+namespace evo2 {
+
+typedef __attribute__((ext_vector_type(16))) float mf32x16_t;
+typedef __attribute__((ext_vector_type(4))) short ms16x4_t;
+typedef __attribute__((address_space(3))) ms16x4_t mlds_s16x4_t;
+
+enum MatForm { MAT_NT = 0, MAT_NN = 1, MAT_TN = 2 };
+enum MatEpi {
+  MAT_BF16 = 0,   // out as bf16
+  MAT_F32 = 1,    // fp32 partial sums, one plane per split (or added to what is there)
+  MAT_GATED = 2,  // act(x w^T) * (x w2^T), and both products for the backward pass
+  MAT_STATS = 3,  // each row's max and sum of exponentials over 128 columns
+  MAT_DLOG = 4,   // the gradient of the cross entropy at the logits
+};
+
+constexpr int MAT_CUS = 256;     // workgroups a launch fills the card with
+constexpr int MAT_BN = 256;      // output columns per workgroup
+constexpr int MAT_BK = 64;       // K per slice
+constexpr uint32_t MAT_OUT = 0x80000000u;  // an offset past every descriptor here
+
+constexpr int mat_stages(int tm) { return tm == 1 ? 4 : 2; }
+
+struct MatArgs {
+  const bf16_t *x; int64_t sx;            // row strides in elements
+  const bf16_t *w, *w2; int64_t sw;
+  int M, N, K;                            // K: contraction of w (of each half of a pair)
+  int Kx;                                 // contraction columns x holds (K-contiguous x)
+  int kpair;                              // MAT_NN: slices of w before w2's follow
+  int mpair, xpair;                       // MAT_TN: row tiles of out before out2's, and x's
+                                          // column where they start
+  int kt;                                 // slices per tile, a multiple of the stages
+  int tiles_m, tiles_n, splits;
+  void *out, *out2; int64_t so;
+  int64_t plane;                          // MAT_F32: elements between the splits' partial sums
+  int add;                                // MAT_F32: add to out
+  float *z1, *z2; int gelu;               // MAT_GATED: the two products (rows of N), or null
+  // cross entropy: rows' targets (less col0), log-sum-exp, upstream gradient
+  const int64_t *targets; int64_t ignore; int64_t V; int64_t col0;
+  const float *lse; const float *grad; int64_t sgrad; const float *count;
+  float2 *part; float *tgt;
+};
+
+// Tile of the t-th work item: whole items go to the XCDs in turn (workgroup b
+// runs on XCD b mod 8), each XCD taking one run of a sequence that walks panels of
+// four column tiles row by row, so that the 32 tiles an XCD has in flight share
+// 4 w tiles and 8 x tiles in its L2.  A bijection onto the items.
+__host__ __device__ inline void mat_tile(int t, int tiles_m, int tiles_n, int splits, int &bm, int &bn,
+                                         int &sp) {
+  const int total = tiles_m * tiles_n * splits;
+  const int xcd = t & 7, q = total >> 3, r = total & 7;
+  int s = xcd * q + (xcd < r ? xcd : r) + (t >> 3);
+  const int plane = tiles_m * tiles_n;
+  sp = s / plane;
+  s -= sp * plane;
+  const int panel = s / (4 * tiles_m);
+  s -= panel * 4 * tiles_m;
+  const int width = tiles_n - 4 * panel < 4 ? tiles_n - 4 * panel : 4;
+  bm = s / width;
+  bn = 4 * panel + (s - bm * width);
+}
+
+__device__ __forceinline__ float gelu_f(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+// d gelu / dx = cdf(x) + x pdf(x)
+__device__ __forceinline__ float gelu_slope(float x) {
+  return 0.5f * (1.0f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * expf(-0.5f * x * x);
+}
+
+// The upstream gradient of a row's loss: 0 of an ignored row, NaN of a target
+// outside the vocabulary.
+__device__ __forceinline__ float loss_weight(const float *grad, int64_t sgrad, const float *count,
+                                             int64_t m, int64_t target, int64_t ignore, int64_t V) {
+  if (target == ignore) return 0.0f;
+  if (target < 0 || target >= V) return __builtin_nanf("");
+  const float g = grad[m * sgrad];
+  return count ? g / *count : g;
+}
+
+template <int FORM, int TM, int EPI>
+__global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
+  constexpr int BM = 64 * TM, NST = mat_stages(TM);
+  constexpr bool WR = FORM != MAT_NT, XR = FORM == MAT_TN;  // rows along N / M
+  constexpr int WST = MAT_BN * MAT_BK, XST = BM * MAT_BK;   // elements per stage
+  __shared__ __align__(16) bf16_t w0[WST], w1[WST], w2s[NST > 2 ? WST : 8], w3[NST > 2 ? WST : 8];
+  __shared__ __align__(16) bf16_t x0[XST], x1[XST], x2s[NST > 2 ? XST : 8], x3[NST > 2 ? XST : 8];
+  constexpr int DB = 8, DX = 2 * TM;  // 1 KB loads of w and x per wave and slice
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int total = p.tiles_m * p.tiles_n * p.splits;
+  const int grid = static_cast<int>(gridDim.x);
+  const int ntile = (total - static_cast<int>(blockIdx.x) + grid - 1) / grid;
+  if (ntile <= 0) return;  // uniform; (the host launches no such workgroup)
+  const int KT = p.kt;
+
+  // Load block j of a wave: RPI rows of LPR lanes; lane i fills physical chunk
+  // i % LPR of row RPI j + i / LPR.  The swizzle depends on the row's low bits,
+  // hence on j's parity alone.
+  constexpr int LPW = WR ? 32 : 8, RPW = 64 / LPW;           // w
+  constexpr int LPX = XR ? BM / 8 : 8, RPX = 64 / LPX;       // x
+  auto logical = [](bool rows, int width, int row, int pc) {
+    if (!rows) return pc ^ ((row >> 1) & 7);
+    return pc ^ ((width == 64 ? (row >> 1) & 1 : row & 3) << 2);
+  };
+  int cw[2], cx[2];            // logical chunk
+  uint32_t lw[2], lx[2];       // byte offset from the block's first row
+#pragma unroll
+  for (int par = 0; par < 2; ++par) {
+    const int rw = lane / LPW, rx = lane / LPX;
+    cw[par] = logical(WR, MAT_BN, RPW * par + rw, lane % LPW);
+    cx[par] = logical(XR, BM, RPX * par + rx, lane % LPX);
+    lw[par] = static_cast<uint32_t>(rw) * static_cast<uint32_t>(p.sw * 2) + 16u * cw[par];
+    lx[par] = static_cast<uint32_t>(rx) * static_cast<uint32_t>(p.sx * 2) + 16u * cx[par];
+  }
+  auto stage_w = [&](auto st) __attribute__((always_inline)) -> bf16_t * {
+    constexpr int S = decltype(st)::value;
+    return S == 0 ? w0 : S == 1 ? w1 : S == 2 ? w2s : w3;
+  };
+  auto stage_x = [&](auto st) __attribute__((always_inline)) -> bf16_t * {
+    constexpr int S = decltype(st)::value;
+    return S == 0 ? x0 : S == 1 ? x1 : S == 2 ? x2s : x3;
+  };
+
+  // The next slice to load: slice ds of this workgroup's tile dj, at (bm, bn, sp).
+  int dj = 0, ds = 0, dbm, dbn, dsp;
+  mat_tile(static_cast<int>(blockIdx.x), p.tiles_m, p.tiles_n, p.splits, dbm, dbn, dsp);
+  auto issue = [&](auto st) __attribute__((always_inline)) {
+    if (ds == KT) {  // (past the last slice the loads repeat it: every step issues as many)
+      if (dj + 1 < ntile) {
+        ds = 0;
+        ++dj;
+        mat_tile(static_cast<int>(blockIdx.x) + dj * grid, p.tiles_m, p.tiles_n, p.splits, dbm, dbn, dsp);
+      } else {
+        ds = KT - 1;
+      }
+    }
+    const int s = dsp * KT + ds;
+    ++ds;
+    // w: this wave's rows of the slice, their first element, how many there are
+    const bf16_t *wb;
+    int wrows, wleft;  // valid rows; valid elements of the last one
+    if constexpr (WR) {
+      const bool second = s >= p.kpair;
+      const int k0 = (second ? s - p.kpair : s) * MAT_BK + 16 * wave;
+      wb = (second ? p.w2 : p.w) + k0 * p.sw + dbn * MAT_BN;
+      wrows = max(0, min(16, p.K - k0));
+      wleft = ((p.N + 7) & ~7) - dbn * MAT_BN;
+    } else {
+      const int k0 = s * MAT_BK;
+      // a gated tile takes 64 rows of each weight for a wave's 128 columns
+      const int n0 = EPI == MAT_GATED ? dbn * (MAT_BN / 2) + 64 * (wave >> 1) : dbn * MAT_BN + 64 * wave;
+      wb = (EPI == MAT_GATED && (wave & 1) ? p.w2 : p.w) + n0 * p.sw + k0;
+      wrows = max(0, min(64, p.N - n0));
+      wleft = max(0, p.K - k0);
+    }
+    const bf16_t *xb;
+    int xrows, xleft;
+    if constexpr (XR) {
+      const int k0 = s * MAT_BK + 16 * wave;
+      const bool second = dbm >= p.mpair;
+      const int m0 = (second ? dbm - p.mpair : dbm) * BM;
+      xb = p.x + k0 * p.sx + (second ? p.xpair : 0) + m0;
+      xrows = max(0, min(16, p.K - k0));
+      xleft = ((p.M + 7) & ~7) - m0;
+    } else {
+      const int k0 = s * MAT_BK, m0 = dbm * BM + 16 * TM * wave;
+      xb = p.x + m0 * p.sx + k0;
+      xrows = max(0, min(16 * TM, p.M - m0));
+      xleft = max(0, p.Kx - k0);
+    }
+    const uint32_t wbytes = wrows > 0 ? static_cast<uint32_t>(((wrows - 1) * p.sw + wleft) * 2) : 0u;
+    const uint32_t xbytes = xrows > 0 ? static_cast<uint32_t>(((xrows - 1) * p.sx + xleft) * 2) : 0u;
+    const __amdgpu_buffer_rsrc_t wrs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t *>(wb), 0, wbytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t xrs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t *>(xb), 0, xbytes, 0x00020000);
+    uint32_t vw[2], vx[2];
+#pragma unroll
+    for (int par = 0; par < 2; ++par) {  // chunks past the end of K read zeros
+      vw[par] = WR || 8 * cw[par] < wleft ? lw[par] : MAT_OUT;
+      vx[par] = XR || 8 * cx[par] < xleft ? lx[par] : MAT_OUT;
+    }
+    bf16_t *lwp = stage_w(st) + wave * DB * 512, *lxp = stage_x(st) + wave * DX * 512;
+#pragma unroll
+    for (int j = 0; j < DB; ++j) {
+      // a block past the last row reads zeros (its row offset has to stay inside
+      // the buffer)
+      const uint32_t ow = static_cast<uint32_t>(j * RPW * 2 * p.sw);
+      const bool wl = ow < wbytes;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (alds_void *)(lwp + 512 * j), 16, wl ? vw[j & 1] : MAT_OUT,
+                                               wl ? static_cast<int>(ow) : 0, 0, 0);
+      if (j < DX) {
+        const uint32_t ox = static_cast<uint32_t>(j * RPX * 2 * p.sx);
+        const bool xl = ox < xbytes;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xrs, (alds_void *)(lxp + 512 * j), 16,
+                                                 xl ? vx[j & 1] : MAT_OUT, xl ? static_cast<int>(ox) : 0, 0, 0);
+      }
+    }
+  };
+
+  const int wn = (wave & 1) * 128, wm = (wave >> 1) * (32 * TM);  // wave's columns and rows
+  const int g = lane >> 5, lr = lane & 31;
+  // K-contiguous reads: row base + lr, chunk 2 kk + g of 16-wide K step kk
+  const int swz = (lr >> 1) & 7;
+  // transposing reads: 16-lane group q reads K rows 16 kk + 8 (q >> 1) + 0..3 (then
+  // + 4 .. 7) of columns 16 (q & 1) + 0..15 of a 32-column tile; lane i of it row
+  // i >> 2, columns 4 (i & 3) .. + 3
+  const int ti = lane & 15, tq = lane >> 4;
+  const int trow = 8 * (tq >> 1) + (ti >> 2), tcol = 16 * (tq & 1) + 4 * (ti & 3);
+  auto read_w = [&](auto st, int tn, int kk) __attribute__((always_inline)) -> abf16x8_t {
+    const bf16_t *b = stage_w(st);
+    if constexpr (WR) {
+      const int T = ((wn >> 5) + tn) ^ (ti >> 2);  // 32-column tile, swizzled
+      const bf16_t *a = b + (trow + 16 * kk) * MAT_BN + 32 * T + tcol;
+      const ms16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mlds_s16x4_t *)(a));
+      const ms16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mlds_s16x4_t *)(a + 4 * MAT_BN));
+      return __builtin_bit_cast(abf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const bf16_t *a = b + (wn + 32 * tn + lr) * MAT_BK + 8 * ((2 * kk + g) ^ swz);
+      return __builtin_bit_cast(abf16x8_t, *reinterpret_cast<const au32x4_t *>(a));
+    }
+  };
+  auto read_x = [&](auto st, int tm, int kk) __attribute__((always_inline)) -> abf16x8_t {
+    const bf16_t *b = stage_x(st);
+    if constexpr (XR) {
+      const int T = ((wm >> 5) + tm) ^ (BM == 64 ? (ti >> 3) & 1 : ti >> 2);
+      const bf16_t *a = b + (trow + 16 * kk) * BM + 32 * T + tcol;
+      const ms16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mlds_s16x4_t *)(a));
+      const ms16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mlds_s16x4_t *)(a + 4 * BM));
+      return __builtin_bit_cast(abf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const bf16_t *a = b + (wm + 32 * tm + lr) * MAT_BK + 8 * ((2 * kk + g) ^ swz);
+      return __builtin_bit_cast(abf16x8_t, *reinterpret_cast<const au32x4_t *>(a));
+    }
+  };
+
+  mf32x16_t acc[4][TM];
+  abf16x8_t fa[2][4][2], fb[2][TM][2];  // fragments of a half slice (two 16-wide K steps)
+  auto read_frags = [&](auto st, auto half) __attribute__((always_inline)) {
+    constexpr int H = decltype(half)::value;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+      for (int t = 0; t < TM; ++t) fb[H][t][kk] = read_x(st, t, 2 * H + kk);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) fa[H][t][kk] = read_w(st, t, 2 * H + kk);
+    }
+  };
+  auto mma = [&](auto half) __attribute__((always_inline)) {
+    constexpr int H = decltype(half)::value;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm)
+          acc[tn][tm] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[H][tn][kk], fb[H][tm][kk], acc[tn][tm], 0, 0, 0);
+  };
+  // every MFMA is followed by its share of the fragment reads and of the loads
+  auto interleave = [&](auto dma) __attribute__((always_inline)) {
+    static_for<8 * TM>([&](auto i) __attribute__((always_inline)) {
+      constexpr int I = decltype(i)::value, NM = 8 * TM;
+      constexpr int ND = 8 * (WR ? 2 : 1) + 2 * TM * (XR ? 2 : 1), NV = DB + DX;
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, (I + 1) * ND / NM - I * ND / NM, 0);  // DS read
+      if constexpr (decltype(dma)::value)
+        __builtin_amdgcn_sched_group_barrier(0x020, (I + 1) * NV / NM - I * NV / NM, 0);  // VMEM read
+    });
+  };
+  using std::integral_constant;
+  using I0 = integral_constant<int, 0>;
+  using I1 = integral_constant<int, 1>;
+  // Step over the slice in stage S: the MFMAs of its first half while its second
+  // is read; every wave's loads of the next slice have landed (its own, waited
+  // for, before the barrier) and nobody reads stage S again: it is refilled; the
+  // MFMAs of the second half while the next slice's first is read.
+  auto step = [&](auto st) __attribute__((always_inline)) {
+    constexpr int S = decltype(st)::value;
+    read_frags(st, I1{});
+    mma(I0{});
+    interleave(integral_constant<bool, false>{});
+    vmcnt_wait<(NST - 2) * (DB + DX)>();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    issue(st);
+    read_frags(integral_constant<int, (S + 1) % NST>{}, I0{});
+    mma(I1{});
+    interleave(integral_constant<bool, true>{});
+  };
+
+  // Lane (lr, g) holds, for row m = wm + 32 tm + lr of the tile, columns
+  // wn + 32 tn + 8 q + 4 g + i in acc[tn][tm][4 q + i].
+  auto epilogue = [&](int j) __attribute__((always_inline)) {
+    int bm, bn, sp;
+    mat_tile(static_cast<int>(blockIdx.x) + j * grid, p.tiles_m, p.tiles_n, p.splits, bm, bn, sp);
+    const bool second = FORM == MAT_TN && bm >= p.mpair;
+    const int m0 = (second ? bm - p.mpair : bm) * BM + wm;      // wave's first row
+    const int n0 = bn * (EPI == MAT_GATED ? MAT_BN / 2 : MAT_BN) + (EPI == MAT_GATED ? wn / 2 : wn);
+    // Lanes l and l + 32 hold the same row: they swap halves of each pair of
+    // column groups so that each stores 16 contiguous bytes.
+    auto store_pair = [&](bf16_t *row, int c, int limit, const float (&v)[8]) __attribute__((always_inline)) {
+      // v: columns 16 pq + 4 g + i (i < 4) and 16 pq + 8 + 4 g + i
+      const auto s0 = __builtin_amdgcn_permlane32_swap(pack_bf(v[0], v[1]), pack_bf(v[4], v[5]), false, false);
+      const auto s1 = __builtin_amdgcn_permlane32_swap(pack_bf(v[2], v[3]), pack_bf(v[6], v[7]), false, false);
+      if (c + 8 * g < limit)
+        *reinterpret_cast<au32x4_t *>(row + c + 8 * g) = au32x4_t{s0[0], s1[0], s0[1], s1[1]};
+    };
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) {
+      const int m = m0 + 32 * tm + lr;
+      const bool live = m < p.M;
+      if constexpr (EPI == MAT_BF16) {
+        bf16_t *row = static_cast<bf16_t *>(second ? p.out2 : p.out) + m * p.so + n0;
+        const int limit = live ? p.N - n0 : 0;
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int pq = 0; pq < 2; ++pq) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = acc[tn][tm][8 * pq + i];
+            store_pair(row, 32 * tn + 16 * pq, limit, v);
+          }
+      } else if constexpr (EPI == MAT_F32) {
+        float *row = static_cast<float *>(second ? p.out2 : p.out) + sp * p.plane + m * p.so + n0;
+        const int limit = live ? p.N - n0 : 0;
+        const bool vec = p.so % 4 == 0;  // uniform
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c = 32 * tn + 8 * q + 4 * g;
+            af32x4_t v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = acc[tn][tm][4 * q + i];
+            if (vec && c + 4 <= limit) {
+              af32x4_t *d = reinterpret_cast<af32x4_t *>(row + c);
+              if (p.add) v += *d;
+              *d = v;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (c + i < limit) row[c + i] = p.add ? row[c + i] + v[i] : v[i];
+            }
+          }
+      } else if constexpr (EPI == MAT_GATED) {
+        bf16_t *row = static_cast<bf16_t *>(p.out) + m * p.so + n0;
+        const int limit = live ? p.N - n0 : 0;
+#pragma unroll
+        for (int tn = 0; tn < 2; ++tn)
+#pragma unroll
+          for (int pq = 0; pq < 2; ++pq) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float a = acc[tn][tm][8 * pq + i];
+              v[i] = (p.gelu ? gelu_f(a) : a) * acc[tn + 2][tm][8 * pq + i];
+            }
+            store_pair(row, 32 * tn + 16 * pq, limit, v);
+            if (p.z1) {
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                const int c = 32 * tn + 16 * pq + 8 * hh + 4 * g;
+                if (c < limit) {
+                  const int64_t at = static_cast<int64_t>(m) * p.N + n0 + c;
+                  af32x4_t a, b;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    a[i] = acc[tn][tm][8 * pq + 4 * hh + i];
+                    b[i] = acc[tn + 2][tm][8 * pq + 4 * hh + i];
+                  }
+                  *reinterpret_cast<af32x4_t *>(p.z1 + at) = a;
+                  *reinterpret_cast<af32x4_t *>(p.z2 + at) = b;
+                }
+              }
+            }
+          }
+      } else if constexpr (EPI == MAT_STATS) {
+        // max and sum of exp over the wave's 128 columns of the row, and the
+        // target's logit where it lies among them
+        const int limit = p.N - n0;  // columns of the vocabulary from the wave's first
+        float mx = -INFINITY;
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (32 * tn + 8 * (i >> 2) + 4 * g + (i & 3) >= limit) acc[tn][tm][i] = -INFINITY;
+            mx = fmaxf(mx, acc[tn][tm][i]);
+          }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float sub = mx == -INFINITY ? 0.0f : mx * 1.44269504088896341f;
+        const int64_t t = live ? p.targets[m] - n0 : -1;
+        const int tc = t >= 0 && t < min(128, limit) ? static_cast<int>(t) : -1;
+        float sum = 0.0f, zt = 0.0f;
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float v = acc[tn][tm][i];
+            sum += __builtin_amdgcn_exp2f(fmaf(v, 1.44269504088896341f, -sub));
+            if (32 * tn + 8 * (i >> 2) + 4 * g + (i & 3) == tc) zt = v;
+          }
+        sum += __shfl_xor(sum, 32);
+        if (live) {
+          if (g == 0) p.part[static_cast<int64_t>(2 * bn + (wave & 1)) * p.M + m] = make_float2(mx, sum);
+          if (tc >= 0 && ((tc >> 2) & 1) == g) p.tgt[m] = zt;
+        }
+      } else {
+        // d = (exp(z - lse) - [n = target]) * weight, zeros in the columns that
+        // pad the vocabulary to eights
+        bf16_t *row = static_cast<bf16_t *>(p.out) + m * p.so + n0;
+        const int limit = live ? ((p.N + 7) & ~7) - n0 : 0, valid = p.N - n0;
+        const int64_t t = live ? p.targets[m] : p.ignore;
+        const float wgt = live ? loss_weight(p.grad, p.sgrad, p.count, m, t, p.ignore, p.V) : 0.0f;
+        const float lse2 = live ? p.lse[m] * 1.44269504088896341f : 0.0f;
+        const int64_t tl = t - p.col0 - n0;
+        const int tc = tl >= 0 && tl < 128 ? static_cast<int>(tl) : -1;
+        const bool used = live && t != p.ignore;
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int pq = 0; pq < 2; ++pq) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int c = 32 * tn + 16 * pq + 8 * (i >> 2) + 4 * g + (i & 3);
+              float e = __builtin_amdgcn_exp2f(fmaf(acc[tn][tm][8 * pq + i], 1.44269504088896341f, -lse2));
+              if (c == tc) e -= 1.0f;
+              v[i] = used && c < valid ? e * wgt : 0.0f;
+            }
+            store_pair(row, 32 * tn + 16 * pq, limit, v);
+          }
+      }
+    }
+  };
+
+  issue(I0{});
+  issue(I1{});
+  if constexpr (NST > 2) {
+    issue(integral_constant<int, 2>{});
+    issue(integral_constant<int, 3>{});
+  }
+  vmcnt_wait<(NST - 1) * (DB + DX)>();  // slice 0
+  asm volatile("s_barrier" ::: "memory");
+  read_frags(I0{}, I0{});
+  for (int j = 0; j < ntile; ++j) {
+#pragma unroll
+    for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+      for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[tn][tm][i] = 0.0f;
+    for (int k = 0; k < KT; k += NST)
+      static_for<NST>([&](auto st) __attribute__((always_inline)) { step(st); });
+    epilogue(j);
+  }
+  // No direct-to-LDS write may still be landing when the workgroup's LDS is
+  // handed to the next one.
+  vmcnt_wait<0>();
+}
+
+// How a product is cut: tiles of 64 tm rows, K in `splits` runs of kt slices.
+struct MatPlan {
+  int tm, tiles_m, tiles_n, splits, kt;
+};
+
+// M: rows of one of `pair` outputs; slices: of K; width: output columns per tile.
+inline MatPlan mat_plan(int64_t M, int64_t N, int64_t slices, int pair, int width, bool may_split) {
+  MatPlan best{};
+  double least = 1e300;
+  for (int tm : {4, 2, 1}) {
+    const int nst = mat_stages(tm);
+    const int64_t tm_tiles = cdiv(M, 64 * tm) * pair, tn_tiles = cdiv(N, width), tiles = tm_tiles * tn_tiles;
+    int64_t splits = 1;
+    if (may_split && tiles < MAT_CUS) splits = std::max<int64_t>(1, std::min<int64_t>(MAT_CUS / tiles, slices / nst));
+    const int64_t kt = cdiv(cdiv(slices, splits), nst) * nst;
+    splits = std::max<int64_t>(1, cdiv(slices, kt));
+    const double rounds = double(cdiv(tiles * splits, MAT_CUS));
+    double cost = rounds * kt * (tm + 1.3);
+    // the partial sums' second launch, and their bytes there and back (in the time
+    // of 0.16 us that a slice takes per unit of tm + 1.3)
+    if (splits > 1) cost += 20.0 + double(splits) * M * pair * N * 1.25e-5;
+    if (cost < least - 1e-9) {
+      least = cost;
+      best = MatPlan{tm, static_cast<int>(tm_tiles), static_cast<int>(tn_tiles), static_cast<int>(splits),
+                     static_cast<int>(kt)};
+    }
+  }
+  return best;
+}
+
+template <int FORM, int EPI>
+inline void mat_launch(MatArgs a, const MatPlan &pl, hipStream_t st) {
+  a.tiles_m = pl.tiles_m;
+  a.tiles_n = pl.tiles_n;
+  a.splits = pl.splits;
+  a.kt = pl.kt;
+  const int64_t items = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n * pl.splits;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(MAT_CUS, items)));
+  if (pl.tm == 4) hipLaunchKernelGGL((mat_kernel<FORM, 4, EPI>), grid, dim3(256), 0, st, a);
+  else if (pl.tm == 2) hipLaunchKernelGGL((mat_kernel<FORM, 2, EPI>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((mat_kernel<FORM, 1, EPI>), grid, dim3(256), 0, st, a);
+}
+
+// Products compiled once (bf16_mat.hip): out as bf16, or fp32 partial sums.
+void mat_nn(const MatArgs &a, const MatPlan &pl, bool f32, hipStream_t st);
+void mat_tn(const MatArgs &a, const MatPlan &pl, bool f32, hipStream_t st);
+void mat_nt_f32(const MatArgs &a, const MatPlan &pl, hipStream_t st);
+// out (rows, cols) bf16 = the sum of `splits` fp32 planes (rows of cols, contiguous);
+// cols a multiple of 8.
+void mat_join(const float *part, int64_t plane, int splits, bf16_t *out, int64_t so, int64_t rows,
+              int64_t cols, hipStream_t st);
+
+// Sizes and strides the kernel's 32-bit offsets take.
+inline bool mat_fits(int64_t M, int64_t N, int64_t K, int64_t s) {
+  return M < (int64_t(1) << 30) && N < (int64_t(1) << 30) && K < (int64_t(1) << 30) && s < (int64_t(1) << 22) &&
+         cdiv(M, 64) * cdiv(N, 128) < (int64_t(1) << 24);
+}
+
+}  // namespace evo2

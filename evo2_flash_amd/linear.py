@@ -1,13 +1,15 @@
 """bf16 projections (out_proj, the attention projections, the MLP, the head):
 `linear` and `gated` run on this build's weight-streaming kernel
 (csrc/bf16_stream.hip) at decode batch sizes and on the platform's library GEMM
-otherwise.
+otherwise.  `gated_linear` is the gated product of any number of rows in one launch,
+with its backward pass (csrc/gated.hip).
 """
 
 from typing import Optional
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 from torch.utils._device import DeviceContext
 
 from . import _lib
@@ -146,4 +148,87 @@ def gated(x, w1, w2, gelu):
     return (torch.nn.functional.gelu(z1) if gelu else z1) * z2
 
 
-__all__ = ["linear", "gated", "plain", "STREAM_ROWS"]
+def _weight_rows(w1, w2):
+    """Both weights as 16-byte aligned rows of one stride."""
+    w1, w2 = _lib.rows16(w1), _lib.rows16(w2)
+    if w1.stride(0) != w2.stride(0):
+        w1, w2 = w1.contiguous(), w2.contiguous()
+    return w1, w2
+
+
+def _gated_forward(x, w1, w2, gelu, keep):
+    """(h, z1, z2): act(x w1^T) * (x w2^T) in bf16 and, to `keep`, both products in
+    fp32 (else None)."""
+    M, (I, H) = x.shape[0], w1.shape
+    h = torch.empty(M, I, dtype=x.dtype, device=x.device)
+    z1 = z2 = None
+    if keep:
+        z1, z2 = torch.empty(2, M, I, dtype=torch.float32, device=x.device).unbind(0)
+    if M:
+        xr, (a, b) = _lib.rows16(x), _weight_rows(w1, w2)
+        with _lib.on_device(xr):
+            _lib.call("evo2_gated_linear", _lib.ptr(xr), xr.stride(0), _lib.ptr(a), _lib.ptr(b),
+                      a.stride(0), int(gelu), _lib.ptr(h), h.stride(0), _lib.ptr(z1), _lib.ptr(z2),
+                      M, I, H, _lib.stream_of(xr))
+    return h, z1, z2
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w1, w2, gelu):
+        h, z1, z2 = _gated_forward(x, w1, w2, gelu, True)
+        ctx.save_for_backward(x, w1, w2, z1, z2)
+        ctx.gelu = gelu
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        x, w1, w2, z1, z2 = ctx.saved_tensors
+        M, (I, H) = x.shape[0], w1.shape
+        dx = dw1 = dw2 = None
+        if ctx.needs_input_grad[0]:
+            dx = torch.empty(M, H, dtype=x.dtype, device=x.device)
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            make = torch.empty if M else torch.zeros
+            dw1, dw2 = (make(I, H, dtype=x.dtype, device=x.device) for _ in range(2))
+        if M:
+            g, xr, (a, b) = _lib.rows16(dh), _lib.rows16(x), _weight_rows(w1, w2)
+            with _lib.on_device(xr):
+                n = _lib.lib().evo2_gated_linear_workspace_bytes(M, I, H)
+                ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+                _lib.call("evo2_gated_linear_backward", _lib.ptr(g), g.stride(0), _lib.ptr(xr),
+                          xr.stride(0), _lib.ptr(a), _lib.ptr(b), a.stride(0), int(ctx.gelu),
+                          _lib.ptr(z1), _lib.ptr(z2), _lib.ptr(dx), _lib.ptr(dw1), _lib.ptr(dw2),
+                          _lib.ptr(ws), n, M, I, H, _lib.stream_of(xr))
+        return (dx, dw1 if ctx.needs_input_grad[1] else None,
+                dw2 if ctx.needs_input_grad[2] else None, None)
+
+
+def gated_linear(x, w1, w2, gelu):
+    """act(x @ w1^T) * (x @ w2^T), act the exact GELU or the identity, differentiable in
+    x, w1 and w2 (once): `gated` with its backward pass, both projections, the
+    activation and the product in one launch at any number of rows.
+
+    x (..., H), w1 and w2 (I, H) bf16 on one device, I and H multiples of 8.  The
+    products and the activation are fp32 and the result is rounded once (`gated`
+    rounds each step, as the library's separate operators do)."""
+    _lib.require_device(x, w1, w2)
+    if any(t.dtype != torch.bfloat16 for t in (x, w1, w2)):
+        raise ValueError(f"gated_linear takes bf16 x, w1, w2, got {x.dtype}, {w1.dtype}, {w2.dtype}")
+    if (w1.dim() != 2 or w1.shape != w2.shape or x.dim() < 1 or x.shape[-1] != w1.shape[1]):
+        raise ValueError(f"gated_linear: shapes x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 "
+                         f"{tuple(w2.shape)} do not match")
+    if any(n == 0 or n % 8 for n in w1.shape):
+        raise ValueError(f"gated_linear takes weights of multiples of 8, got {tuple(w1.shape)}")
+    if not x.device == w1.device == w2.device:
+        raise ValueError(f"gated_linear: operands on {x.device}, {w1.device}, {w2.device}")
+    rows = x.reshape(-1, x.shape[-1])
+    if torch.is_grad_enabled() and (rows.requires_grad or w1.requires_grad or w2.requires_grad):
+        h = _GatedLinear.apply(rows, w1, w2, bool(gelu))
+    else:
+        h = _gated_forward(rows, w1, w2, gelu, False)[0]
+    return h.view(*x.shape[:-1], w1.shape[0])
+
+
+__all__ = ["linear", "gated", "gated_linear", "plain", "STREAM_ROWS"]

@@ -1,0 +1,119 @@
+"""The head's softmax cross entropy from hidden rows and the head's weight, with its
+gradient, without the logits tensor (csrc/linear_loss.hip): what scoring and
+training need of RMSNorm(x) @ embed^T (model.py:343-348).
+
+Forward leaves each row's log-sum-exp; backward computes the logits again in pieces
+of the vocabulary.  The sums are fp32 (over rows: 64 bits, in a fixed order, so a
+result does not depend on timing).
+"""
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_REDUCTIONS = ("none", "sum", "mean")
+
+
+def _workspace(T, V, H, backward, device):
+    n = _lib.lib().evo2_linear_loss_workspace_bytes(T, V, H, int(backward))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _forward(hidden, weight, targets, ignore_index, reduction):
+    """(nll (T,), lse (T,), loss (), count ()) fp32; loss and count None with "none"."""
+    T, (V, H) = hidden.shape[0], weight.shape
+    dev = hidden.device
+    nll, lse = torch.empty(2, T, dtype=torch.float32, device=dev).unbind(0)
+    loss = count = None
+    if reduction:
+        loss, count = torch.empty(2, dtype=torch.float32, device=dev).unbind(0)
+    if T == 0:
+        if reduction:
+            loss.fill_(0.0 if reduction == 1 else float("nan"))
+            count.zero_()
+        return nll, lse, loss, count
+    h, w = _lib.rows16(hidden), _lib.rows16(weight)
+    with _lib.on_device(h):
+        ws = _workspace(T, V, H, False, dev)
+        _lib.call("evo2_linear_loss", _lib.ptr(h), h.stride(0), _lib.ptr(w), w.stride(0),
+                  _lib.ptr(targets), ignore_index, reduction, _lib.ptr(nll), _lib.ptr(lse),
+                  _lib.ptr(loss), _lib.ptr(count), _lib.ptr(ws), ws.numel(), T, V, H,
+                  _lib.stream_of(h))
+    return nll, lse, loss, count
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
+        nll, lse, loss, count = _forward(hidden, weight, targets, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, targets, lse, count if reduction == 2 else None)
+        ctx.ignore_index = ignore_index
+        return loss if reduction else nll
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, targets, lse, count = ctx.saved_tensors
+        T, (V, H) = hidden.shape[0], weight.shape
+        dev = hidden.device
+        dh = dw = None
+        if ctx.needs_input_grad[0]:
+            dh = torch.empty(T, H, dtype=hidden.dtype, device=dev)
+        if ctx.needs_input_grad[1]:
+            dw = (torch.empty if T else torch.zeros)(V, H, dtype=weight.dtype, device=dev)
+        if T:
+            h, w = _lib.rows16(hidden), _lib.rows16(weight)
+            grad = grad.to(torch.float32)
+            with _lib.on_device(h):
+                ws = _workspace(T, V, H, True, dev)
+                _lib.call("evo2_linear_loss_backward", _lib.ptr(h), h.stride(0), _lib.ptr(w),
+                          w.stride(0), _lib.ptr(targets), ctx.ignore_index, _lib.ptr(lse),
+                          _lib.ptr(grad), grad.stride(0) if grad.dim() else 0, _lib.ptr(count),
+                          _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(ws), ws.numel(), T, V, H,
+                          _lib.stream_of(h))
+        return dh, dw, None, None, None
+
+
+def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="mean"):
+    """Cross entropy of the logits hidden @ weight^T against `targets`, differentiable
+    in hidden and weight (once).
+
+    hidden (..., H) and weight (V, H) bf16 on one device, H a multiple of 8; targets
+    (...) of an integer type.  Rows whose target is `ignore_index` have loss 0 and no
+    gradient; a target outside [0, V) otherwise makes its row's loss and gradient NaN
+    (nothing is read through it).  reduction: "none" (fp32 losses of targets' shape:
+    the negative log-likelihoods), "sum" or "mean" over the rows that are not ignored
+    (fp32 scalar; the mean of no rows is NaN).  The logits are fp32 sums of the bf16
+    products and never rounded."""
+    _lib.require_device(hidden, weight, targets)
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise ValueError(f"linear_cross_entropy takes bf16 hidden and weight, got {hidden.dtype}, "
+                         f"{weight.dtype}")
+    if (weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]
+            or targets.shape != hidden.shape[:-1]):
+        raise ValueError(f"linear_cross_entropy: shapes hidden {tuple(hidden.shape)}, weight "
+                         f"{tuple(weight.shape)}, targets {tuple(targets.shape)} do not match")
+    if weight.shape[0] == 0 or weight.shape[1] == 0 or weight.shape[1] % 8:
+        raise ValueError(f"linear_cross_entropy takes a weight of at least one row and rows of a "
+                         f"multiple of 8, got {tuple(weight.shape)}")
+    if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
+        raise ValueError(f"targets must be integers, got {targets.dtype}")
+    if not hidden.device == weight.device == targets.device:
+        raise ValueError(f"linear_cross_entropy: operands on {hidden.device}, {weight.device}, "
+                         f"{targets.device}")
+    shape = targets.shape
+    h = hidden.reshape(-1, hidden.shape[-1])
+    t = targets.reshape(-1).to(torch.int64).contiguous()
+    red = _REDUCTIONS.index(reduction)
+    if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
+        out = _LinearCrossEntropy.apply(h, weight, t, int(ignore_index), red)
+    else:
+        nll, _, loss, _ = _forward(h, weight, t, int(ignore_index), red)
+        out = loss if red else nll
+    return out if red else out.view(shape)
+
+
+__all__ = ["linear_cross_entropy"]

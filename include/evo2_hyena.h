@@ -432,6 +432,53 @@ int evo2_bf16_stream_gated(const void *x, int64_t sx, const void *w1, const void
                            void *stream);
 
 /*
+ * The gated product of a feed-forward block at any number of rows, and its backward
+ * pass (evo2_flash/model.py:77-101 before the down projection):
+ *   z1 = x w1^T, z2 = x w2^T, h = bf16(act(z1) * z2), act the exact GELU with
+ *   gelu != 0, else the identity; d1 = dh z2 act'(z1), d2 = dh act(z1);
+ *   dx = d1 w1 + d2 w2, dw1 = d1^T x, dw2 = d2^T x
+ *   x (M, H) row stride sx, w1, w2 (I, H) row stride sw, h (M, I) row stride sh,
+ *   dh (M, I) row stride sdh, dx (M, H), dw1, dw2 (I, H) contiguous, all bf16;
+ *   z1, z2 (M, I) fp32 contiguous, written by the forward call where not NULL (both
+ *   or neither) and read by the backward call.  I and H multiples of 8, rows 16-byte
+ *   aligned.  dx may be NULL; dw1 and dw2 may be NULL together.  The backward call
+ *   takes M >= 1 and a workspace of _workspace_bytes(M, I, H) bytes.
+ */
+int64_t evo2_gated_linear_workspace_bytes(int64_t M, int64_t I, int64_t H);
+int evo2_gated_linear(const void *x, int64_t sx, const void *w1, const void *w2, int64_t sw,
+                      int32_t gelu, void *h, int64_t sh, float *z1, float *z2, int64_t M, int64_t I,
+                      int64_t H, void *stream);
+int evo2_gated_linear_backward(const void *dh, int64_t sdh, const void *x, int64_t sx, const void *w1,
+                               const void *w2, int64_t sw, int32_t gelu, const float *z1,
+                               const float *z2, void *dx, void *dw1, void *dw2, void *workspace,
+                               int64_t workspace_bytes, int64_t M, int64_t I, int64_t H, void *stream);
+
+/*
+ * Softmax cross entropy of the logits h w^T (evo2_flash/model.py:343-348), which are
+ * never stored whole, and its gradient:
+ *   lse = log sum_n exp(h w_n), nll = lse - h w_target (0 where target == ignore,
+ *   NaN where it is otherwise outside [0, V)); loss their sum (reduction 1) or mean
+ *   over the count rows that are not ignored (2); reduction 0: nll alone, loss and
+ *   count may be NULL.
+ *   d = (exp(h w_n - lse) - [n = target]) g, dh = d w, dw = d^T h, with g =
+ *   grad[m * sgrad], divided by *count where count is not NULL (a mean's)
+ *   h (T, H) row stride sh, w (V, H) row stride sw, dh (T, H) and dw (V, H)
+ *   contiguous, bf16, H a multiple of 8, rows 16-byte aligned; targets (T,) int64;
+ *   nll, lse (T,), loss, count (1,), grad fp32.  dh or dw may be NULL.  T >= 1; the
+ *   workspace has _workspace_bytes(T, V, H, backward) bytes.
+ */
+int64_t evo2_linear_loss_workspace_bytes(int64_t T, int64_t V, int64_t H, int32_t backward);
+int evo2_linear_loss(const void *h, int64_t sh, const void *w, int64_t sw, const int64_t *targets,
+                     int64_t ignore, int32_t reduction, float *nll, float *lse, float *loss,
+                     float *count, void *workspace, int64_t workspace_bytes, int64_t T, int64_t V,
+                     int64_t H, void *stream);
+int evo2_linear_loss_backward(const void *h, int64_t sh, const void *w, int64_t sw,
+                              const int64_t *targets, int64_t ignore, const float *lse,
+                              const float *grad, int64_t sgrad, const float *count, void *dh, void *dw,
+                              void *workspace, int64_t workspace_bytes, int64_t T, int64_t V, int64_t H,
+                              void *stream);
+
+/*
  * Neox rotary of q and k with linear position scaling, and the write of k and
  * v into 16-position KV pages, from rows of a qkv projection (q | k | v, each
  * heads * head_dim bf16; row stride sqkv):
