@@ -160,6 +160,19 @@ SIGNATURES = {
         _c_i64, _c_i64, _c_i64,                   # out strides (n, h, row)
         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_f, _c_p,  # N, heads, L, Lv, head_dim, scale, stream
     ],
+    "evo2_packed_attention": [
+        _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,  # q, k + strides (row, head)
+        _c_p, _c_i64, _c_i64,                     # v + strides
+        _c_p, _c_i64, _c_p, _c_p, _c_p,           # cu, nseq, out, out_lo, lse
+        _c_i64, _c_i64, _c_i64, _c_i64, _c_f, _c_p,  # T, heads, kv, head_dim, scale, stream
+    ],
+    "evo2_packed_attention_backward": [
+        _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,  # dout, q + strides (row, head)
+        _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,  # k, v + strides
+        _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p,     # cu, nseq, out, out_lo, lse, delta
+        _c_p, _c_p, _c_p,                         # dq, dk, dv
+        _c_i64, _c_i64, _c_i64, _c_i64, _c_f, _c_p,  # T, heads, kv, head_dim, scale, stream
+    ],
     "evo2_bf16_stream_linear": [
         _c_p, _c_i64, _c_p, _c_i64, _c_p,         # x, sx, w, sw, bias
         _c_p, _c_i64, _c_p, _c_i64,               # residual, sr, out, so

@@ -18,9 +18,13 @@ rotary_prefill or once per call; fp32 scores and softmax, bf16 softmax weights i
 product); other head dims on torch's fused attention kernels where the
 platform has them for the inputs, else a chunked product with contiguous
 operands and an fp32 softmax.
+
+packed_attention is the causal attention of packed sequences of any lengths with its
+backward pass (csrc/packed_attention.hip), for scoring and training.
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -352,6 +356,107 @@ def causal_prefill_attention(q, k, v, scale):
     return _causal_chunked(q, k, v, scale)
 
 
-__all__ = ["decode_attention", "workspace", "paged_decode_attention", "check_block_table",
+def _head_rows(t):
+    """t (T, heads, hd) as the packed kernels read it: unit last stride, rows that do
+    not overlap, 16-byte aligned; itself or a copy."""
+    if (t.stride(2) == 1 and t.shape[2] <= t.stride(0) < 1 << 23 and t.stride(0) % 8 == 0
+            and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _packed_forward(q, k, v, cu, scale, keep):
+    """(out, out_lo, lse): the attention's output and, to `keep`, what the backward pass
+    needs (else None)."""
+    T, heads, hd = q.shape
+    out = torch.empty(T, heads, hd, dtype=q.dtype, device=q.device)
+    lo = lse = None
+    if keep:
+        lo = torch.empty_like(out)
+        lse = torch.empty(heads, T, dtype=torch.float32, device=q.device)
+    if T:
+        q, k, v = (_head_rows(t) for t in (q, k, v))
+        with _lib.on_device(q):
+            _lib.call("evo2_packed_attention", _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k),
+                      k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1), _lib.ptr(cu),
+                      cu.shape[0] - 1, _lib.ptr(out), _lib.ptr(lo), _lib.ptr(lse), T, heads,
+                      k.shape[1], hd, scale, _lib.stream_of(q))
+    return out, lo, lse
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu, scale):
+        out, lo, lse = _packed_forward(q, k, v, cu, scale, True)
+        ctx.save_for_backward(q, k, v, cu, out, lo, lse)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, cu, out, lo, lse = ctx.saved_tensors
+        T, heads, hd = q.shape
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if T:
+            d, q, k, v = (_head_rows(t) for t in (dout, q, k, v))
+            with _lib.on_device(q):
+                delta = torch.empty_like(lse)
+                _lib.call("evo2_packed_attention_backward", _lib.ptr(d), d.stride(0), d.stride(1),
+                          _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k), k.stride(0),
+                          k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1), _lib.ptr(cu),
+                          cu.shape[0] - 1, _lib.ptr(out), _lib.ptr(lo), _lib.ptr(lse),
+                          _lib.ptr(delta), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), T, heads,
+                          k.shape[1], hd, ctx.scale, _lib.stream_of(q))
+        need = ctx.needs_input_grad
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None,
+                None)
+
+
+def packed_attention(q, k, v, cu_seqlens, scale):
+    """Causal self-attention of packed sequences, differentiable in q, k and v (once):
+    q (T, heads, head_dim), k and v (T, kv_heads, head_dim) bf16 with head_dim 64 or
+    128 and heads a multiple of kv_heads (query head h reads key head
+    h // (heads // kv_heads)); views of any strides (the qkv projection's rows are read
+    in place), unaligned or overlapping rows are copied.  Sequence s takes rows
+    cu_seqlens[s] .. cu_seqlens[s + 1] - 1; cu_seqlens (nseq + 1,) is an integer tensor
+    on q's device that never decreases (the host does not read it; its entries are
+    clamped to [0, T]).  Rows outside every sequence give zeros and get zero gradients.
+    Returns (T, heads, head_dim) bf16.
+
+    Scores, softmax and sums are fp32; the probabilities and their gradients enter the
+    products as bf16.  A key's infinite or NaN value also reaches the queries before it
+    in its 64-row tile."""
+    _lib.require_device(q, k, v, cu_seqlens)
+    if any(t.dim() != 3 or t.dtype != torch.bfloat16 for t in (q, k, v)):
+        raise ValueError("packed_attention takes bf16 q (T, heads, head_dim), k and v (T, kv_heads, "
+                         "head_dim)")
+    T, heads, hd = q.shape
+    if (k.shape != v.shape or k.shape[0] != T or k.shape[2] != hd or heads == 0
+            or k.shape[1] == 0 or heads % k.shape[1]):
+        raise ValueError(f"packed_attention: shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v "
+                         f"{tuple(v.shape)} do not match")
+    if hd not in (64, 128):
+        raise ValueError(f"packed_attention takes head_dim 64 or 128, got {hd}")
+    if (cu_seqlens.dim() != 1 or cu_seqlens.shape[0] == 0
+            or cu_seqlens.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"cu_seqlens must be (nseq + 1,) int32 or int64, got "
+                         f"{tuple(cu_seqlens.shape)} {cu_seqlens.dtype}")
+    if not q.device == k.device == v.device == cu_seqlens.device:
+        raise ValueError(f"packed_attention: operands on {q.device}, {k.device}, {v.device}, "
+                         f"{cu_seqlens.device}")
+    scale = float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"packed_attention takes a positive scale, got {scale}")
+    cu = cu_seqlens
+    if cu.dtype != torch.int32:
+        cu = cu.clamp(0, T).to(torch.int32)
+    cu = cu.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _PackedAttention.apply(q, k, v, cu, scale)
+    return _packed_forward(q, k, v, cu, scale, False)[0]
+
+
+__all__ = ["packed_attention", "decode_attention", "workspace", "paged_decode_attention", "check_block_table",
            "PagedKVCache", "causal_prefill_attention", "prefill_attention",
            "prefill_attention_rows", "rotary_prefill", "rotary_decode", "PAGE"]

@@ -412,6 +412,33 @@ int evo2_iir_verify_gated(const void *zf, int64_t zs, const float *log_poles, in
                           void *stream);
 
 /*
+ * Causal self-attention of packed sequences and its backward pass: sequence s takes
+ * rows cu[s] .. cu[s + 1] - 1 of T, query head h reads key head h / (heads / kv):
+ *   p_ij = softmax_{j <= i in the sequence}(scale q_i . k_j), o = p v
+ *   ds = p (do v^T - delta), delta_i = do_i . o_i; dv = p^T do, dq = scale ds k,
+ *   dk = scale ds^T q, dk and dv summed over the query heads that share them
+ *   q, dout (T, heads, hd), k, v (T, kv, hd) bf16, strides st (row, at least hd), sh
+ *   (head), unit last stride, 16-byte aligned; cu (nseq + 1) int32 on the device,
+ *   never decreasing (entries are clamped to [0, T]; nothing is read or written
+ *   outside the tensors whatever it holds)
+ *   out, dq (T, heads, hd), dk, dv (T, kv, hd) bf16 contiguous; rows outside every
+ *   sequence are zero
+ *   out_lo (T, heads, hd) bf16 and lse (heads, T) fp32: what the backward call needs
+ *   of the forward one (both NULL without one); delta (heads, T) fp32 scratch
+ *   heads a multiple of kv, hd 64 or 128, scale > 0
+ */
+int evo2_packed_attention(const void *q, int64_t sqt, int64_t sqh, const void *k, int64_t skt,
+                          int64_t skh, const void *v, int64_t svt, int64_t svh, const int32_t *cu,
+                          int64_t nseq, void *out, void *out_lo, float *lse, int64_t T, int64_t heads,
+                          int64_t kv, int64_t head_dim, float scale, void *stream);
+int evo2_packed_attention_backward(const void *dout, int64_t sdt, int64_t sdh, const void *q,
+                                   int64_t sqt, int64_t sqh, const void *k, int64_t skt, int64_t skh,
+                                   const void *v, int64_t svt, int64_t svh, const int32_t *cu,
+                                   int64_t nseq, const void *out, const void *out_lo, const float *lse,
+                                   float *delta, void *dq, void *dk, void *dv, int64_t T, int64_t heads,
+                                   int64_t kv, int64_t head_dim, float scale, void *stream);
+
+/*
  * bf16 projections of at most 16 rows (decode steps), fp32 sums:
  *   _linear  out[m, n] = bf16(sum_k x[m, k] w[n, k] [+ bias[n]]), then with
  *            residual (row stride sr) bf16(that + residual[m, n])

@@ -1,0 +1,126 @@
+"""attention.packed_attention and its gradients against 64-bit arithmetic.
+
+Bounds (u = 2^-8, half a bf16 step; e = 2^-24): a score is off by es = (hd + 4) e scale
+sum |q k| and a probability relatively by twice the row's largest es plus the rounding
+of the exponent's argument; as a bf16 operand it is off by u p more.  o is rounded once.
+In the backward pass p (dp - delta) is rounded once as an operand, delta from o to 2^-16;
+each gradient is rounded once.
+"""
+
+import pytest
+import torch
+
+from evo2_flash_amd.attention import packed_attention
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF = torch.bfloat16
+U, E = 2.0 ** -8, 2.0 ** -24
+
+
+def _case(lens, heads, kv, hd, seed, pad=(0, 0), dev=1.3):
+    g = torch.Generator().manual_seed(seed)
+    T = sum(lens) + sum(pad)
+    q, k, v, d = ((torch.randn(T, n, hd, generator=g) * dev).to(BF).to(DEV)
+                  for n in (heads, kv, kv, heads))
+    cu = torch.tensor([pad[0], *lens]).cumsum(0).to(torch.int32).to(DEV)
+    return q, k, v, d, cu
+
+
+def _exact(q, k, v, d, cu, scale):
+    """{name: (value, bound)} in 64 bits."""
+    q, k, v, d = (t.detach().cpu().double() for t in (q, k, v, d))
+    cu = cu.cpu().tolist()
+    heads, kv, hd = q.shape[1], k.shape[1], q.shape[2]
+    r = {n: torch.zeros_like(t) for n, t in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+    b = {n: torch.zeros_like(t) for n, t in r.items()}
+    for s0, s1 in zip(cu[:-1], cu[1:]):
+        n = s1 - s0
+        if n <= 0:
+            continue
+        s = slice(s0, s1)
+        live = torch.ones(n, n, dtype=torch.bool).tril()
+        for h in range(heads):
+            j = h // (heads // kv)
+            sc = (q[s, h] @ k[s, j].t()) * scale
+            mag = (q[s, h].abs() @ k[s, j].abs().t()) * scale * live
+            p = torch.softmax(sc.masked_fill(~live, float("-inf")), 1)
+            top = (sc.abs() * live).amax(1, keepdim=True)
+            rp = 2 * (hd + 4) * E * mag.amax(1, keepdim=True) + (8 * top + n + 16) * E
+            o = p @ v[s, j]
+            so = p @ v[s, j].abs()
+            eo = (U + rp + (n + 8) * E) * so
+            r["o"][s, h] = o
+            b["o"][s, h] = U * o.abs() + eo
+            dp = d[s, h] @ v[s, j].t()
+            sdp = d[s, h].abs() @ v[s, j].abs().t()
+            delta = (p * dp).sum(1, keepdim=True)
+            # delta = do . o: o to a bf16 pair, whose error is e_o (fp32) + u^2 |o| / 2,
+            # the probabilities' own roundings (u p, before the value product) among it
+            edelta = (d[s, h].abs() * (eo + U * U * o.abs())).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            eds = (U + 2 * rp) * ds.abs() + p * (2 * (hd + 4) * E * sdp + edelta * 1.01)
+            if n >= 1:  # a query of one key: exactly 0
+                ds[0] = 0.0
+                eds[0] = 0.0
+            ep = (U + rp) * p
+            r["dq"][s, h] = scale * (ds @ k[s, j])
+            b["dq"][s, h] = scale * ((eds + n * E * ds.abs()) @ k[s, j].abs())
+            r["dk"][s, j] += scale * (ds.t() @ q[s, h])
+            b["dk"][s, j] += scale * ((eds + n * E * ds.abs()).t() @ q[s, h].abs())
+            r["dv"][s, j] += p.t() @ d[s, h]
+            b["dv"][s, j] += (ep + n * E * p).t() @ d[s, h].abs()
+    for n in ("dq", "dk", "dv"):
+        b[n] = b[n] * 1.01 + U * r[n].abs()
+    return {n: (r[n], b[n]) for n in r}
+
+
+def _check(got, want, what):
+    for n, t in got.items():
+        v, bound = want[n]
+        off = (t.detach().cpu().double() - v).abs()
+        assert bool((off <= bound * (1 + 2 * U) + 1e-38).all()), (
+            what, n, float((off / (bound + 1e-30)).max()))
+
+
+def _grads(q, k, v, d, cu, scale):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = packed_attention(*leaves, cu, scale)
+    return dict(zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, d))))
+
+
+CASES = [
+    ([1], 1, 1, 128), ([2], 2, 1, 64), ([1, 1, 1], 8, 8, 64), ([31, 32, 33], 4, 2, 128),
+    ([63, 64, 65], 3, 3, 64), ([127, 128, 129], 2, 2, 128), ([5, 0, 7, 0, 0, 200], 4, 1, 128),
+    ([257], 8, 8, 128), ([400, 3, 77], 16, 8, 64), ([640], 2, 1, 64), ([1000], 1, 1, 128),
+    ([1] * 150 + [3, 70], 2, 2, 64),
+]
+
+
+@pytest.mark.parametrize("lens,heads,kv,hd", CASES)
+def test_against_64_bits(lens, heads, kv, hd):
+    q, k, v, d, cu = _case(lens, heads, kv, hd, seed=sum(lens) + hd)
+    scale = hd ** -0.5
+    print(f"packed_attention {lens[:8]} {heads} {kv} {hd}", flush=True)
+    want = _exact(q, k, v, d, cu, scale)
+    with torch.no_grad():
+        _check({"o": packed_attention(q, k, v, cu, scale)}, want, "forward")
+    _check(_grads(q, k, v, d, cu, scale), want, "training")
+
+
+@pytest.mark.parametrize("pad", [(0, 9), (130, 0), (3, 300)])
+def test_rows_outside_the_sequences(pad):
+    """Rows before the first and behind the last sequence: zeros, and zero gradients,
+    whatever they hold."""
+    q, k, v, d, cu = _case([70, 1, 33], 4, 2, 128, seed=5, pad=pad)
+    out = torch.ones(q.shape[0], dtype=torch.bool)
+    out[pad[0]:q.shape[0] - pad[1]] = False
+    for t in (q, k, v, d):
+        t[out.to(DEV)] = float("nan")
+    got = _grads(q, k, v, d, cu, 0.09)
+    for t in (q, k, v, d):
+        t[out.to(DEV)] = 0.0
+    want = _exact(q, k, v, d, cu, 0.09)
+    _check(got, want, pad)
+    for n, t in got.items():
+        assert not t[out.to(DEV)].any(), n
