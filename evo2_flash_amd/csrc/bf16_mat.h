@@ -71,8 +71,10 @@ struct MatArgs {
   float *z1, *z2; int gelu;               // MAT_GATED: the two products (rows of N), or null
   // cross entropy: rows' targets (less col0), log-sum-exp, upstream gradient
   const int64_t *targets; int64_t ignore; int64_t V; int64_t col0;
-  const float *lse; const float *grad; int64_t sgrad; const float *count;
+  const float *lse; const float *grad; int64_t sgrad;
+  int weighted;                           // MAT_DLOG: rows times their upstream gradient
   float2 *part; float *tgt;
+  const float *num, *den;                 // MAT_BF16: out times *num / *den (each may be null)
 };
 
 // Tile of the t-th work item: whole items go to the XCDs in turn (workgroup b
@@ -100,14 +102,46 @@ __device__ __forceinline__ float gelu_slope(float x) {
   return 0.5f * (1.0f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * expf(-0.5f * x * x);
 }
 
-// The upstream gradient of a row's loss: 0 of an ignored row, NaN of a target
-// outside the vocabulary.
-__device__ __forceinline__ float loss_weight(const float *grad, int64_t sgrad, const float *count,
-                                             int64_t m, int64_t target, int64_t ignore, int64_t V) {
-  if (target == ignore) return 0.0f;
-  if (target < 0 || target >= V) return __builtin_nanf("");
-  const float g = grad[m * sgrad];
-  return count ? g / *count : g;
+// What a row's softmax less its target is multiplied by: its upstream gradient, 0 of an
+// ignored row, NaN of a target outside the vocabulary.  Where all rows share the
+// upstream gradient (a sum or a mean) it is left to the products' results: times one
+// factor, the values near -1 at the targets would all be rounded the same way.
+__device__ __forceinline__ float loss_weight(const MatArgs &p, int64_t m, int64_t target) {
+  if (target == p.ignore) return 0.0f;
+  if (target < 0 || target >= p.V) return __builtin_nanf("");
+  return p.weighted ? p.grad[m * p.sgrad] : 1.0f;
+}
+
+__device__ __forceinline__ float mat_factor(const float *num, const float *den) {
+  const float n = num ? *num : 1.0f;
+  return den ? n / *den : n;
+}
+
+// A raw buffer descriptor over `bytes` bytes from p.
+__device__ __forceinline__ au32x4_t mat_rsrc(const void *p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  // (uniform values; stated, for an operand that has to be in SGPRs)
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
+  return au32x4_t{lo, hi & 0xffffu, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(bytes)), 0x00020000u};
+}
+
+// One direct-to-LDS load: 64 lanes x 16 bytes at byte offset v (zeros past the
+// descriptor) to lds .. lds + 1 KB.  In asm so that the compiler does not know of it:
+// before each transposing LDS read it would wait for all such loads in flight.  The
+// kernel waits for them itself (mat_sync), and no register is written.
+__device__ __forceinline__ void mat_load(au32x4_t rsrc, uint32_t v, const bf16_t *lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds_addr(lds)), "v"(v), "s"(rsrc)
+               : "m0");
+}
+
+// All but N of the wave's loads and stores and all its LDS reads are done; then the
+// workgroup meets, and LDS holds what every wave's loads brought.
+template <int N>
+__device__ __forceinline__ void mat_sync() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
 template <int FORM, int TM, int EPI>
@@ -127,9 +161,9 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   if (ntile <= 0) return;  // uniform; (the host launches no such workgroup)
   const int KT = p.kt;
 
-  // Load block j of a wave: RPI rows of LPR lanes; lane i fills physical chunk
-  // i % LPR of row RPI j + i / LPR.  The swizzle depends on the row's low bits,
-  // hence on j's parity alone.
+  // Load block j of a wave: RP rows of LP lanes; lane i fills physical chunk i % LP of
+  // row RP j + i / LP.  The swizzle depends on the row's low bits, hence on j's
+  // parity alone.
   constexpr int LPW = WR ? 32 : 8, RPW = 64 / LPW;           // w
   constexpr int LPX = XR ? BM / 8 : 8, RPX = 64 / LPX;       // x
   auto logical = [](bool rows, int width, int row, int pc) {
@@ -137,15 +171,18 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     return pc ^ ((width == 64 ? (row >> 1) & 1 : row & 3) << 2);
   };
   int cw[2], cx[2];            // logical chunk
-  uint32_t lw[2], lx[2];       // byte offset from the block's first row
+  uint32_t lw[DB], lx[DX];     // byte offset of block j from the wave's first row
 #pragma unroll
   for (int par = 0; par < 2; ++par) {
-    const int rw = lane / LPW, rx = lane / LPX;
-    cw[par] = logical(WR, MAT_BN, RPW * par + rw, lane % LPW);
-    cx[par] = logical(XR, BM, RPX * par + rx, lane % LPX);
-    lw[par] = static_cast<uint32_t>(rw) * static_cast<uint32_t>(p.sw * 2) + 16u * cw[par];
-    lx[par] = static_cast<uint32_t>(rx) * static_cast<uint32_t>(p.sx * 2) + 16u * cx[par];
+    cw[par] = logical(WR, MAT_BN, RPW * par + lane / LPW, lane % LPW);
+    cx[par] = logical(XR, BM, RPX * par + lane / LPX, lane % LPX);
   }
+#pragma unroll
+  for (int j = 0; j < DB; ++j)
+    lw[j] = static_cast<uint32_t>(RPW * j + lane / LPW) * static_cast<uint32_t>(p.sw * 2) + 16u * cw[j & 1];
+#pragma unroll
+  for (int j = 0; j < DX; ++j)
+    lx[j] = static_cast<uint32_t>(RPX * j + lane / LPX) * static_cast<uint32_t>(p.sx * 2) + 16u * cx[j & 1];
   auto stage_w = [&](auto st) __attribute__((always_inline)) -> bf16_t * {
     constexpr int S = decltype(st)::value;
     return S == 0 ? w0 : S == 1 ? w1 : S == 2 ? w2s : w3;
@@ -158,7 +195,9 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   // The next slice to load: slice ds of this workgroup's tile dj, at (bm, bn, sp).
   int dj = 0, ds = 0, dbm, dbn, dsp;
   mat_tile(static_cast<int>(blockIdx.x), p.tiles_m, p.tiles_n, p.splits, dbm, dbn, dsp);
-  auto issue = [&](auto st) __attribute__((always_inline)) {
+  au32x4_t nw, nx;  // its descriptors
+  int wpast, xpast;
+  auto next = [&]() __attribute__((always_inline)) {
     if (ds == KT) {  // (past the last slice the loads repeat it: every step issues as many)
       if (dj + 1 < ntile) {
         ds = 0;
@@ -204,32 +243,28 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     }
     const uint32_t wbytes = wrows > 0 ? static_cast<uint32_t>(((wrows - 1) * p.sw + wleft) * 2) : 0u;
     const uint32_t xbytes = xrows > 0 ? static_cast<uint32_t>(((xrows - 1) * p.sx + xleft) * 2) : 0u;
-    const __amdgpu_buffer_rsrc_t wrs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t *>(wb), 0, wbytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t xrs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t *>(xb), 0, xbytes, 0x00020000);
-    uint32_t vw[2], vx[2];
-#pragma unroll
-    for (int par = 0; par < 2; ++par) {  // chunks past the end of K read zeros
-      vw[par] = WR || 8 * cw[par] < wleft ? lw[par] : MAT_OUT;
-      vx[par] = XR || 8 * cx[par] < xleft ? lx[par] : MAT_OUT;
+    nw = mat_rsrc(wb, wbytes);
+    nx = mat_rsrc(xb, xbytes);
+    // chunks past the end of K read zeros (of rows along N or M the descriptor ends
+    // with the last row)
+    wpast = WR ? 0 : wleft;
+    xpast = XR ? 0 : xleft;
+  };
+  // Load i of the slice that `next` found, into a stage.
+  auto load = [&](auto st, int i) __attribute__((always_inline)) {
+    if (i < DB) {
+      const uint32_t v = WR || 8 * cw[i & 1] < wpast ? lw[i] : MAT_OUT;
+      mat_load(nw, v, stage_w(st) + (wave * DB + i) * 512);
+    } else {
+      const int j = i - DB;
+      const uint32_t v = XR || 8 * cx[j & 1] < xpast ? lx[j] : MAT_OUT;
+      mat_load(nx, v, stage_x(st) + (wave * DX + j) * 512);
     }
-    bf16_t *lwp = stage_w(st) + wave * DB * 512, *lxp = stage_x(st) + wave * DX * 512;
+  };
+  auto issue = [&](auto st) __attribute__((always_inline)) {
+    next();
 #pragma unroll
-    for (int j = 0; j < DB; ++j) {
-      // a block past the last row reads zeros (its row offset has to stay inside
-      // the buffer)
-      const uint32_t ow = static_cast<uint32_t>(j * RPW * 2 * p.sw);
-      const bool wl = ow < wbytes;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (alds_void *)(lwp + 512 * j), 16, wl ? vw[j & 1] : MAT_OUT,
-                                               wl ? static_cast<int>(ow) : 0, 0, 0);
-      if (j < DX) {
-        const uint32_t ox = static_cast<uint32_t>(j * RPX * 2 * p.sx);
-        const bool xl = ox < xbytes;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(xrs, (alds_void *)(lxp + 512 * j), 16,
-                                                 xl ? vx[j & 1] : MAT_OUT, xl ? static_cast<int>(ox) : 0, 0, 0);
-      }
-    }
+    for (int i = 0; i < DB + DX; ++i) load(st, i);
   };
 
   const int wn = (wave & 1) * 128, wm = (wave >> 1) * (32 * TM);  // wave's columns and rows
@@ -270,15 +305,17 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
 
   mf32x16_t acc[4][TM];
   abf16x8_t fa[2][4][2], fb[2][TM][2];  // fragments of a half slice (two 16-wide K steps)
+  // fragment f of a half slice, in the order the MFMAs take them
+  auto read_frag = [&](auto st, auto half, int f) __attribute__((always_inline)) {
+    constexpr int H = decltype(half)::value;
+    const int kk = f / (TM + 4), t = f % (TM + 4);
+    if (t < TM) fb[H][t][kk] = read_x(st, t, 2 * H + kk);
+    else fa[H][t - TM][kk] = read_w(st, t - TM, 2 * H + kk);
+  };
   auto read_frags = [&](auto st, auto half) __attribute__((always_inline)) {
     constexpr int H = decltype(half)::value;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-#pragma unroll
-      for (int t = 0; t < TM; ++t) fb[H][t][kk] = read_x(st, t, 2 * H + kk);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) fa[H][t][kk] = read_w(st, t, 2 * H + kk);
-    }
+    for (int f = 0; f < 2 * (TM + 4); ++f) read_frag(st, half, f);
   };
   auto mma = [&](auto half) __attribute__((always_inline)) {
     constexpr int H = decltype(half)::value;
@@ -290,15 +327,12 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
         for (int tm = 0; tm < TM; ++tm)
           acc[tn][tm] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[H][tn][kk], fb[H][tm][kk], acc[tn][tm], 0, 0, 0);
   };
-  // every MFMA is followed by its share of the fragment reads and of the loads
-  auto interleave = [&](auto dma) __attribute__((always_inline)) {
+  // every MFMA is followed by its share of the fragment reads
+  auto interleave = [&]() __attribute__((always_inline)) {
     static_for<8 * TM>([&](auto i) __attribute__((always_inline)) {
-      constexpr int I = decltype(i)::value, NM = 8 * TM;
-      constexpr int ND = 8 * (WR ? 2 : 1) + 2 * TM * (XR ? 2 : 1), NV = DB + DX;
+      constexpr int I = decltype(i)::value, NM = 8 * TM, ND = 8 * (WR ? 2 : 1) + 2 * TM * (XR ? 2 : 1);
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
       __builtin_amdgcn_sched_group_barrier(0x100, (I + 1) * ND / NM - I * ND / NM, 0);  // DS read
-      if constexpr (decltype(dma)::value)
-        __builtin_amdgcn_sched_group_barrier(0x020, (I + 1) * NV / NM - I * NV / NM, 0);  // VMEM read
     });
   };
   using std::integral_constant;
@@ -310,15 +344,22 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   // MFMAs of the second half while the next slice's first is read.
   auto step = [&](auto st) __attribute__((always_inline)) {
     constexpr int S = decltype(st)::value;
+    using N = integral_constant<int, (S + 1) % NST>;
+    next();
     read_frags(st, I1{});
     mma(I0{});
-    interleave(integral_constant<bool, false>{});
-    vmcnt_wait<(NST - 2) * (DB + DX)>();
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    issue(st);
-    read_frags(integral_constant<int, (S + 1) % NST>{}, I0{});
+    interleave();
+    mat_sync<(NST - 2) * (DB + DX)>();
+    // the loads stand between the fragment reads, in this order
+    constexpr int NF = 2 * (TM + 4), NV = DB + DX;
+    static_for<NF>([&](auto f) __attribute__((always_inline)) {
+      constexpr int F = decltype(f)::value;
+#pragma unroll
+      for (int i = F * NV / NF; i < (F + 1) * NV / NF; ++i) load(st, i);
+      read_frag(N{}, I0{}, F);
+    });
     mma(I1{});
-    interleave(integral_constant<bool, true>{});
+    interleave();
   };
 
   // Lane (lr, g) holds, for row m = wm + 32 tm + lr of the tile, columns
@@ -329,6 +370,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     const bool second = FORM == MAT_TN && bm >= p.mpair;
     const int m0 = (second ? bm - p.mpair : bm) * BM + wm;      // wave's first row
     const int n0 = bn * (EPI == MAT_GATED ? MAT_BN / 2 : MAT_BN) + (EPI == MAT_GATED ? wn / 2 : wn);
+    const float factor = EPI == MAT_BF16 ? mat_factor(p.num, p.den) : 1.0f;
     // Lanes l and l + 32 hold the same row: they swap halves of each pair of
     // column groups so that each stores 16 contiguous bytes.
     auto store_pair = [&](bf16_t *row, int c, int limit, const float (&v)[8]) __attribute__((always_inline)) {
@@ -351,7 +393,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
           for (int pq = 0; pq < 2; ++pq) {
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = acc[tn][tm][8 * pq + i];
+            for (int i = 0; i < 8; ++i) v[i] = acc[tn][tm][8 * pq + i] * factor;
             store_pair(row, 32 * tn + 16 * pq, limit, v);
           }
       } else if constexpr (EPI == MAT_F32) {
@@ -444,7 +486,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
         bf16_t *row = static_cast<bf16_t *>(p.out) + m * p.so + n0;
         const int limit = live ? ((p.N + 7) & ~7) - n0 : 0, valid = p.N - n0;
         const int64_t t = live ? p.targets[m] : p.ignore;
-        const float wgt = live ? loss_weight(p.grad, p.sgrad, p.count, m, t, p.ignore, p.V) : 0.0f;
+        const float wgt = live ? loss_weight(p, m, t) : 0.0f;
         const float lse2 = live ? p.lse[m] * 1.44269504088896341f : 0.0f;
         const int64_t tl = t - p.col0 - n0;
         const int tc = tl >= 0 && tl < 128 ? static_cast<int>(tl) : -1;
@@ -473,8 +515,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     issue(integral_constant<int, 2>{});
     issue(integral_constant<int, 3>{});
   }
-  vmcnt_wait<(NST - 1) * (DB + DX)>();  // slice 0
-  asm volatile("s_barrier" ::: "memory");
+  mat_sync<(NST - 1) * (DB + DX)>();  // slice 0
   read_frags(I0{}, I0{});
   for (int j = 0; j < ntile; ++j) {
 #pragma unroll
@@ -539,10 +580,10 @@ inline void mat_launch(MatArgs a, const MatPlan &pl, hipStream_t st) {
 void mat_nn(const MatArgs &a, const MatPlan &pl, bool f32, hipStream_t st);
 void mat_tn(const MatArgs &a, const MatPlan &pl, bool f32, hipStream_t st);
 void mat_nt_f32(const MatArgs &a, const MatPlan &pl, hipStream_t st);
-// out (rows, cols) bf16 = the sum of `splits` fp32 planes (rows of cols, contiguous);
-// cols a multiple of 8.
+// out (rows, cols) bf16 = the sum of `splits` fp32 planes (rows of cols, contiguous)
+// times *num / *den (each may be null); cols a multiple of 8.
 void mat_join(const float *part, int64_t plane, int splits, bf16_t *out, int64_t so, int64_t rows,
-              int64_t cols, hipStream_t st);
+              int64_t cols, hipStream_t st, const float *num = nullptr, const float *den = nullptr);
 
 // Sizes and strides the kernel's 32-bit offsets take.
 inline bool mat_fits(int64_t M, int64_t N, int64_t K, int64_t s) {

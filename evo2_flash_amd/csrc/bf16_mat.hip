@@ -15,7 +15,8 @@ void mat_nt_f32(const MatArgs &a, const MatPlan &pl, hipStream_t st) {
 
 // A thread sums eight columns of a row over the planes, in the planes' order.
 __global__ __launch_bounds__(256) void mat_join_kernel(const float *part, int64_t plane, int splits,
-                                                       bf16_t *out, int64_t so, int64_t chunks, int cols8) {
+                                                       bf16_t *out, int64_t so, int64_t chunks, int cols8,
+                                                       const float *num, const float *den) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (at >= chunks) return;
   const int64_t r = at / cols8;
@@ -26,15 +27,18 @@ __global__ __launch_bounds__(256) void mat_join_kernel(const float *part, int64_
     a += *reinterpret_cast<const af32x4_t *>(src);
     b += *reinterpret_cast<const af32x4_t *>(src + 4);
   }
+  const float f = mat_factor(num, den);
+  a *= f;
+  b *= f;
   *reinterpret_cast<au32x4_t *>(out + r * so + c) =
       au32x4_t{pack_bf(a[0], a[1]), pack_bf(a[2], a[3]), pack_bf(b[0], b[1]), pack_bf(b[2], b[3])};
 }
 
 void mat_join(const float *part, int64_t plane, int splits, bf16_t *out, int64_t so, int64_t rows,
-              int64_t cols, hipStream_t st) {
+              int64_t cols, hipStream_t st, const float *num, const float *den) {
   const int64_t chunks = rows * (cols / 8);
   hipLaunchKernelGGL(mat_join_kernel, dim3(static_cast<unsigned>(cdiv(chunks, 256))), dim3(256), 0, st, part,
-                     plane, splits, out, so, chunks, static_cast<int>(cols / 8));
+                     plane, splits, out, so, chunks, static_cast<int>(cols / 8), num, den);
 }
 
 }  // namespace evo2

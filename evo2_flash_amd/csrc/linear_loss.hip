@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void loss_rows_grad_kernel(MatArgs p, const fl
   const int m = blockIdx.x;
   const int64_t plane = static_cast<int64_t>(p.M) * p.V, row = static_cast<int64_t>(m) * p.V;
   const int64_t t = p.targets[m];
-  const float wgt = loss_weight(p.grad, p.sgrad, p.count, m, t, p.ignore, p.V);
+  const float wgt = loss_weight(p, m, t);
   const float lse2 = p.lse[m] * L_LOG2E;
   bf16_t *out = static_cast<bf16_t *>(p.out) + static_cast<int64_t>(m) * p.so;
   for (int n = threadIdx.x; n < Vp; n += 256) {
@@ -277,7 +277,7 @@ extern "C" int evo2_linear_loss_backward(const void *h, int64_t sh, const void *
                                          int64_t V, int64_t H, void *stream) {
   int rc = check_sizes("linear_loss_backward", T, V, H, sh, sw);
   if (rc) return rc;
-  if (!h || !w || !targets || !lse || !grad || !workspace)
+  if (!h || !w || !targets || !lse || !grad || !workspace || (count && sgrad))
     return fail(EVO2_ERR_INVALID, "linear_loss_backward: null pointer argument");
   if (!aligned(h) || !aligned(w) || !aligned(dh) || !aligned(dw) || !aligned(workspace))
     return fail(EVO2_ERR_UNSUPPORTED, "linear_loss_backward: operands must be 16-byte aligned rows");
@@ -291,6 +291,8 @@ extern "C" int evo2_linear_loss_backward(const void *h, int64_t sh, const void *
   bf16_t *d = reinterpret_cast<bf16_t *>(at);
   float *acc = reinterpret_cast<float *>(at + up(T * b.ld * 2, 256));
   float *part = reinterpret_cast<float *>(reinterpret_cast<char *>(acc) + b.acc);
+  const bool shared = sgrad == 0;  // one upstream gradient for all rows
+  const float *num = shared ? grad : nullptr, *den = shared ? count : nullptr;
   for (int64_t v0 = 0; v0 < V; v0 += b.vp) {
     const int64_t vn = std::min(b.vp, V - v0);
     const bf16_t *wp = static_cast<const bf16_t *>(w) + v0 * sw;
@@ -311,7 +313,7 @@ extern "C" int evo2_linear_loss_backward(const void *h, int64_t sh, const void *
     a.lse = lse;
     a.grad = grad;
     a.sgrad = sgrad;
-    a.count = count;
+    a.weighted = !shared;
     if (b.z.splits > 1) {  // (one piece)
       a.out = part;
       a.so = V;
@@ -339,15 +341,17 @@ extern "C" int evo2_linear_loss_backward(const void *h, int64_t sh, const void *
       c.Kx = static_cast<int>(up(vn, 8));
       c.so = H;
       c.plane = T * H;
+      c.num = num;
+      c.den = den;
       if (b.pieces > 1) {
         c.out = acc;
         c.add = v0 > 0;
         mat_nn(c, mat_plan(T, H, cdiv(vn, MAT_BK), 1, MAT_BN, false), true, st);
-        if (v0 + vn == V) mat_join(acc, 0, 1, static_cast<bf16_t *>(dh), H, T, H, st);
+        if (v0 + vn == V) mat_join(acc, 0, 1, static_cast<bf16_t *>(dh), H, T, H, st, num, den);
       } else {
         c.out = b.dh.splits > 1 ? static_cast<void *>(part) : dh;
         mat_nn(c, b.dh, b.dh.splits > 1, st);
-        if (b.dh.splits > 1) mat_join(part, T * H, b.dh.splits, static_cast<bf16_t *>(dh), H, T, H, st);
+        if (b.dh.splits > 1) mat_join(part, T * H, b.dh.splits, static_cast<bf16_t *>(dh), H, T, H, st, num, den);
       }
     }
     if (dw) {
@@ -366,9 +370,11 @@ extern "C" int evo2_linear_loss_backward(const void *h, int64_t sh, const void *
       if (pl.splits > 1 && pl.splits * vn * H * 4 > b.part) pl = mat_plan(vn, H, cdiv(T, MAT_BK), 1, MAT_BN, false);
       bf16_t *to = static_cast<bf16_t *>(dw) + v0 * H;
       c.plane = vn * H;
+      c.num = num;
+      c.den = den;
       c.out = pl.splits > 1 ? static_cast<void *>(part) : to;
       mat_tn(c, pl, pl.splits > 1, st);
-      if (pl.splits > 1) mat_join(part, vn * H, pl.splits, to, H, vn, H, st);
+      if (pl.splits > 1) mat_join(part, vn * H, pl.splits, to, H, vn, H, st, num, den);
     }
   }
   return check_launch("linear_loss_backward");
