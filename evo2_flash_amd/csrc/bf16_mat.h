@@ -53,7 +53,7 @@ constexpr int MAT_BN = 256;      // output columns per workgroup
 constexpr int MAT_BK = 64;       // K per slice
 constexpr uint32_t MAT_OUT = 0x80000000u;  // an offset past every descriptor here
 
-constexpr int mat_stages(int tm) { return tm == 1 ? 4 : 2; }
+constexpr int mat_stages(int tm) { return tm == 1 ? 3 : 2; }
 
 struct MatArgs {
   const bf16_t *x; int64_t sx;            // row strides in elements
@@ -149,8 +149,9 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   constexpr int BM = 64 * TM, NST = mat_stages(TM);
   constexpr bool WR = FORM != MAT_NT, XR = FORM == MAT_TN;  // rows along N / M
   constexpr int WST = MAT_BN * MAT_BK, XST = BM * MAT_BK;   // elements per stage
-  __shared__ __align__(16) bf16_t w0[WST], w1[WST], w2s[NST > 2 ? WST : 8], w3[NST > 2 ? WST : 8];
-  __shared__ __align__(16) bf16_t x0[XST], x1[XST], x2s[NST > 2 ? XST : 8], x3[NST > 2 ? XST : 8];
+  __shared__ __align__(16) bf16_t w0[WST], w1[WST], w2s[NST > 2 ? WST : 8];
+  __shared__ __align__(16) bf16_t x0[XST], x1[XST], x2s[NST > 2 ? XST : 8];
+  __shared__ __align__(16) float turned[4][32 * 36];        // a wave's 32 x 32 results, by rows
   constexpr int DB = 8, DX = 2 * TM;  // 1 KB loads of w and x per wave and slice
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -185,11 +186,11 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     lx[j] = static_cast<uint32_t>(RPX * j + lane / LPX) * static_cast<uint32_t>(p.sx * 2) + 16u * cx[j & 1];
   auto stage_w = [&](auto st) __attribute__((always_inline)) -> bf16_t * {
     constexpr int S = decltype(st)::value;
-    return S == 0 ? w0 : S == 1 ? w1 : S == 2 ? w2s : w3;
+    return S == 0 ? w0 : S == 1 ? w1 : w2s;
   };
   auto stage_x = [&](auto st) __attribute__((always_inline)) -> bf16_t * {
     constexpr int S = decltype(st)::value;
-    return S == 0 ? x0 : S == 1 ? x1 : S == 2 ? x2s : x3;
+    return S == 0 ? x0 : S == 1 ? x1 : x2s;
   };
 
   // The next slice to load: slice ds of this workgroup's tile dj, at (bm, bn, sp).
@@ -207,7 +208,12 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
         ds = KT - 1;
       }
     }
-    const int s = dsp * KT + ds;
+    // K-contiguous rows at a power-of-two stride put all of a slice's lines on a few
+    // cache channels: workgroups of different rows start up to seven slices apart
+    // (4096 x 32768 x 4096: 1000 -> 925 us; further apart they lose the L2's sharing)
+    int s = ds + (FORM == MAT_NT && KT >= 16 ? dbm & 7 : 0);
+    if (s >= KT) s -= KT;
+    s += dsp * KT;
     ++ds;
     // w: this wave's rows of the slice, their first element, how many there are
     const bf16_t *wb;
@@ -363,7 +369,10 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   };
 
   // Lane (lr, g) holds, for row m = wm + 32 tm + lr of the tile, columns
-  // wn + 32 tn + 8 q + 4 g + i in acc[tn][tm][4 q + i].
+  // wn + 32 tn + 8 q + 4 g + i in acc[tn][tm][4 q + i].  Results go to memory by way of
+  // a wave's own 32 rows of 144 bytes in LDS, which turn them so that eight lanes
+  // store one whole 128-byte line of a row: stored as they lie, each line takes four
+  // requests, and the caches' request rate bounds the burst at a tile's end.
   auto epilogue = [&](int j) __attribute__((always_inline)) {
     int bm, bn, sp;
     mat_tile(static_cast<int>(blockIdx.x) + j * grid, p.tiles_m, p.tiles_n, p.splits, bm, bn, sp);
@@ -371,150 +380,141 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     const int m0 = (second ? bm - p.mpair : bm) * BM + wm;      // wave's first row
     const int n0 = bn * (EPI == MAT_GATED ? MAT_BN / 2 : MAT_BN) + (EPI == MAT_GATED ? wn / 2 : wn);
     const float factor = EPI == MAT_BF16 ? mat_factor(p.num, p.den) : 1.0f;
-    // Lanes l and l + 32 hold the same row: they swap halves of each pair of
-    // column groups so that each stores 16 contiguous bytes.
-    auto store_pair = [&](bf16_t *row, int c, int limit, const float (&v)[8]) __attribute__((always_inline)) {
-      // v: columns 16 pq + 4 g + i (i < 4) and 16 pq + 8 + 4 g + i
-      const auto s0 = __builtin_amdgcn_permlane32_swap(pack_bf(v[0], v[1]), pack_bf(v[4], v[5]), false, false);
-      const auto s1 = __builtin_amdgcn_permlane32_swap(pack_bf(v[2], v[3]), pack_bf(v[6], v[7]), false, false);
-      if (c + 8 * g < limit)
-        *reinterpret_cast<au32x4_t *>(row + c + 8 * g) = au32x4_t{s0[0], s1[0], s0[1], s1[1]};
+    float *tb = turned[wave];
+    const int tr = lane >> 3, tc = lane & 7;  // turned: lane's row of eight, 16-byte chunk
+    // (LDS serves a wave in order; the compiler is kept to it)
+    auto fence = [] { asm volatile("" ::: "memory"); };
+    // rows m .. m + 31, 64 columns from n0 + c: v(t, i) of tile t (0, 1), element i
+    auto put_bf16 = [&](bf16_t *out, int m, int c, int cols, auto &&v) __attribute__((always_inline)) {
+      bf16_t *b = reinterpret_cast<bf16_t *>(tb);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint2 *>(b + lr * 72 + 32 * t + 8 * q + 4 * g) =
+              make_uint2(pack_bf(v(t, 4 * q), v(t, 4 * q + 1)), pack_bf(v(t, 4 * q + 2), v(t, 4 * q + 3)));
+      fence();
+      bf16_t *o = out + m * p.so + n0 + c;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 8 * k + tr;
+        const au32x4_t w = *reinterpret_cast<const au32x4_t *>(b + r * 72 + 8 * tc);
+        if (m + r < p.M && n0 + c + 8 * tc < cols) *reinterpret_cast<au32x4_t *>(o + r * p.so + 8 * tc) = w;
+      }
+      fence();
+    };
+    // rows m .. m + 31, 32 columns from n0 + c of fp32 rows of `so` elements
+    auto put_f32 = [&](float *out, int64_t so, int m, int c, bool add, auto &&v) __attribute__((always_inline)) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<af32x4_t *>(tb + lr * 36 + 8 * q + 4 * g) =
+            af32x4_t{v(4 * q), v(4 * q + 1), v(4 * q + 2), v(4 * q + 3)};
+      fence();
+      float *o = out + m * so + n0 + c;
+      if (so % 4 == 0 && p.N % 4 == 0) {  // uniform
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 8 * k + tr;
+          af32x4_t w = *reinterpret_cast<const af32x4_t *>(tb + r * 36 + 4 * tc);
+          if (m + r < p.M && n0 + c + 4 * tc < p.N) {
+            af32x4_t *d = reinterpret_cast<af32x4_t *>(o + r * so + 4 * tc);
+            if (add) w += *d;
+            *d = w;
+          }
+        }
+      } else {  // (an odd vocabulary's partial logits)
+#pragma unroll 1
+        for (int k = 0; k < 16; ++k) {
+          const int r = 2 * k + (lane >> 5), cc = lane & 31;
+          const float w = tb[r * 36 + cc];
+          if (m + r < p.M && n0 + c + cc < p.N) o[r * so + cc] = w;
+        }
+      }
+      fence();
     };
 #pragma unroll
     for (int tm = 0; tm < TM; ++tm) {
-      const int m = m0 + 32 * tm + lr;
+      const int mr = m0 + 32 * tm, m = mr + lr;
       const bool live = m < p.M;
       if constexpr (EPI == MAT_BF16) {
-        bf16_t *row = static_cast<bf16_t *>(second ? p.out2 : p.out) + m * p.so + n0;
-        const int limit = live ? p.N - n0 : 0;
+        bf16_t *out = static_cast<bf16_t *>(second ? p.out2 : p.out);
 #pragma unroll
-        for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-          for (int pq = 0; pq < 2; ++pq) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = acc[tn][tm][8 * pq + i] * factor;
-            store_pair(row, 32 * tn + 16 * pq, limit, v);
-          }
+        for (int h = 0; h < 2; ++h)
+          put_bf16(out, mr, 64 * h, p.N, [&](int t, int i) { return acc[2 * h + t][tm][i] * factor; });
       } else if constexpr (EPI == MAT_F32) {
-        float *row = static_cast<float *>(second ? p.out2 : p.out) + sp * p.plane + m * p.so + n0;
-        const int limit = live ? p.N - n0 : 0;
-        const bool vec = p.so % 4 == 0;  // uniform
+        float *out = static_cast<float *>(second ? p.out2 : p.out) + sp * p.plane;
 #pragma unroll
         for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int c = 32 * tn + 8 * q + 4 * g;
-            af32x4_t v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = acc[tn][tm][4 * q + i];
-            if (vec && c + 4 <= limit) {
-              af32x4_t *d = reinterpret_cast<af32x4_t *>(row + c);
-              if (p.add) v += *d;
-              *d = v;
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (c + i < limit) row[c + i] = p.add ? row[c + i] + v[i] : v[i];
-            }
-          }
+          put_f32(out, p.so, mr, 32 * tn, p.add != 0, [&](int i) { return acc[tn][tm][i]; });
       } else if constexpr (EPI == MAT_GATED) {
-        bf16_t *row = static_cast<bf16_t *>(p.out) + m * p.so + n0;
-        const int limit = live ? p.N - n0 : 0;
+        put_bf16(static_cast<bf16_t *>(p.out), mr, 0, p.N, [&](int t, int i) {
+          const float a = acc[t][tm][i];
+          return (p.gelu ? gelu_f(a) : a) * acc[t + 2][tm][i];
+        });
+        if (p.z1) {
 #pragma unroll
-        for (int tn = 0; tn < 2; ++tn)
-#pragma unroll
-          for (int pq = 0; pq < 2; ++pq) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float a = acc[tn][tm][8 * pq + i];
-              v[i] = (p.gelu ? gelu_f(a) : a) * acc[tn + 2][tm][8 * pq + i];
-            }
-            store_pair(row, 32 * tn + 16 * pq, limit, v);
-            if (p.z1) {
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                const int c = 32 * tn + 16 * pq + 8 * hh + 4 * g;
-                if (c < limit) {
-                  const int64_t at = static_cast<int64_t>(m) * p.N + n0 + c;
-                  af32x4_t a, b;
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    a[i] = acc[tn][tm][8 * pq + 4 * hh + i];
-                    b[i] = acc[tn + 2][tm][8 * pq + 4 * hh + i];
-                  }
-                  *reinterpret_cast<af32x4_t *>(p.z1 + at) = a;
-                  *reinterpret_cast<af32x4_t *>(p.z2 + at) = b;
-                }
-              }
-            }
+          for (int t = 0; t < 2; ++t) {
+            put_f32(p.z1, p.N, mr, 32 * t, false, [&](int i) { return acc[t][tm][i]; });
+            put_f32(p.z2, p.N, mr, 32 * t, false, [&](int i) { return acc[t + 2][tm][i]; });
           }
+        }
       } else if constexpr (EPI == MAT_STATS) {
         // max and sum of exp over the wave's 128 columns of the row, and the
         // target's logit where it lies among them
         const int limit = p.N - n0;  // columns of the vocabulary from the wave's first
+        const int lim = limit - 4 * g;
+        auto logit = [&](int tn, int i) {
+          return 32 * tn + 8 * (i >> 2) + (i & 3) < lim ? acc[tn][tm][i] : -INFINITY;
+        };
         float mx = -INFINITY;
 #pragma unroll
         for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (32 * tn + 8 * (i >> 2) + 4 * g + (i & 3) >= limit) acc[tn][tm][i] = -INFINITY;
-            mx = fmaxf(mx, acc[tn][tm][i]);
-          }
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, logit(tn, i));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float sub = mx == -INFINITY ? 0.0f : mx * 1.44269504088896341f;
         const int64_t t = live ? p.targets[m] - n0 : -1;
-        const int tc = t >= 0 && t < min(128, limit) ? static_cast<int>(t) : -1;
+        // the target's place among the lane's own columns (the lane with none: past all)
+        const int at = t >= 0 && t < min(128, limit) && ((t >> 2) & 1) == g ? static_cast<int>(t) - 4 * g : -1;
         float sum = 0.0f, zt = 0.0f;
 #pragma unroll
         for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float v = acc[tn][tm][i];
+            const float v = logit(tn, i);
             sum += __builtin_amdgcn_exp2f(fmaf(v, 1.44269504088896341f, -sub));
-            if (32 * tn + 8 * (i >> 2) + 4 * g + (i & 3) == tc) zt = v;
+            zt = at == 32 * tn + 8 * (i >> 2) + (i & 3) ? v : zt;
           }
         sum += __shfl_xor(sum, 32);
         if (live) {
           if (g == 0) p.part[static_cast<int64_t>(2 * bn + (wave & 1)) * p.M + m] = make_float2(mx, sum);
-          if (tc >= 0 && ((tc >> 2) & 1) == g) p.tgt[m] = zt;
+          if (at >= 0) p.tgt[m] = zt;
         }
       } else {
         // d = (exp(z - lse) - [n = target]) * weight, zeros in the columns that
         // pad the vocabulary to eights
-        bf16_t *row = static_cast<bf16_t *>(p.out) + m * p.so + n0;
-        const int limit = live ? ((p.N + 7) & ~7) - n0 : 0, valid = p.N - n0;
+        const int valid = p.N - n0 - 4 * g;
         const int64_t t = live ? p.targets[m] : p.ignore;
         const float wgt = live ? loss_weight(p, m, t) : 0.0f;
         const float lse2 = live ? p.lse[m] * 1.44269504088896341f : 0.0f;
-        const int64_t tl = t - p.col0 - n0;
-        const int tc = tl >= 0 && tl < 128 ? static_cast<int>(tl) : -1;
+        const int64_t tl = t - p.col0 - n0 - 4 * g;
+        const int at = tl >= 0 && tl < 128 ? static_cast<int>(tl) : -1;
         const bool used = live && t != p.ignore;
 #pragma unroll
-        for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-          for (int pq = 0; pq < 2; ++pq) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int c = 32 * tn + 16 * pq + 8 * (i >> 2) + 4 * g + (i & 3);
-              float e = __builtin_amdgcn_exp2f(fmaf(acc[tn][tm][8 * pq + i], 1.44269504088896341f, -lse2));
-              if (c == tc) e -= 1.0f;
-              v[i] = used && c < valid ? e * wgt : 0.0f;
-            }
-            store_pair(row, 32 * tn + 16 * pq, limit, v);
-          }
+        for (int h = 0; h < 2; ++h)
+          put_bf16(static_cast<bf16_t *>(p.out), mr, 64 * h, (p.N + 7) & ~7, [&](int u, int i) {
+            const int c = 64 * h + 32 * u + 8 * (i >> 2) + (i & 3);
+            float e = __builtin_amdgcn_exp2f(fmaf(acc[2 * h + u][tm][i], 1.44269504088896341f, -lse2));
+            e = at == c ? e - 1.0f : e;
+            return used && c < valid ? e * wgt : 0.0f;
+          });
       }
     }
   };
 
   issue(I0{});
   issue(I1{});
-  if constexpr (NST > 2) {
-    issue(integral_constant<int, 2>{});
-    issue(integral_constant<int, 3>{});
-  }
+  if constexpr (NST > 2) issue(integral_constant<int, 2>{});
   mat_sync<(NST - 1) * (DB + DX)>();  // slice 0
   read_frags(I0{}, I0{});
   for (int j = 0; j < ntile; ++j) {
