@@ -166,11 +166,12 @@ SIGNATURES = {
         _c_p, _c_i64, _c_p, _c_p, _c_p,           # cu, nseq, out, out_lo, lse
         _c_i64, _c_i64, _c_i64, _c_i64, _c_f, _c_p,  # T, heads, kv, head_dim, scale, stream
     ],
+    "evo2_packed_attention_workspace_bytes": [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64],
     "evo2_packed_attention_backward": [
         _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,  # dout, q + strides (row, head)
         _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,  # k, v + strides
-        _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p,     # cu, nseq, out, out_lo, lse, delta
-        _c_p, _c_p, _c_p,                         # dq, dk, dv
+        _c_p, _c_i64, _c_p, _c_p, _c_p,           # cu, nseq, out, out_lo, lse
+        _c_p, _c_i64, _c_p, _c_p, _c_p,           # workspace, bytes, dq, dk, dv
         _c_i64, _c_i64, _c_i64, _c_i64, _c_f, _c_p,  # T, heads, kv, head_dim, scale, stream
     ],
     "evo2_bf16_stream_linear": [
@@ -336,6 +337,7 @@ SIGNATURES = {
 RESTYPES = {"evo2_last_error": ctypes.c_char_p, "evo2_hcl_workspace_bytes": ctypes.c_int64,
             "evo2_decode_attention_workspace_bytes": ctypes.c_int64,
             "evo2_fp8_gemm_persist_order": ctypes.c_int64,
+            "evo2_packed_attention_workspace_bytes": ctypes.c_int64,
             "evo2_gated_linear_workspace_bytes": ctypes.c_int64,
             "evo2_linear_loss_workspace_bytes": ctypes.c_int64}
 

@@ -401,12 +401,14 @@ class _PackedAttention(torch.autograd.Function):
         if T:
             d, q, k, v = (_head_rows(t) for t in (dout, q, k, v))
             with _lib.on_device(q):
-                delta = torch.empty_like(lse)
+                nseq = cu.shape[0] - 1
+                n = _lib.lib().evo2_packed_attention_workspace_bytes(T, nseq, heads, k.shape[1], hd)
+                ws = torch.empty(n, dtype=torch.uint8, device=q.device)
                 _lib.call("evo2_packed_attention_backward", _lib.ptr(d), d.stride(0), d.stride(1),
                           _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k), k.stride(0),
                           k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1), _lib.ptr(cu),
-                          cu.shape[0] - 1, _lib.ptr(out), _lib.ptr(lo), _lib.ptr(lse),
-                          _lib.ptr(delta), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), T, heads,
+                          nseq, _lib.ptr(out), _lib.ptr(lo), _lib.ptr(lse), _lib.ptr(ws), n,
+                          _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), T, heads,
                           k.shape[1], hd, ctx.scale, _lib.stream_of(q))
         need = ctx.needs_input_grad
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None,

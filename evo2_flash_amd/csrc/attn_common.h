@@ -1,6 +1,6 @@
-// Pieces shared by the matrix-core attention kernels: operand vector types,
-// a compile-time loop, and LDS reads that the compiler does not order after
-// direct-to-LDS loads.
+// Pieces shared by the matrix-core attention and product kernels: operand vector
+// types, a compile-time loop, LDS reads that the compiler does not order after
+// direct-to-LDS loads, and such loads that it does not know of.
 #pragma once
 
 #include <type_traits>
@@ -67,6 +67,41 @@ __device__ __forceinline__ void lds_read4(au32x4_t (&r)[4], uint32_t a) {
 // LDS byte address of a pointer into a __shared__ array.
 __device__ __forceinline__ uint32_t lds_addr(const void *p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p));
+}
+
+// A raw buffer descriptor over `bytes` bytes from p.
+__device__ __forceinline__ au32x4_t lds_rsrc(const void *p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  // (uniform values; stated, for an operand that has to be in SGPRs)
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
+  return au32x4_t{lo, hi & 0xffffu, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(bytes)), 0x00020000u};
+}
+
+// One direct-to-LDS load: 64 lanes x 16 bytes at byte offset v (zeros past the
+// descriptor) to lds .. lds + 1 KB.  In asm so that the compiler does not know of it:
+// before each transposing LDS read it would wait for all such loads in flight.  The
+// kernel waits for them itself (lds_sync), and no register is written.
+__device__ __forceinline__ void lds_load(au32x4_t rsrc, uint32_t v, const bf16_t *lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds_addr(lds)), "v"(v), "s"(rsrc)
+               : "m0");
+}
+
+// The same, 64 lanes x 4 bytes.
+__device__ __forceinline__ void lds_load4(au32x4_t rsrc, uint32_t v, const void *lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds_addr(lds)), "v"(v), "s"(rsrc)
+               : "m0");
+}
+
+// All but N of the wave's loads and stores and all its LDS reads are done; then the
+// workgroup meets, and LDS holds what every wave's loads brought.
+template <int N>
+__device__ __forceinline__ void lds_sync() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
 }  // namespace evo2

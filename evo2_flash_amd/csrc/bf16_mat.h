@@ -117,33 +117,6 @@ __device__ __forceinline__ float mat_factor(const float *num, const float *den) 
   return den ? n / *den : n;
 }
 
-// A raw buffer descriptor over `bytes` bytes from p.
-__device__ __forceinline__ au32x4_t mat_rsrc(const void *p, uint32_t bytes) {
-  const uint64_t a = reinterpret_cast<uint64_t>(p);
-  // (uniform values; stated, for an operand that has to be in SGPRs)
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
-  return au32x4_t{lo, hi & 0xffffu, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(bytes)), 0x00020000u};
-}
-
-// One direct-to-LDS load: 64 lanes x 16 bytes at byte offset v (zeros past the
-// descriptor) to lds .. lds + 1 KB.  In asm so that the compiler does not know of it:
-// before each transposing LDS read it would wait for all such loads in flight.  The
-// kernel waits for them itself (mat_sync), and no register is written.
-__device__ __forceinline__ void mat_load(au32x4_t rsrc, uint32_t v, const bf16_t *lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(lds_addr(lds)), "v"(v), "s"(rsrc)
-               : "m0");
-}
-
-// All but N of the wave's loads and stores and all its LDS reads are done; then the
-// workgroup meets, and LDS holds what every wave's loads brought.
-template <int N>
-__device__ __forceinline__ void mat_sync() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
-}
-
 template <int FORM, int TM, int EPI>
 __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   constexpr int BM = 64 * TM, NST = mat_stages(TM);
@@ -249,8 +222,8 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     }
     const uint32_t wbytes = wrows > 0 ? static_cast<uint32_t>(((wrows - 1) * p.sw + wleft) * 2) : 0u;
     const uint32_t xbytes = xrows > 0 ? static_cast<uint32_t>(((xrows - 1) * p.sx + xleft) * 2) : 0u;
-    nw = mat_rsrc(wb, wbytes);
-    nx = mat_rsrc(xb, xbytes);
+    nw = lds_rsrc(wb, wbytes);
+    nx = lds_rsrc(xb, xbytes);
     // chunks past the end of K read zeros (of rows along N or M the descriptor ends
     // with the last row)
     wpast = WR ? 0 : wleft;
@@ -260,11 +233,11 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   auto load = [&](auto st, int i) __attribute__((always_inline)) {
     if (i < DB) {
       const uint32_t v = WR || 8 * cw[i & 1] < wpast ? lw[i] : MAT_OUT;
-      mat_load(nw, v, stage_w(st) + (wave * DB + i) * 512);
+      lds_load(nw, v, stage_w(st) + (wave * DB + i) * 512);
     } else {
       const int j = i - DB;
       const uint32_t v = XR || 8 * cx[j & 1] < xpast ? lx[j] : MAT_OUT;
-      mat_load(nx, v, stage_x(st) + (wave * DX + j) * 512);
+      lds_load(nx, v, stage_x(st) + (wave * DX + j) * 512);
     }
   };
   auto issue = [&](auto st) __attribute__((always_inline)) {
@@ -355,7 +328,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     read_frags(st, I1{});
     mma(I0{});
     interleave();
-    mat_sync<(NST - 2) * (DB + DX)>();
+    lds_sync<(NST - 2) * (DB + DX)>();
     // the loads stand between the fragment reads, in this order
     constexpr int NF = 2 * (TM + 4), NV = DB + DX;
     static_for<NF>([&](auto f) __attribute__((always_inline)) {
@@ -437,10 +410,24 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
       const int mr = m0 + 32 * tm, m = mr + lr;
       const bool live = m < p.M;
       if constexpr (EPI == MAT_BF16) {
-        bf16_t *out = static_cast<bf16_t *>(second ? p.out2 : p.out);
+        // (one output of half the size: as it lies, lanes l and l + 32, which hold the
+        // same row, swapping halves of each pair of column groups for 16-byte stores;
+        // by way of LDS 32768 x 4096 x 512 took 203 us, so 175)
+        bf16_t *row = static_cast<bf16_t *>(second ? p.out2 : p.out) + m * p.so + n0;
+        const int limit = live ? p.N - n0 : 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          put_bf16(out, mr, 64 * h, p.N, [&](int t, int i) { return acc[2 * h + t][tm][i] * factor; });
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int pq = 0; pq < 2; ++pq) {
+            uint32_t v[4];  // columns 16 pq + 4 g + i and 16 pq + 8 + 4 g + i
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[i] = pack_bf(acc[tn][tm][8 * pq + 2 * i] * factor, acc[tn][tm][8 * pq + 2 * i + 1] * factor);
+            const auto s0 = __builtin_amdgcn_permlane32_swap(v[0], v[2], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(v[1], v[3], false, false);
+            const int c = 32 * tn + 16 * pq + 8 * g;
+            if (c < limit) *reinterpret_cast<au32x4_t *>(row + c) = au32x4_t{s0[0], s1[0], s0[1], s1[1]};
+          }
       } else if constexpr (EPI == MAT_F32) {
         float *out = static_cast<float *>(second ? p.out2 : p.out) + sp * p.plane;
 #pragma unroll
@@ -515,7 +502,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   issue(I0{});
   issue(I1{});
   if constexpr (NST > 2) issue(integral_constant<int, 2>{});
-  mat_sync<(NST - 1) * (DB + DX)>();  // slice 0
+  lds_sync<(NST - 1) * (DB + DX)>();  // slice 0
   read_frags(I0{}, I0{});
   for (int j = 0; j < ntile; ++j) {
 #pragma unroll

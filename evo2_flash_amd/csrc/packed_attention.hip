@@ -7,7 +7,7 @@
 //   dv = p^T do, dp = do v^T, ds = p (dp - delta), delta_i = sum_j p_ij dp_ij = do_i . o_i
 //   dq = scale ds k, dk = scale ds^T q
 //
-// Three kernels of one shape, four waves of 32 rows each over tiles of 64 rows that
+// Three kernels of one shape, waves of 32 rows each (four, eight for dk and dv) over tiles of 64 rows that
 // come through LDS by direct-to-LDS loads, double-buffered, one barrier a tile:
 //   forward  32 queries a wave, sweeping keys and values:  s^T = k q^T, o^T += v^T p^T
 //   dq       32 queries a wave, sweeping keys and values:  s^T, dp^T = v do^T,
@@ -22,9 +22,10 @@
 // one wave in a fixed order: no atomics, so results repeat bit for bit; the price is
 // that the backward pass computes s and dp twice (seven products for five).
 //
-// LDS rows are 2 HD bytes; 16-byte chunk c of row r sits at c ^ swizzle(r), chosen so
-// that both the 16 rows of a 16-byte read and the four rows of a transposing read
-// fall on distinct banks.
+// LDS holds a tile as the load instructions' blocks of 1 KB (four rows of 128, eight of
+// 64), 16 bytes apart, 16-byte chunk c of a block's row i at c ^ p_swizzle(i): the 16
+// rows of a 16-byte read and the four rows of a transposing read fall on distinct
+// banks, and few addresses are not constant offsets of one another.
 //
 // Scores, softmax statistics and sums are fp32; p and ds are rounded to bf16 as
 // operands, the results once.  The forward pass keeps each row's log-sum-exp and, for
@@ -42,6 +43,8 @@ typedef __attribute__((address_space(3))) ps16x4_t plds_s16x4_t;
 constexpr int P_NW = 4;             // waves per workgroup
 constexpr int P_WR = 32;            // rows a wave owns
 constexpr int P_WG = P_NW * P_WR;   // rows a workgroup owns
+constexpr int P_KW = 8;             // waves per workgroup of the dk, dv kernel
+constexpr int P_KG = P_KW * P_WR;   // keys it owns
 constexpr int P_TR = 64;            // rows per swept tile
 constexpr int P_FILL = 32;          // workgroups that clear rows outside the sequences
 constexpr float P_SLACK = 8.0f;     // log2 headroom of the reference max
@@ -55,7 +58,7 @@ struct PackedArgs {
   Rows q, k, v, d;                  // d: do
   const int32_t *cu;
   int nseq, T, heads, kv;
-  int tiles;                        // row-tile slots: T / P_WG + nseq
+  int tiles;                        // row-tile slots: T / (rows of a workgroup) + nseq
   int items;                        // workgroups that own rows; P_FILL follow
   float c2, scale;                  // scale * log2(e), scale
   bf16_t *out, *lo;                 // (T, heads, HD)
@@ -63,11 +66,22 @@ struct PackedArgs {
   const bf16_t *o, *olo;
   float *delta;                     // (heads, T)
   bf16_t *dq, *dk, *dv;
+  float *part;                      // (heads, T, 2, HD): dk and dv by query head
 };
 
+constexpr int P_BLK = 520;          // elements from one 1 KB block to the next
+
 template <int HD>
-__device__ __forceinline__ int p_swizzle(int r) {
-  return HD == 128 ? ((r & 7) << 1) | ((r >> 3) & 1) : (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+__device__ __forceinline__ int p_swizzle(int i) {
+  return HD == 128 ? (i & 3) << 2 : (((i >> 1) & 1) << 2) | (((i >> 2) & 1) << 1);
+}
+// Elements a tile of `rows` rows takes, and where chunk c of its row r is.
+template <int HD>
+constexpr int p_tile(int rows) { return rows * HD / 512 * P_BLK; }
+template <int HD>
+__device__ __forceinline__ int p_at(int r, int c) {
+  constexpr int RPI = 512 / HD;
+  return r / RPI * P_BLK + r % RPI * HD + 8 * (c ^ p_swizzle<HD>(r % RPI));
 }
 
 // Rows of sequence s, inside the tensor whatever the table holds.
@@ -76,21 +90,22 @@ __device__ __forceinline__ void p_bounds(const PackedArgs &p, int s, int &begin,
   len = min(max(p.cu[s + 1], begin), p.T) - begin;
 }
 
-// Slot t of the row tiles: sequence s's start at cu[s] / P_WG + s, which leaves it at
+// Slot t of the tiles of `rows` rows: sequence s's start at cu[s] / rows + s, which leaves it at
 // least as many as it needs, so a slot finds its sequence from the table alone (one
 // load per 64 sequences) and the host never reads it.  False: nothing there.
-__device__ __forceinline__ bool p_slot(const PackedArgs &p, int t, int lane, int &begin, int &len, int &r0) {
+__device__ __forceinline__ bool p_slot(const PackedArgs &p, int t, int lane, int rows, int &begin, int &len,
+                                      int &r0) {
   int s = -1;
   for (int b = 0; b < p.nseq; b += 64) {
     const int i = b + lane;
-    const bool at = i < p.nseq && min(max(p.cu[i], 0), p.T) / P_WG + i <= t;
+    const bool at = i < p.nseq && min(max(p.cu[i], 0), p.T) / rows + i <= t;
     const int n = __popcll(__ballot(at));
     s += n;
     if (n < 64) break;
   }
   if (s < 0) return false;
   p_bounds(p, s, begin, len);
-  r0 = (t - begin / P_WG - s) * P_WG;
+  r0 = (t - begin / rows - s) * rows;
   return r0 >= 0 && r0 < len;
 }
 
@@ -121,11 +136,11 @@ __device__ __forceinline__ void p_clear(const PackedArgs &p, bf16_t *out, int n,
 }
 
 // One workgroup's loads of tiles of P_TR rows: lane i of load block j fills physical
-// chunk i % CH of row RPI j + i / CH; wave w takes blocks w, w + 4, .., whose rows
+// chunk i % CH of row RPI j + i / CH; wave w takes blocks w, w + NW, .., whose rows
 // share the swizzle.
-template <int HD>
+template <int HD, int NW = P_NW>
 struct TileLoad {
-  static constexpr int CH = HD / 8, RPI = 64 / CH, PER = P_TR / RPI / P_NW;
+  static constexpr int CH = HD / 8, RPI = 64 / CH, PER = P_TR / RPI / NW;
   const bf16_t *p;
   int64_t st;
   uint32_t voff;
@@ -136,21 +151,17 @@ struct TileLoad {
     wave = w;
     const int r = lane / CH;
     voff = static_cast<uint32_t>(r) * static_cast<uint32_t>(st * 2) +
-           16u * ((lane % CH) ^ p_swizzle<HD>(RPI * w + r));
+           16u * ((lane % CH) ^ p_swizzle<HD>(r));
   }
   // rows row0 .. of the sequence's `len`; the rest of the tile reads zeros
   __device__ __forceinline__ void issue(bf16_t *lds, int row0, int len) const {
     const int rows = min(P_TR, len - row0);
     const uint32_t bytes = rows > 0 ? static_cast<uint32_t>(((rows - 1) * st + HD) * 2) : 0u;
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t *>(p + row0 * st), 0, bytes, 0x00020000);
+    const au32x4_t rs = lds_rsrc(p + row0 * st, bytes);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int j = wave + P_NW * i;
-      const uint32_t off = static_cast<uint32_t>(j * RPI * 2 * st);
-      const bool live = (j * RPI) < rows;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (alds_void *)(lds + 512 * j), 16, live ? voff : 0x80000000u,
-                                               live ? static_cast<int>(off) : 0, 0, 0);
+      const int j = wave + NW * i;
+      lds_load(rs, voff + static_cast<uint32_t>(j * RPI) * static_cast<uint32_t>(st * 2), lds + P_BLK * j);
     }
   }
 };
@@ -159,7 +170,7 @@ struct TileLoad {
 template <int HD>
 __device__ __forceinline__ abf16x8_t p_rows(const bf16_t *tile, int t, int kk, int lr, int g) {
   return __builtin_bit_cast(abf16x8_t, *reinterpret_cast<const au32x4_t *>(
-                                           tile + (32 * t + lr) * HD + 8 * ((2 * kk + g) ^ p_swizzle<HD>(lr))));
+                                           tile + t * p_tile<HD>(32) + p_at<HD>(lr, 2 * kk + g)));
 }
 
 // A operand of the second product, transposed: columns 32 e .. + 31 as its rows, K
@@ -167,13 +178,11 @@ __device__ __forceinline__ abf16x8_t p_rows(const bf16_t *tile, int t, int kk, i
 template <int HD>
 __device__ __forceinline__ abf16x8_t p_cols(const bf16_t *tile, int e, int kp, int lane) {
   const int ti = lane & 15, tq = lane >> 4;
-  const int r = 16 * kp + 4 * (tq >> 1) + (ti >> 2);
-  const int c = 4 * e + 2 * (tq & 1) + ((ti & 3) >> 1), in = 4 * (ti & 1);
-  const ps16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (plds_s16x4_t *)(tile + r * HD + 8 * (c ^ p_swizzle<HD>(r)) + in));
-  const ps16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (plds_s16x4_t *)(tile + (r + 8) * HD + 8 * (c ^ p_swizzle<HD>(r + 8)) + in));
-  return __builtin_bit_cast(abf16x8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  const bf16_t *a = tile + kp * p_tile<HD>(16) + 4 * (ti & 1) +
+                    p_at<HD>(4 * (tq >> 1) + (ti >> 2), 4 * e + 2 * (tq & 1) + ((ti & 3) >> 1));
+  const ps16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((plds_s16x4_t *)a);
+  const ps16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((plds_s16x4_t *)(a + p_tile<HD>(8)));
+  return __builtin_bit_cast(abf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // B operand: eight products of a lane as bf16.
@@ -221,15 +230,9 @@ __device__ __forceinline__ void p_store(const pf32x16_t (&acc)[HD / 32], float f
     }
 }
 
-// Every wave's loads have landed, and every wave is done with the other stage.
-__device__ __forceinline__ void p_sync() {
-  vmcnt_wait<0>();
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 template <int HD>
 __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs p) {
-  __shared__ __align__(16) bf16_t k0[P_TR * HD], k1[P_TR * HD], v0[P_TR * HD], v1[P_TR * HD];
+  __shared__ __align__(16) bf16_t k0[p_tile<HD>(P_TR)], k1[p_tile<HD>(P_TR)], v0[p_tile<HD>(P_TR)], v1[p_tile<HD>(P_TR)];
   const int w = static_cast<int>(blockIdx.x);
   if (w >= p.items) {
     p_clear(p, p.out, p.heads * HD, w - p.items);
@@ -239,7 +242,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int h, t, begin, len, q0;
   p_item(w, p.heads, p.tiles, true, h, t);
-  if (!p_slot(p, t, lane, begin, len, q0)) return;
+  if (!p_slot(p, t, lane, P_WG, begin, len, q0)) return;
   begin = __builtin_amdgcn_readfirstlane(begin);
   len = __builtin_amdgcn_readfirstlane(len);
   q0 = __builtin_amdgcn_readfirstlane(q0);
@@ -258,7 +261,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs p) {
 
   auto block = [&](int b, const bf16_t *ks, const bf16_t *vs, bf16_t *kn, bf16_t *vn)
       __attribute__((always_inline)) {
-    p_sync();
+    lds_sync<0>();  // every wave's loads have landed, and it is done with the other stage
     if (b + 1 < nkb) {
       lk.issue(kn, (b + 1) * P_TR, len);
       lv.issue(vn, (b + 1) * P_TR, len);
@@ -348,7 +351,7 @@ __global__ __launch_bounds__(256) void packed_delta_kernel(PackedArgs p) {
 
 template <int HD>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
-  __shared__ __align__(16) bf16_t k0[P_TR * HD], k1[P_TR * HD], v0[P_TR * HD], v1[P_TR * HD];
+  __shared__ __align__(16) bf16_t k0[p_tile<HD>(P_TR)], k1[p_tile<HD>(P_TR)], v0[p_tile<HD>(P_TR)], v1[p_tile<HD>(P_TR)];
   const int w = static_cast<int>(blockIdx.x);
   if (w >= p.items) {
     p_clear(p, p.dq, p.heads * HD, w - p.items);
@@ -358,7 +361,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int h, t, begin, len, q0;
   p_item(w, p.heads, p.tiles, true, h, t);
-  if (!p_slot(p, t, lane, begin, len, q0)) return;
+  if (!p_slot(p, t, lane, P_WG, begin, len, q0)) return;
   begin = __builtin_amdgcn_readfirstlane(begin);
   len = __builtin_amdgcn_readfirstlane(len);
   q0 = __builtin_amdgcn_readfirstlane(q0);
@@ -380,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
 
   auto block = [&](int b, const bf16_t *ks, const bf16_t *vs, bf16_t *kn, bf16_t *vn)
       __attribute__((always_inline)) {
-    p_sync();
+    lds_sync<0>();  // every wave's loads have landed, and it is done with the other stage
     if (b + 1 < nkb) {
       lk.issue(kn, (b + 1) * P_TR, len);
       lv.issue(vn, (b + 1) * P_TR, len);
@@ -420,43 +423,54 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
   p_store<HD>(acc, p.scale, p.dq + (static_cast<int64_t>(begin + qi) * p.heads + h) * HD, nullptr, g, qi < len);
 }
 
-template <int HD>
-__global__ __launch_bounds__(256, 2) void packed_dkv_kernel(PackedArgs p) {
-  __shared__ __align__(16) bf16_t q0s[P_TR * HD], q1s[P_TR * HD], d0s[P_TR * HD], d1s[P_TR * HD];
+// dk and dv of eight waves' keys.  A wave's 32 x HD sums of both take half its
+// registers, its keys' B operands an eighth; its values' are read from LDS again for
+// every tile.  SPLIT: one query head per workgroup, fp32 sums to `part`, which a second
+// kernel joins over the heads that share a key head.
+template <int HD, bool SPLIT>
+__global__ __launch_bounds__(64 * P_KW, 1) void packed_dkv_kernel(PackedArgs p) {
+  constexpr int TILE = p_tile<HD>(P_TR);
+  __shared__ __align__(16) bf16_t q0s[TILE], q1s[TILE], d0s[TILE], d1s[TILE];
+  __shared__ __align__(16) bf16_t vs[p_tile<HD>(P_KG)];                   // the workgroup's values
   __shared__ __align__(16) float l0s[P_TR], l1s[P_TR], e0s[P_TR], e1s[P_TR];  // log-sum-exp, delta
   const int w = static_cast<int>(blockIdx.x);
   if (w >= p.items) {
-    p_clear(p, p.dk, p.kv * HD, w - p.items);
-    p_clear(p, p.dv, p.kv * HD, w - p.items);
+    if (!SPLIT) {
+      p_clear(p, p.dk, p.kv * HD, w - p.items);
+      p_clear(p, p.dv, p.kv * HD, w - p.items);
+    }
     return;
   }
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, lr = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = p.heads / p.kv;
   int hk, t, begin, len, r0;
-  p_item(w, p.kv, p.tiles, false, hk, t);
-  if (!p_slot(p, t, lane, begin, len, r0)) return;
+  p_item(w, SPLIT ? p.heads : p.kv, p.tiles, false, hk, t);
+  const int h0 = SPLIT ? hk : hk * group;  // first query head
+  if (SPLIT) hk /= group;
+  if (!p_slot(p, t, lane, P_KG, begin, len, r0)) return;
   begin = __builtin_amdgcn_readfirstlane(begin);
   len = __builtin_amdgcn_readfirstlane(len);
   r0 = __builtin_amdgcn_readfirstlane(r0);
-  const int group = p.heads / p.kv;
   const int wk0 = r0 + P_WR * wave, ki = wk0 + lr;
-  const int nqb = (len - r0 + P_TR - 1) / P_TR, total = nqb * group;  // swept tiles, of all heads
+  const int nqb = (len - r0 + P_TR - 1) / P_TR, total = SPLIT ? nqb : nqb * group;  // swept tiles
 
-  TileLoad<HD> lq, ld;
+  TileLoad<HD, P_KW> lq, ld, lv;
   lq.init(p.q.p, p.q.st, wave, lane);
   ld.init(p.d.p, p.d.st, wave, lane);
+  lv.init(p.v.p + begin * p.v.st + hk * p.v.sh, p.v.st, wave, lane);
+#pragma unroll
+  for (int i = 0; i < P_KG / P_TR; ++i) lv.issue(vs + i * TILE, r0 + i * P_TR, len);
   int ih = 0, ib = 0;  // the next tile to load: head of the group, tile of its sweep
   auto issue = [&](bf16_t *qs, bf16_t *ds, float *ls, float *es) __attribute__((always_inline)) {
-    const int h = hk * group + ih, row = r0 + ib * P_TR;
+    const int h = h0 + ih, row = r0 + ib * P_TR;
     lq.p = p.q.p + begin * p.q.st + h * p.q.sh;
     ld.p = p.d.p + begin * p.d.st + h * p.d.sh;
     lq.issue(qs, row, len);
     ld.issue(ds, row, len);
     if (wave < 2) {  // 64 log-sum-exps, 64 deltas
       const float *src = (wave ? p.delta : p.lse) + static_cast<int64_t>(h) * p.T + begin + row;
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<float *>(src), 0, 4u * static_cast<uint32_t>(min(P_TR, len - row)), 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (alds_void *)(wave ? es : ls), 4, 4 * lane, 0, 0, 0);
+      lds_load4(lds_rsrc(src, 4u * static_cast<uint32_t>(min(P_TR, len - row))), 4 * lane, wave ? es : ls);
     }
     if (++ib == nqb) {
       ib = 0;
@@ -464,19 +478,19 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(PackedArgs p) {
     }
   };
   issue(q0s, d0s, l0s, e0s);
-  abf16x8_t k[HD / 16], v[HD / 16];
+  abf16x8_t k[HD / 16];
   p_own<HD>(k, p.k, begin + min(ki, len - 1), hk, g);
-  p_own<HD>(v, p.v, begin + min(ki, len - 1), hk, g);
   pf32x16_t dk[HD / 32] = {}, dv[HD / 32] = {};
 
   int cb = 0;  // tile of the current sweep
   auto block = [&](int it, const bf16_t *qs, const bf16_t *ds, const float *ls, const float *es, bf16_t *qn,
                    bf16_t *dn, float *ln, float *en) __attribute__((always_inline)) {
-    p_sync();
+    lds_sync<0>();  // every wave's loads have landed, and it is done with the other stage
     if (it + 1 < total) issue(qn, dn, ln, en);
     const int qb0 = r0 + cb * P_TR;
     if (++cb == nqb) cb = 0;
-#pragma unroll
+    if (wk0 >= len) return;  // wave-uniform: no keys
+#pragma unroll 1
     for (int u = 0; u < 2; ++u) {
       const int qt0 = qb0 + 32 * u;
       if (qt0 < wk0) continue;  // wave-uniform: queries before all of the wave's keys
@@ -484,7 +498,8 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(PackedArgs p) {
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
         s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(qs, u, kk, lr, g), k[kk], s, 0, 0, 0);
-        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(ds, u, kk, lr, g), v[kk], dp, 0, 0, 0);
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(ds, u, kk, lr, g), p_rows<HD>(vs, wave, kk, lr, g),
+                                                     dp, 0, 0, 0);
       }
       // (queries past the sequence: zero rows of q and do, whose log-sum-exp and
       // delta read as 0, so that ds = 0 and p meets do = 0)
@@ -521,9 +536,52 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(PackedArgs p) {
     block(it, q0s, d0s, l0s, e0s, q1s, d1s, l1s, e1s);
     if (it + 1 < total) block(it + 1, q1s, d1s, l1s, e1s, q0s, d0s, l0s, e0s);
   }
-  const int64_t at = (static_cast<int64_t>(begin + ki) * p.kv + hk) * HD;
-  p_store<HD>(dk, p.scale, p.dk + at, nullptr, g, ki < len);
-  p_store<HD>(dv, 1.0f, p.dv + at, nullptr, g, ki < len);
+  if constexpr (SPLIT) {
+    if (ki >= len) return;
+    // element 32 e + 8 q + 4 g + i of the row
+    float *o = p.part + (static_cast<int64_t>(h0) * p.T + begin + ki) * (2 * HD) + 4 * g;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        *reinterpret_cast<af32x4_t *>(o + 32 * e + 8 * b) =
+            af32x4_t{dk[e][4 * b], dk[e][4 * b + 1], dk[e][4 * b + 2], dk[e][4 * b + 3]};
+        *reinterpret_cast<af32x4_t *>(o + HD + 32 * e + 8 * b) =
+            af32x4_t{dv[e][4 * b], dv[e][4 * b + 1], dv[e][4 * b + 2], dv[e][4 * b + 3]};
+      }
+  } else {
+    const int64_t at = (static_cast<int64_t>(begin + ki) * p.kv + hk) * HD;
+    p_store<HD>(dk, p.scale, p.dk + at, nullptr, g, ki < len);
+    p_store<HD>(dv, 1.0f, p.dv + at, nullptr, g, ki < len);
+  }
+}
+
+// dk and dv rows from the sums of the heads that share them, in the heads' order; rows
+// outside the sequences zero.  HD / 8 lanes per row and key head.
+template <int HD>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs p) {
+  constexpr int CH = HD / 8;
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / CH;  // row * kv + key head
+  const int c = 8 * (threadIdx.x % CH);
+  if (at >= static_cast<int64_t>(p.T) * p.kv) return;
+  const int64_t row = at / p.kv;
+  const int hk = static_cast<int>(at - row * p.kv), group = p.heads / p.kv;
+  float k[8] = {}, v[8] = {};
+  if (row >= p.cu[0] && row < p.cu[p.nseq])
+    for (int i = 0; i < group; ++i) {
+      const float *s = p.part + (static_cast<int64_t>(hk * group + i) * p.T + row) * (2 * HD) + c;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        k[j] += s[j];
+        v[j] += s[HD + j];
+      }
+    }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) k[j] *= p.scale;
+  *reinterpret_cast<au32x4_t *>(p.dk + at * HD + c) =
+      au32x4_t{pack_bf(k[0], k[1]), pack_bf(k[2], k[3]), pack_bf(k[4], k[5]), pack_bf(k[6], k[7])};
+  *reinterpret_cast<au32x4_t *>(p.dv + at * HD + c) =
+      au32x4_t{pack_bf(v[0], v[1]), pack_bf(v[2], v[3]), pack_bf(v[4], v[5]), pack_bf(v[6], v[7])};
 }
 
 // 16-byte aligned rows that do not overlap (a tile's rows past its sequence have to
@@ -569,8 +627,18 @@ template <int HD>
 static void launch_backward(PackedArgs a, hipStream_t st) {
   const int64_t lanes = static_cast<int64_t>(a.T) * a.heads * (HD / 8);
   hipLaunchKernelGGL((packed_delta_kernel<HD>), dim3(static_cast<unsigned>(cdiv(lanes, 256))), dim3(256), 0, st, a);
-  a.items = a.tiles * a.kv;
-  hipLaunchKernelGGL((packed_dkv_kernel<HD>), dim3(a.items + P_FILL), dim3(256), 0, st, a);
+  const int tiles = a.tiles;
+  a.tiles = a.T / P_KG + a.nseq;
+  if (a.part) {
+    a.items = a.tiles * a.heads;
+    hipLaunchKernelGGL((packed_dkv_kernel<HD, true>), dim3(a.items), dim3(64 * P_KW), 0, st, a);
+    const int64_t rows = static_cast<int64_t>(a.T) * a.kv * (HD / 8);
+    hipLaunchKernelGGL((packed_join_kernel<HD>), dim3(static_cast<unsigned>(cdiv(rows, 256))), dim3(256), 0, st, a);
+  } else {
+    a.items = a.tiles * a.kv;
+    hipLaunchKernelGGL((packed_dkv_kernel<HD, false>), dim3(a.items + P_FILL), dim3(64 * P_KW), 0, st, a);
+  }
+  a.tiles = tiles;
   a.items = a.tiles * a.heads;
   hipLaunchKernelGGL((packed_dq_kernel<HD>), dim3(a.items + P_FILL), dim3(256), 0, st, a);
 }
@@ -602,20 +670,38 @@ extern "C" int evo2_packed_attention(const void *q, int64_t sqt, int64_t sqh, co
   return check_launch("packed_attention");
 }
 
+// Whether a workgroup of the dk, dv kernel takes one query head rather than all that
+// share its keys: where whole groups leave fewer workgroups than two for each CU.
+static bool packed_split(int64_t T, int64_t nseq, int64_t heads, int64_t kv) {
+  return heads > kv && (T / P_KG + nseq) * kv < 512;
+}
+
+extern "C" int64_t evo2_packed_attention_workspace_bytes(int64_t T, int64_t nseq, int64_t heads, int64_t kv,
+                                                         int64_t head_dim) {
+  if (T <= 0 || nseq < 0 || heads <= 0 || kv <= 0 || head_dim <= 0) return 0;
+  // delta, then the sums by query head
+  return cdiv(heads * T * 4, 256) * 256 + (packed_split(T, nseq, heads, kv) ? heads * T * 2 * head_dim * 4 : 0);
+}
+
 extern "C" int evo2_packed_attention_backward(const void *dout, int64_t sdt, int64_t sdh, const void *q,
                                               int64_t sqt, int64_t sqh, const void *k, int64_t skt, int64_t skh,
                                               const void *v, int64_t svt, int64_t svh, const int32_t *cu,
                                               int64_t nseq, const void *out, const void *out_lo,
-                                              const float *lse, float *delta, void *dq, void *dk, void *dv,
-                                              int64_t T, int64_t heads, int64_t kv, int64_t head_dim, float scale,
+                                              const float *lse, void *workspace, int64_t workspace_bytes,
+                                              void *dq, void *dk, void *dv, int64_t T, int64_t heads, int64_t kv, int64_t head_dim, float scale,
                                               void *stream) {
   const int rc = check_sizes("packed_attention_backward", T, nseq, heads, kv, head_dim, scale);
   if (rc || T == 0) return rc;
-  if (!dout || !q || !k || !v || !cu || !out || !out_lo || !lse || !delta || !dq || !dk || !dv)
+  if (!dout || !q || !k || !v || !cu || !out || !out_lo || !lse || !workspace || !dq || !dk || !dv)
     return fail(EVO2_ERR_INVALID, "packed_attention_backward: null pointer argument");
   if (!rows_ok(dout, sdt, sdh, head_dim) || !rows_ok(q, sqt, sqh, head_dim) || !rows_ok(k, skt, skh, head_dim) || !rows_ok(v, svt, svh, head_dim) ||
-      !aligned(out) || !aligned(out_lo) || !aligned(dq) || !aligned(dk) || !aligned(dv))
+      !aligned(out) || !aligned(out_lo) || !aligned(dq) || !aligned(dk) || !aligned(dv) ||
+      !aligned(workspace))
     return fail(EVO2_ERR_UNSUPPORTED, "packed_attention_backward: operands must be 16-byte aligned rows");
+  if (workspace_bytes < evo2_packed_attention_workspace_bytes(T, nseq, heads, kv, head_dim))
+    return fail(EVO2_ERR_INVALID, "packed_attention_backward: workspace of %lld bytes, %lld needed",
+                (long long)workspace_bytes,
+                (long long)evo2_packed_attention_workspace_bytes(T, nseq, heads, kv, head_dim));
   PackedArgs a = packed_args(cu, nseq, T, heads, kv, scale);
   a.q = Rows{static_cast<const bf16_t *>(q), sqt, sqh};
   a.k = Rows{static_cast<const bf16_t *>(k), skt, skh};
@@ -624,7 +710,9 @@ extern "C" int evo2_packed_attention_backward(const void *dout, int64_t sdt, int
   a.o = static_cast<const bf16_t *>(out);
   a.olo = static_cast<const bf16_t *>(out_lo);
   a.lse = const_cast<float *>(lse);
-  a.delta = delta;
+  a.delta = static_cast<float *>(workspace);
+  if (packed_split(T, nseq, heads, kv))
+    a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + cdiv(heads * T * 4, 256) * 256);
   a.dq = static_cast<bf16_t *>(dq);
   a.dk = static_cast<bf16_t *>(dk);
   a.dv = static_cast<bf16_t *>(dv);

@@ -424,19 +424,23 @@ int evo2_iir_verify_gated(const void *zf, int64_t zs, const float *log_poles, in
  *   out, dq (T, heads, hd), dk, dv (T, kv, hd) bf16 contiguous; rows outside every
  *   sequence are zero
  *   out_lo (T, heads, hd) bf16 and lse (heads, T) fp32: what the backward call needs
- *   of the forward one (both NULL without one); delta (heads, T) fp32 scratch
+ *   of the forward one (both NULL without one); the backward call's workspace has
+ *   _workspace_bytes(T, nseq, heads, kv, hd) bytes
  *   heads a multiple of kv, hd 64 or 128, scale > 0
  */
 int evo2_packed_attention(const void *q, int64_t sqt, int64_t sqh, const void *k, int64_t skt,
                           int64_t skh, const void *v, int64_t svt, int64_t svh, const int32_t *cu,
                           int64_t nseq, void *out, void *out_lo, float *lse, int64_t T, int64_t heads,
                           int64_t kv, int64_t head_dim, float scale, void *stream);
+int64_t evo2_packed_attention_workspace_bytes(int64_t T, int64_t nseq, int64_t heads, int64_t kv,
+                                              int64_t head_dim);
 int evo2_packed_attention_backward(const void *dout, int64_t sdt, int64_t sdh, const void *q,
                                    int64_t sqt, int64_t sqh, const void *k, int64_t skt, int64_t skh,
                                    const void *v, int64_t svt, int64_t svh, const int32_t *cu,
                                    int64_t nseq, const void *out, const void *out_lo, const float *lse,
-                                   float *delta, void *dq, void *dk, void *dv, int64_t T, int64_t heads,
-                                   int64_t kv, int64_t head_dim, float scale, void *stream);
+                                   void *workspace, int64_t workspace_bytes, void *dq, void *dk,
+                                   void *dv, int64_t T, int64_t heads, int64_t kv, int64_t head_dim,
+                                   float scale, void *stream);
 
 /*
  * bf16 projections of at most 16 rows (decode steps), fp32 sums:
