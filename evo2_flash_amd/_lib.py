@@ -187,13 +187,13 @@ SIGNATURES = {
     "evo2_gated_linear_workspace_bytes": [_c_i64, _c_i64, _c_i64],
     "evo2_gated_linear": [
         _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i32,  # x, sx, w1, w2, sw, gelu
-        _c_p, _c_i64, _c_p, _c_p,                 # h, sh, z1, z2
+        _c_p, _c_i64, _c_p,                       # h, sh, kept
         _c_i64, _c_i64, _c_i64, _c_p,             # M, I, H, stream
     ],
     "evo2_gated_linear_backward": [
         _c_p, _c_i64, _c_p, _c_i64,               # dh, sdh, x, sx
-        _c_p, _c_p, _c_i64, _c_i32,               # w1, w2, sw, gelu
-        _c_p, _c_p, _c_p, _c_p, _c_p,             # z1, z2, dx, dw1, dw2
+        _c_p, _c_p, _c_i64,                       # w1, w2, sw
+        _c_p, _c_p, _c_p, _c_p,                   # kept, dx, dw1, dw2
         _c_p, _c_i64,                             # workspace, bytes
         _c_i64, _c_i64, _c_i64, _c_p,             # M, I, H, stream
     ],

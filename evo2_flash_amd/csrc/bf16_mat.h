@@ -43,7 +43,7 @@ enum MatForm { MAT_NT = 0, MAT_NN = 1, MAT_TN = 2 };
 enum MatEpi {
   MAT_BF16 = 0,   // out as bf16
   MAT_F32 = 1,    // fp32 partial sums, one plane per split (or added to what is there)
-  MAT_GATED = 2,  // act(x w^T) * (x w2^T), and both products for the backward pass
+  MAT_GATED = 2,  // act(x w^T) * (x w2^T), and both factors of its gradients
   MAT_STATS = 3,  // each row's max and sum of exponentials over 128 columns
   MAT_DLOG = 4,   // the gradient of the cross entropy at the logits
 };
@@ -68,7 +68,7 @@ struct MatArgs {
   void *out, *out2; int64_t so;
   int64_t plane;                          // MAT_F32: elements between the splits' partial sums
   int add;                                // MAT_F32: add to out
-  float *z1, *z2; int gelu;               // MAT_GATED: the two products (rows of N), or null
+  bf16_t *kept; int64_t kplane; int gelu; // MAT_GATED: what the backward pass needs, or null
   // cross entropy: rows' targets (less col0), log-sum-exp, upstream gradient
   const int64_t *targets; int64_t ignore; int64_t V; int64_t col0;
   const float *lse; const float *grad; int64_t sgrad;
@@ -96,10 +96,11 @@ __host__ __device__ inline void mat_tile(int t, int tiles_m, int tiles_n, int sp
   bn = 4 * panel + (s - bm * width);
 }
 
-__device__ __forceinline__ float gelu_f(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
-// d gelu / dx = cdf(x) + x pdf(x)
-__device__ __forceinline__ float gelu_slope(float x) {
-  return 0.5f * (1.0f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * expf(-0.5f * x * x);
+// gelu(x) = x cdf(x), and its slope cdf(x) + x pdf(x).
+__device__ __forceinline__ void gelu_both(const float x, float &value, float &slope) {
+  const float cdf = fmaf(0.5f, erff(x * 0.70710678118654752f), 0.5f);
+  slope = fmaf(x * 0.39894228040143268f, __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f), cdf);
+  value = x * cdf;
 }
 
 // What a row's softmax less its target is multiplied by: its upstream gradient, 0 of an
@@ -119,6 +120,7 @@ __device__ __forceinline__ float mat_factor(const float *num, const float *den) 
 
 template <int FORM, int TM, int EPI>
 __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
+  static_assert(FORM != MAT_TN || TM != 3, "rows of 192 do not fill whole load blocks");
   constexpr int BM = 64 * TM, NST = mat_stages(TM);
   constexpr bool WR = FORM != MAT_NT, XR = FORM == MAT_TN;  // rows along N / M
   constexpr int WST = MAT_BN * MAT_BK, XST = BM * MAT_BK;   // elements per stage
@@ -357,22 +359,22 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     const int tr = lane >> 3, tc = lane & 7;  // turned: lane's row of eight, 16-byte chunk
     // (LDS serves a wave in order; the compiler is kept to it)
     auto fence = [] { asm volatile("" ::: "memory"); };
-    // rows m .. m + 31, 64 columns from n0 + c: v(t, i) of tile t (0, 1), element i
-    auto put_bf16 = [&](bf16_t *out, int m, int c, int cols, auto &&v) __attribute__((always_inline)) {
+    // rows m .. m + 31, 64 columns from n0 + c of rows of `so` 16-bit values: v(t, i) holds
+    // elements i and i + 1 of tile t (0, 1)
+    auto put16 = [&](bf16_t *out, int64_t so, int m, int c, int cols, auto &&v) __attribute__((always_inline)) {
       bf16_t *b = reinterpret_cast<bf16_t *>(tb);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint2 *>(b + lr * 72 + 32 * t + 8 * q + 4 * g) =
-              make_uint2(pack_bf(v(t, 4 * q), v(t, 4 * q + 1)), pack_bf(v(t, 4 * q + 2), v(t, 4 * q + 3)));
+          *reinterpret_cast<uint2 *>(b + lr * 72 + 32 * t + 8 * q + 4 * g) = make_uint2(v(t, 4 * q), v(t, 4 * q + 2));
       fence();
-      bf16_t *o = out + m * p.so + n0 + c;
+      bf16_t *o = out + m * so + n0 + c;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int r = 8 * k + tr;
         const au32x4_t w = *reinterpret_cast<const au32x4_t *>(b + r * 72 + 8 * tc);
-        if (m + r < p.M && n0 + c + 8 * tc < cols) *reinterpret_cast<au32x4_t *>(o + r * p.so + 8 * tc) = w;
+        if (m + r < p.M && n0 + c + 8 * tc < cols) *reinterpret_cast<au32x4_t *>(o + r * so + 8 * tc) = w;
       }
       fence();
     };
@@ -434,16 +436,39 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
         for (int tn = 0; tn < 4; ++tn)
           put_f32(out, p.so, mr, 32 * tn, p.add != 0, [&](int i) { return acc[tn][tm][i]; });
       } else if constexpr (EPI == MAT_GATED) {
-        put_bf16(static_cast<bf16_t *>(p.out), mr, 0, p.N, [&](int t, int i) {
-          const float a = acc[t][tm][i];
-          return (p.gelu ? gelu_f(a) : a) * acc[t + 2][tm][i];
-        });
-        if (p.z1) {
+        // h = act(z1) z2, and for the backward pass a = z2 act'(z1) and b = act(z1), in
+        // place of z1 and z2, as three planes of 16 bits: the high halves of both and
+        // the next eight bits of each (24 of 32 bits, off by at most 2^-16: rounded to
+        // bf16 they would put a second rounding under d1 and d2; as fp32 the tile's
+        // stores and the gradient kernel's loads are a third more)
+        float slope[2][16];
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            put_f32(p.z1, p.N, mr, 32 * t, false, [&](int i) { return acc[t][tm][i]; });
-            put_f32(p.z2, p.N, mr, 32 * t, false, [&](int i) { return acc[t + 2][tm][i]; });
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float value = acc[t][tm][i];
+            slope[t][i] = 1.0f;
+            if (p.gelu) gelu_both(value, value, slope[t][i]);  // uniform
+            acc[t][tm][i] = value;
           }
+        put16(static_cast<bf16_t *>(p.out), p.so, mr, 0, p.N, [&](int t, int i) {
+          return pack_bf(acc[t][tm][i] * acc[t + 2][tm][i], acc[t][tm][i + 1] * acc[t + 2][tm][i + 1]);
+        });
+        if (p.kept) {  // uniform
+          auto bits = [&](int t, int i, int which) {
+            const float v = which ? acc[t][tm][i] : acc[t + 2][tm][i] * slope[t][i];
+            return __float_as_uint(v);
+          };
+#pragma unroll
+          for (int which = 0; which < 2; ++which)
+            put16(p.kept + which * p.kplane, p.N, mr, 0, p.N, [&](int t, int i) {
+              return (bits(t, i, which) >> 16) | (bits(t, i + 1, which) & 0xffff0000u);
+            });
+          put16(p.kept + 2 * p.kplane, p.N, mr, 0, p.N, [&](int t, int i) {
+            const uint32_t lo = ((bits(t, i, 0) >> 8) & 0xffu) | (bits(t, i, 1) & 0xff00u);
+            const uint32_t hi = ((bits(t, i + 1, 0) >> 8) & 0xffu) | (bits(t, i + 1, 1) & 0xff00u);
+            return lo | (hi << 16);
+          });
         }
       } else if constexpr (EPI == MAT_STATS) {
         // max and sum of exp over the wave's 128 columns of the row, and the
@@ -489,11 +514,16 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
         const bool used = live && t != p.ignore;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          put_bf16(static_cast<bf16_t *>(p.out), mr, 64 * h, (p.N + 7) & ~7, [&](int u, int i) {
-            const int c = 64 * h + 32 * u + 8 * (i >> 2) + (i & 3);
-            float e = __builtin_amdgcn_exp2f(fmaf(acc[2 * h + u][tm][i], 1.44269504088896341f, -lse2));
-            e = at == c ? e - 1.0f : e;
-            return used && c < valid ? e * wgt : 0.0f;
+          put16(static_cast<bf16_t *>(p.out), p.so, mr, 64 * h, (p.N + 7) & ~7, [&](int u, int i0) {
+            float d[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int i = i0 + k, c = 64 * h + 32 * u + 8 * (i >> 2) + (i & 3);
+              float e = __builtin_amdgcn_exp2f(fmaf(acc[2 * h + u][tm][i], 1.44269504088896341f, -lse2));
+              e = at == c ? e - 1.0f : e;
+              d[k] = used && c < valid ? e * wgt : 0.0f;
+            }
+            return pack_bf(d[0], d[1]);
           });
       }
     }
@@ -526,10 +556,12 @@ struct MatPlan {
 };
 
 // M: rows of one of `pair` outputs; slices: of K; width: output columns per tile.
-inline MatPlan mat_plan(int64_t M, int64_t N, int64_t slices, int pair, int width, bool may_split) {
+inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int pair, int width,
+                        bool may_split) {
   MatPlan best{};
   double least = 1e300;
-  for (int tm : {4, 2, 1}) {
+  for (int tm : {4, 3, 2, 1}) {
+    if (form == MAT_TN && tm == 3) continue;  // (rows of 192 do not fill whole load blocks)
     const int nst = mat_stages(tm);
     const int64_t tm_tiles = cdiv(M, 64 * tm) * pair, tn_tiles = cdiv(N, width), tiles = tm_tiles * tn_tiles;
     int64_t splits = 1;
@@ -559,6 +591,8 @@ inline void mat_launch(MatArgs a, const MatPlan &pl, hipStream_t st) {
   const int64_t items = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n * pl.splits;
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(MAT_CUS, items)));
   if (pl.tm == 4) hipLaunchKernelGGL((mat_kernel<FORM, 4, EPI>), grid, dim3(256), 0, st, a);
+  else if (FORM != MAT_TN && pl.tm == 3)
+    hipLaunchKernelGGL((mat_kernel<FORM, FORM == MAT_TN ? 4 : 3, EPI>), grid, dim3(256), 0, st, a);
   else if (pl.tm == 2) hipLaunchKernelGGL((mat_kernel<FORM, 2, EPI>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((mat_kernel<FORM, 1, EPI>), grid, dim3(256), 0, st, a);
 }

@@ -5,18 +5,17 @@
 // (the reference's MLP, evo2_flash/model.py:77-101, before its down projection).
 // Both projections, the activation and the product are one launch whose tile takes
 // 128 columns of each weight, so a lane holds z1 and z2 of the same element; h is
-// rounded to bf16 once.  With a backward pass to come the products are kept in fp32:
-// rounded to bf16 they would put a second rounding under d1 and d2, which enter two
-// more products as bf16 themselves.
+// rounded to bf16 once.  With a backward pass to come the launch also keeps the factors
+// of d1 and d2, z2 act'(z1) and act(z1), to 24 bits.
 #include "bf16_mat.h"
 
 namespace evo2 {
 
 // d1 | d2 as (M, 2 Ip) bf16, Ip = I rounded up to whole K slices with zeros there:
 // one thread per eight columns.
-__global__ __launch_bounds__(256) void gated_grad_kernel(const bf16_t *dh, int64_t sdh, const float *z1,
-                                                         const float *z2, int gelu, bf16_t *dz, int64_t chunks,
-                                                         int I, int Ip) {
+__global__ __launch_bounds__(256) void gated_grad_kernel(const bf16_t *dh, int64_t sdh, const bf16_t *kept,
+                                                         int64_t plane, bf16_t *dz, int64_t chunks, int I,
+                                                         int Ip) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (at >= chunks) return;
   const int per = Ip >> 3;
@@ -25,20 +24,20 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const bf16_t *dh, int64
   bf16_t *o = dz + m * 2 * Ip + c;
   au32x4_t d1 = {0, 0, 0, 0}, d2 = {0, 0, 0, 0};
   if (c < I) {
+    const bf16_t *k = kept + m * I + c;
     const au32x4_t g = *reinterpret_cast<const au32x4_t *>(dh + m * sdh + c);
-    const float *a = z1 + m * I + c, *b = z2 + m * I + c;
+    const au32x4_t a = *reinterpret_cast<const au32x4_t *>(k);
+    const au32x4_t b = *reinterpret_cast<const au32x4_t *>(k + plane);
+    const au32x4_t l = *reinterpret_cast<const au32x4_t *>(k + 2 * plane);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float p[2], q[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float d = i ? hi_bf(g[k]) : lo_bf(g[k]);
-        const float u = a[2 * k + i], v = b[2 * k + i];
-        p[i] = d * v * (gelu ? gelu_slope(u) : 1.0f);
-        q[i] = d * (gelu ? gelu_f(u) : u);
-      }
-      d1[k] = pack_bf(p[0], p[1]);
-      d2[k] = pack_bf(q[0], q[1]);
+    for (int j = 0; j < 4; ++j) {
+      // the high half, then the next eight bits: of a the low byte, of b the high one
+      const float a0 = __uint_as_float((a[j] << 16) | ((l[j] & 0xffu) << 8));
+      const float a1 = __uint_as_float((a[j] & 0xffff0000u) | ((l[j] >> 8) & 0xff00u));
+      const float b0 = __uint_as_float((b[j] << 16) | (l[j] & 0xff00u));
+      const float b1 = __uint_as_float((b[j] & 0xffff0000u) | ((l[j] >> 16) & 0xff00u));
+      d1[j] = pack_bf(lo_bf(g[j]) * a0, hi_bf(g[j]) * a1);
+      d2[j] = pack_bf(lo_bf(g[j]) * b0, hi_bf(g[j]) * b1);
     }
   }
   *reinterpret_cast<au32x4_t *>(o) = d1;
@@ -49,10 +48,10 @@ static int64_t up(int64_t n, int64_t a) { return cdiv(n, a) * a; }
 
 // dx: K = both halves of dz; dw: K = the rows.
 static MatPlan plan_dx(int64_t M, int64_t I, int64_t H) {
-  return mat_plan(M, H, 2 * cdiv(I, MAT_BK), 1, MAT_BN, true);
+  return mat_plan(MAT_NN, M, H, 2 * cdiv(I, MAT_BK), 1, MAT_BN, true);
 }
 static MatPlan plan_dw(int64_t M, int64_t I, int64_t H) {
-  return mat_plan(I, H, cdiv(M, MAT_BK), 2, MAT_BN, true);
+  return mat_plan(MAT_TN, I, H, cdiv(M, MAT_BK), 2, MAT_BN, true);
 }
 
 static int check_sizes(const char *what, int64_t M, int64_t I, int64_t H, int64_t sx, int64_t sw) {
@@ -82,13 +81,13 @@ extern "C" int64_t evo2_gated_linear_workspace_bytes(int64_t M, int64_t I, int64
 }
 
 extern "C" int evo2_gated_linear(const void *x, int64_t sx, const void *w1, const void *w2, int64_t sw,
-                                 int32_t gelu, void *h, int64_t sh, float *z1, float *z2, int64_t M,
-                                 int64_t I, int64_t H, void *stream) {
+                                 int32_t gelu, void *h, int64_t sh, void *kept, int64_t M, int64_t I,
+                                 int64_t H, void *stream) {
   int rc = check_sizes("gated_linear", M, I, H, sx, sw);
   if (rc || M == 0) return rc;
-  if (!x || !w1 || !w2 || !h || !z1 != !z2) return fail(EVO2_ERR_INVALID, "gated_linear: null pointer argument");
+  if (!x || !w1 || !w2 || !h) return fail(EVO2_ERR_INVALID, "gated_linear: null pointer argument");
   if (sx < H || sw < H || sh < I || sx % 8 || sw % 8 || sh % 8 || !aligned(x) || !aligned(w1) || !aligned(w2) ||
-      !aligned(h) || !aligned(z1) || !aligned(z2))
+      !aligned(h) || !aligned(kept))
     return fail(EVO2_ERR_UNSUPPORTED, "gated_linear: operands must be 16-byte aligned rows");
   MatArgs a{};
   a.x = static_cast<const bf16_t *>(x);
@@ -102,27 +101,25 @@ extern "C" int evo2_gated_linear(const void *x, int64_t sx, const void *w1, cons
   a.kpair = a.mpair = INT_MAX;
   a.out = h;
   a.so = sh;
-  a.z1 = z1;
-  a.z2 = z2;
+  a.kept = static_cast<bf16_t *>(kept);
+  a.kplane = M * I;
   a.gelu = gelu != 0;
-  mat_launch<MAT_NT, MAT_GATED>(a, mat_plan(M, I, cdiv(H, MAT_BK), 1, MAT_BN / 2, false),
+  mat_launch<MAT_NT, MAT_GATED>(a, mat_plan(MAT_NT, M, I, cdiv(H, MAT_BK), 1, MAT_BN / 2, false),
                                 static_cast<hipStream_t>(stream));
   return check_launch("gated_linear");
 }
 
 extern "C" int evo2_gated_linear_backward(const void *dh, int64_t sdh, const void *x, int64_t sx,
-                                          const void *w1, const void *w2, int64_t sw, int32_t gelu,
-                                          const float *z1, const float *z2, void *dx, void *dw1, void *dw2,
-                                          void *workspace, int64_t workspace_bytes, int64_t M, int64_t I,
-                                          int64_t H, void *stream) {
+                                          const void *w1, const void *w2, int64_t sw, const void *kept,
+                                          void *dx, void *dw1, void *dw2, void *workspace,
+                                          int64_t workspace_bytes, int64_t M, int64_t I, int64_t H, void *stream) {
   int rc = check_sizes("gated_linear_backward", M, I, H, sx, sw);
   if (rc) return rc;
   if (M == 0) return fail(EVO2_ERR_INVALID, "gated_linear_backward: no rows");
-  if (!dh || !x || !w1 || !w2 || !z1 || !z2 || !workspace || !dw1 != !dw2)
+  if (!dh || !x || !w1 || !w2 || !kept || !workspace || !dw1 != !dw2)
     return fail(EVO2_ERR_INVALID, "gated_linear_backward: null pointer argument");
   if (sdh < I || sx < H || sw < H || sdh % 8 || sx % 8 || sw % 8 || !aligned(dh) || !aligned(x) || !aligned(w1) ||
-      !aligned(w2) || !aligned(z1) || !aligned(z2) || !aligned(dx) || !aligned(dw1) || !aligned(dw2) ||
-      !aligned(workspace))
+      !aligned(w2) || !aligned(kept) || !aligned(dx) || !aligned(dw1) || !aligned(dw2) || !aligned(workspace))
     return fail(EVO2_ERR_UNSUPPORTED, "gated_linear_backward: operands must be 16-byte aligned rows");
   if (workspace_bytes < evo2_gated_linear_workspace_bytes(M, I, H))
     return fail(EVO2_ERR_INVALID, "gated_linear_backward: workspace of %lld bytes, %lld needed",
@@ -132,8 +129,8 @@ extern "C" int evo2_gated_linear_backward(const void *dh, int64_t sdh, const voi
   bf16_t *dz = static_cast<bf16_t *>(workspace);
   float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + up(M * 2 * Ip * 2, 256));
   hipLaunchKernelGGL(gated_grad_kernel, dim3(static_cast<unsigned>(cdiv(chunks, 256))), dim3(256), 0, st,
-                     static_cast<const bf16_t *>(dh), sdh, z1, z2, gelu != 0, dz, chunks, static_cast<int>(I),
-                     static_cast<int>(Ip));
+                     static_cast<const bf16_t *>(dh), sdh, static_cast<const bf16_t *>(kept), M * I, dz, chunks,
+                     static_cast<int>(I), static_cast<int>(Ip));
   MatArgs a{};
   a.x = dz;
   a.sx = 2 * Ip;

@@ -163,7 +163,7 @@ static int64_t up(int64_t n, int64_t a) { return cdiv(n, a) * a; }
 static bool aligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 static MatPlan plan_logits(int64_t T, int64_t V, int64_t H, bool split) {
-  return mat_plan(T, V, cdiv(H, MAT_BK), 1, MAT_BN, split);
+  return mat_plan(MAT_NT, T, V, cdiv(H, MAT_BK), 1, MAT_BN, split);
 }
 
 // Vocabulary columns per piece of the backward pass: d takes at most 256 MB, or
@@ -185,8 +185,8 @@ static BackPlan plan_back(int64_t T, int64_t V, int64_t H) {
   b.pieces = cdiv(V, b.vp);
   b.ld = up(b.vp, 8);
   b.z = plan_logits(T, b.vp, H, b.pieces == 1);
-  b.dh = mat_plan(T, H, cdiv(b.vp, MAT_BK), 1, MAT_BN, b.pieces == 1);
-  b.dw = mat_plan(b.vp, H, cdiv(T, MAT_BK), 1, MAT_BN, true);
+  b.dh = mat_plan(MAT_NN, T, H, cdiv(b.vp, MAT_BK), 1, MAT_BN, b.pieces == 1);
+  b.dw = mat_plan(MAT_TN, b.vp, H, cdiv(T, MAT_BK), 1, MAT_BN, true);
   b.acc = b.pieces > 1 ? up(T * H * 4, 256) : 0;
   b.part = std::max({b.z.splits > 1 ? b.z.splits * T * b.vp * 4 : 0, b.dh.splits > 1 ? b.dh.splits * T * H * 4 : 0,
                      b.dw.splits > 1 ? b.dw.splits * b.vp * H * 4 : 0});
@@ -346,7 +346,7 @@ extern "C" int evo2_linear_loss_backward(const void *h, int64_t sh, const void *
       if (b.pieces > 1) {
         c.out = acc;
         c.add = v0 > 0;
-        mat_nn(c, mat_plan(T, H, cdiv(vn, MAT_BK), 1, MAT_BN, false), true, st);
+        mat_nn(c, mat_plan(MAT_NN, T, H, cdiv(vn, MAT_BK), 1, MAT_BN, false), true, st);
         if (v0 + vn == V) mat_join(acc, 0, 1, static_cast<bf16_t *>(dh), H, T, H, st, num, den);
       } else {
         c.out = b.dh.splits > 1 ? static_cast<void *>(part) : dh;
@@ -366,8 +366,8 @@ extern "C" int evo2_linear_loss_backward(const void *h, int64_t sh, const void *
       c.K = static_cast<int>(T);
       c.so = H;
       // a last piece is smaller than the others: its splits are no more than theirs
-      MatPlan pl = mat_plan(vn, H, cdiv(T, MAT_BK), 1, MAT_BN, true);
-      if (pl.splits > 1 && pl.splits * vn * H * 4 > b.part) pl = mat_plan(vn, H, cdiv(T, MAT_BK), 1, MAT_BN, false);
+      MatPlan pl = mat_plan(MAT_TN, vn, H, cdiv(T, MAT_BK), 1, MAT_BN, true);
+      if (pl.splits > 1 && pl.splits * vn * H * 4 > b.part) pl = mat_plan(MAT_TN, vn, H, cdiv(T, MAT_BK), 1, MAT_BN, false);
       bf16_t *to = static_cast<bf16_t *>(dw) + v0 * H;
       c.plane = vn * H;
       c.num = num;

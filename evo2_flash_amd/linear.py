@@ -157,34 +157,31 @@ def _weight_rows(w1, w2):
 
 
 def _gated_forward(x, w1, w2, gelu, keep):
-    """(h, z1, z2): act(x w1^T) * (x w2^T) in bf16 and, to `keep`, both products in
-    fp32 (else None)."""
+    """(h, kept): act(x w1^T) * (x w2^T) in bf16 and, to `keep`, what the backward pass
+    needs of the products (else None)."""
     M, (I, H) = x.shape[0], w1.shape
     h = torch.empty(M, I, dtype=x.dtype, device=x.device)
-    z1 = z2 = None
-    if keep:
-        z1, z2 = torch.empty(2, M, I, dtype=torch.float32, device=x.device).unbind(0)
+    kept = torch.empty(3, M, I, dtype=torch.int16, device=x.device) if keep else None
     if M:
         xr, (a, b) = _lib.rows16(x), _weight_rows(w1, w2)
         with _lib.on_device(xr):
             _lib.call("evo2_gated_linear", _lib.ptr(xr), xr.stride(0), _lib.ptr(a), _lib.ptr(b),
-                      a.stride(0), int(gelu), _lib.ptr(h), h.stride(0), _lib.ptr(z1), _lib.ptr(z2),
-                      M, I, H, _lib.stream_of(xr))
-    return h, z1, z2
+                      a.stride(0), int(gelu), _lib.ptr(h), h.stride(0), _lib.ptr(kept), M, I, H,
+                      _lib.stream_of(xr))
+    return h, kept
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, w2, gelu):
-        h, z1, z2 = _gated_forward(x, w1, w2, gelu, True)
-        ctx.save_for_backward(x, w1, w2, z1, z2)
-        ctx.gelu = gelu
+        h, kept = _gated_forward(x, w1, w2, gelu, True)
+        ctx.save_for_backward(x, w1, w2, kept)
         return h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        x, w1, w2, z1, z2 = ctx.saved_tensors
+        x, w1, w2, kept = ctx.saved_tensors
         M, (I, H) = x.shape[0], w1.shape
         dx = dw1 = dw2 = None
         if ctx.needs_input_grad[0]:
@@ -198,8 +195,8 @@ class _GatedLinear(torch.autograd.Function):
                 n = _lib.lib().evo2_gated_linear_workspace_bytes(M, I, H)
                 ws = torch.empty(n, dtype=torch.uint8, device=x.device)
                 _lib.call("evo2_gated_linear_backward", _lib.ptr(g), g.stride(0), _lib.ptr(xr),
-                          xr.stride(0), _lib.ptr(a), _lib.ptr(b), a.stride(0), int(ctx.gelu),
-                          _lib.ptr(z1), _lib.ptr(z2), _lib.ptr(dx), _lib.ptr(dw1), _lib.ptr(dw2),
+                          xr.stride(0), _lib.ptr(a), _lib.ptr(b), a.stride(0),
+                          _lib.ptr(kept), _lib.ptr(dx), _lib.ptr(dw1), _lib.ptr(dw2),
                           _lib.ptr(ws), n, M, I, H, _lib.stream_of(xr))
         return (dx, dw1 if ctx.needs_input_grad[1] else None,
                 dw2 if ctx.needs_input_grad[2] else None, None)

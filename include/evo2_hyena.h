@@ -470,19 +470,18 @@ int evo2_bf16_stream_gated(const void *x, int64_t sx, const void *w1, const void
  *   dx = d1 w1 + d2 w2, dw1 = d1^T x, dw2 = d2^T x
  *   x (M, H) row stride sx, w1, w2 (I, H) row stride sw, h (M, I) row stride sh,
  *   dh (M, I) row stride sdh, dx (M, H), dw1, dw2 (I, H) contiguous, all bf16;
- *   z1, z2 (M, I) fp32 contiguous, written by the forward call where not NULL (both
- *   or neither) and read by the backward call.  I and H multiples of 8, rows 16-byte
- *   aligned.  dx may be NULL; dw1 and dw2 may be NULL together.  The backward call
+ *   kept: 6 M I bytes, written by the forward call where not NULL (z2 act'(z1) and
+ *   act(z1) to 24 bits) and read by the backward call.  I and H multiples of 8, rows
+ *   16-byte aligned.  dx may be NULL; dw1 and dw2 may be NULL together.  The backward call
  *   takes M >= 1 and a workspace of _workspace_bytes(M, I, H) bytes.
  */
 int64_t evo2_gated_linear_workspace_bytes(int64_t M, int64_t I, int64_t H);
 int evo2_gated_linear(const void *x, int64_t sx, const void *w1, const void *w2, int64_t sw,
-                      int32_t gelu, void *h, int64_t sh, float *z1, float *z2, int64_t M, int64_t I,
-                      int64_t H, void *stream);
+                      int32_t gelu, void *h, int64_t sh, void *kept, int64_t M, int64_t I, int64_t H,
+                      void *stream);
 int evo2_gated_linear_backward(const void *dh, int64_t sdh, const void *x, int64_t sx, const void *w1,
-                               const void *w2, int64_t sw, int32_t gelu, const float *z1,
-                               const float *z2, void *dx, void *dw1, void *dw2, void *workspace,
-                               int64_t workspace_bytes, int64_t M, int64_t I, int64_t H, void *stream);
+                               const void *w2, int64_t sw, const void *kept, void *dx, void *dw1,
+                               void *dw2, void *workspace, int64_t workspace_bytes, int64_t M, int64_t I, int64_t H, void *stream);
 
 /*
  * Softmax cross entropy of the logits h w^T (evo2_flash/model.py:343-348), which are
