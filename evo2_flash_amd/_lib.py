@@ -12,6 +12,7 @@ import os
 import threading
 
 import torch  # noqa: F401  (must precede the library load, see above)
+from torch.autograd.function import once_differentiable
 
 from .build import LIB_PATH
 
@@ -421,20 +422,33 @@ def overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(t):
     """A context in which t's device is the current one (launches go there)."""
-    if t.get_device() == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def rows16(t):
     """t (rows, n of a multiple of 8, 16-bit) with rows of unit stride that start
     on 16 bytes and do not overlap: itself, or a copy."""
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] \
-            and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    row, unit = t.stride()
+    if unit != 1 or row & 7 or row < t.shape[1] or t.data_ptr() & 15:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def once(backward):
+    """A backward pass that is not differentiable itself, as a static method.  (Where
+    no graph of it is asked for, torch's once_differentiable would only add its own
+    bookkeeping to calls that small steps wait for.)"""
+    guarded = once_differentiable(backward)
+
+    def call_backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return staticmethod(call_backward)
 
 
 def require_device(*tensors):

@@ -24,7 +24,6 @@ backward pass (csrc/packed_attention.hip), for scoring and training.
 """
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -358,61 +357,70 @@ def causal_prefill_attention(q, k, v, scale):
 
 def _head_rows(t):
     """t (T, heads, hd) as the packed kernels read it: unit last stride, rows that do
-    not overlap, 16-byte aligned; itself or a copy."""
-    if (t.stride(2) == 1 and t.shape[2] <= t.stride(0) < 1 << 23 and t.stride(0) % 8 == 0
-            and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    not overlap, 16-byte aligned; (itself or a copy, address, row and head stride)."""
+    row, head, unit = t.stride()
+    at = t.data_ptr()
+    if unit != 1 or (row | head) & 7 or at & 15 or not t.shape[2] <= row < 1 << 23:
+        t = t.clone(memory_format=torch.contiguous_format)
+        row, head, unit = t.stride()
+        at = t.data_ptr()
+    return t, at, row, head
 
 
 def _packed_forward(q, k, v, cu, scale, keep):
-    """(out, out_lo, lse): the attention's output and, to `keep`, what the backward pass
-    needs (else None)."""
+    """(out, kept): the attention's output and, to `keep`, what the backward pass needs
+    beside it, as bytes (what rounding took from the output (T, heads, hd) bf16, then
+    the rows' log-sum-exp (heads, T) fp32)."""
     T, heads, hd = q.shape
     out = torch.empty(T, heads, hd, dtype=q.dtype, device=q.device)
-    lo = lse = None
+    kept = lo = lse = None
     if keep:
-        lo = torch.empty_like(out)
-        lse = torch.empty(heads, T, dtype=torch.float32, device=q.device)
+        n = 2 * T * heads * hd
+        kept = torch.empty(n + 4 * T * heads, dtype=torch.uint8, device=q.device)
+        lo = kept.data_ptr()
+        lse = lo + n
     if T:
-        q, k, v = (_head_rows(t) for t in (q, k, v))
+        q, qp, qt, qh = _head_rows(q)
+        k, kp, kt, kh = _head_rows(k)
+        v, vp, vt, vh = _head_rows(v)
         with _lib.on_device(q):
-            _lib.call("evo2_packed_attention", _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k),
-                      k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1), _lib.ptr(cu),
-                      cu.shape[0] - 1, _lib.ptr(out), _lib.ptr(lo), _lib.ptr(lse), T, heads,
-                      k.shape[1], hd, scale, _lib.stream_of(q))
-    return out, lo, lse
+            _lib.call("evo2_packed_attention", qp, qt, qh, kp, kt, kh, vp, vt, vh, cu.data_ptr(),
+                      cu.shape[0] - 1, out.data_ptr(), lo, lse, T, heads, k.shape[1], hd, scale,
+                      _lib.stream_of(q))
+    return out, kept
+
+
+def _packed_backward(ctx, dout):
+    q, k, v, cu, out, kept = ctx.saved_tensors
+    T, heads, hd = q.shape
+    kv, nseq = k.shape[1], cu.shape[0] - 1
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    if T:
+        d, dp, dt, dh = _head_rows(dout)
+        q, qp, qt, qh = _head_rows(q)
+        k, kp, kt, kh = _head_rows(k)
+        v, vp, vt, vh = _head_rows(v)
+        lo = kept.data_ptr()
+        with _lib.on_device(q):
+            n = _lib.lib().evo2_packed_attention_workspace_bytes(T, nseq, heads, kv, hd)
+            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+            _lib.call("evo2_packed_attention_backward", dp, dt, dh, qp, qt, qh, kp, kt, kh, vp, vt,
+                      vh, cu.data_ptr(), nseq, out.data_ptr(), lo, lo + 2 * T * heads * hd,
+                      ws.data_ptr(), n, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, heads, kv,
+                      hd, ctx.scale, _lib.stream_of(q))
+    need = ctx.needs_input_grad
+    return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None)
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, scale):
-        out, lo, lse = _packed_forward(q, k, v, cu, scale, True)
-        ctx.save_for_backward(q, k, v, cu, out, lo, lse)
+        out, kept = _packed_forward(q, k, v, cu, scale, True)
+        ctx.save_for_backward(q, k, v, cu, out, kept)
         ctx.scale = scale
         return out
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, cu, out, lo, lse = ctx.saved_tensors
-        T, heads, hd = q.shape
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        if T:
-            d, q, k, v = (_head_rows(t) for t in (dout, q, k, v))
-            with _lib.on_device(q):
-                nseq = cu.shape[0] - 1
-                n = _lib.lib().evo2_packed_attention_workspace_bytes(T, nseq, heads, k.shape[1], hd)
-                ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-                _lib.call("evo2_packed_attention_backward", _lib.ptr(d), d.stride(0), d.stride(1),
-                          _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k), k.stride(0),
-                          k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1), _lib.ptr(cu),
-                          nseq, _lib.ptr(out), _lib.ptr(lo), _lib.ptr(lse), _lib.ptr(ws), n,
-                          _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), T, heads,
-                          k.shape[1], hd, ctx.scale, _lib.stream_of(q))
-        need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None,
-                None)
+    backward = _lib.once(_packed_backward)
 
 
 def packed_attention(q, k, v, cu_seqlens, scale):
@@ -430,7 +438,8 @@ def packed_attention(q, k, v, cu_seqlens, scale):
     products as bf16.  A key's infinite or NaN value also reaches the queries before it
     in its 64-row tile."""
     _lib.require_device(q, k, v, cu_seqlens)
-    if any(t.dim() != 3 or t.dtype != torch.bfloat16 for t in (q, k, v)):
+    bf = torch.bfloat16
+    if not (q.dim() == k.dim() == v.dim() == 3 and q.dtype == k.dtype == v.dtype == bf):
         raise ValueError("packed_attention takes bf16 q (T, heads, head_dim), k and v (T, kv_heads, "
                          "head_dim)")
     T, heads, hd = q.shape

@@ -83,6 +83,7 @@ __global__ __launch_bounds__(256) void loss_join_kernel(LossRows p, const float2
 // One row's logit n from the partial sums over K.
 __device__ __forceinline__ float loss_logit(const float *part, int64_t plane, int splits, int64_t at) {
   float z = 0.0f;
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) z += part[s * plane + at];
   return z;
 }

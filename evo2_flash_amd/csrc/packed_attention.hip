@@ -326,29 +326,6 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs p) {
     p.lse[static_cast<int64_t>(h) * p.T + begin + qi] = m + __builtin_amdgcn_logf(l);
 }
 
-// delta = do . o per row and head, from both halves of o: HD / 8 lanes a row.
-template <int HD>
-__global__ __launch_bounds__(256) void packed_delta_kernel(PackedArgs p) {
-  constexpr int CH = HD / 8;
-  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / CH;  // row * heads + head
-  const int c = 8 * (threadIdx.x % CH);
-  if (at >= static_cast<int64_t>(p.T) * p.heads) return;  // (whole groups of CH lanes)
-  const int64_t row = at / p.heads;
-  const int h = static_cast<int>(at - row * p.heads);
-  const au32x4_t d = *reinterpret_cast<const au32x4_t *>(p.d.p + row * p.d.st + h * p.d.sh + c);
-  const au32x4_t a = *reinterpret_cast<const au32x4_t *>(p.o + at * HD + c);
-  const au32x4_t b = *reinterpret_cast<const au32x4_t *>(p.olo + at * HD + c);
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    s = fmaf(lo_bf(d[i]), lo_bf(a[i]) + lo_bf(b[i]), s);
-    s = fmaf(hi_bf(d[i]), hi_bf(a[i]) + hi_bf(b[i]), s);
-  }
-#pragma unroll
-  for (int o = 1; o < CH; o <<= 1) s += __shfl_xor(s, o);
-  if (c == 0) p.delta[static_cast<int64_t>(h) * p.T + row] = s;
-}
-
 template <int HD>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
   __shared__ __align__(16) bf16_t k0[p_tile<HD>(P_TR)], k1[p_tile<HD>(P_TR)], v0[p_tile<HD>(P_TR)], v1[p_tile<HD>(P_TR)];
@@ -378,7 +355,20 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
   p_own<HD>(q, p.q, row, h, g);
   p_own<HD>(d, p.d, row, h, g);
   const float lse = p.lse[static_cast<int64_t>(h) * p.T + row];
-  const float delta = p.delta[static_cast<int64_t>(h) * p.T + row];
+  // delta = do . o of the wave's rows, from both parts of o; the dk, dv launch reads it
+  float delta = 0.0f;
+  {
+    abf16x8_t o[HD / 16], lo[HD / 16];
+    p_own<HD>(o, Rows{p.o, static_cast<int64_t>(p.heads) * HD, HD}, row, h, g);
+    p_own<HD>(lo, Rows{p.olo, static_cast<int64_t>(p.heads) * HD, HD}, row, h, g);
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        delta = fmaf(static_cast<float>(d[kk][j]), static_cast<float>(o[kk][j]) + static_cast<float>(lo[kk][j]), delta);
+  }
+  delta += __shfl_xor(delta, 32);
+  if (g == 0 && qi < len) p.delta[static_cast<int64_t>(h) * p.T + row] = delta;
   pf32x16_t acc[HD / 32] = {};
 
   auto block = [&](int b, const bf16_t *ks, const bf16_t *vs, bf16_t *kn, bf16_t *vn)
@@ -490,7 +480,8 @@ __global__ __launch_bounds__(64 * P_KW, 1) void packed_dkv_kernel(PackedArgs p) 
     const int qb0 = r0 + cb * P_TR;
     if (++cb == nqb) cb = 0;
     if (wk0 >= len) return;  // wave-uniform: no keys
-#pragma unroll 1
+    // (both tiles at once where the registers allow it)
+#pragma unroll HD == 64 ? 2 : 1
     for (int u = 0; u < 2; ++u) {
       const int qt0 = qb0 + 32 * u;
       if (qt0 < wk0) continue;  // wave-uniform: queries before all of the wave's keys
@@ -625,9 +616,8 @@ static void launch_forward(PackedArgs a, hipStream_t st) {
 
 template <int HD>
 static void launch_backward(PackedArgs a, hipStream_t st) {
-  const int64_t lanes = static_cast<int64_t>(a.T) * a.heads * (HD / 8);
-  hipLaunchKernelGGL((packed_delta_kernel<HD>), dim3(static_cast<unsigned>(cdiv(lanes, 256))), dim3(256), 0, st, a);
-  const int tiles = a.tiles;
+  a.items = a.tiles * a.heads;  // first: it writes delta
+  hipLaunchKernelGGL((packed_dq_kernel<HD>), dim3(a.items + P_FILL), dim3(256), 0, st, a);
   a.tiles = a.T / P_KG + a.nseq;
   if (a.part) {
     a.items = a.tiles * a.heads;
@@ -638,9 +628,6 @@ static void launch_backward(PackedArgs a, hipStream_t st) {
     a.items = a.tiles * a.kv;
     hipLaunchKernelGGL((packed_dkv_kernel<HD, false>), dim3(a.items + P_FILL), dim3(64 * P_KW), 0, st, a);
   }
-  a.tiles = tiles;
-  a.items = a.tiles * a.heads;
-  hipLaunchKernelGGL((packed_dq_kernel<HD>), dim3(a.items + P_FILL), dim3(256), 0, st, a);
 }
 
 }  // namespace evo2

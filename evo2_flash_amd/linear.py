@@ -9,7 +9,6 @@ from typing import Optional
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 from torch.utils._device import DeviceContext
 
 from . import _lib
@@ -163,12 +162,34 @@ def _gated_forward(x, w1, w2, gelu, keep):
     h = torch.empty(M, I, dtype=x.dtype, device=x.device)
     kept = torch.empty(3, M, I, dtype=torch.int16, device=x.device) if keep else None
     if M:
-        xr, (a, b) = _lib.rows16(x), _weight_rows(w1, w2)
-        with _lib.on_device(xr):
-            _lib.call("evo2_gated_linear", _lib.ptr(xr), xr.stride(0), _lib.ptr(a), _lib.ptr(b),
-                      a.stride(0), int(gelu), _lib.ptr(h), h.stride(0), _lib.ptr(kept), M, I, H,
-                      _lib.stream_of(xr))
+        x = _lib.rows16(x)
+        w1, w2 = _weight_rows(w1, w2)
+        with _lib.on_device(x):
+            _lib.call("evo2_gated_linear", x.data_ptr(), x.stride(0), w1.data_ptr(), w2.data_ptr(),
+                      w1.stride(0), int(gelu), h.data_ptr(), I, _lib.ptr(kept), M, I, H,
+                      _lib.stream_of(x))
     return h, kept
+
+
+def _gated_backward(ctx, dh):
+    x, w1, w2, kept = ctx.saved_tensors
+    M, (I, H) = x.shape[0], w1.shape
+    need = ctx.needs_input_grad
+    dx = x.new_empty(M, H) if need[0] else None
+    dw1 = dw2 = None
+    if need[1] or need[2]:
+        dw1, dw2 = ((w.new_empty if M else w.new_zeros)((I, H)) for w in (w1, w2))
+    if M:
+        dh, x = _lib.rows16(dh), _lib.rows16(x)
+        w1, w2 = _weight_rows(w1, w2)
+        with _lib.on_device(x):
+            n = _lib.lib().evo2_gated_linear_workspace_bytes(M, I, H)
+            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+            _lib.call("evo2_gated_linear_backward", dh.data_ptr(), dh.stride(0), x.data_ptr(),
+                      x.stride(0), w1.data_ptr(), w2.data_ptr(), w1.stride(0), kept.data_ptr(),
+                      _lib.ptr(dx), _lib.ptr(dw1), _lib.ptr(dw2), ws.data_ptr(), n, M, I, H,
+                      _lib.stream_of(x))
+    return dx, dw1 if need[1] else None, dw2 if need[2] else None, None
 
 
 class _GatedLinear(torch.autograd.Function):
@@ -178,28 +199,7 @@ class _GatedLinear(torch.autograd.Function):
         ctx.save_for_backward(x, w1, w2, kept)
         return h
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh):
-        x, w1, w2, kept = ctx.saved_tensors
-        M, (I, H) = x.shape[0], w1.shape
-        dx = dw1 = dw2 = None
-        if ctx.needs_input_grad[0]:
-            dx = torch.empty(M, H, dtype=x.dtype, device=x.device)
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            make = torch.empty if M else torch.zeros
-            dw1, dw2 = (make(I, H, dtype=x.dtype, device=x.device) for _ in range(2))
-        if M:
-            g, xr, (a, b) = _lib.rows16(dh), _lib.rows16(x), _weight_rows(w1, w2)
-            with _lib.on_device(xr):
-                n = _lib.lib().evo2_gated_linear_workspace_bytes(M, I, H)
-                ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-                _lib.call("evo2_gated_linear_backward", _lib.ptr(g), g.stride(0), _lib.ptr(xr),
-                          xr.stride(0), _lib.ptr(a), _lib.ptr(b), a.stride(0),
-                          _lib.ptr(kept), _lib.ptr(dx), _lib.ptr(dw1), _lib.ptr(dw2),
-                          _lib.ptr(ws), n, M, I, H, _lib.stream_of(xr))
-        return (dx, dw1 if ctx.needs_input_grad[1] else None,
-                dw2 if ctx.needs_input_grad[2] else None, None)
+    backward = _lib.once(_gated_backward)
 
 
 def gated_linear(x, w1, w2, gelu):
@@ -211,21 +211,22 @@ def gated_linear(x, w1, w2, gelu):
     products and the activation are fp32 and the result is rounded once (`gated`
     rounds each step, as the library's separate operators do)."""
     _lib.require_device(x, w1, w2)
-    if any(t.dtype != torch.bfloat16 for t in (x, w1, w2)):
+    if not x.dtype == w1.dtype == w2.dtype == torch.bfloat16:
         raise ValueError(f"gated_linear takes bf16 x, w1, w2, got {x.dtype}, {w1.dtype}, {w2.dtype}")
     if (w1.dim() != 2 or w1.shape != w2.shape or x.dim() < 1 or x.shape[-1] != w1.shape[1]):
         raise ValueError(f"gated_linear: shapes x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 "
                          f"{tuple(w2.shape)} do not match")
-    if any(n == 0 or n % 8 for n in w1.shape):
+    I, H = w1.shape
+    if I == 0 or H == 0 or (I | H) & 7:
         raise ValueError(f"gated_linear takes weights of multiples of 8, got {tuple(w1.shape)}")
     if not x.device == w1.device == w2.device:
         raise ValueError(f"gated_linear: operands on {x.device}, {w1.device}, {w2.device}")
-    rows = x.reshape(-1, x.shape[-1])
+    rows = x if x.dim() == 2 else x.reshape(-1, H)
     if torch.is_grad_enabled() and (rows.requires_grad or w1.requires_grad or w2.requires_grad):
         h = _GatedLinear.apply(rows, w1, w2, bool(gelu))
     else:
         h = _gated_forward(rows, w1, w2, gelu, False)[0]
-    return h.view(*x.shape[:-1], w1.shape[0])
+    return h if x.dim() == 2 else h.view(*x.shape[:-1], I)
 
 
 __all__ = ["linear", "gated", "gated_linear", "plain", "STREAM_ROWS"]

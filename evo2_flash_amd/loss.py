@@ -8,39 +8,54 @@ result does not depend on timing).
 """
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 _REDUCTIONS = ("none", "sum", "mean")
 
 
-def _workspace(T, V, H, backward, device):
-    n = _lib.lib().evo2_linear_loss_workspace_bytes(T, V, H, int(backward))
-    return torch.empty(n, dtype=torch.uint8, device=device)
-
-
 def _forward(hidden, weight, targets, ignore_index, reduction):
     """(nll (T,), lse (T,), loss (), count ()) fp32; loss and count None with "none"."""
     T, (V, H) = hidden.shape[0], weight.shape
-    dev = hidden.device
-    nll, lse = torch.empty(2, T, dtype=torch.float32, device=dev).unbind(0)
+    dev, f32 = hidden.device, torch.float32
+    nll, lse = torch.empty(T, dtype=f32, device=dev), torch.empty(T, dtype=f32, device=dev)
     loss = count = None
     if reduction:
-        loss, count = torch.empty(2, dtype=torch.float32, device=dev).unbind(0)
+        loss, count = torch.empty((), dtype=f32, device=dev), torch.empty((), dtype=f32, device=dev)
     if T == 0:
         if reduction:
             loss.fill_(0.0 if reduction == 1 else float("nan"))
             count.zero_()
         return nll, lse, loss, count
-    h, w = _lib.rows16(hidden), _lib.rows16(weight)
-    with _lib.on_device(h):
-        ws = _workspace(T, V, H, False, dev)
-        _lib.call("evo2_linear_loss", _lib.ptr(h), h.stride(0), _lib.ptr(w), w.stride(0),
-                  _lib.ptr(targets), ignore_index, reduction, _lib.ptr(nll), _lib.ptr(lse),
-                  _lib.ptr(loss), _lib.ptr(count), _lib.ptr(ws), ws.numel(), T, V, H,
-                  _lib.stream_of(h))
+    hidden, weight = _lib.rows16(hidden), _lib.rows16(weight)
+    with _lib.on_device(hidden):
+        n = _lib.lib().evo2_linear_loss_workspace_bytes(T, V, H, 0)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _lib.call("evo2_linear_loss", hidden.data_ptr(), hidden.stride(0), weight.data_ptr(),
+                  weight.stride(0), targets.data_ptr(), ignore_index, reduction, nll.data_ptr(),
+                  lse.data_ptr(), _lib.ptr(loss), _lib.ptr(count), ws.data_ptr(), n, T, V, H,
+                  _lib.stream_of(hidden))
     return nll, lse, loss, count
+
+
+def _backward(ctx, grad):
+    hidden, weight, targets, lse, count = ctx.saved_tensors
+    T, (V, H) = hidden.shape[0], weight.shape
+    need = ctx.needs_input_grad
+    dh = hidden.new_empty((T, H)) if need[0] else None
+    dw = (weight.new_empty if T else weight.new_zeros)((V, H)) if need[1] else None
+    if T:
+        hidden, weight = _lib.rows16(hidden), _lib.rows16(weight)
+        grad = grad.to(torch.float32)
+        with _lib.on_device(hidden):
+            n = _lib.lib().evo2_linear_loss_workspace_bytes(T, V, H, 1)
+            ws = torch.empty(n, dtype=torch.uint8, device=hidden.device)
+            _lib.call("evo2_linear_loss_backward", hidden.data_ptr(), hidden.stride(0),
+                      weight.data_ptr(), weight.stride(0), targets.data_ptr(), ctx.ignore_index,
+                      lse.data_ptr(), grad.data_ptr(), grad.stride(0) if grad.dim() else 0,
+                      _lib.ptr(count), _lib.ptr(dh), _lib.ptr(dw), ws.data_ptr(), n, T, V, H,
+                      _lib.stream_of(hidden))
+    return dh, dw, None, None, None
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -51,28 +66,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ctx.ignore_index = ignore_index
         return loss if reduction else nll
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        hidden, weight, targets, lse, count = ctx.saved_tensors
-        T, (V, H) = hidden.shape[0], weight.shape
-        dev = hidden.device
-        dh = dw = None
-        if ctx.needs_input_grad[0]:
-            dh = torch.empty(T, H, dtype=hidden.dtype, device=dev)
-        if ctx.needs_input_grad[1]:
-            dw = (torch.empty if T else torch.zeros)(V, H, dtype=weight.dtype, device=dev)
-        if T:
-            h, w = _lib.rows16(hidden), _lib.rows16(weight)
-            grad = grad.to(torch.float32)
-            with _lib.on_device(h):
-                ws = _workspace(T, V, H, True, dev)
-                _lib.call("evo2_linear_loss_backward", _lib.ptr(h), h.stride(0), _lib.ptr(w),
-                          w.stride(0), _lib.ptr(targets), ctx.ignore_index, _lib.ptr(lse),
-                          _lib.ptr(grad), grad.stride(0) if grad.dim() else 0, _lib.ptr(count),
-                          _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(ws), ws.numel(), T, V, H,
-                          _lib.stream_of(h))
-        return dh, dw, None, None, None
+    backward = _lib.once(_backward)
 
 
 def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="mean"):
@@ -105,7 +99,7 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="
         raise ValueError(f"linear_cross_entropy: operands on {hidden.device}, {weight.device}, "
                          f"{targets.device}")
     shape = targets.shape
-    h = hidden.reshape(-1, hidden.shape[-1])
+    h = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     t = targets.reshape(-1).to(torch.int64).contiguous()
     red = _REDUCTIONS.index(reduction)
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
