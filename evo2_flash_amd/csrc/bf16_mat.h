@@ -185,7 +185,8 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     }
     // K-contiguous rows at a power-of-two stride put all of a slice's lines on a few
     // cache channels: workgroups of different rows start up to seven slices apart
-    // (4096 x 32768 x 4096: 1000 -> 925 us; further apart they lose the L2's sharing)
+    // (gated, 8192 x 11264 x 4096: 1566 -> 1330 us; further apart they lose the L2's
+    // sharing, 1890 with the starts spread over all of K)
     int s = ds + (FORM == MAT_NT && KT >= 16 ? dbm & 7 : 0);
     if (s >= KT) s -= KT;
     s += dsp * KT;
@@ -555,9 +556,20 @@ struct MatPlan {
   int tm, tiles_m, tiles_n, splits, kt;
 };
 
+// The tile height and split of least time: rounds of tiles over the CUs, times what a
+// tile costs -- us per slice and us at its end, measured over 512 to 10240 of K -- and
+// where few tiles let K be split, the partial sums' second launch and their bytes
+// there and back.  Measured, us for tm 1 / 2 / 3 / 4: NT 777 x 49999 x 1920 238 / 209
+// / 191 / 214; gated 777 x 11264 x 4096 187 / 162 / 152 / 231, 2048 x 5120 x 1920 131
+// / 114 / 124 / 177; NN 2048 x 1920 x 10240, split by 1, 2, 2, 4, 111 / 93 / 102 / 91;
+// TN 512 x 4096 x 32768, split by 2, 4, -, 8, 210 / 183 / - / 147 and 49999 x 1920 x
+// 777 296 / 236 / - / 206.
 // M: rows of one of `pair` outputs; slices: of K; width: output columns per tile.
 inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int pair, int width,
                         bool may_split) {
+  const bool gated = width < MAT_BN;  // (four 16-bit outputs rather than one)
+  const double slice[5] = {0, 0.60, form == MAT_TN ? 1.05 : 0.90, 1.30, 1.72};
+  const double end[5] = {0, gated ? 7.0 : 4.0, gated ? 11.0 : 6.0, gated ? 19.0 : 9.0, gated ? 25.0 : 12.0};
   MatPlan best{};
   double least = 1e300;
   for (int tm : {4, 3, 2, 1}) {
@@ -569,10 +581,8 @@ inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int 
     const int64_t kt = cdiv(cdiv(slices, splits), nst) * nst;
     splits = std::max<int64_t>(1, cdiv(slices, kt));
     const double rounds = double(cdiv(tiles * splits, MAT_CUS));
-    double cost = rounds * kt * (tm + 1.3);
-    // the partial sums' second launch, and their bytes there and back (in the time
-    // of 0.16 us that a slice takes per unit of tm + 1.3)
-    if (splits > 1) cost += 20.0 + double(splits) * M * pair * N * 1.25e-5;
+    double cost = rounds * (kt * slice[tm] + end[tm]);
+    if (splits > 1) cost += 6.0 + double(splits) * M * pair * N * 1.3e-6;
     if (cost < least - 1e-9) {
       least = cost;
       best = MatPlan{tm, static_cast<int>(tm_tiles), static_cast<int>(tn_tiles), static_cast<int>(splits),

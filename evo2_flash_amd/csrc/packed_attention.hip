@@ -274,6 +274,12 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs p) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(ks, u, kk, lr, g), q[kk], s[u], 0, 0, 0);
+    // the first half of the values' fragments: on their way during the softmax
+    abf16x8_t vf[2][HD / 32];
+#pragma unroll
+    for (int kp = 0; kp < 2; ++kp)
+#pragma unroll
+      for (int e = 0; e < HD / 32; ++e) vf[kp][e] = p_cols<HD>(vs, e, kp, lane);
     if (kb0 + P_TR - 1 > wq0) {  // wave-uniform: some keys come after some queries
       const int lim = qi - kb0 - 4 * g;
 #pragma unroll
@@ -310,7 +316,8 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs p) {
       const abf16x8_t pb = p_pack(s[kp >> 1], kp & 1);
 #pragma unroll
       for (int e = 0; e < HD / 32; ++e)
-        acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_cols<HD>(vs, e, kp, lane), pb, acc[e], 0, 0, 0);
+        acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kp < 2 ? vf[kp][e] : p_cols<HD>(vs, e, kp, lane), pb,
+                                                         acc[e], 0, 0, 0);
     }
   };
   for (int b = 0; b < nkb; b += 2) {
