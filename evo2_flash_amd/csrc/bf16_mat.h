@@ -113,9 +113,10 @@ __device__ __forceinline__ float loss_weight(const MatArgs &p, int64_t m, int64_
   return p.weighted ? p.grad[m * p.sgrad] : 1.0f;
 }
 
+// (a mean of no rows has no gradient)
 __device__ __forceinline__ float mat_factor(const float *num, const float *den) {
   const float n = num ? *num : 1.0f;
-  return den ? n / *den : n;
+  return !den ? n : *den == 0.0f ? 0.0f : n / *den;
 }
 
 template <int FORM, int TM, int EPI>

@@ -628,7 +628,8 @@ static void launch_backward(PackedArgs a, hipStream_t st) {
   a.tiles = a.T / P_KG + a.nseq;
   if (a.part) {
     a.items = a.tiles * a.heads;
-    hipLaunchKernelGGL((packed_dkv_kernel<HD, true>), dim3(a.items), dim3(64 * P_KW), 0, st, a);
+    if (a.items > 0)  // (fewer than P_KG rows and no sequences: the join clears them)
+      hipLaunchKernelGGL((packed_dkv_kernel<HD, true>), dim3(a.items), dim3(64 * P_KW), 0, st, a);
     const int64_t rows = static_cast<int64_t>(a.T) * a.kv * (HD / 8);
     hipLaunchKernelGGL((packed_join_kernel<HD>), dim3(static_cast<unsigned>(cdiv(rows, 256))), dim3(256), 0, st, a);
   } else {

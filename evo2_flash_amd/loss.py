@@ -75,8 +75,9 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="
 
     hidden (..., H) and weight (V, H) bf16 on one device, H a multiple of 8; targets
     (...) of an integer type.  Rows whose target is `ignore_index` have loss 0 and no
-    gradient; a target outside [0, V) otherwise makes its row's loss and gradient NaN
-    (nothing is read through it).  reduction: "none" (fp32 losses of targets' shape:
+    gradient (but their infinite or NaN hidden values reach the weight's, times 0); a target
+    outside [0, V) otherwise makes its row's loss and gradient NaN (nothing is read
+    through it).  reduction: "none" (fp32 losses of targets' shape:
     the negative log-likelihoods), "sum" or "mean" over the rows that are not ignored
     (fp32 scalar; the mean of no rows is NaN).  The logits are fp32 sums of the bf16
     products and never rounded."""

@@ -24,6 +24,13 @@ kernel at head_dim 128 and in torch otherwise; rotary and the page writes are
 one launch (attention.py).  The projections and MLPs run on the weight-streaming
 kernel at decode batch sizes and in torch otherwise (linear.py).
 
+Scoring (Evo2DecodeModel.score) reduces the head's logits to log-likelihoods without
+keeping them (loss.py).  Training (training_loss) takes gradients through the
+attention layers above the last Hyena mixer -- layer 31 of the 7B map -- the final
+norm and the head, on features of the layers below that stay as they are: packed
+attention, the gated product and the cross entropy run on this build's kernels in both
+directions, the projections on the library's, the norms and the rotary in torch.
+
 Weights are random, seeded, in the benchmark's distributions.
 """
 
@@ -31,9 +38,11 @@ import torch
 from torch import nn
 
 from .attention import (PAGE, PagedKVCache, causal_prefill_attention, check_block_table,
-                        paged_decode_attention, prefill_attention_rows, rotary_decode,
-                        rotary_prefill, shared_prefix_pages, workspace as attention_workspace)
-from .linear import gated, linear, plain
+                        packed_attention, paged_decode_attention, prefill_attention_rows,
+                        rotary_decode, rotary_prefill, shared_prefix_pages,
+                        workspace as attention_workspace)
+from .linear import gated, gated_linear, linear, plain
+from .loss import linear_cross_entropy
 from .metadata import build_metadata
 from .mixers import Linear, load_mixer_params, make_mixer, set_forward_context
 from .norm import Evo2RMSNorm
@@ -79,6 +88,23 @@ class Evo2MLP(nn.Module):
         if not _bare(self.l3, Linear):
             return self.forward(x) + residual
         return linear(self._product(x), self.l3.weight, self.l3.bias, residual=residual)
+
+    def forward_train(self, x):
+        """forward(x) with gradients: the product is one launch (projections with a bias
+        or hooks are called as modules)."""
+        if all(_bare(m, Linear) and m.bias is None for m in (self.l1, self.l2)):
+            h = gated_linear(x, self.l1.weight, self.l2.weight, self.use_act)
+        else:
+            h = self._product(x)
+        out, _ = self.l3(h)
+        return out
+
+
+def _norm_train(norm, x):
+    """norm(x) with gradients: Evo2RMSNorm's rounding points (bf16 after every op) in
+    torch's operators."""
+    size = x.float().norm(dim=-1, keepdim=True).to(x.dtype) * norm.hidden_size ** -0.5
+    return norm.weight * (x / (size + norm.eps))
 
 
 def rotary_neox(x, positions, inv_freq, factor):
@@ -154,6 +180,16 @@ class Evo2Attention(nn.Module):
         return o
 
 
+    def forward_train(self, x, cu_seqlens, positions):
+        """x (T, H): packed sequences (rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1) at
+        `positions` (T,), with gradients; the KV pages are neither read nor written."""
+        qkv, _ = self.qkv_proj(x)
+        q, k, v = self._rotated(qkv, positions)
+        out = packed_attention(q, k, v, cu_seqlens, self.hd ** -0.5)
+        o, _ = self.o_proj(out.reshape(-1, self.heads * self.hd))
+        return o
+
+
 class Evo2DecoderLayer(nn.Module):
     """pre_norm -> mixer -> post_norm (+ residual) -> MLP (+ residual)
     (model.py:156-200)."""
@@ -195,6 +231,14 @@ class Evo2DecoderLayer(nn.Module):
             m = self.mixer(pre, token_ids=token_ids)
         post, x = self.post_norm(m, x)
         return self._mlp(post, x)
+
+
+    def forward_train(self, x, cu_seqlens, positions):
+        """An attention layer over packed sequences, with gradients."""
+        if self.kind != "attn":
+            raise NotImplementedError(f"no gradients through Hyena mixers ({self.kind})")
+        x = x + self.mixer.forward_train(_norm_train(self.pre_norm, x), cu_seqlens, positions)
+        return x + self.mlp.forward_train(_norm_train(self.post_norm, x))
 
 
 class Evo2DecodeModel(nn.Module):
@@ -300,11 +344,19 @@ class Evo2DecodeModel(nn.Module):
         kernels write each sequence's final state and windows into its
         blocks) and KV pages for positions 0..L-1.  Returns the logits of the
         last position (B, vocab)."""
+        L = tokens.shape[1]
+        last = [x.view(n, L, -1)[:, -1] for _, n, x in self._prompts(tokens, chunk_seqs,
+                                                                     self.layers)]
+        h = self.norm(torch.cat(last))
+        return linear(h, self.embed)
+
+    def _prompts(self, tokens, chunk_seqs, layers):
+        """Prompts tokens (B, L) through `layers` (the first ones), in groups of
+        `chunk_seqs` sequences: (first sequence, how many, their rows (n * L, H))."""
         B, L = tokens.shape
         if B > self.max_batch or L > self.max_pages * PAGE:
             raise ValueError(f"prompts ({B}, {L}) exceed the model's {self.max_batch} sequences "
                              f"of {self.max_pages * PAGE} positions")
-        last = []
         for b0 in range(0, B, chunk_seqs):
             n = min(chunk_seqs, B - b0)
             tok = tokens[b0:b0 + n].reshape(-1)
@@ -312,11 +364,52 @@ class Evo2DecodeModel(nn.Module):
                                has_init=[0] * n, device=tokens.device)
             x = self.embed[tok]
             with set_forward_context(m):
-                for layer in self.layers:
+                for layer in layers:
                     x = layer.forward_prefill(x, tok, n, L, self.block_table[b0:b0 + n])
-            last.append(x.view(n, L, -1)[:, -1])
-        h = self.norm(torch.cat(last))
-        return linear(h, self.embed)
+            yield b0, n, x
+
+    @torch.no_grad()
+    def score(self, tokens, chunk_seqs=8):
+        """Log-likelihoods of prompts tokens (B, L) of sequences 0..B-1: (B, L - 1) fp32,
+        entry l that of token l + 1 given the tokens up to l.  The prompts run as in
+        `prefill` (fresh Hyena states, KV pages written); no logits are kept."""
+        B, L = tokens.shape
+        out = torch.empty(B, max(L - 1, 0), dtype=torch.float32, device=tokens.device)
+        for b0, n, x in self._prompts(tokens, chunk_seqs, self.layers):
+            h = self.norm(x).view(n, L, -1)[:, :-1]
+            out[b0:b0 + n] = -linear_cross_entropy(h, self.embed, tokens[b0:b0 + n, 1:],
+                                                   reduction="none")
+        return out
+
+    def trained_layers(self):
+        """The layers that training_loss takes gradients through: the attention layers
+        above the last Hyena mixer."""
+        n = len(self.layers)
+        while n and self.layers[n - 1].kind == "attn":
+            n -= 1
+        return list(self.layers[n:])
+
+    def training_loss(self, tokens, targets=None, ignore_index=-100, chunk_seqs=8):
+        """Mean cross entropy of sequences tokens (B, L) against targets (B, L) (by
+        default each sequence's next tokens; entries of ignore_index do not count, so
+        shorter sequences are padded behind), with gradients in those parameters of
+        `trained_layers()`, the final norm and the head (`embed`, as the head alone)
+        that require them.  The layers below run as in `prefill`, without gradients."""
+        B, L = tokens.shape
+        if targets is None:
+            targets = torch.full_like(tokens, ignore_index)
+            targets[:, :-1] = tokens[:, 1:]
+        top = self.trained_layers()
+        with torch.no_grad():
+            below = list(self._prompts(tokens, chunk_seqs,
+                                       self.layers[:len(self.layers) - len(top)]))
+        x = torch.cat([rows for _, _, rows in below])
+        cu = torch.arange(0, B * L + 1, L, dtype=torch.int32, device=x.device)
+        positions = torch.arange(L, device=x.device).repeat(B)
+        for layer in top:
+            x = layer.forward_train(x, cu, positions)
+        return linear_cross_entropy(_norm_train(self.norm, x), self.embed, targets.reshape(-1),
+                                    ignore_index=ignore_index)
 
     def prefill_shared(self, prompt):
         """Prefill one prompt (L,) with L = shared_prefix into sequence 0 and

@@ -79,3 +79,110 @@ def test_against_64_bits(M, I, H, gelu):
     with torch.no_grad():
         _check({"h": gated_linear(x, w1, w2, gelu)}, want, "forward")
     _check(_grads(x, w1, w2, gelu, dh), want, "training")
+
+
+def test_gradient_against_differences():
+    """The product is quadratic in x and in each weight linear (identity): along a
+    direction exact in bf16, central differences are the gradient but for the outputs'
+    roundings, u |h| each."""
+    M, I, H = 40, 136, 72
+    x, w1, w2, dh = _case(M, I, H, seed=7)
+    got = _grads(x, w1, w2, False, dh)
+    g = torch.Generator().manual_seed(8)
+    for i, n in enumerate(("dx", "dw1", "dw2")):
+        ops = [x, w1, w2]
+        step = (torch.randint(0, 2, ops[i].shape, generator=g) * 2 - 1).to(DEV) * 2.0 ** -3
+        lo, hi = ((ops[i].float() + s * step).to(BF) for s in (-1, 1))
+        with torch.no_grad():
+            a, b = (gated_linear(*ops[:i], t, *ops[i + 1:], False).double() for t in (lo, hi))
+        # the steps as bf16 holds them
+        want = ((b - a) * dh.double()).sum()
+        moved = (hi.double() - lo.double())
+        have = (got[n].double() * moved).sum()
+        noise = U * ((a.abs() + b.abs()) * dh.double().abs()).square().sum().sqrt()
+        if n == "dx":  # quadratic: the midpoint is not x where the two steps round apart
+            noise = noise + ((lo.double() + hi.double()) / 2 - x.double()).abs().max() * 64 * I
+        assert abs(have - want) <= 4 * noise + U * (got[n].double() * moved).norm() * 2, n
+
+
+@pytest.mark.parametrize("gelu", [False, True])
+def test_near_the_streamed_product(gelu):
+    """gated's values (each step rounded to bf16): within three roundings."""
+    x, w1, w2, _ = _case(5, 640, 264, seed=9)
+    a, b = gated_linear(x, w1, w2, gelu).double(), gated(x, w1, w2, gelu).double()
+    z1, z2 = (x.double() @ w.double().t() for w in (w1, w2))
+    assert ((a - b).abs() <= 4 * U * (z1.abs() + 0.2) * z2.abs() + 4 * U * a.abs()).all()
+
+
+def test_forms_of_call():
+    """Leading dimensions, strided and unaligned operands, weights of two strides, an
+    expanded upstream gradient, one gradient asked for, no rows: the same values."""
+    M, I, H = 24, 136, 72
+    x, w1, w2, dh = _case(M, I, H, seed=11)
+    want = _grads(x, w1, w2, True, dh)
+    wide = torch.zeros(I, H + 16, dtype=BF, device=DEV)
+    wide[:, 8:H + 8] = w2
+    odd = torch.zeros(M * H + 3, dtype=BF, device=DEV)[3:].view(M, H).copy_(x)
+    got = _grads(odd, w1, wide[:, 8:H + 8], True, dh.t().contiguous().t())
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    lead = gated_linear(x.view(2, 3, 4, H), w1, w2, True)
+    assert lead.shape == (2, 3, 4, I) and torch.equal(lead.view(M, I), want["h"])
+    xs = x.clone().requires_grad_()
+    gated_linear(xs, w1, w2, True).sum().backward()
+    ones = _grads(x, w1, w2, True, torch.ones_like(dh))
+    assert torch.equal(xs.grad, ones["dx"])
+    for i, n in enumerate(("dx", "dw1", "dw2")):
+        ops = [x.clone(), w1.clone(), w2.clone()]
+        ops[i].requires_grad_()
+        gated_linear(*ops, True).backward(dh)
+        assert torch.equal(ops[i].grad, want[n]), n
+    w = w1.clone().requires_grad_()
+    none = gated_linear(x[:0], w, w2, False)
+    assert none.shape == (0, I) and not torch.autograd.grad(none.sum(), w)[0].any()
+    # the same weight twice: its gradient is both
+    both = gated_linear(x, w, w, False)
+    got = torch.autograd.grad(both, w, dh)[0]
+    twice = _grads(x, w1, w1, False, dh)
+    assert ((got.float() - twice["dw1"].float() - twice["dw2"].float()).abs()
+            <= 2 * U * got.float().abs() + 1e-30).all()
+
+
+def test_nothing_spreads_between_rows():
+    """A row of NaN or infinities reaches its own outputs only (and the weights'
+    gradients)."""
+    x, w1, w2, dh = _case(130, 136, 72, seed=12)
+    want = _grads(x, w1, w2, True, dh)
+    x[64], x[65, 3] = float("nan"), float("inf")
+    got = _grads(x, w1, w2, True, dh)
+    rows = torch.ones(130, dtype=torch.bool, device=DEV)
+    rows[64:66] = False
+    for n in ("h", "dx"):
+        assert torch.equal(got[n][rows], want[n][rows]), n
+    assert got["h"][64].isnan().all()
+
+
+def test_repeats_bit_for_bit_in_a_graph():
+    """Replays of a captured forward and backward pass, with eager work between, give the
+    eager bits; the split sums (few tiles) too."""
+    for M, I, H in ((300, 264, 328), (5, 1920, 640)):
+        x, w1, w2, dh = _case(M, I, H, seed=13)
+        leaves = [t.detach().clone().requires_grad_() for t in (x, w1, w2)]
+
+        def step():
+            h = gated_linear(*leaves, True)
+            return (h.detach(), *torch.autograd.grad(h, leaves, dh))
+
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+            with torch.cuda.graph(graph, stream=side):
+                outs = step()
+        torch.cuda.synchronize()
+        for rep in range(3):
+            with torch.no_grad():
+                leaves[0].copy_(x * (rep + 1))
+            graph.replay()
+            torch.cuda.synchronize()
+            eager = _grads(x * (rep + 1), w1, w2, True, dh)
+            assert all(torch.equal(a, b) for a, b in zip(outs, eager.values())), (M, rep)

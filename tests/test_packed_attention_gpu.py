@@ -124,3 +124,113 @@ def test_rows_outside_the_sequences(pad):
     _check(got, want, pad)
     for n, t in got.items():
         assert not t[out.to(DEV)].any(), n
+
+
+def test_gradient_against_differences():
+    """The output is linear in v: along a direction exact in bf16 the difference is the
+    gradient but for the outputs' roundings.  In q and k along a small direction, the
+    second order below the roundings."""
+    q, k, v, d, cu = _case([40, 1, 90], 4, 2, 64, seed=21)
+    got = _grads(q, k, v, d, cu, 0.125)
+    g = torch.Generator().manual_seed(22)
+    for i, (n, size) in enumerate((("dq", 2.0 ** -4), ("dk", 2.0 ** -4), ("dv", 0.5))):
+        ops = [q, k, v]
+        step = (torch.randint(0, 2, ops[i].shape, generator=g) * 2 - 1).to(DEV) * size
+        lo, hi = ((ops[i].float() + s * step).to(BF) for s in (-1, 1))
+        with torch.no_grad():
+            a, b = (packed_attention(*ops[:i], t, *ops[i + 1:], cu, 0.125).double() for t in (lo, hi))
+        want = ((b - a) * d.double()).sum()
+        have = (got[n].double() * (hi.double() - lo.double())).sum()
+        noise = U * ((a.abs() + b.abs()) * d.double().abs()).square().sum().sqrt()
+        # third order: (0.125 sum |step| |k|)^3 / 6 of the values, some 0.1 of a step's
+        third = 0.0 if n == "dv" else 0.02 * noise / U * size
+        assert abs(have - want) <= 4 * noise + third, (n, have.item(), want.item())
+
+
+def test_one_key_rows_have_no_score_gradient():
+    """Sequences of one token: out = v, dv = do, dq and dk exactly 0 (also of scores far
+    from 0)."""
+    q, k, v, d, cu = _case([1] * 9, 4, 4, 128, seed=23, dev=30.0)
+    got = _grads(q, k, v, d, cu, 1.0)
+    assert torch.equal(got["o"], v) and torch.equal(got["dv"], d)
+    assert not got["dq"].any() and not got["dk"].any()
+
+
+def test_large_scores():
+    """Scores of some +-4000: probabilities of 0 and 1 without overflow, the neighbours'
+    rows untouched by a sequence of infinities."""
+    q, k, v, d, cu = _case([70, 65, 130], 2, 1, 128, seed=24)
+    want = _grads(q, k, v, d, cu, 0.09)
+    big = _grads(q * 32, k * 32, v, d, cu, 0.09)
+    assert all(t.isfinite().all() for t in big.values())
+    for t in (q, k, v):
+        t[70:135] = float("inf")
+    got = _grads(q, k, v, d, cu, 0.09)
+    for n in want:
+        assert torch.equal(got[n][:70], want[n][:70]) and torch.equal(got[n][135:], want[n][135:]), n
+
+
+def test_forms_of_call():
+    """Views of the projection's rows, unaligned and expanded operands, int64 lengths, one
+    gradient asked for, no rows, no sequences: the same values."""
+    lens, heads, kv, hd = [50, 7, 140], 4, 2, 64
+    q, k, v, d, cu = _case(lens, heads, kv, hd, seed=25)
+    T = sum(lens)
+    want = _grads(q, k, v, d, cu, 0.1)
+    rows = torch.zeros(T, (heads + 2 * kv) * hd + 24, dtype=BF, device=DEV)
+    rows[:, 8:-16] = torch.cat([t.reshape(T, -1) for t in (q, k, v)], 1)
+    qv, kvw, vv = rows[:, 8:-16].view(T, heads + 2 * kv, hd).split([heads, kv, kv], 1)
+    assert qv.data_ptr() % 16 == 0 and not qv.is_contiguous()
+    got = _grads(qv, kvw, vv, d.transpose(0, 1).contiguous().transpose(0, 1), cu.long(), 0.1)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    odd = torch.zeros(T * heads * hd + 1, dtype=BF, device=DEV)[1:].view(T, heads, hd).copy_(q)
+    assert torch.equal(packed_attention(odd, k, v, cu, 0.1), want["o"])
+    # a key head expanded over the query heads equals sharing it
+    ke, ve = (t[:, :1].expand(T, heads, hd) for t in (k, v))
+    assert torch.equal(packed_attention(q, ke, ve, cu, 0.1),
+                       packed_attention(q, k[:, :1], v[:, :1], cu, 0.1))
+    qs = q.clone().requires_grad_()
+    packed_attention(qs, k, v, cu, 0.1).sum().backward()
+    assert torch.equal(qs.grad, _grads(q, k, v, torch.ones_like(d), cu, 0.1)["dq"])
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = _grads(q, k, v, d, none, 0.1)  # no sequences: every row is outside
+    assert not any(t.any() for t in got.values())
+    assert packed_attention(q[:0], k[:0], v[:0], none, 0.1).shape == (0, heads, hd)
+
+
+def test_lengths_that_lie_outside():
+    """Entries past the rows are clamped: nothing outside is read or written."""
+    q, k, v, d, cu = _case([100, 60], 2, 2, 64, seed=26)
+    far = cu.clone()
+    far[-1], far[0] = 100000, -7
+    want, got = _grads(q, k, v, d, cu, 0.1), _grads(q, k, v, d, far, 0.1)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 4), (8, 2)])
+def test_repeats_bit_for_bit_in_a_graph(heads, kv):
+    """Replays of a captured forward and backward pass, with eager work between, give the
+    eager bits; so does another stream."""
+    q, k, v, d, cu = _case([200, 33, 64], heads, kv, 128, seed=27)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+
+    def step():
+        o = packed_attention(*leaves, cu, 0.1)
+        return (o.detach(), *torch.autograd.grad(o, leaves, d))
+
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = step()
+        with torch.cuda.graph(graph, stream=side):
+            outs = step()
+    torch.cuda.synchronize()
+    want = _grads(q, k, v, d, cu, 0.1)
+    assert all(torch.equal(a, b) for a, b in zip(first, want.values()))
+    for rep in range(3):
+        with torch.no_grad():
+            leaves[2].copy_(v * (rep + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = _grads(q, k, v * (rep + 1), d, cu, 0.1)
+        assert all(torch.equal(a, b) for a, b in zip(outs, eager.values())), rep
