@@ -49,6 +49,10 @@ constexpr int P_TR = 64;            // rows per swept tile
 constexpr int P_FILL = 32;          // workgroups that clear rows outside the sequences
 constexpr float P_SLACK = 8.0f;     // log2 headroom of the reference max
 
+// Keeps a wave-uniform condition a branch: the masks of the few tiles on the diagonal
+// were computed for every tile otherwise, a third of the vector instructions.
+#define P_BRANCH asm volatile("")
+
 struct Rows {                       // (T, heads, HD) bf16, unit last stride
   const bf16_t *p;
   int64_t st, sh;
@@ -281,6 +285,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs p) {
 #pragma unroll
       for (int e = 0; e < HD / 32; ++e) vf[kp][e] = p_cols<HD>(vs, e, kp, lane);
     if (kb0 + P_TR - 1 > wq0) {  // wave-uniform: some keys come after some queries
+      P_BRANCH;
       const int lim = qi - kb0 - 4 * g;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -399,6 +404,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c2, -lse)) * (dp[i] - delta);
       if (edge) {  // keys after the query; a query of one key
+        P_BRANCH;
         const int lim = qi == 0 ? -1 : qi - kb0 - 4 * g;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -512,6 +518,7 @@ __global__ __launch_bounds__(64 * P_KW, 1) void packed_dkv_kernel(PackedArgs p) 
         }
       }
       if (qt0 == wk0) {  // wave-uniform: the diagonal tile (rows of both start on 32s)
+        P_BRANCH;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int qr = 8 * (i >> 2) + 4 * g + (i & 3);
