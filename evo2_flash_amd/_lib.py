@@ -8,6 +8,7 @@ fallback: if the library is missing or fails to load, every operator raises.
 
 import contextlib
 import ctypes
+import functools
 import os
 import threading
 
@@ -386,6 +387,12 @@ def lib():
         return _lib
 
 
+@functools.lru_cache(maxsize=4096)
+def workspace_bytes(name, *sizes):
+    """What the C ABI's workspace query `name` gives for these sizes."""
+    return getattr(lib(), name)(*sizes)
+
+
 def call(name, *args):
     """Call a C-ABI entry point; raise Evo2Error on a nonzero status."""
     l = lib()
@@ -449,6 +456,15 @@ def once(backward):
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return staticmethod(call_backward)
+
+
+def same_device(*tensors):
+    """Whether the (CUDA) tensors are on one device."""
+    first = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != first:
+            return False
+    return True
 
 
 def require_device(*tensors):

@@ -394,7 +394,7 @@ def _packed_backward(ctx, dout):
     q, k, v, cu, out, kept = ctx.saved_tensors
     T, heads, hd = q.shape
     kv, nseq = k.shape[1], cu.shape[0] - 1
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dq, dk, dv = q.new_empty((T, heads, hd)), k.new_empty((T, kv, hd)), v.new_empty((T, kv, hd))
     if T:
         d, dp, dt, dh = _head_rows(dout)
         q, qp, qt, qh = _head_rows(q)
@@ -402,7 +402,7 @@ def _packed_backward(ctx, dout):
         v, vp, vt, vh = _head_rows(v)
         lo = kept.data_ptr()
         with _lib.on_device(q):
-            n = _lib.lib().evo2_packed_attention_workspace_bytes(T, nseq, heads, kv, hd)
+            n = _lib.workspace_bytes("evo2_packed_attention_workspace_bytes", T, nseq, heads, kv, hd)
             ws = torch.empty(n, dtype=torch.uint8, device=q.device)
             _lib.call("evo2_packed_attention_backward", dp, dt, dh, qp, qt, qh, kp, kt, kh, vp, vt,
                       vh, cu.data_ptr(), nseq, out.data_ptr(), lo, lo + 2 * T * heads * hd,
@@ -453,7 +453,7 @@ def packed_attention(q, k, v, cu_seqlens, scale):
             or cu_seqlens.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"cu_seqlens must be (nseq + 1,) int32 or int64, got "
                          f"{tuple(cu_seqlens.shape)} {cu_seqlens.dtype}")
-    if not q.device == k.device == v.device == cu_seqlens.device:
+    if not _lib.same_device(q, k, v, cu_seqlens):
         raise ValueError(f"packed_attention: operands on {q.device}, {k.device}, {v.device}, "
                          f"{cu_seqlens.device}")
     scale = float(scale)
@@ -462,7 +462,8 @@ def packed_attention(q, k, v, cu_seqlens, scale):
     cu = cu_seqlens
     if cu.dtype != torch.int32:
         cu = cu.clamp(0, T).to(torch.int32)
-    cu = cu.contiguous()
+    if cu.stride(0) != 1:
+        cu = cu.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, cu, scale)
     return _packed_forward(q, k, v, cu, scale, False)[0]

@@ -178,12 +178,13 @@ def _gated_backward(ctx, dh):
     dx = x.new_empty(M, H) if need[0] else None
     dw1 = dw2 = None
     if need[1] or need[2]:
-        dw1, dw2 = ((w.new_empty if M else w.new_zeros)((I, H)) for w in (w1, w2))
+        make = w1.new_empty if M else w1.new_zeros
+        dw1, dw2 = make((I, H)), make((I, H))
     if M:
         dh, x = _lib.rows16(dh), _lib.rows16(x)
         w1, w2 = _weight_rows(w1, w2)
         with _lib.on_device(x):
-            n = _lib.lib().evo2_gated_linear_workspace_bytes(M, I, H)
+            n = _lib.workspace_bytes("evo2_gated_linear_workspace_bytes", M, I, H)
             ws = torch.empty(n, dtype=torch.uint8, device=x.device)
             _lib.call("evo2_gated_linear_backward", dh.data_ptr(), dh.stride(0), x.data_ptr(),
                       x.stride(0), w1.data_ptr(), w2.data_ptr(), w1.stride(0), kept.data_ptr(),
@@ -219,7 +220,7 @@ def gated_linear(x, w1, w2, gelu):
     I, H = w1.shape
     if I == 0 or H == 0 or (I | H) & 7:
         raise ValueError(f"gated_linear takes weights of multiples of 8, got {tuple(w1.shape)}")
-    if not x.device == w1.device == w2.device:
+    if not _lib.same_device(x, w1, w2):
         raise ValueError(f"gated_linear: operands on {x.device}, {w1.device}, {w2.device}")
     rows = x if x.dim() == 2 else x.reshape(-1, H)
     if torch.is_grad_enabled() and (rows.requires_grad or w1.requires_grad or w2.requires_grad):

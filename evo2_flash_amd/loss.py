@@ -29,7 +29,7 @@ def _forward(hidden, weight, targets, ignore_index, reduction):
         return nll, lse, loss, count
     hidden, weight = _lib.rows16(hidden), _lib.rows16(weight)
     with _lib.on_device(hidden):
-        n = _lib.lib().evo2_linear_loss_workspace_bytes(T, V, H, 0)
+        n = _lib.workspace_bytes("evo2_linear_loss_workspace_bytes", T, V, H, 0)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         _lib.call("evo2_linear_loss", hidden.data_ptr(), hidden.stride(0), weight.data_ptr(),
                   weight.stride(0), targets.data_ptr(), ignore_index, reduction, nll.data_ptr(),
@@ -48,7 +48,7 @@ def _backward(ctx, grad):
         hidden, weight = _lib.rows16(hidden), _lib.rows16(weight)
         grad = grad.to(torch.float32)
         with _lib.on_device(hidden):
-            n = _lib.lib().evo2_linear_loss_workspace_bytes(T, V, H, 1)
+            n = _lib.workspace_bytes("evo2_linear_loss_workspace_bytes", T, V, H, 1)
             ws = torch.empty(n, dtype=torch.uint8, device=hidden.device)
             _lib.call("evo2_linear_loss_backward", hidden.data_ptr(), hidden.stride(0),
                       weight.data_ptr(), weight.stride(0), targets.data_ptr(), ctx.ignore_index,
@@ -96,12 +96,14 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="
                          f"multiple of 8, got {tuple(weight.shape)}")
     if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
         raise ValueError(f"targets must be integers, got {targets.dtype}")
-    if not hidden.device == weight.device == targets.device:
+    if not _lib.same_device(hidden, weight, targets):
         raise ValueError(f"linear_cross_entropy: operands on {hidden.device}, {weight.device}, "
                          f"{targets.device}")
     shape = targets.shape
     h = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
-    t = targets.reshape(-1).to(torch.int64).contiguous()
+    t = targets.reshape(-1).to(torch.int64)
+    if t.stride(0) != 1:  # (an expanded target)
+        t = t.contiguous()
     red = _REDUCTIONS.index(reduction)
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
         out = _LinearCrossEntropy.apply(h, weight, t, int(ignore_index), red)
