@@ -31,6 +31,7 @@
 #include <algorithm>
 #include <climits>
 
+
 #include "attn_common.h"
 
 namespace evo2 {
@@ -53,7 +54,7 @@ constexpr int MAT_BN = 256;      // output columns per workgroup
 constexpr int MAT_BK = 64;       // K per slice
 constexpr uint32_t MAT_OUT = 0x80000000u;  // an offset past every descriptor here
 
-constexpr int mat_stages(int tm) { return tm == 1 ? 3 : 2; }
+constexpr int mat_stages(int tm) { return tm <= 2 ? 3 : 2; }
 
 struct MatArgs {
   const bf16_t *x; int64_t sx;            // row strides in elements
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   constexpr int WST = MAT_BN * MAT_BK, XST = BM * MAT_BK;   // elements per stage
   __shared__ __align__(16) bf16_t w0[WST], w1[WST], w2s[NST > 2 ? WST : 8];
   __shared__ __align__(16) bf16_t x0[XST], x1[XST], x2s[NST > 2 ? XST : 8];
-  __shared__ __align__(16) float turned[4][32 * 36];        // a wave's 32 x 32 results, by rows
+  __shared__ __align__(16) float turned[4][32 * 32];        // a wave's 32 x 32 results, by rows
   constexpr int DB = 8, DX = 2 * TM;  // 1 KB loads of w and x per wave and slice
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
 
   // Lane (lr, g) holds, for row m = wm + 32 tm + lr of the tile, columns
   // wn + 32 tn + 8 q + 4 g + i in acc[tn][tm][4 q + i].  Results go to memory by way of
-  // a wave's own 32 rows of 144 bytes in LDS, which turn them so that eight lanes
+  // a wave's own 32 rows of 128 bytes in LDS (16-byte chunk c of row r at c ^ (r & 7)), which turn them so that eight lanes
   // store one whole 128-byte line of a row: stored as they lie, each line takes four
   // requests, and the caches' request rate bounds the burst at a tile's end.
   auto epilogue = [&](int j) __attribute__((always_inline)) {
@@ -369,13 +370,13 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint2 *>(b + lr * 72 + 32 * t + 8 * q + 4 * g) = make_uint2(v(t, 4 * q), v(t, 4 * q + 2));
+          *reinterpret_cast<uint2 *>(b + lr * 64 + 8 * ((4 * t + q) ^ (lr & 7)) + 4 * g) = make_uint2(v(t, 4 * q), v(t, 4 * q + 2));
       fence();
       bf16_t *o = out + m * so + n0 + c;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int r = 8 * k + tr;
-        const au32x4_t w = *reinterpret_cast<const au32x4_t *>(b + r * 72 + 8 * tc);
+        const au32x4_t w = *reinterpret_cast<const au32x4_t *>(b + r * 64 + 8 * (tc ^ (r & 7)));
         if (m + r < p.M && n0 + c + 8 * tc < cols) *reinterpret_cast<au32x4_t *>(o + r * so + 8 * tc) = w;
       }
       fence();
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     auto put_f32 = [&](float *out, int64_t so, int m, int c, bool add, auto &&v) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<af32x4_t *>(tb + lr * 36 + 8 * q + 4 * g) =
+        *reinterpret_cast<af32x4_t *>(tb + lr * 32 + 4 * ((2 * q + g) ^ (lr & 7))) =
             af32x4_t{v(4 * q), v(4 * q + 1), v(4 * q + 2), v(4 * q + 3)};
       fence();
       float *o = out + m * so + n0 + c;
@@ -392,7 +393,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int r = 8 * k + tr;
-          af32x4_t w = *reinterpret_cast<const af32x4_t *>(tb + r * 36 + 4 * tc);
+          af32x4_t w = *reinterpret_cast<const af32x4_t *>(tb + r * 32 + 4 * (tc ^ (r & 7)));
           if (m + r < p.M && n0 + c + 4 * tc < p.N) {
             af32x4_t *d = reinterpret_cast<af32x4_t *>(o + r * so + 4 * tc);
             if (add) w += *d;
@@ -403,7 +404,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
 #pragma unroll 1
         for (int k = 0; k < 16; ++k) {
           const int r = 2 * k + (lane >> 5), cc = lane & 31;
-          const float w = tb[r * 36 + cc];
+          const float w = tb[r * 32 + 4 * ((cc >> 2) ^ (r & 7)) + (cc & 3)];
           if (m + r < p.M && n0 + c + cc < p.N) o[r * so + cc] = w;
         }
       }
@@ -560,20 +561,26 @@ struct MatPlan {
 // The tile height and split of least time: rounds of tiles over the CUs, times what a
 // tile costs -- us per slice and us at its end, measured over 512 to 10240 of K -- and
 // where few tiles let K be split, the partial sums' second launch and their bytes
-// there and back.  Measured, us for tm 1 / 2 / 3 / 4: NT 777 x 49999 x 1920 238 / 209
-// / 191 / 214; gated 777 x 11264 x 4096 187 / 162 / 152 / 231, 2048 x 5120 x 1920 131
-// / 114 / 124 / 177; NN 2048 x 1920 x 10240, split by 1, 2, 2, 4, 111 / 93 / 102 / 91;
-// TN 512 x 4096 x 32768, split by 2, 4, -, 8, 210 / 183 / - / 147 and 49999 x 1920 x
-// 777 296 / 236 / - / 206.
+// there and back.  Measured, us for tm 1 / 2 / 3 / 4: NT 777 x 49999 x 1920 223 / 207
+// / 191 / 214; gated 777 x 11264 x 4096 184 / 163 / 152 / 189, 2048 x 5120 x 1920 126
+// / 126 / 124 / 167, 8192 x 11264 x 4096 1665 / 1350 / - / 1412; NN 2048 x 1920 x 10240,
+// split by 1, 2, 2, 4, 106 / 95 / 102 / 90, 8192 x 4096 x 22528 1749 / 1474 / - / 1157;
+// TN 512 x 4096 x 32768, split by 2, 4, -, 8, 208 / 163 / - / 147, 49999 x 1920 x 777
+// 294 / 235 / - / 206 and 22528 x 4096 x 8192 1926 / 1285 / - / 1177.
 // M: rows of one of `pair` outputs; slices: of K; width: output columns per tile.
 inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int pair, int width,
                         bool may_split) {
   const bool gated = width < MAT_BN;  // (four 16-bit outputs rather than one)
-  const double slice[5] = {0, 0.60, form == MAT_TN ? 1.05 : 0.90, 1.30, 1.72};
-  const double end[5] = {0, gated ? 7.0 : 4.0, gated ? 11.0 : 6.0, gated ? 19.0 : 9.0, gated ? 25.0 : 12.0};
+  static const double slice[4][5] = {{0, 0.60, 0.93, 1.30, 1.72},   // NT
+                                     {0, 0.60, 1.00, 1.30, 1.72},   // NN
+                                     {0, 0.66, 1.00, 1.30, 1.72},   // TN
+                                     {0, 0.60, 0.80, 1.20, 1.72}};  // NT, gated
+  static const double ends[2][5] = {{0, 4.0, 6.0, 9.0, 12.0}, {0, 7.0, 11.0, 17.0, 25.0}};
+  const double *each = slice[gated ? 3 : form], *end = ends[gated];
   MatPlan best{};
   double least = 1e300;
   for (int tm : {4, 3, 2, 1}) {
+    
     if (form == MAT_TN && tm == 3) continue;  // (rows of 192 do not fill whole load blocks)
     const int nst = mat_stages(tm);
     const int64_t tm_tiles = cdiv(M, 64 * tm) * pair, tn_tiles = cdiv(N, width), tiles = tm_tiles * tn_tiles;
@@ -582,7 +589,7 @@ inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int 
     const int64_t kt = cdiv(cdiv(slices, splits), nst) * nst;
     splits = std::max<int64_t>(1, cdiv(slices, kt));
     const double rounds = double(cdiv(tiles * splits, MAT_CUS));
-    double cost = rounds * (kt * slice[tm] + end[tm]);
+    double cost = rounds * (kt * each[tm] + end[tm]);
     if (splits > 1) cost += 6.0 + double(splits) * M * pair * N * 1.3e-6;
     if (cost < least - 1e-9) {
       least = cost;
