@@ -572,7 +572,7 @@ inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int 
                         bool may_split) {
   const bool gated = width < MAT_BN;  // (four 16-bit outputs rather than one)
   static const double slice[4][5] = {{0, 0.60, 0.93, 1.30, 1.72},   // NT
-                                     {0, 0.60, 1.00, 1.30, 1.72},   // NN
+                                     {0, 0.66, 1.00, 1.40, 1.72},   // NN
                                      {0, 0.66, 1.00, 1.30, 1.72},   // TN
                                      {0, 0.60, 0.80, 1.20, 1.72}};  // NT, gated
   static const double ends[2][5] = {{0, 4.0, 6.0, 9.0, 12.0}, {0, 7.0, 11.0, 17.0, 25.0}};

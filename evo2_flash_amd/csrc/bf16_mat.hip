@@ -23,6 +23,7 @@ __global__ __launch_bounds__(256) void mat_join_kernel(const float *part, int64_
   const int c = static_cast<int>(at - r * cols8) * 8;
   const float *src = part + at * 8;
   af32x4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll 4
   for (int s = 0; s < splits; ++s, src += plane) {
     a += *reinterpret_cast<const af32x4_t *>(src);
     b += *reinterpret_cast<const af32x4_t *>(src + 4);

@@ -19,7 +19,8 @@
 namespace evo2 {
 
 constexpr float L_LOG2E = 1.44269504088896341f, L_LN2 = 0.69314718055994531f;
-constexpr int L_ROWS = 32;   // rows per workgroup of the joining kernel
+constexpr int L_ROWS = 16;             // rows per workgroup of the joining kernel
+constexpr int L_RUNS = 256 / L_ROWS;   // and the runs of parts it cuts each into
 
 struct LossRows {
   const int64_t *targets;
@@ -46,23 +47,31 @@ __device__ __forceinline__ void loss_join(float &mx, float &sum, float mx2, floa
   mx = top;
 }
 
-// Joins the tiles' (max, sum): 32 rows by 8 runs of the parts per workgroup.
+// Joins the tiles' (max, sum), 16 rows by 16 runs of the parts per workgroup: a run's
+// max first, then its sum, so that the loads of neither pass wait for one another (one
+// pass that rescales as it goes: 20 us for 777 rows of 392 parts, JOIN_NOW so).
 __global__ __launch_bounds__(256) void loss_join_kernel(LossRows p, const float2 *part, const float *tgt,
                                                         int nparts) {
-  __shared__ float smx[8][L_ROWS], ssum[8][L_ROWS];
-  const int r = threadIdx.x & 31, run = threadIdx.x >> 5;
+  __shared__ float smx[L_RUNS][L_ROWS], ssum[L_RUNS][L_ROWS];
+  const int r = threadIdx.x % L_ROWS, run = threadIdx.x / L_ROWS;
   const int m = blockIdx.x * L_ROWS + r;
   float mx = -INFINITY, sum = 0.0f;
-  if (m < p.T)
-    for (int i = run; i < nparts; i += 8) {
-      const float2 v = part[static_cast<int64_t>(i) * p.T + m];
-      loss_join(mx, sum, v.x, v.y);
+  if (m < p.T) {
+    const float2 *at = part + m;
+#pragma unroll 8
+    for (int i = run; i < nparts; i += L_RUNS) mx = fmaxf(mx, at[static_cast<int64_t>(i) * p.T].x);
+    const float sub = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll 8
+    for (int i = run; i < nparts; i += L_RUNS) {
+      const float2 v = at[static_cast<int64_t>(i) * p.T];
+      sum = fmaf(v.y, __builtin_amdgcn_exp2f((v.x - sub) * L_LOG2E), sum);
     }
+  }
   smx[run][r] = mx;
   ssum[run][r] = sum;
   __syncthreads();
   if (run != 0) return;
-  for (int i = 1; i < 8; ++i) loss_join(mx, sum, smx[i][r], ssum[i][r]);
+  for (int i = 1; i < L_RUNS; ++i) loss_join(mx, sum, smx[i][r], ssum[i][r]);
   double loss = 0.0, n = 0.0;
   if (m < p.T) {
     const int64_t t = p.targets[m];
@@ -70,7 +79,7 @@ __global__ __launch_bounds__(256) void loss_join_kernel(LossRows p, const float2
     loss = loss_row(p, m, mx, sum, ok ? tgt[m] : 0.0f);
     n = t != p.ignore ? 1.0 : 0.0;
   }
-  for (int o = 16; o; o >>= 1) {
+  for (int o = L_ROWS / 2; o; o >>= 1) {
     loss += __shfl_xor(loss, o);
     n += __shfl_xor(n, o);
   }
