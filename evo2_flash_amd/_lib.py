@@ -13,6 +13,7 @@ import os
 import threading
 
 import torch  # noqa: F401  (must precede the library load, see above)
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .build import LIB_PATH
@@ -456,6 +457,19 @@ def once(backward):
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return staticmethod(call_backward)
+
+
+def recorded(*tensors):
+    """Whether a call on these goes through its autograd function: a gradient to
+    record, or a forward-mode level (for whose tangents the function, which has no such
+    derivative, raises)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    return False
 
 
 def same_device(*tensors):

@@ -464,7 +464,7 @@ def packed_attention(q, k, v, cu_seqlens, scale):
         cu = cu.clamp(0, T).to(torch.int32)
     if cu.stride(0) != 1:
         cu = cu.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _lib.recorded(q, k, v):
         return _PackedAttention.apply(q, k, v, cu, scale)
     return _packed_forward(q, k, v, cu, scale, False)[0]
 

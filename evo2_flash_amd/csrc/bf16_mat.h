@@ -31,7 +31,6 @@
 #include <algorithm>
 #include <climits>
 
-
 #include "attn_common.h"
 
 namespace evo2 {

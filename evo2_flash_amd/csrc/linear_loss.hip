@@ -49,7 +49,7 @@ __device__ __forceinline__ void loss_join(float &mx, float &sum, float mx2, floa
 
 // Joins the tiles' (max, sum), 16 rows by 16 runs of the parts per workgroup: a run's
 // max first, then its sum, so that the loads of neither pass wait for one another (one
-// pass that rescales as it goes: 20 us for 777 rows of 392 parts, JOIN_NOW so).
+// pass that rescales as it goes: 20 us for 777 rows of 392 parts, 6 so).
 __global__ __launch_bounds__(256) void loss_join_kernel(LossRows p, const float2 *part, const float *tgt,
                                                         int nparts) {
   __shared__ float smx[L_RUNS][L_ROWS], ssum[L_RUNS][L_ROWS];
@@ -208,7 +208,8 @@ static int check_sizes(const char *what, int64_t T, int64_t V, int64_t H, int64_
     return fail(EVO2_ERR_INVALID, "%s: bad sizes T=%lld V=%lld H=%lld", what, (long long)T, (long long)V,
                 (long long)H);
   if (H % 8) return fail(EVO2_ERR_UNSUPPORTED, "%s: H=%lld must be a multiple of 8", what, (long long)H);
-  if (!mat_fits(T, V, H, std::max(sh, sw)) || !mat_fits(V, H, T, H))
+  // (a piece's rows of d take V columns at most)
+  if (V >= (int64_t(1) << 22) || !mat_fits(T, V, H, std::max(sh, sw)) || !mat_fits(V, H, T, H))
     return fail(EVO2_ERR_UNSUPPORTED, "%s: problem too large", what);
   if (sh < H || sw < H || sh % 8 || sw % 8)
     return fail(EVO2_ERR_UNSUPPORTED, "%s: operands must be 16-byte aligned rows", what);

@@ -223,7 +223,7 @@ def gated_linear(x, w1, w2, gelu):
     if not _lib.same_device(x, w1, w2):
         raise ValueError(f"gated_linear: operands on {x.device}, {w1.device}, {w2.device}")
     rows = x if x.dim() == 2 else x.reshape(-1, H)
-    if torch.is_grad_enabled() and (rows.requires_grad or w1.requires_grad or w2.requires_grad):
+    if _lib.recorded(rows, w1, w2):
         h = _GatedLinear.apply(rows, w1, w2, bool(gelu))
     else:
         h = _gated_forward(rows, w1, w2, gelu, False)[0]

@@ -73,7 +73,7 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="
     """Cross entropy of the logits hidden @ weight^T against `targets`, differentiable
     in hidden and weight (once).
 
-    hidden (..., H) and weight (V, H) bf16 on one device, H a multiple of 8; targets
+    hidden (..., H) and weight (V, H) bf16 on one device, H a multiple of 8, V < 2^22; targets
     (...) of an integer type.  Rows whose target is `ignore_index` have loss 0 and no
     gradient (but their infinite or NaN hidden values reach the weight's, times 0); a target
     outside [0, V) otherwise makes its row's loss and gradient NaN (nothing is read
@@ -105,7 +105,7 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="
     if t.stride(0) != 1:  # (an expanded target)
         t = t.contiguous()
     red = _REDUCTIONS.index(reduction)
-    if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
+    if _lib.recorded(h, weight):
         out = _LinearCrossEntropy.apply(h, weight, t, int(ignore_index), red)
     else:
         nll, _, loss, _ = _forward(h, weight, t, int(ignore_index), red)

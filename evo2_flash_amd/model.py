@@ -90,10 +90,13 @@ class Evo2MLP(nn.Module):
         return linear(self._product(x), self.l3.weight, self.l3.bias, residual=residual)
 
     def forward_train(self, x):
-        """forward(x) with gradients: the product is one launch (projections with a bias
-        or hooks are called as modules)."""
-        if all(_bare(m, Linear) and m.bias is None for m in (self.l1, self.l2)):
-            h = gated_linear(x, self.l1.weight, self.l2.weight, self.use_act)
+        """forward(x) with gradients: the product is one launch (projections of another
+        type or size, with a bias or hooks, are called as modules)."""
+        w1, w2 = self.l1.weight, self.l2.weight
+        if (all(_bare(m, Linear) and m.bias is None for m in (self.l1, self.l2))
+                and x.dtype == w1.dtype == w2.dtype == torch.bfloat16
+                and all(n % 8 == 0 for n in w1.shape)):
+            h = gated_linear(x, w1, w2, self.use_act)
         else:
             h = self._product(x)
         out, _ = self.l3(h)

@@ -493,7 +493,7 @@ int evo2_gated_linear_backward(const void *dh, int64_t sdh, const void *x, int64
  *   d = (exp(h w_n - lse) - [n = target]) g, dh = d w, dw = d^T h, with g =
  *   grad[m * sgrad], divided by *count where count is not NULL (a mean's, sgrad 0)
  *   h (T, H) row stride sh, w (V, H) row stride sw, dh (T, H) and dw (V, H)
- *   contiguous, bf16, H a multiple of 8, rows 16-byte aligned; targets (T,) int64;
+ *   contiguous, bf16, H a multiple of 8, V < 2^22, rows 16-byte aligned; targets (T,) int64;
  *   nll, lse (T,), loss, count (1,), grad fp32.  dh or dw may be NULL.  T >= 1; the
  *   workspace has _workspace_bytes(T, V, H, backward) bytes.
  */

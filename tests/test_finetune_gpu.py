@@ -129,3 +129,59 @@ def test_layers_with_hooks_and_hyena_layers():
     assert abs(plain.item() - hooked.item()) <= 1e-2 * abs(plain.item())
     with pytest.raises(NotImplementedError, match="Hyena"):
         model.layers[0].forward_train(torch.zeros(4, 256, device=DEV), None, None)
+
+
+def test_training_under_compile_and_checkpoints():
+    """The operators inside a compiled function, a checkpointed one and autocast give the
+    eager bits; forward-mode tangents, which they have not, are refused."""
+    from torch.utils.checkpoint import checkpoint
+
+    from evo2_flash_amd.attention import packed_attention
+    from evo2_flash_amd.linear import gated_linear
+    from evo2_flash_amd.loss import linear_cross_entropy
+
+    g = torch.Generator().manual_seed(6)
+
+    def leaf(*shape):
+        return torch.randn(*shape, generator=g).to(torch.bfloat16).to(DEV).requires_grad_()
+
+    q, k, v = (leaf(40, 2, 64) for _ in range(3))
+    w1, w2 = leaf(72, 128), leaf(72, 128)
+    cu = torch.tensor([0, 15, 40], dtype=torch.int32, device=DEV)
+    t = torch.randint(72, (40,), generator=g).to(DEV)
+    leaves = (q, k, v, w1, w2)
+
+    def f(q, k, v, w1, w2):
+        x = packed_attention(q, k, v, cu, 0.1).view(40, 128)
+        return linear_cross_entropy(x, w1, t) + gated_linear(x, w1, w2, True).float().mean()
+
+    want = f(*leaves)
+    grads = torch.autograd.grad(want, leaves)
+
+    def same(loss):
+        got = torch.autograd.grad(loss, leaves)
+        return torch.equal(loss, want) and all(torch.equal(a, b) for a, b in zip(got, grads))
+
+    assert same(torch.compile(f)(*leaves))
+    assert same(checkpoint(f, *leaves, use_reentrant=False))
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = f(*leaves)
+    assert same(loss)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q.detach(), torch.ones_like(q))
+        with pytest.raises(Exception, match="jvp"):
+            packed_attention(dual, k.detach(), v.detach(), cu, 0.1)
+
+
+def test_other_sizes_take_the_modules():
+    """An MLP off the operator's sizes trains through its modules."""
+    from evo2_flash_amd.model import Evo2MLP
+
+    mlp = Evo2MLP(64, 36, True, device=DEV).requires_grad_()
+    for m in (mlp.l1, mlp.l2, mlp.l3):
+        torch.nn.init.normal_(m.weight, std=0.1)
+    x = torch.randn(5, 64, device=DEV).to(torch.bfloat16)
+    out = mlp.forward_train(x)
+    assert torch.equal(out, mlp(x))
+    out.sum().backward()
+    assert all(m.weight.grad.isfinite().all() for m in (mlp.l1, mlp.l2, mlp.l3))
