@@ -560,21 +560,27 @@ struct MatPlan {
 // The tile height and split of least time: rounds of tiles over the CUs, times what a
 // tile costs -- us per slice and us at its end, measured over 512 to 10240 of K -- and
 // where few tiles let K be split, the partial sums' second launch and their bytes
-// there and back.  Measured, us for tm 1 / 2 / 3 / 4: NT 777 x 49999 x 1920 223 / 207
-// / 191 / 214; gated 777 x 11264 x 4096 184 / 163 / 152 / 189, 2048 x 5120 x 1920 126
-// / 126 / 124 / 167, 8192 x 11264 x 4096 1665 / 1350 / - / 1412; NN 2048 x 1920 x 10240,
-// split by 1, 2, 2, 4, 106 / 95 / 102 / 90, 8192 x 4096 x 22528 1749 / 1474 / - / 1157;
-// TN 512 x 4096 x 32768, split by 2, 4, -, 8, 208 / 163 / - / 147, 49999 x 1920 x 777
-// 294 / 235 / - / 206 and 22528 x 4096 x 8192 1926 / 1285 / - / 1177.
+// there and back.  Measured, us for tm 1 / 2 / 3 / 4:
+//   NT     777 x 49999 x 1920             223 / 207 / 191 / 214
+//          4096 x 131072 x 4096           - / - / 3472 / 3280
+//   gated  777 x 11264 x 4096             184 / 163 / 152 / 189
+//          2048 x 5120 x 1920             126 / 126 / 124 / 167
+//          8192 x 11264 x 4096            1665 / 1350 / - / 1412
+//   NN     2048 x 1920 x 10240            106 / 95 / 102 / 90 (split by 1, 2, 2, 4)
+//          32768 x 4096 x 512             262 / 214 / 180 / 202
+//          8192 x 4096 x 22528            1749 / 1474 / - / 1157
+//   TN     512 x 4096 x 32768             208 / 163 / - / 147 (split by 2, 4, -, 8)
+//          49999 x 1920 x 777             294 / 235 / - / 206
+//          22528 x 4096 x 8192            1926 / 1285 / - / 1177
 // M: rows of one of `pair` outputs; slices: of K; width: output columns per tile.
 inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int pair, int width,
                         bool may_split) {
   const bool gated = width < MAT_BN;  // (four 16-bit outputs rather than one)
-  static const double slice[4][5] = {{0, 0.60, 0.93, 1.30, 1.72},   // NT
+  static const double slice[4][5] = {{0, 0.60, 0.93, 1.30, 1.62},   // NT
                                      {0, 0.66, 1.00, 1.40, 1.72},   // NN
                                      {0, 0.66, 1.00, 1.30, 1.72},   // TN
                                      {0, 0.60, 0.80, 1.20, 1.72}};  // NT, gated
-  static const double ends[2][5] = {{0, 4.0, 6.0, 9.0, 12.0}, {0, 7.0, 11.0, 17.0, 25.0}};
+  static const double ends[2][5] = {{0, 4.0, 6.0, 7.0, 14.0}, {0, 7.0, 11.0, 17.0, 25.0}};
   const double *each = slice[gated ? 3 : form], *end = ends[gated];
   MatPlan best{};
   double least = 1e300;
@@ -589,7 +595,7 @@ inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int 
     splits = std::max<int64_t>(1, cdiv(slices, kt));
     const double rounds = double(cdiv(tiles * splits, MAT_CUS));
     double cost = rounds * (kt * each[tm] + end[tm]);
-    if (splits > 1) cost += 6.0 + double(splits) * M * pair * N * 1.3e-6;
+    if (splits > 1) cost += 4.0 + double(splits) * M * pair * N * 1.0e-6;
     if (cost < least - 1e-9) {
       least = cost;
       best = MatPlan{tm, static_cast<int>(tm_tiles), static_cast<int>(tn_tiles), static_cast<int>(splits),
