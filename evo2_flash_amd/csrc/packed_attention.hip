@@ -7,8 +7,9 @@
 //   dv = p^T do, dp = do v^T, ds = p (dp - delta), delta_i = sum_j p_ij dp_ij = do_i . o_i
 //   dq = scale ds k, dk = scale ds^T q
 //
-// Three kernels of one shape, waves of 32 rows each (four, eight for dk and dv) over tiles of 64 rows that
-// come through LDS by direct-to-LDS loads, double-buffered, one barrier a tile:
+// Three kernels of one shape, waves of 32 rows each (four; four or eight for dk and dv)
+// over tiles of 64 rows that come through LDS by direct-to-LDS loads, double-buffered,
+// one barrier a tile:
 //   forward  32 queries a wave, sweeping keys and values:  s^T = k q^T, o^T += v^T p^T
 //   dq       32 queries a wave, sweeping keys and values:  s^T, dp^T = v do^T,
 //            dq^T += k^T ds^T
@@ -43,8 +44,6 @@ typedef __attribute__((address_space(3))) ps16x4_t plds_s16x4_t;
 constexpr int P_NW = 4;             // waves per workgroup
 constexpr int P_WR = 32;            // rows a wave owns
 constexpr int P_WG = P_NW * P_WR;   // rows a workgroup owns
-constexpr int P_KW = 8;             // waves per workgroup of the dk, dv kernel
-constexpr int P_KG = P_KW * P_WR;   // keys it owns
 constexpr int P_TR = 64;            // rows per swept tile
 constexpr int P_FILL = 32;          // workgroups that clear rows outside the sequences
 constexpr float P_SLACK = 8.0f;     // log2 headroom of the reference max
@@ -115,15 +114,18 @@ __device__ __forceinline__ bool p_slot(const PackedArgs &p, int t, int lane, int
 
 // Workgroup -> (head, row-tile slot).  Whole heads per XCD (workgroup b runs on XCD
 // b mod 8) where they split evenly, so that an XCD's workgroups sweep the same rows
-// through its L2; reversed: the longest sweeps (the last queries) first.
+// through its L2; the longest sweeps of all its heads first (reversed: those of the last
+// queries), so that what is left at the end is short: head by head, 8192 tokens of 32
+// heads of 128 took 609, 812 and 1321 us forward, for dq and for dk, dv, so 588, 770 and
+// 1282 (dk, dv by now 1056).
 __device__ __forceinline__ void p_item(int w, int heads, int tiles, bool reversed, int &h, int &t) {
   if (heads % 8 == 0) {
-    const int j = w >> 3;
-    h = (w & 7) + 8 * (j / tiles);
-    t = j % tiles;
+    const int j = w >> 3, per = heads >> 3;
+    t = j / per;
+    h = (w & 7) + 8 * (j - t * per);
   } else {
-    h = w / tiles;
-    t = w % tiles;
+    t = w / heads;
+    h = w - t * heads;
   }
   if (reversed) t = tiles - 1 - t;
 }
@@ -426,15 +428,17 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
   p_store<HD>(acc, p.scale, p.dq + (static_cast<int64_t>(begin + qi) * p.heads + h) * HD, nullptr, g, qi < len);
 }
 
-// dk and dv of eight waves' keys.  A wave's 32 x HD sums of both take half its
+// dk and dv of KW waves' keys.  A wave's 32 x HD sums of both take half its
 // registers, its keys' B operands an eighth; its values' are read from LDS again for
-// every tile.  SPLIT: one query head per workgroup, fp32 sums to `part`, which a second
-// kernel joins over the heads that share a key head.
-template <int HD, bool SPLIT>
-__global__ __launch_bounds__(64 * P_KW, 1) void packed_dkv_kernel(PackedArgs p) {
+// every tile.  Heads of 64: held to what three workgroups of a CU can have (16384 tokens
+// of 16 heads 1139 -> 1070 us).  SPLIT: one query head per workgroup, fp32 sums to
+// `part`, which a second kernel joins over the heads that share a key head.
+template <int HD, bool SPLIT, int KW>
+__global__ __launch_bounds__(64 * KW, HD == 64 ? 3 : 1) void packed_dkv_kernel(PackedArgs p) {
+  constexpr int KG = KW * P_WR;  // keys of the workgroup
   constexpr int TILE = p_tile<HD>(P_TR);
   __shared__ __align__(16) bf16_t q0s[TILE], q1s[TILE], d0s[TILE], d1s[TILE];
-  __shared__ __align__(16) bf16_t vs[p_tile<HD>(P_KG)];                   // the workgroup's values
+  __shared__ __align__(16) bf16_t vs[p_tile<HD>(KG)];                   // the workgroup's values
   __shared__ __align__(16) float l0s[P_TR], l1s[P_TR], e0s[P_TR], e1s[P_TR];  // log-sum-exp, delta
   const int w = static_cast<int>(blockIdx.x);
   if (w >= p.items) {
@@ -451,19 +455,19 @@ __global__ __launch_bounds__(64 * P_KW, 1) void packed_dkv_kernel(PackedArgs p) 
   p_item(w, SPLIT ? p.heads : p.kv, p.tiles, false, hk, t);
   const int h0 = SPLIT ? hk : hk * group;  // first query head
   if (SPLIT) hk /= group;
-  if (!p_slot(p, t, lane, P_KG, begin, len, r0)) return;
+  if (!p_slot(p, t, lane, KG, begin, len, r0)) return;
   begin = __builtin_amdgcn_readfirstlane(begin);
   len = __builtin_amdgcn_readfirstlane(len);
   r0 = __builtin_amdgcn_readfirstlane(r0);
   const int wk0 = r0 + P_WR * wave, ki = wk0 + lr;
   const int nqb = (len - r0 + P_TR - 1) / P_TR, total = SPLIT ? nqb : nqb * group;  // swept tiles
 
-  TileLoad<HD, P_KW> lq, ld, lv;
+  TileLoad<HD, KW> lq, ld, lv;
   lq.init(p.q.p, p.q.st, wave, lane);
   ld.init(p.d.p, p.d.st, wave, lane);
   lv.init(p.v.p + begin * p.v.st + hk * p.v.sh, p.v.st, wave, lane);
 #pragma unroll
-  for (int i = 0; i < P_KG / P_TR; ++i) lv.issue(vs + i * TILE, r0 + i * P_TR, len);
+  for (int i = 0; i < KG / P_TR; ++i) lv.issue(vs + i * TILE, r0 + i * P_TR, len);
   int ih = 0, ib = 0;  // the next tile to load: head of the group, tile of its sweep
   auto issue = [&](bf16_t *qs, bf16_t *ds, float *ls, float *es) __attribute__((always_inline)) {
     const int h = h0 + ih, row = r0 + ib * P_TR;
@@ -494,7 +498,7 @@ __global__ __launch_bounds__(64 * P_KW, 1) void packed_dkv_kernel(PackedArgs p) 
     if (++cb == nqb) cb = 0;
     if (wk0 >= len) return;  // wave-uniform: no keys
     // (both tiles at once where the registers allow it)
-#pragma unroll HD == 64 ? 2 : 1
+#pragma unroll HD == 64 ? 3 : 1
     for (int u = 0; u < 2; ++u) {
       const int qt0 = qb0 + 32 * u;
       if (qt0 < wk0) continue;  // wave-uniform: queries before all of the wave's keys
@@ -519,12 +523,11 @@ __global__ __launch_bounds__(64 * P_KW, 1) void packed_dkv_kernel(PackedArgs p) 
       }
       if (qt0 == wk0) {  // wave-uniform: the diagonal tile (rows of both start on 32s)
         P_BRANCH;
+        const int lim = lr - 4 * g;  // (the rows as constants: as sums they held 16 registers)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int qr = 8 * (i >> 2) + 4 * g + (i & 3);
-          if (qr < lr) s[i] = dp[i] = 0.0f;
-          if (qt0 + qr == 0) dp[i] = 0.0f;  // a query of one key
-        }
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i >> 2) + (i & 3) < lim) s[i] = dp[i] = 0.0f;
+        if (qt0 + 4 * g == 0) dp[0] = 0.0f;  // a query of one key
       }
 #pragma unroll
       for (int kp = 0; kp < 2; ++kp) {
@@ -628,21 +631,40 @@ static void launch_forward(PackedArgs a, hipStream_t st) {
   hipLaunchKernelGGL((packed_forward_kernel<HD>), dim3(a.items + P_FILL), dim3(256), 0, st, a);
 }
 
-template <int HD>
-static void launch_backward(PackedArgs a, hipStream_t st) {
-  a.items = a.tiles * a.heads;  // first: it writes delta
-  hipLaunchKernelGGL((packed_dq_kernel<HD>), dim3(a.items + P_FILL), dim3(256), 0, st, a);
-  a.tiles = a.T / P_KG + a.nseq;
+// Whether the dk, dv kernel's workgroups take eight waves rather than four.  Heads of
+// 128: eight share a swept tile, but such a workgroup fills a CU, so that up to about one
+// round of the CUs half as many keys in twice as many workgroups end sooner (us with
+// eight and with four waves, by workgroups of eight: 128 of them 57 and 46, 208: 153 and
+// 129, 272: 158 and 140, 288: 115 and 108 or 124 and 131, 320: 61 and 62, 384: 90 and
+// 115, 1056: 1056 and 1746).  Heads of 64: always four, three workgroups to a CU, which
+// fill each other's waits (8192 tokens of 32 heads 754 and 625 us, 8 x 1024 tokens 120
+// and 93).
+static bool packed_wide(const PackedArgs &a) {
+  return (a.T / (8 * P_WR) + a.nseq) * (a.part ? a.heads : a.kv) >= 304;
+}
+
+template <int HD, int KW>
+static void launch_dkv(PackedArgs a, hipStream_t st) {
+  a.tiles = a.T / (KW * P_WR) + a.nseq;
   if (a.part) {
     a.items = a.tiles * a.heads;
-    if (a.items > 0)  // (fewer than P_KG rows and no sequences: the join clears them)
-      hipLaunchKernelGGL((packed_dkv_kernel<HD, true>), dim3(a.items), dim3(64 * P_KW), 0, st, a);
+    if (a.items > 0)  // (few rows and no sequences: the join clears them)
+      hipLaunchKernelGGL((packed_dkv_kernel<HD, true, KW>), dim3(a.items), dim3(64 * KW), 0, st, a);
     const int64_t rows = static_cast<int64_t>(a.T) * a.kv * (HD / 8);
     hipLaunchKernelGGL((packed_join_kernel<HD>), dim3(static_cast<unsigned>(cdiv(rows, 256))), dim3(256), 0, st, a);
   } else {
     a.items = a.tiles * a.kv;
-    hipLaunchKernelGGL((packed_dkv_kernel<HD, false>), dim3(a.items + P_FILL), dim3(64 * P_KW), 0, st, a);
+    hipLaunchKernelGGL((packed_dkv_kernel<HD, false, KW>), dim3(a.items + P_FILL), dim3(64 * KW), 0, st, a);
   }
+}
+
+template <int HD>
+static void launch_backward(PackedArgs a, hipStream_t st) {
+  a.items = a.tiles * a.heads;  // first: it writes delta
+  hipLaunchKernelGGL((packed_dq_kernel<HD>), dim3(a.items + P_FILL), dim3(256), 0, st, a);
+  if constexpr (HD == 128)
+    if (packed_wide(a)) return launch_dkv<HD, 8>(a, st);
+  launch_dkv<HD, 4>(a, st);
 }
 
 }  // namespace evo2
@@ -657,8 +679,8 @@ extern "C" int evo2_packed_attention(const void *q, int64_t sqt, int64_t sqh, co
   if (rc || T == 0) return rc;
   if (!q || !k || !v || !cu || !out || !out_lo != !lse)
     return fail(EVO2_ERR_INVALID, "packed_attention: null pointer argument");
-  if (!rows_ok(q, sqt, sqh, head_dim) || !rows_ok(k, skt, skh, head_dim) || !rows_ok(v, svt, svh, head_dim) || !aligned(out) ||
-      !aligned(out_lo))
+  if (!rows_ok(q, sqt, sqh, head_dim) || !rows_ok(k, skt, skh, head_dim) || !rows_ok(v, svt, svh, head_dim) ||
+      !aligned(out) || !aligned(out_lo))
     return fail(EVO2_ERR_UNSUPPORTED, "packed_attention: operands must be 16-byte aligned rows");
   PackedArgs a = packed_args(cu, nseq, T, heads, kv, scale);
   a.q = Rows{static_cast<const bf16_t *>(q), sqt, sqh};
@@ -675,7 +697,7 @@ extern "C" int evo2_packed_attention(const void *q, int64_t sqt, int64_t sqh, co
 // Whether a workgroup of the dk, dv kernel takes one query head rather than all that
 // share its keys: where whole groups leave fewer workgroups than two for each CU.
 static bool packed_split(int64_t T, int64_t nseq, int64_t heads, int64_t kv) {
-  return heads > kv && (T / P_KG + nseq) * kv < 512;
+  return heads > kv && (T / (8 * P_WR) + nseq) * kv < 512;
 }
 
 extern "C" int64_t evo2_packed_attention_workspace_bytes(int64_t T, int64_t nseq, int64_t heads, int64_t kv,
@@ -690,14 +712,14 @@ extern "C" int evo2_packed_attention_backward(const void *dout, int64_t sdt, int
                                               const void *v, int64_t svt, int64_t svh, const int32_t *cu,
                                               int64_t nseq, const void *out, const void *out_lo,
                                               const float *lse, void *workspace, int64_t workspace_bytes,
-                                              void *dq, void *dk, void *dv, int64_t T, int64_t heads, int64_t kv, int64_t head_dim, float scale,
-                                              void *stream) {
+                                              void *dq, void *dk, void *dv, int64_t T, int64_t heads, int64_t kv,
+                                              int64_t head_dim, float scale, void *stream) {
   const int rc = check_sizes("packed_attention_backward", T, nseq, heads, kv, head_dim, scale);
   if (rc || T == 0) return rc;
   if (!dout || !q || !k || !v || !cu || !out || !out_lo || !lse || !workspace || !dq || !dk || !dv)
     return fail(EVO2_ERR_INVALID, "packed_attention_backward: null pointer argument");
-  if (!rows_ok(dout, sdt, sdh, head_dim) || !rows_ok(q, sqt, sqh, head_dim) || !rows_ok(k, skt, skh, head_dim) || !rows_ok(v, svt, svh, head_dim) ||
-      !aligned(out) || !aligned(out_lo) || !aligned(dq) || !aligned(dk) || !aligned(dv) ||
+  if (!rows_ok(dout, sdt, sdh, head_dim) || !rows_ok(q, sqt, sqh, head_dim) || !rows_ok(k, skt, skh, head_dim) ||
+      !rows_ok(v, svt, svh, head_dim) || !aligned(out) || !aligned(out_lo) || !aligned(dq) || !aligned(dk) || !aligned(dv) ||
       !aligned(workspace))
     return fail(EVO2_ERR_UNSUPPORTED, "packed_attention_backward: operands must be 16-byte aligned rows");
   if (workspace_bytes < evo2_packed_attention_workspace_bytes(T, nseq, heads, kv, head_dim))

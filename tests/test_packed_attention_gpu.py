@@ -108,6 +108,17 @@ def test_against_64_bits(lens, heads, kv, hd):
     _check(_grads(q, k, v, d, cu, scale), want, "training")
 
 
+@pytest.mark.parametrize("heads,kv,hd,pad", [(8, 8, 128, (3, 40)), (16, 2, 128, (260, 5)), (6, 3, 128, (0, 1)),
+                                             (16, 4, 64, (7, 300))])
+def test_enough_workgroups_for_larger_ones(heads, kv, hd, pad):
+    """Key tiles of 256 rows, whole, cut short and of one key, behind one another; rows
+    outside the sequences cleared by workgroups of that size."""
+    lens = [513, 31, 257, 0, 256] + [2, 1] * 30 + [300]
+    q, k, v, d, cu = _case(lens, heads, kv, hd, seed=heads + pad[0], pad=pad)
+    print(f"packed_attention, larger workgroups {heads} {kv} {hd} {pad}", flush=True)
+    _check(_grads(q, k, v, d, cu, hd ** -0.5), _exact(q, k, v, d, cu, hd ** -0.5), "training")
+
+
 @pytest.mark.parametrize("pad", [(0, 9), (130, 0), (3, 300)])
 def test_rows_outside_the_sequences(pad):
     """Rows before the first and behind the last sequence: zeros, and zero gradients,
