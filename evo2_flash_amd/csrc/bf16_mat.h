@@ -43,9 +43,10 @@ enum MatForm { MAT_NT = 0, MAT_NN = 1, MAT_TN = 2 };
 enum MatEpi {
   MAT_BF16 = 0,   // out as bf16
   MAT_F32 = 1,    // fp32 partial sums, one plane per split (or added to what is there)
-  MAT_GATED = 2,  // act(x w^T) * (x w2^T), and both factors of its gradients
+  MAT_GATED = 2,  // (x w^T) * (x w2^T), and both factors of its gradients
   MAT_STATS = 3,  // each row's max and sum of exponentials over 128 columns
   MAT_DLOG = 4,   // the gradient of the cross entropy at the logits
+  MAT_GELU = 5,   // gelu(x w^T) * (x w2^T), as MAT_GATED
 };
 
 constexpr int MAT_CUS = 256;     // workgroups a launch fills the card with
@@ -68,7 +69,7 @@ struct MatArgs {
   void *out, *out2; int64_t so;
   int64_t plane;                          // MAT_F32: elements between the splits' partial sums
   int add;                                // MAT_F32: add to out
-  bf16_t *kept; int64_t kplane; int gelu; // MAT_GATED: what the backward pass needs, or null
+  bf16_t *kept; int64_t kplane;           // MAT_GATED, MAT_GELU: what the backward pass needs, or null
   // cross entropy: rows' targets (less col0), log-sum-exp, upstream gradient
   const int64_t *targets; int64_t ignore; int64_t V; int64_t col0;
   const float *lse; const float *grad; int64_t sgrad;
@@ -96,10 +97,23 @@ __host__ __device__ inline void mat_tile(int t, int tiles_m, int tiles_n, int sp
   bn = 4 * panel + (s - bm * width);
 }
 
-// gelu(x) = x cdf(x), and its slope cdf(x) + x pdf(x).
+// gelu(x) = x cdf(x), and its slope cdf(x) + x pdf(x).  The tail cdf(-|x|) is
+// exp(-x^2 / 2) t Q(t) with t = 1 / (1 + |x| / 4): Q, a polynomial of degree 6 fitted to
+// erfc(|x| / sqrt 2) exp(x^2 / 2) / (2 t) over |x| < 14, is off by 3e-9 of the cdf, the
+// fp32 steps by up to 3e-7; the tail keeps its leading digits (to 1e-3 at -13), which
+// 1 + erf loses below -5, and one exponential serves both results without a branch (by
+// erff 2048 rows of 5120 x 1920, kept, took 118 us, so 100).
 __device__ __forceinline__ void gelu_both(const float x, float &value, float &slope) {
-  const float cdf = fmaf(0.5f, erff(x * 0.70710678118654752f), 0.5f);
-  slope = fmaf(x * 0.39894228040143268f, __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f), cdf);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.25f, fabsf(x), 1.0f));
+  const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
+  float q = fmaf(-0.08913502097129822f, t, 0.3290213942527771f);
+  q = fmaf(q, t, -0.24036912620067596f);
+  q = fmaf(q, t, 0.2513173818588257f);
+  q = fmaf(q, t, 0.043495841324329376f);
+  q = fmaf(q, t, 0.10600420832633972f);
+  q = fmaf(q, t, 0.0996653363108635f);
+  const float tail = q * t * e, cdf = x > 0.0f ? 1.0f - tail : tail;
+  slope = fmaf(x * 0.39894228040143268f, e, cdf);
   value = x * cdf;
 }
 
@@ -128,6 +142,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   __shared__ __align__(16) bf16_t w0[WST], w1[WST], w2s[NST > 2 ? WST : 8];
   __shared__ __align__(16) bf16_t x0[XST], x1[XST], x2s[NST > 2 ? XST : 8];
   __shared__ __align__(16) float turned[4][32 * 32];        // a wave's 32 x 32 results, by rows
+  constexpr bool PAIR = EPI == MAT_GATED || EPI == MAT_GELU;
   constexpr int DB = 8, DX = 2 * TM;  // 1 KB loads of w and x per wave and slice
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -204,8 +219,8 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     } else {
       const int k0 = s * MAT_BK;
       // a gated tile takes 64 rows of each weight for a wave's 128 columns
-      const int n0 = EPI == MAT_GATED ? dbn * (MAT_BN / 2) + 64 * (wave >> 1) : dbn * MAT_BN + 64 * wave;
-      wb = (EPI == MAT_GATED && (wave & 1) ? p.w2 : p.w) + n0 * p.sw + k0;
+      const int n0 = PAIR ? dbn * (MAT_BN / 2) + 64 * (wave >> 1) : dbn * MAT_BN + 64 * wave;
+      wb = (PAIR && (wave & 1) ? p.w2 : p.w) + n0 * p.sw + k0;
       wrows = max(0, min(64, p.N - n0));
       wleft = max(0, p.K - k0);
     }
@@ -347,15 +362,16 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
 
   // Lane (lr, g) holds, for row m = wm + 32 tm + lr of the tile, columns
   // wn + 32 tn + 8 q + 4 g + i in acc[tn][tm][4 q + i].  Results go to memory by way of
-  // a wave's own 32 rows of 128 bytes in LDS (16-byte chunk c of row r at c ^ (r & 7)), which turn them so that eight lanes
-  // store one whole 128-byte line of a row: stored as they lie, each line takes four
-  // requests, and the caches' request rate bounds the burst at a tile's end.
+  // a wave's own 32 rows of 128 bytes in LDS (16-byte chunk c of row r at c ^ (r & 7)),
+  // which turn them so that eight lanes store one whole 128-byte line of a row: stored
+  // as they lie, each line takes four requests, and the caches' request rate bounds the
+  // burst at a tile's end.
   auto epilogue = [&](int j) __attribute__((always_inline)) {
     int bm, bn, sp;
     mat_tile(static_cast<int>(blockIdx.x) + j * grid, p.tiles_m, p.tiles_n, p.splits, bm, bn, sp);
     const bool second = FORM == MAT_TN && bm >= p.mpair;
     const int m0 = (second ? bm - p.mpair : bm) * BM + wm;      // wave's first row
-    const int n0 = bn * (EPI == MAT_GATED ? MAT_BN / 2 : MAT_BN) + (EPI == MAT_GATED ? wn / 2 : wn);
+    const int n0 = bn * (PAIR ? MAT_BN / 2 : MAT_BN) + (PAIR ? wn / 2 : wn);
     const float factor = EPI == MAT_BF16 ? mat_factor(p.num, p.den) : 1.0f;
     float *tb = turned[wave];
     const int tr = lane >> 3, tc = lane & 7;  // turned: lane's row of eight, 16-byte chunk
@@ -369,7 +385,8 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint2 *>(b + lr * 64 + 8 * ((4 * t + q) ^ (lr & 7)) + 4 * g) = make_uint2(v(t, 4 * q), v(t, 4 * q + 2));
+          *reinterpret_cast<uint2 *>(b + lr * 64 + 8 * ((4 * t + q) ^ (lr & 7)) + 4 * g) =
+              make_uint2(v(t, 4 * q), v(t, 4 * q + 2));
       fence();
       bf16_t *o = out + m * so + n0 + c;
 #pragma unroll
@@ -437,28 +454,32 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
 #pragma unroll
         for (int tn = 0; tn < 4; ++tn)
           put_f32(out, p.so, mr, 32 * tn, p.add != 0, [&](int i) { return acc[tn][tm][i]; });
-      } else if constexpr (EPI == MAT_GATED) {
+      } else if constexpr (PAIR) {
         // h = act(z1) z2, and for the backward pass a = z2 act'(z1) and b = act(z1), in
         // place of z1 and z2, as three planes of 16 bits: the high halves of both and
         // the next eight bits of each (24 of 32 bits, off by at most 2^-16: rounded to
         // bf16 they would put a second rounding under d1 and d2; as fp32 the tile's
         // stores and the gradient kernel's loads are a third more)
+        // (gelu is a kernel of its own: its slopes held registers of the other, 777 x 11264
+        // x 4096 151 us rather than 142)
         float slope[2][16];
+        if constexpr (EPI == MAT_GELU) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float value = acc[t][tm][i];
-            slope[t][i] = 1.0f;
-            if (p.gelu) gelu_both(value, value, slope[t][i]);  // uniform
-            acc[t][tm][i] = value;
-          }
+            for (int i = 0; i < 16; ++i) {
+              float value;
+              gelu_both(acc[t][tm][i], value, slope[t][i]);
+              acc[t][tm][i] = value;
+            }
+        }
         put16(static_cast<bf16_t *>(p.out), p.so, mr, 0, p.N, [&](int t, int i) {
           return pack_bf(acc[t][tm][i] * acc[t + 2][tm][i], acc[t][tm][i + 1] * acc[t + 2][tm][i + 1]);
         });
         if (p.kept) {  // uniform
           auto bits = [&](int t, int i, int which) {
-            const float v = which ? acc[t][tm][i] : acc[t + 2][tm][i] * slope[t][i];
+            const float a = EPI == MAT_GELU ? acc[t + 2][tm][i] * slope[t][i] : acc[t + 2][tm][i];
+            const float v = which ? acc[t][tm][i] : a;
             return __float_as_uint(v);
           };
 #pragma unroll
@@ -477,28 +498,35 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
         // target's logit where it lies among them
         const int limit = p.N - n0;  // columns of the vocabulary from the wave's first
         const int lim = limit - 4 * g;
-        auto logit = [&](int tn, int i) {
-          return 32 * tn + 8 * (i >> 2) + (i & 3) < lim ? acc[tn][tm][i] : -INFINITY;
-        };
-        float mx = -INFINITY;
-#pragma unroll
-        for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, logit(tn, i));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float sub = mx == -INFINITY ? 0.0f : mx * 1.44269504088896341f;
         const int64_t t = live ? p.targets[m] - n0 : -1;
         // the target's place among the lane's own columns (the lane with none: past all)
         const int at = t >= 0 && t < min(128, limit) && ((t >> 2) & 1) == g ? static_cast<int>(t) - 4 * g : -1;
-        float sum = 0.0f, zt = 0.0f;
+        float mx = -INFINITY, sum = 0.0f, zt = 0.0f;
+        // EDGE: with columns past the vocabulary or a target among them.  A wave whose 128
+        // columns have neither, as most, compares nothing (4096 x 131072 x 4096: 3230 ->
+        // 3160 us; the same for MAT_DLOG gained nothing)
+        auto stats = [&](auto edge) __attribute__((always_inline)) {
+          constexpr bool EDGE = decltype(edge)::value;
+          auto logit = [&](int tn, int i) {
+            return !EDGE || 32 * tn + 8 * (i >> 2) + (i & 3) < lim ? acc[tn][tm][i] : -INFINITY;
+          };
 #pragma unroll
-        for (int tn = 0; tn < 4; ++tn)
+          for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float v = logit(tn, i);
-            sum += __builtin_amdgcn_exp2f(fmaf(v, 1.44269504088896341f, -sub));
-            zt = at == 32 * tn + 8 * (i >> 2) + (i & 3) ? v : zt;
-          }
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, logit(tn, i));
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float sub = mx == -INFINITY ? 0.0f : mx * 1.44269504088896341f;
+#pragma unroll
+          for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float v = logit(tn, i);
+              sum += __builtin_amdgcn_exp2f(fmaf(v, 1.44269504088896341f, -sub));
+              if (EDGE) zt = at == 32 * tn + 8 * (i >> 2) + (i & 3) ? v : zt;
+            }
+        };
+        if (limit >= 128 && !__any(at >= 0)) stats(std::false_type{});
+        else stats(std::true_type{});
         sum += __shfl_xor(sum, 32);
         if (live) {
           if (g == 0) p.part[static_cast<int64_t>(2 * bn + (wave & 1)) * p.M + m] = make_float2(mx, sum);
@@ -561,31 +589,37 @@ struct MatPlan {
 // tile costs -- us per slice and us at its end, measured over 512 to 10240 of K -- and
 // where few tiles let K be split, the partial sums' second launch and their bytes
 // there and back.  Measured, us for tm 1 / 2 / 3 / 4:
-//   NT     777 x 49999 x 1920             223 / 207 / 191 / 214
-//          4096 x 131072 x 4096           - / - / 3472 / 3280
-//   gated  777 x 11264 x 4096             184 / 163 / 152 / 189
-//          2048 x 5120 x 1920             126 / 126 / 124 / 167
-//          8192 x 11264 x 4096            1665 / 1350 / - / 1412
+//   NT     777 x 49999 x 1920             190 / 165 / 154 / 184
+//          4096 x 131072 x 4096           4999 / 3808 / 3590 / 3341
+//   gated  777 x 11264 x 4096             182 / 159 / 145 / 188
+//          the same, gelu                 179 / 160 / 156 / 187
+//          2048 x 5120 x 1920, kept       94 / 88 / 82 / 138
+//          the same, gelu                 101 / 97 / 113 / 132
+//          8192 x 11264 x 4096, kept      1740 / 1363 / 1283 / 1363
+//          the same, gelu                 1815 / 1418 / 1471 / 1369
 //   NN     2048 x 1920 x 10240            106 / 95 / 102 / 90 (split by 1, 2, 2, 4)
 //          32768 x 4096 x 512             262 / 214 / 180 / 202
 //          8192 x 4096 x 22528            1749 / 1474 / - / 1157
 //   TN     512 x 4096 x 32768             208 / 163 / - / 147 (split by 2, 4, -, 8)
 //          49999 x 1920 x 777             294 / 235 / - / 206
 //          22528 x 4096 x 8192            1926 / 1285 / - / 1177
-// M: rows of one of `pair` outputs; slices: of K; width: output columns per tile.
+// M: rows of one of `pair` outputs; slices: of K; width: output columns per tile;
+// gated: 0, or 1 + (kept: four 16-bit outputs rather than one) + 2 (gelu).
 inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int pair, int width,
-                        bool may_split) {
-  const bool gated = width < MAT_BN;  // (four 16-bit outputs rather than one)
+                        bool may_split, int gated = 0) {
   static const double slice[4][5] = {{0, 0.60, 0.93, 1.30, 1.62},   // NT
                                      {0, 0.66, 1.00, 1.40, 1.72},   // NN
                                      {0, 0.66, 1.00, 1.30, 1.72},   // TN
-                                     {0, 0.60, 0.80, 1.20, 1.72}};  // NT, gated
-  static const double ends[2][5] = {{0, 4.0, 6.0, 7.0, 14.0}, {0, 7.0, 11.0, 17.0, 25.0}};
+                                     {0, 0.52, 0.83, 1.19, 1.54}};  // NT, gated
+  static const double ends[5][5] = {{0, 4.0, 6.0, 7.0, 14.0},
+                                    {0, 3.5, 4.5, 4.5, 14.0},
+                                    {0, 5.5, 10.0, 10.5, 33.0},
+                                    {0, 5.0, 7.0, 13.0, 17.0},
+                                    {0, 7.5, 12.5, 24.0, 31.0}};
   const double *each = slice[gated ? 3 : form], *end = ends[gated];
   MatPlan best{};
   double least = 1e300;
   for (int tm : {4, 3, 2, 1}) {
-    
     if (form == MAT_TN && tm == 3) continue;  // (rows of 192 do not fill whole load blocks)
     const int nst = mat_stages(tm);
     const int64_t tm_tiles = cdiv(M, 64 * tm) * pair, tn_tiles = cdiv(N, width), tiles = tm_tiles * tn_tiles;

@@ -81,6 +81,29 @@ def test_against_64_bits(M, I, H, gelu):
     _check(_grads(x, w1, w2, gelu, dh), want, "training")
 
 
+def test_gelu_tails():
+    """gelu of values set by the input (z1 = v, z2 = 1): to a relative 1e-3 down to -12,
+    where the 24 bits of 1 + erf have long been lost, and one rounding; its slope, by
+    way of dx, to 2e-6 and the roundings of dz, of its kept factor and of dx."""
+    v = torch.cat([torch.linspace(-12, 12, 1023), torch.tensor([0.0])]).to(BF).to(DEV)
+    x = torch.zeros(v.numel(), 64, device=DEV, dtype=BF)
+    x[:, 0], x[:, 1] = v, 1.0
+    w1, w2 = (torch.zeros(8, 64, device=DEV, dtype=BF) for _ in range(2))
+    w1[0, 0] = w2[0, 1] = 1.0
+    x.requires_grad_()
+    h = gated_linear(x, w1, w2, True)
+    dh = torch.zeros_like(h)
+    dh[:, 0] = 1.0
+    dx, = torch.autograd.grad(h, x, dh)
+    z = v.double()
+    cdf = 0.5 * torch.special.erfc(-z / 2 ** 0.5)
+    value = z * cdf
+    assert ((h[:, 0].double() - value).abs() <= (U + 1.1e-3) * value.abs()).all()
+    assert not h[:, 1:].any()
+    slope = cdf + z * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+    assert ((dx[:, 0].double() - slope).abs() <= (2.02 * U + 2.0 ** -16) * slope.abs() + 2e-6).all()
+
+
 def test_gradient_against_differences():
     """The product is quadratic in x and in each weight linear (identity): along a
     direction exact in bf16, central differences are the gradient but for the outputs'
