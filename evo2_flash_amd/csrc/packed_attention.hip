@@ -93,20 +93,24 @@ __device__ __forceinline__ void p_bounds(const PackedArgs &p, int s, int &begin,
   len = min(max(p.cu[s + 1], begin), p.T) - begin;
 }
 
-// Slot t of the tiles of `rows` rows: sequence s's start at cu[s] / rows + s, which leaves it at
-// least as many as it needs, so a slot finds its sequence from the table alone (one
-// load per 64 sequences) and the host never reads it.  False: nothing there.
+// Slot t of the tiles of `rows` rows: sequence s's start at cu[s] / rows + s, which leaves
+// it at least as many as it needs, so a slot finds its sequence, the last that starts at
+// or before it, from the table alone (a search by 64ths, one load a step) and the host
+// never reads it.  False: nothing there.
 __device__ __forceinline__ bool p_slot(const PackedArgs &p, int t, int lane, int rows, int &begin, int &len,
                                       int &r0) {
-  int s = -1;
-  for (int b = 0; b < p.nseq; b += 64) {
-    const int i = b + lane;
-    const bool at = i < p.nseq && min(max(p.cu[i], 0), p.T) / rows + i <= t;
-    const int n = __popcll(__ballot(at));
-    s += n;
-    if (n < 64) break;
+  int s = 0;  // it is among s .. s + n - 1
+  for (int n = p.nseq, step; n > 0; n = min(step, n)) {
+    step = (n - 1) / 64 + 1;
+    const int i = s + lane * step;  // (below 2^31: step is at most nseq / 64 + 1)
+    const bool at = i < s + n && min(max(p.cu[i], 0), p.T) / rows + i <= t;
+    const int c = __popcll(__ballot(at));
+    if (c == 0) return false;  // (none starts at or before the slot: the first step's only)
+    s += (c - 1) * step;
+    n -= (c - 1) * step;
+    if (step == 1) break;
   }
-  if (s < 0) return false;
+  if (p.nseq == 0) return false;
   p_bounds(p, s, begin, len);
   r0 = (t - begin / rows - s) * rows;
   return r0 >= 0 && r0 < len;

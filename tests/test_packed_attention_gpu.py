@@ -119,6 +119,17 @@ def test_enough_workgroups_for_larger_ones(heads, kv, hd, pad):
     _check(_grads(q, k, v, d, cu, hd ** -0.5), _exact(q, k, v, d, cu, hd ** -0.5), "training")
 
 
+@pytest.mark.parametrize("nseq", [64, 65, 4097])
+def test_many_sequences(nseq):
+    """Tables of one, two and three search steps, empty sequences among them."""
+    g = torch.Generator().manual_seed(nseq)
+    lens = torch.randint(0, 4, (nseq,), generator=g).tolist()
+    lens[nseq // 2] = 300
+    q, k, v, d, cu = _case(lens, 2, 1, 64, seed=nseq, pad=(1, 2))
+    print(f"packed_attention, {nseq} sequences", flush=True)
+    _check(_grads(q, k, v, d, cu, 0.125), _exact(q, k, v, d, cu, 0.125), "training")
+
+
 @pytest.mark.parametrize("pad", [(0, 9), (130, 0), (3, 300)])
 def test_rows_outside_the_sequences(pad):
     """Rows before the first and behind the last sequence: zeros, and zero gradients,
