@@ -604,17 +604,17 @@ struct MatPlan {
 //          49999 x 1920 x 777             294 / 235 / - / 206
 //          22528 x 4096 x 8192            1926 / 1285 / - / 1177
 // M: rows of one of `pair` outputs; slices: of K; width: output columns per tile;
-// gated: 0, or 1 + (kept: four 16-bit outputs rather than one) + 2 (gelu).
+// gated: 0, or 1 + gelu (costs with what the backward pass needs kept; without, a tile's
+// end is 2 to 19 us shorter and the choice the same or 3% behind at these sizes, but a
+// plan by it would sum K in another order where a gradient is recorded).
 inline MatPlan mat_plan(MatForm form, int64_t M, int64_t N, int64_t slices, int pair, int width,
                         bool may_split, int gated = 0) {
   static const double slice[4][5] = {{0, 0.60, 0.93, 1.30, 1.62},   // NT
                                      {0, 0.66, 1.00, 1.40, 1.72},   // NN
                                      {0, 0.66, 1.00, 1.30, 1.72},   // TN
                                      {0, 0.52, 0.83, 1.19, 1.54}};  // NT, gated
-  static const double ends[5][5] = {{0, 4.0, 6.0, 7.0, 14.0},
-                                    {0, 3.5, 4.5, 4.5, 14.0},
+  static const double ends[3][5] = {{0, 4.0, 6.0, 7.0, 14.0},
                                     {0, 5.5, 10.0, 10.5, 33.0},
-                                    {0, 5.0, 7.0, 13.0, 17.0},
                                     {0, 7.5, 12.5, 24.0, 31.0}};
   const double *each = slice[gated ? 3 : form], *end = ends[gated];
   MatPlan best{};

@@ -103,7 +103,7 @@ extern "C" int evo2_gated_linear(const void *x, int64_t sx, const void *w1, cons
   a.so = sh;
   a.kept = static_cast<bf16_t *>(kept);
   a.kplane = M * I;
-  const MatPlan pl = mat_plan(MAT_NT, M, I, cdiv(H, MAT_BK), 1, MAT_BN / 2, false, 1 + !!kept + 2 * !!gelu);
+  const MatPlan pl = mat_plan(MAT_NT, M, I, cdiv(H, MAT_BK), 1, MAT_BN / 2, false, 1 + !!gelu);
   if (gelu) mat_launch<MAT_NT, MAT_GELU>(a, pl, static_cast<hipStream_t>(stream));
   else mat_launch<MAT_NT, MAT_GATED>(a, pl, static_cast<hipStream_t>(stream));
   return check_launch("gated_linear");

@@ -170,6 +170,15 @@ def test_forms_of_call():
             <= 2 * U * got.float().abs() + 1e-30).all()
 
 
+@pytest.mark.parametrize("gelu", [False, True])
+@pytest.mark.parametrize("M,I,H", [(777, 2056, 1032), (2048, 1288, 1032)])
+def test_same_bits_with_and_without_a_gradient(M, I, H, gelu):
+    x, w1, w2, _ = _case(M, I, H, seed=14)
+    with torch.no_grad():
+        want = gated_linear(x, w1, w2, gelu)
+    assert torch.equal(gated_linear(x.requires_grad_(), w1, w2, gelu), want)
+
+
 def test_nothing_spreads_between_rows():
     """A row of NaN or infinities reaches its own outputs only (and the weights'
     gradients)."""
