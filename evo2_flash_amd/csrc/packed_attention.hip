@@ -434,15 +434,18 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
 
 // dk and dv of KW waves' keys.  A wave's 32 x HD sums of both take half its
 // registers, its keys' B operands an eighth; its values' are read from LDS again for
-// every tile.  Heads of 64: held to what three workgroups of a CU can have (16384 tokens
-// of 16 heads 1139 -> 1070 us).  SPLIT: one query head per workgroup, fp32 sums to
-// `part`, which a second kernel joins over the heads that share a key head.
+// every tile, but by four waves of heads of 128, which have the registers (2048 tokens of
+// 32 heads 107 -> 102 us; with eight waves they spilled, 1133 -> 1420 us for 8192 tokens).
+// Heads of 64: held to what three workgroups of a CU can have (16384 tokens of 16 heads
+// 1139 -> 1070 us).  SPLIT: one query head per workgroup, fp32 sums to `part`, which a
+// second kernel joins over the heads that share a key head.
 template <int HD, bool SPLIT, int KW>
 __global__ __launch_bounds__(64 * KW, HD == 64 ? 3 : 1) void packed_dkv_kernel(PackedArgs p) {
   constexpr int KG = KW * P_WR;  // keys of the workgroup
   constexpr int TILE = p_tile<HD>(P_TR);
+  constexpr bool OWN = HD == 128 && KW == 4;  // values in registers
   __shared__ __align__(16) bf16_t q0s[TILE], q1s[TILE], d0s[TILE], d1s[TILE];
-  __shared__ __align__(16) bf16_t vs[p_tile<HD>(KG)];                   // the workgroup's values
+  __shared__ __align__(16) bf16_t vs[OWN ? 8 : p_tile<HD>(KG)];         // the workgroup's values
   __shared__ __align__(16) float l0s[P_TR], l1s[P_TR], e0s[P_TR], e1s[P_TR];  // log-sum-exp, delta
   const int w = static_cast<int>(blockIdx.x);
   if (w >= p.items) {
@@ -470,8 +473,8 @@ __global__ __launch_bounds__(64 * KW, HD == 64 ? 3 : 1) void packed_dkv_kernel(P
   lq.init(p.q.p, p.q.st, wave, lane);
   ld.init(p.d.p, p.d.st, wave, lane);
   lv.init(p.v.p + begin * p.v.st + hk * p.v.sh, p.v.st, wave, lane);
-#pragma unroll
-  for (int i = 0; i < KG / P_TR; ++i) lv.issue(vs + i * TILE, r0 + i * P_TR, len);
+  if constexpr (!OWN)
+    for (int i = 0; i < KG / P_TR; ++i) lv.issue(vs + i * TILE, r0 + i * P_TR, len);
   int ih = 0, ib = 0;  // the next tile to load: head of the group, tile of its sweep
   auto issue = [&](bf16_t *qs, bf16_t *ds, float *ls, float *es) __attribute__((always_inline)) {
     const int h = h0 + ih, row = r0 + ib * P_TR;
@@ -491,6 +494,8 @@ __global__ __launch_bounds__(64 * KW, HD == 64 ? 3 : 1) void packed_dkv_kernel(P
   issue(q0s, d0s, l0s, e0s);
   abf16x8_t k[HD / 16];
   p_own<HD>(k, p.k, begin + min(ki, len - 1), hk, g);
+  abf16x8_t v[OWN ? HD / 16 : 1];
+  if constexpr (OWN) p_own<HD>(v, p.v, begin + min(ki, len - 1), hk, g);
   pf32x16_t dk[HD / 32] = {}, dv[HD / 32] = {};
 
   int cb = 0;  // tile of the current sweep
@@ -510,8 +515,10 @@ __global__ __launch_bounds__(64 * KW, HD == 64 ? 3 : 1) void packed_dkv_kernel(P
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
         s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(qs, u, kk, lr, g), k[kk], s, 0, 0, 0);
-        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(ds, u, kk, lr, g), p_rows<HD>(vs, wave, kk, lr, g),
-                                                     dp, 0, 0, 0);
+        abf16x8_t vk;
+        if constexpr (OWN) vk = v[kk];
+        else vk = p_rows<HD>(vs, wave, kk, lr, g);
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(ds, u, kk, lr, g), vk, dp, 0, 0, 0);
       }
       // (queries past the sequence: zero rows of q and do, whose log-sum-exp and
       // delta read as 0, so that ds = 0 and p meets do = 0)
@@ -638,11 +645,11 @@ static void launch_forward(PackedArgs a, hipStream_t st) {
 // Whether the dk, dv kernel's workgroups take eight waves rather than four.  Heads of
 // 128: eight share a swept tile, but such a workgroup fills a CU, so that up to about one
 // round of the CUs half as many keys in twice as many workgroups end sooner (us with
-// eight and with four waves, by workgroups of eight: 128 of them 57 and 46, 208: 153 and
-// 129, 272: 158 and 140, 288: 115 and 108 or 124 and 131, 320: 61 and 62, 384: 90 and
-// 115, 1056: 1056 and 1746).  Heads of 64: always four, three workgroups to a CU, which
-// fill each other's waits (8192 tokens of 32 heads 754 and 625 us, 8 x 1024 tokens 120
-// and 93).
+// eight and with four waves, by workgroups of eight: 160 of them 61 and 48, 208: 156 and
+// 124, 272: 163 and 142, 288: 114 and 102, 131 and 133 or 244 and 244, 320: 62 and 60 or
+// 260 and 270, 352: 147 and 166, 1056: 1085 and 1393).  Heads of 64: always four, three
+// workgroups to a CU, which fill each other's waits (8192 tokens of 32 heads 754 and 625
+// us, 8 x 1024 tokens 120 and 93).
 static bool packed_wide(const PackedArgs &a) {
   return (a.T / (8 * P_WR) + a.nseq) * (a.part ? a.heads : a.kv) >= 304;
 }
