@@ -67,7 +67,7 @@ struct PackedArgs {
   bf16_t *out, *lo;                 // (T, heads, HD)
   float *lse;                       // (heads, T), log2 units
   const bf16_t *o, *olo;
-  float *delta;                     // (heads, T)
+  float *delta;                     // (heads, T): -delta
   bf16_t *dq, *dk, *dv;
   float *part;                      // (heads, T, 2, HD): dk and dv by query head
 };
@@ -121,7 +121,7 @@ __device__ __forceinline__ bool p_slot(const PackedArgs &p, int t, int lane, int
 // through its L2; the longest sweeps of all its heads first (reversed: those of the last
 // queries), so that what is left at the end is short: head by head, 8192 tokens of 32
 // heads of 128 took 609, 812 and 1321 us forward, for dq and for dk, dv, so 588, 770 and
-// 1282 (dk, dv by now 1056).
+// 1282.
 __device__ __forceinline__ void p_item(int w, int heads, int tiles, bool reversed, int &h, int &t) {
   if (heads % 8 == 0) {
     const int j = w >> 3, per = heads >> 3;
@@ -386,8 +386,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
         delta = fmaf(static_cast<float>(d[kk][j]), static_cast<float>(o[kk][j]) + static_cast<float>(lo[kk][j]), delta);
   }
   delta += __shfl_xor(delta, 32);
-  if (g == 0 && qi < len) p.delta[static_cast<int64_t>(h) * p.T + row] = delta;
+  const float less = -delta;  // (dk and dv's kernel starts its sums from it)
+  if (g == 0 && qi < len) p.delta[static_cast<int64_t>(h) * p.T + row] = less;
   pf32x16_t acc[HD / 32] = {};
+  // dp starts from -delta where that is the faster (8192 tokens, 32 heads of 64: 395 ->
+  // 381 us; 2048 tokens, heads of 128: 72 -> 75)
+  constexpr bool START = HD == 64;
 
   auto block = [&](int b, const bf16_t *ks, const bf16_t *vs, bf16_t *kn, bf16_t *vn)
       __attribute__((always_inline)) {
@@ -401,14 +405,16 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs p) {
     const bool edge = kb0 + P_TR - 1 > wq0;  // wave-uniform: some keys come after some queries
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      pf32x16_t s = {}, dp = {};
+      pf32x16_t s = {}, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[i] = START ? less : 0.0f;
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
         s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(ks, u, kk, lr, g), q[kk], s, 0, 0, 0);
         dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(vs, u, kk, lr, g), d[kk], dp, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c2, -lse)) * (dp[i] - delta);
+      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c2, -lse)) * (START ? dp[i] : dp[i] - delta);
       if (edge) {  // keys after the query; a query of one key
         P_BRANCH;
         const int lim = qi == 0 ? -1 : qi - kb0 - 4 * g;
@@ -446,7 +452,7 @@ __global__ __launch_bounds__(64 * KW, HD == 64 ? 3 : 1) void packed_dkv_kernel(P
   constexpr bool OWN = HD == 128 && KW == 4;  // values in registers
   __shared__ __align__(16) bf16_t q0s[TILE], q1s[TILE], d0s[TILE], d1s[TILE];
   __shared__ __align__(16) bf16_t vs[OWN ? 8 : p_tile<HD>(KG)];         // the workgroup's values
-  __shared__ __align__(16) float l0s[P_TR], l1s[P_TR], e0s[P_TR], e1s[P_TR];  // log-sum-exp, delta
+  __shared__ __align__(16) float l0s[P_TR], l1s[P_TR], e0s[P_TR], e1s[P_TR];  // log-sum-exp, -delta
   const int w = static_cast<int>(blockIdx.x);
   if (w >= p.items) {
     if (!SPLIT) {
@@ -511,7 +517,13 @@ __global__ __launch_bounds__(64 * KW, HD == 64 ? 3 : 1) void packed_dkv_kernel(P
     for (int u = 0; u < 2; ++u) {
       const int qt0 = qb0 + 32 * u;
       if (qt0 < wk0) continue;  // wave-uniform: queries before all of the wave's keys
-      pf32x16_t s = {}, dp = {};
+      pf32x16_t s = {}, dp;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {  // dp - delta
+        const af32x4_t ee = *reinterpret_cast<const af32x4_t *>(es + 32 * u + 8 * b + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dp[4 * b + i] = ee[i];  // from LDS, no subtraction (1144 -> 1129 us)
+      }
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
         s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p_rows<HD>(qs, u, kk, lr, g), k[kk], s, 0, 0, 0);
@@ -525,11 +537,10 @@ __global__ __launch_bounds__(64 * KW, HD == 64 ? 3 : 1) void packed_dkv_kernel(P
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const af32x4_t ll = *reinterpret_cast<const af32x4_t *>(ls + 32 * u + 8 * b + 4 * g);
-        const af32x4_t ee = *reinterpret_cast<const af32x4_t *>(es + 32 * u + 8 * b + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s[4 * b + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * b + i], p.c2, -ll[i]));
-          dp[4 * b + i] = s[4 * b + i] * (dp[4 * b + i] - ee[i]);
+          dp[4 * b + i] *= s[4 * b + i];
         }
       }
       if (qt0 == wk0) {  // wave-uniform: the diagonal tile (rows of both start on 32s)
