@@ -203,6 +203,13 @@ __device__ __forceinline__ abf16x8_t p_pack(const pf32x16_t &s, int half) {
   return __builtin_bit_cast(abf16x8_t, u);
 }
 
+// Max of lanes l and l + 32, in both (by a swap of registers: a shuffle through LDS waits
+// for the fragments read before it; 8192 tokens, 32 heads of 64 on 8: 322 -> 303 us).
+__device__ __forceinline__ float p_max_pair(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
 // A wave's own rows as B operands: row lr, K step kk.
 template <int HD>
 __device__ __forceinline__ void p_own(abf16x8_t (&f)[HD / 16], const Rows &r, int64_t row, int h, int g) {
@@ -304,7 +311,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs p) {
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-    top = fmaxf(top, __shfl_xor(top, 32)) * p.c2;
+    top = p_max_pair(top) * p.c2;
     // the reference max moves only past the slack (from -inf: at the first score)
     const bool move = top > m + P_SLACK;
     const float mn = move ? top : m, sub = mn == -INFINITY ? 0.0f : mn;
