@@ -81,9 +81,13 @@ __device__ __forceinline__ au32x4_t lds_rsrc(const void *p, uint32_t bytes) {
 // One direct-to-LDS load: 64 lanes x 16 bytes at byte offset v (zeros past the
 // descriptor) to lds .. lds + 1 KB.  In asm so that the compiler does not know of it:
 // before each transposing LDS read it would wait for all such loads in flight.  The
-// kernel waits for them itself (lds_sync), and no register is written.
+// kernel waits for them itself (lds_sync), and no register is written.  The wait states
+// that the compiler would put before the load stand in the asm: one after the write of m0,
+// and five after a vector instruction that wrote part of the descriptor (lds_rsrc's
+// readfirstlane, or the reload of a spilled register, wherever those land), which the
+// hardware does not interlock: the load would go by the old word.
 __device__ __forceinline__ void lds_load(au32x4_t rsrc, uint32_t v, const bf16_t *lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds_addr(lds)), "v"(v), "s"(rsrc)
                : "m0");
@@ -91,7 +95,7 @@ __device__ __forceinline__ void lds_load(au32x4_t rsrc, uint32_t v, const bf16_t
 
 // The same, 64 lanes x 4 bytes.
 __device__ __forceinline__ void lds_load4(au32x4_t rsrc, uint32_t v, const void *lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(lds_addr(lds)), "v"(v), "s"(rsrc)
                : "m0");
