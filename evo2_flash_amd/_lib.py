@@ -440,9 +440,11 @@ def on_device(t):
 
 def rows16(t):
     """t (rows, n of a multiple of 8, 16-bit) with rows of unit stride that start
-    on 16 bytes and do not overlap: itself, or a copy."""
+    on 16 bytes, do not overlap and lie within the matrix kernels' 32-bit offsets of one
+    another (fewer than 2^22 elements: the last position of long sequences is a view of
+    rows further apart, also where it has one row): itself, or a copy."""
     row, unit = t.stride()
-    if unit != 1 or row & 7 or row < t.shape[1] or t.data_ptr() & 15:
+    if unit != 1 or row & 7 or not t.shape[1] <= row < 1 << 22 or t.data_ptr() & 15:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 

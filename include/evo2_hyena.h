@@ -472,7 +472,8 @@ int evo2_bf16_stream_gated(const void *x, int64_t sx, const void *w1, const void
  *   dh (M, I) row stride sdh, dx (M, H), dw1, dw2 (I, H) contiguous, all bf16;
  *   kept: 6 M I bytes, written by the forward call where not NULL (z2 act'(z1) and
  *   act(z1) to 24 bits) and read by the backward call.  I and H multiples of 8, rows
- *   16-byte aligned.  dx may be NULL; dw1 and dw2 may be NULL together.  The backward call
+ *   16-byte aligned, sx and sw below 2^22.  dx may be NULL; dw1 and dw2 may be NULL
+ *   together.  The backward call
  *   takes M >= 1 and a workspace of _workspace_bytes(M, I, H) bytes.
  */
 int64_t evo2_gated_linear_workspace_bytes(int64_t M, int64_t I, int64_t H);
@@ -493,7 +494,8 @@ int evo2_gated_linear_backward(const void *dh, int64_t sdh, const void *x, int64
  *   d = (exp(h w_n - lse) - [n = target]) g, dh = d w, dw = d^T h, with g =
  *   grad[m * sgrad], divided by *count where count is not NULL (a mean's, sgrad 0)
  *   h (T, H) row stride sh, w (V, H) row stride sw, dh (T, H) and dw (V, H)
- *   contiguous, bf16, H a multiple of 8, V < 2^22, rows 16-byte aligned; targets (T,) int64;
+ *   contiguous, bf16, H a multiple of 8, V, sh and sw below 2^22, rows 16-byte aligned;
+ *   targets (T,) int64;
  *   nll, lse (T,), loss, count (1,), grad fp32.  dh or dw may be NULL.  T >= 1; the
  *   workspace has _workspace_bytes(T, V, H, backward) bytes.
  */
