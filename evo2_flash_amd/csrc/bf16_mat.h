@@ -117,6 +117,13 @@ __device__ __forceinline__ void gelu_both(const float x, float &value, float &sl
   value = x * cdf;
 }
 
+// x's bits, of which the high 24 are x rounded to nearest (ties away from 0; an infinity or
+// a NaN stays what it is).
+__device__ __forceinline__ uint32_t round24(const float x) {
+  const uint32_t u = __float_as_uint(x);
+  return x == x ? u + 0x80u : u;  // (an infinity's low byte is dropped again)
+}
+
 // What a row's softmax less its target is multiplied by: its upstream gradient, 0 of an
 // ignored row, NaN of a target outside the vocabulary.  Where all rows share the
 // upstream gradient (a sum or a mean) it is left to the products' results: times one
@@ -457,9 +464,9 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
       } else if constexpr (PAIR) {
         // h = act(z1) z2, and for the backward pass a = z2 act'(z1) and b = act(z1), in
         // place of z1 and z2, as three planes of 16 bits: the high halves of both and
-        // the next eight bits of each (24 of 32 bits, off by at most 2^-16: rounded to
-        // bf16 they would put a second rounding under d1 and d2; as fp32 the tile's
-        // stores and the gradient kernel's loads are a third more)
+        // the next eight bits of each (rounded to 24 of 32 bits, off by at most 2^-16, to
+        // either side: rounded to bf16 they would put a second rounding under d1 and d2; as
+        // fp32 the tile's stores and the gradient kernel's loads are a third more)
         // (gelu is a kernel of its own: its slopes held registers of the other, 777 x 11264
         // x 4096 151 us rather than 142)
         float slope[2][16];
@@ -479,8 +486,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
         if (p.kept) {  // uniform
           auto bits = [&](int t, int i, int which) {
             const float a = EPI == MAT_GELU ? acc[t + 2][tm][i] * slope[t][i] : acc[t + 2][tm][i];
-            const float v = which ? acc[t][tm][i] : a;
-            return __float_as_uint(v);
+            return round24(which ? acc[t][tm][i] : a);
           };
 #pragma unroll
           for (int which = 0; which < 2; ++which)

@@ -35,3 +35,46 @@ def test_the_last_position_of_long_sequences(B):
     tall = torch.empty(8, 1 << 22, dtype=BF, device=DEV)[:, :H].copy_(w[0, :8])
     assert torch.equal(gated_linear(x[:, -1], tall, tall, False),
                        gated_linear(x[:, -1], w[0, :8], w[0, :8], False))
+
+
+def _kept(x, w1, w2, gelu):
+    """Both factors that the gated product keeps for its gradients, from their planes: the
+    high 16 bits of each, then the next eight of both."""
+    from evo2_flash_amd.linear import _gated_forward
+
+    planes = _gated_forward(x, w1, w2, gelu, True)[1].to(torch.int32) & 0xffff
+    a, b, low = planes
+    return [t.view(torch.float32).double()
+            for t in ((a << 16) | ((low & 0xff) << 8), (b << 16) | (low & 0xff00))]
+
+
+@pytest.mark.parametrize("lower", [False, True])
+@pytest.mark.parametrize("M", [300, 2048])
+def test_kept_factors_are_rounded_to_nearest(M, lower):
+    """Products of 24 significant bits, exact in fp32 (a + b 2^-8 + c 2^-16 of 8-bit a, b,
+    c): kept to 16 bits, the nearest.  The last eight bits are 128 + an odd number, which
+    rounds up, or with `lower` (2^-16 taken off) the odd number, which rounds down; no ties.
+    Infinities and NaN stay what they are."""
+    g = torch.Generator().manual_seed(M)
+    x = torch.zeros(M, 64)
+    a, b, c = (torch.randint(0, n, (M,), generator=g) for n in (110, 128, 64))
+    x[:, 0], x[:, 1], x[:, 2] = 1 + a / 128, 1 + b / 128, 1 + (2 * c + 1) / 128
+    x[:, 3] = float(lower)
+    w = torch.zeros(2, 136, 64)
+    w[0, :, :4] = torch.tensor([1.0, 2.0 ** -8, 2.0 ** -16, -2.0 ** -16])
+    w[1] = -2 * w[0]
+    want = x.double() @ w.double().transpose(1, 2)  # z1, z2
+    x, w = x.to(BF).to(DEV), w.to(BF).to(DEV)
+    print(f"kept factors, {M} rows", flush=True)
+    a2, b1 = _kept(x, *w, False)
+    for got, z in ((a2, want[1]), (b1, want[0])):
+        step = 2.0 ** (torch.floor(torch.log2(z.abs())) - 15)
+        assert torch.equal(got.cpu(), torch.round(z / step) * step)
+    x[5], x[6, 0] = float("nan"), float("inf")
+    for gelu in (False, True):
+        a2, b1 = _kept(x, *w, gelu)
+        assert a2[5].isnan().all() and b1[5].isnan().all()
+        assert (b1[6] == float("inf")).all()
+        rest = torch.ones(M, dtype=torch.bool, device=DEV)
+        rest[5:7] = False
+        assert a2[rest].isfinite().all() and b1[rest].isfinite().all()
