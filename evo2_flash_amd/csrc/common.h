@@ -104,4 +104,7 @@ int check_launch(const char *what);
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Whether a launch takes so many workgroups: it counts a dimension's threads in 32 bits.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= 0xffffffff / threads; }
+
 }  // namespace evo2

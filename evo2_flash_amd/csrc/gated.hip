@@ -61,7 +61,8 @@ static int check_sizes(const char *what, int64_t M, int64_t I, int64_t H, int64_
   if (I % 8 || H % 8)
     return fail(EVO2_ERR_UNSUPPORTED, "%s: I=%lld and H=%lld must be multiples of 8", what, (long long)I,
                 (long long)H);
-  if (!mat_fits(M, up(I, 64) * 2, H, std::max({sx, sw, up(I, 64) * 2, H})) || !mat_fits(up(I, 64) * 2, H, M, H))
+  if (!mat_fits(M, up(I, 64) * 2, H, std::max({sx, sw, up(I, 64) * 2, H})) || !mat_fits(up(I, 64) * 2, H, M, H) ||
+      !mat_fits(M, H, I, H))
     return fail(EVO2_ERR_UNSUPPORTED, "%s: problem too large", what);
   return EVO2_OK;
 }
@@ -126,6 +127,8 @@ extern "C" int evo2_gated_linear_backward(const void *dh, int64_t sdh, const voi
                 (long long)workspace_bytes, (long long)evo2_gated_linear_workspace_bytes(M, I, H));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t Ip = up(I, MAT_BK), chunks = M * (Ip / 8);
+  if (!grid_fits(cdiv(chunks, 256), 256))
+    return fail(EVO2_ERR_UNSUPPORTED, "gated_linear_backward: problem too large");
   bf16_t *dz = static_cast<bf16_t *>(workspace);
   float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + up(M * 2 * Ip * 2, 256));
   hipLaunchKernelGGL(gated_grad_kernel, dim3(static_cast<unsigned>(cdiv(chunks, 256))), dim3(256), 0, st,

@@ -208,8 +208,9 @@ static int check_sizes(const char *what, int64_t T, int64_t V, int64_t H, int64_
     return fail(EVO2_ERR_INVALID, "%s: bad sizes T=%lld V=%lld H=%lld", what, (long long)T, (long long)V,
                 (long long)H);
   if (H % 8) return fail(EVO2_ERR_UNSUPPORTED, "%s: H=%lld must be a multiple of 8", what, (long long)H);
-  // (a piece's rows of d take V columns at most)
-  if (V >= (int64_t(1) << 22) || !mat_fits(T, V, H, std::max(sh, sw)) || !mat_fits(V, H, T, H))
+  // (a piece's rows of d take V columns at most; the joining kernel a workgroup for 16 rows)
+  if (V >= (int64_t(1) << 22) || !mat_fits(T, V, H, std::max(sh, sw)) || !mat_fits(V, H, T, H) ||
+      !mat_fits(T, H, V, H) || !grid_fits(cdiv(T, L_ROWS), 256))
     return fail(EVO2_ERR_UNSUPPORTED, "%s: problem too large", what);
   if (sh < H || sw < H || sh % 8 || sw % 8)
     return fail(EVO2_ERR_UNSUPPORTED, "%s: operands must be 16-byte aligned rows", what);
@@ -298,6 +299,8 @@ extern "C" int evo2_linear_loss_backward(const void *h, int64_t sh, const void *
   if (!dh && !dw) return EVO2_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const BackPlan b = plan_back(T, V, H);
+  if (b.pieces > 1 && !grid_fits(cdiv(T * (H / 8), 256), 256))  // dh's pieces are joined
+    return fail(EVO2_ERR_UNSUPPORTED, "linear_loss_backward: problem too large");
   char *at = static_cast<char *>(workspace);
   bf16_t *d = reinterpret_cast<bf16_t *>(at);
   float *acc = reinterpret_cast<float *>(at + up(T * b.ld * 2, 256));

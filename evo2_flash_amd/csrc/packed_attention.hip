@@ -631,9 +631,13 @@ static bool aligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 
 
 static int check_sizes(const char *what, int64_t T, int64_t nseq, int64_t heads, int64_t kv, int64_t hd, float scale) {
   if (T < 0 || nseq < 0 || heads <= 0 || kv <= 0 || heads % kv || T > 0x3fffffff || nseq > 0x3fffffff ||
-      (T / P_WG + nseq) * heads > 0x3fffffff)
+      heads > 0x3fffffff)
     return fail(EVO2_ERR_INVALID, "%s: bad sizes T=%lld nseq=%lld heads=%lld kv=%lld", what, (long long)T,
                 (long long)nseq, (long long)heads, (long long)kv);
+  // (the dk, dv kernel's workgroups are no more; packed_wide sees to those of eight waves)
+  if (!grid_fits((T / P_WG + nseq) * heads + P_FILL, 64 * P_NW))
+    return fail(EVO2_ERR_UNSUPPORTED, "%s: T=%lld nseq=%lld heads=%lld are more workgroups than a launch takes",
+                what, (long long)T, (long long)nseq, (long long)heads);
   if (hd != 64 && hd != 128)
     return fail(EVO2_ERR_UNSUPPORTED, "%s: head_dim %lld (64 or 128)", what, (long long)hd);
   if (!(scale > 0.0f) || !(scale < INFINITY))
@@ -669,7 +673,8 @@ static void launch_forward(PackedArgs a, hipStream_t st) {
 // workgroups to a CU, which fill each other's waits (8192 tokens of 32 heads 754 and 625
 // us, 8 x 1024 tokens 120 and 93).
 static bool packed_wide(const PackedArgs &a) {
-  return (a.T / (8 * P_WR) + a.nseq) * (a.part ? a.heads : a.kv) >= 304;
+  const int64_t groups = (a.T / (8 * P_WR) + static_cast<int64_t>(a.nseq)) * (a.part ? a.heads : a.kv);
+  return groups >= 304 && grid_fits(groups + P_FILL, 64 * 8);
 }
 
 template <int HD, int KW>

@@ -426,7 +426,8 @@ int evo2_iir_verify_gated(const void *zf, int64_t zs, const float *log_poles, in
  *   out_lo (T, heads, hd) bf16 and lse (heads, T) fp32: what the backward call needs
  *   of the forward one (both NULL without one); the backward call's workspace has
  *   _workspace_bytes(T, nseq, heads, kv, hd) bytes
- *   heads a multiple of kv, hd 64 or 128, scale > 0
+ *   heads a multiple of kv, hd 64 or 128, scale > 0, (T / 128 + nseq) * heads below
+ *   2^24 - 32 (a launch's workgroups)
  */
 int evo2_packed_attention(const void *q, int64_t sqt, int64_t sqh, const void *k, int64_t skt,
                           int64_t skh, const void *v, int64_t svt, int64_t svh, const int32_t *cu,

@@ -18,3 +18,36 @@ def test_rows_as_the_matrix_kernels_take_them(rows, stride):
     got = _lib.rows16(t)
     assert torch.equal(got, t) and got.stride(1) == 1 and got.stride(0) < 1 << 22
     assert (got.data_ptr() == t.data_ptr()) == (stride < 1 << 22)
+
+
+UNSUPPORTED = 2
+
+
+def test_more_workgroups_than_a_launch_takes_are_refused():
+    """A launch counts its threads in 32 bits: what takes more is refused before the first of
+    a call's launches, by both passes alike."""
+    lib, n, at = _lib.lib(), None, 4096  # (an aligned address that is never read)
+
+    def attention(T, nseq, heads, kv, backward):
+        if not backward:
+            return lib.evo2_packed_attention(at, heads * 64, 64, at, kv * 64, 64, at, kv * 64, 64, at, nseq,
+                                             at, n, n, T, heads, kv, 64, 0.1, n)
+        return lib.evo2_packed_attention_backward(
+            at, heads * 64, 64, at, heads * 64, 64, at, kv * 64, 64, at, kv * 64, 64, at, nseq, at, at, at, at,
+            1 << 62, at, at, at, T, heads, kv, 64, 0.1, n)
+
+    for backward in (False, True):
+        assert attention(8, (1 << 19) - 1, 32, 32, backward) == UNSUPPORTED
+        assert attention(1 << 20, 600000, 32, 8, backward) == UNSUPPORTED
+        assert attention(1 << 29, 0, 4, 4, backward) == UNSUPPORTED
+    assert b"workgroups" in lib.evo2_last_error()
+    rc = lib.evo2_linear_loss(at, 8, at, 8, at, -100, 2, at, at, at, at, at, 1 << 62, 1 << 28, 8, 8, n)
+    assert rc == UNSUPPORTED
+    # dh's sums over pieces: a thread for eight columns
+    rc = lib.evo2_linear_loss_backward(at, 1 << 15, at, 1 << 15, at, -100, at, at, 0, n, at, at, at, 1 << 62,
+                                       1 << 20, 9000, 1 << 15, n)
+    assert rc == UNSUPPORTED
+    # the elementwise gradient: a thread for eight columns
+    rc = lib.evo2_gated_linear_backward(at, 1 << 15, at, 8, at, at, 8, at, at, at, at, at, 1 << 62,
+                                        1 << 20, 1 << 15, 8, n)
+    assert rc == UNSUPPORTED
