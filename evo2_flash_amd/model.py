@@ -375,7 +375,8 @@ class Evo2DecodeModel(nn.Module):
     def score(self, tokens, chunk_seqs=8):
         """Log-likelihoods of prompts tokens (B, L) of sequences 0..B-1: (B, L - 1) fp32,
         entry l that of token l + 1 given the tokens up to l.  The prompts run as in
-        `prefill` (fresh Hyena states, KV pages written); no logits are kept."""
+        `prefill`: the Hyena states and the KV pages of sequences 0..B-1 are overwritten.
+        No logits are kept."""
         B, L = tokens.shape
         out = torch.empty(B, max(L - 1, 0), dtype=torch.float32, device=tokens.device)
         for b0, n, x in self._prompts(tokens, chunk_seqs, self.layers):
@@ -393,15 +394,20 @@ class Evo2DecodeModel(nn.Module):
         return list(self.layers[n:])
 
     def training_loss(self, tokens, targets=None, ignore_index=-100, chunk_seqs=8):
-        """Mean cross entropy of sequences tokens (B, L) against targets (B, L) (by
-        default each sequence's next tokens; entries of ignore_index do not count, so
-        shorter sequences are padded behind), with gradients in those parameters of
-        `trained_layers()`, the final norm and the head (`embed`, as the head alone)
-        that require them.  The layers below run as in `prefill`, without gradients."""
+        """Mean cross entropy of sequences tokens (B, L) against targets (B, L), or the
+        same flat (by default each sequence's next tokens; entries of ignore_index do not
+        count, so shorter sequences are padded behind), with gradients in those
+        parameters of `trained_layers()`, the final norm and the head (`embed`, as the head
+        alone) that require them.  The layers below run as in `prefill`, without
+        gradients: the Hyena states and the KV pages of sequences 0..B-1 are overwritten.
+        (Trained layers take heads of 64 or 128, as packed_attention does.)"""
         B, L = tokens.shape
         if targets is None:
             targets = torch.full_like(tokens, ignore_index)
             targets[:, :-1] = tokens[:, 1:]
+        elif targets.shape not in (tokens.shape, (B * L,)):
+            raise ValueError(f"targets {tuple(targets.shape)} are not of the tokens' shape "
+                             f"{tuple(tokens.shape)}")
         top = self.trained_layers()
         with torch.no_grad():
             below = list(self._prompts(tokens, chunk_seqs,

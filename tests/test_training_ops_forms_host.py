@@ -51,3 +51,13 @@ def test_more_workgroups_than_a_launch_takes_are_refused():
     rc = lib.evo2_gated_linear_backward(at, 1 << 15, at, 8, at, at, 8, at, at, at, at, at, 1 << 62,
                                         1 << 20, 1 << 15, 8, n)
     assert rc == UNSUPPORTED
+
+
+@pytest.mark.parametrize("shape", [(5, 3), (14,), (15, 1), (3, 1, 5), (3, 4)])
+def test_training_targets_of_another_shape_are_refused(shape):
+    """Among them those of as many entries, which would be taken in another order."""
+    from evo2_flash_amd.model import Evo2DecodeModel
+
+    tokens = torch.zeros(3, 5, dtype=torch.int64)
+    with pytest.raises(ValueError, match="tokens' shape"):
+        Evo2DecodeModel.training_loss(None, tokens, torch.zeros(shape, dtype=torch.int64))
