@@ -37,8 +37,6 @@ DEVICE_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
-    # (the direct-to-LDS loads in asm name m0, a reserved register, as clobbered)
-    "-Wno-inline-asm",
 ]
 
 

@@ -78,6 +78,10 @@ __device__ __forceinline__ au32x4_t lds_rsrc(const void *p, uint32_t bytes) {
   return au32x4_t{lo, hi & 0xffffu, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(bytes)), 0x00020000u};
 }
 
+// (m0, a reserved register, is named as clobbered below)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+
 // One direct-to-LDS load: 64 lanes x 16 bytes at byte offset v (zeros past the
 // descriptor) to lds .. lds + 1 KB.  In asm so that the compiler does not know of it:
 // before each transposing LDS read it would wait for all such loads in flight.  The
@@ -100,6 +104,8 @@ __device__ __forceinline__ void lds_load4(au32x4_t rsrc, uint32_t v, const void 
                : "s"(lds_addr(lds)), "v"(v), "s"(rsrc)
                : "m0");
 }
+
+#pragma clang diagnostic pop
 
 // All but N of the wave's loads and stores and all its LDS reads are done; then the
 // workgroup meets, and LDS holds what every wave's loads brought.

@@ -482,12 +482,14 @@ __global__ __launch_bounds__(64 * KW, HD == 64 ? 3 : 1) void packed_dkv_kernel(P
   const int wk0 = r0 + P_WR * wave, ki = wk0 + lr;
   const int nqb = (len - r0 + P_TR - 1) / P_TR, total = SPLIT ? nqb : nqb * group;  // swept tiles
 
-  TileLoad<HD, KW> lq, ld, lv;
+  TileLoad<HD, KW> lq, ld;
   lq.init(p.q.p, p.q.st, wave, lane);
   ld.init(p.d.p, p.d.st, wave, lane);
-  lv.init(p.v.p + begin * p.v.st + hk * p.v.sh, p.v.st, wave, lane);
-  if constexpr (!OWN)
+  if constexpr (!OWN) {
+    TileLoad<HD, KW> lv;
+    lv.init(p.v.p + begin * p.v.st + hk * p.v.sh, p.v.st, wave, lane);
     for (int i = 0; i < KG / P_TR; ++i) lv.issue(vs + i * TILE, r0 + i * P_TR, len);
+  }
   int ih = 0, ib = 0;  // the next tile to load: head of the group, tile of its sweep
   auto issue = [&](bf16_t *qs, bf16_t *ds, float *ls, float *es) __attribute__((always_inline)) {
     const int h = h0 + ih, row = r0 + ib * P_TR;
