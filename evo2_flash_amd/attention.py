@@ -435,8 +435,10 @@ def packed_attention(q, k, v, cu_seqlens, scale):
     Returns (T, heads, head_dim) bf16.
 
     Scores, softmax and sums are fp32; the probabilities and their gradients enter the
-    products as bf16.  A key's infinite or NaN value also reaches the queries before it
-    in its 64-row tile."""
+    products as bf16.  Infinities and NaN reach some rows that the mask parts them from,
+    in tiles counted from their sequence's start: a value's the outputs and a key's the dq
+    of the queries before it in its 64-row tile; those of a query or of its upstream
+    gradient the dk and dv of the keys behind it in its 32-row tile."""
     _lib.require_device(q, k, v, cu_seqlens)
     bf = torch.bfloat16
     if not (q.dim() == k.dim() == v.dim() == 3 and q.dtype == k.dtype == v.dtype == bf):

@@ -99,10 +99,11 @@ __host__ __device__ inline void mat_tile(int t, int tiles_m, int tiles_n, int sp
 
 // gelu(x) = x cdf(x), and its slope cdf(x) + x pdf(x).  The tail cdf(-|x|) is
 // exp(-x^2 / 2) t Q(t) with t = 1 / (1 + |x| / 4): Q, a polynomial of degree 6 fitted to
-// erfc(|x| / sqrt 2) exp(x^2 / 2) / (2 t) over |x| < 14, is off by 3e-9 of the cdf, the
-// fp32 steps by up to 3e-7; the tail keeps its leading digits (to 1e-3 at -13), which
-// 1 + erf loses below -5, and one exponential serves both results without a branch (by
-// erff 2048 rows of 5120 x 1920, kept, took 118 us, so 100).
+// erfc(|x| / sqrt 2) exp(x^2 / 2) / (2 t) over |x| < 14, is off by 1.9e-8 at most (near
+// 0.05, where that is 4e-8 of the cdf), the fp32 steps by up to 3e-7; the tail keeps its
+// leading digits (to 1e-3 at -13), which 1 + erf loses below -5, and one exponential serves
+// both results without a branch (by erff 2048 rows of 5120 x 1920, kept, took 118 us, so
+// 100).
 __device__ __forceinline__ void gelu_both(const float x, float &value, float &slope) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.25f, fabsf(x), 1.0f));
   const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);

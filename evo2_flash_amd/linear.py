@@ -210,7 +210,9 @@ def gated_linear(x, w1, w2, gelu):
 
     x (..., H), w1 and w2 (I, H) bf16 on one device, I and H multiples of 8.  The
     products and the activation are fp32 and the result is rounded once (`gated`
-    rounds each step, as the library's separate operators do)."""
+    rounds each step, as the library's separate operators do).  The gradients at the
+    products, dh z2 act'(z1) and dh act(z1), from factors kept to 24 bits, enter the
+    products for x, w1 and w2 as bf16; those have fp32 sums, rounded once."""
     _lib.require_device(x, w1, w2)
     if not x.dtype == w1.dtype == w2.dtype == torch.bfloat16:
         raise ValueError(f"gated_linear takes bf16 x, w1, w2, got {x.dtype}, {w1.dtype}, {w2.dtype}")

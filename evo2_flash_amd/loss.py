@@ -80,7 +80,9 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="
     through it).  reduction: "none" (fp32 losses of targets' shape:
     the negative log-likelihoods), "sum" or "mean" over the rows that are not ignored
     (fp32 scalar; the mean of no rows is NaN).  The logits are fp32 sums of the bf16
-    products and never rounded."""
+    products and never rounded; their gradient (the softmax less one at the target; of
+    "none" times the row's upstream gradient) enters the products for hidden and weight as
+    bf16, which have fp32 sums."""
     _lib.require_device(hidden, weight, targets)
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
