@@ -337,7 +337,47 @@ SIGNATURES = {
     ],
 }
 
-RESTYPES = {"evo2_last_error": ctypes.c_char_p, "evo2_hcl_workspace_bytes": ctypes.c_int64,
+_KV_FP8 = [
+    _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,   # k_pages + strides, v_pages + strides
+    _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,   # k_scale + strides, v_scale + strides
+    _c_i64, _c_p, _c_i64, _c_i64,                 # num_pages, table, stride, max_pages
+]
+SIGNATURES.update({
+    "evo2_kv_fp8_write": [
+        _c_p, _c_i64, _c_i64, _c_i64,             # k + strides
+        _c_p, _c_i64, _c_i64, _c_i64,             # v + strides
+        *_KV_FP8, _c_p, _c_p,                     # positions, lengths
+        _c_i64, _c_i64, _c_i64, _c_i64, _c_p,     # B, n, heads, head_dim, stream
+    ],
+    "evo2_kv_fp8_read": [
+        *_KV_FP8, _c_p, _c_p, _c_p,               # lengths, k, v
+        _c_i64, _c_i64, _c_i64, _c_i64, _c_p,     # B, L, heads, head_dim, stream
+    ],
+    "evo2_rotary_decode_fp8": [
+        _c_p, _c_i64, _c_p, _c_f, _c_p,           # qkv, sqkv, inv_freq, factor, q
+        *_KV_FP8, _c_p,                           # positions
+        _c_i64, _c_i64, _c_i64, _c_p,             # B, heads, head_dim, stream
+    ],
+    "evo2_decode_attention_fp8_workspace_bytes": [_c_i64] * 6,
+    "evo2_paged_decode_attention_fp8": [
+        _c_p, _c_i64, _c_i64, _c_i64,             # q + strides
+        *_KV_FP8, _c_i64, _c_p,                   # shared_pages, positions
+        _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_i64,  # workspace, bytes, out + strides
+        _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,   # B, n, heads, kv_heads, head_dim
+        _c_f, _c_p,                               # scale, stream
+    ],
+    "evo2_sample_workspace_bytes": [_c_i64, _c_i64],
+    "evo2_sample": [
+        _c_p, _c_i32, _c_i64, _c_p,               # logits, fp32, stride, uniforms
+        _c_p, _c_f, _c_p, _c_i64,                 # temperature (rows, one), top_k (rows, one)
+        _c_p, _c_f, _c_p, _c_f,                   # top_p (rows, one), min_p (rows, one)
+        _c_p, _c_i64, _c_p,                       # workspace, bytes, tokens
+        _c_i64, _c_i64, _c_p,                     # B, V, stream
+    ],
+})
+
+RESTYPES = {"evo2_decode_attention_fp8_workspace_bytes": ctypes.c_int64,
+            "evo2_sample_workspace_bytes": ctypes.c_int64, "evo2_last_error": ctypes.c_char_p, "evo2_hcl_workspace_bytes": ctypes.c_int64,
             "evo2_decode_attention_workspace_bytes": ctypes.c_int64,
             "evo2_fp8_gemm_persist_order": ctypes.c_int64,
             "evo2_packed_attention_workspace_bytes": ctypes.c_int64,

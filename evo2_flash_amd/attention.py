@@ -202,6 +202,12 @@ def _rotary_operands(qkv, cache, inv_freq):
                          f"heads, {PAGE}, head_dim) with unit last strides, got "
                          f"{tuple(cache.k.shape)} {cache.k.dtype}, {tuple(cache.v.shape)} "
                          f"{cache.v.dtype}")
+    qkv, inv_freq = _rotary_rows(qkv, nh, hd, inv_freq)
+    return qkv, nh, hd, inv_freq
+
+
+def _rotary_rows(qkv, nh, hd, inv_freq):
+    """The rows and the frequencies of `_rotary_operands` for nh heads of hd."""
     if inv_freq.shape != (hd // 2,):
         raise ValueError(f"inv_freq must be ({hd // 2},), got {tuple(inv_freq.shape)}")
     if qkv.dim() != 2 or qkv.shape[1] != 3 * nh * hd or qkv.dtype != torch.bfloat16:
@@ -209,7 +215,7 @@ def _rotary_operands(qkv, cache, inv_freq):
                          f"{qkv.dtype}")
     if qkv.stride(1) != 1:
         qkv = qkv.contiguous()
-    return qkv, nh, hd, inv_freq.to(torch.float32).contiguous()
+    return qkv, inv_freq.to(torch.float32).contiguous()
 
 
 def _page_table(block_table, rows, num_pages, device):

@@ -235,7 +235,8 @@ extern "C" int evo2_rotary_prefill(const void *qkv, int64_t sqkv, const float *i
   if (head_dim != RP_HD)
     return fail(EVO2_ERR_UNSUPPORTED, "rotary_prefill: head_dim %lld (128 only)", (long long)head_dim);
   if (N == 0 || L == 0) return EVO2_OK;
-  if (!qkv || !inv_freq || !q || !k || !vt || !k_pages || !v_pages || !table)
+  // (a cache of no pages: k and v are written to the operands alone)
+  if (!qkv || !inv_freq || !q || !k || !vt || (num_pages > 0 && (!k_pages || !v_pages)) || !table)
     return fail(EVO2_ERR_INVALID, "rotary_prefill: null pointer argument");
   if (cdiv(L, 16) > max_pages)
     return fail(EVO2_ERR_INVALID, "rotary_prefill: %lld positions exceed the block table's %lld pages",

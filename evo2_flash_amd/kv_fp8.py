@@ -1,0 +1,272 @@
+"""The decoder's KV cache in 8 bits, and decode attention over it (model.py:104-153): half
+the bytes of the bf16 pages, which is what decode attention over long contexts waits for.
+
+Keys and values are e4m3 codes in pages of 16 positions named by a block table, as in
+attention.PagedKVCache, in the layouts the kernels load as they lie (csrc/kv_fp8.h):
+
+    k_pages (pages, kv_heads, 16, head_dim)    v_pages (pages, kv_heads, head_dim, 16)
+    k_scale, v_scale (pages, kv_heads) fp32    value = code * scale
+
+The scale of a (page, head) is the smallest power of two, of 2^-110 .. 2^119, with which no
+finite value of the page's tokens is over 448 codes.  A token's place in its page decides:
+the write of a page's first position starts the page's scale, a write behind positions that
+the page holds keeps it, or raises it and re-encodes those (exactly, but for codes that
+reach the subnormal range).  NaN and infinities are held as NaN.  Codes are rounded to
+nearest even.  A page that two sequences share is only read: two sequences of one call that
+write to it leave it undefined.
+
+write_kv_fp8, read_kv_fp8 and paged_decode_attention_fp8 take the tensors; Fp8KVCache holds
+them for one attention layer.  rotary_decode_fp8 is the decode step's rotary with the write.
+"""
+
+import torch
+
+from . import _lib
+from .attention import PAGE, _page_table, _rotary_rows
+
+_F8 = torch.float8_e4m3fn
+_INTS = (torch.int32, torch.int64)
+
+
+def _cache_args(what, k_pages, v_pages, k_scale, v_scale, block_table, B):
+    """Checks of the cache's tensors and the table; the C entries' arguments from the key
+    pages to the table's columns, and (kv_heads, head_dim)."""
+    if not (k_pages.dim() == v_pages.dim() == 4 and k_pages.dtype == v_pages.dtype == _F8):
+        raise ValueError(f"{what} takes float8_e4m3fn pages (pages, kv_heads, {PAGE}, head_dim) and "
+                         f"(pages, kv_heads, head_dim, {PAGE})")
+    pages, kv, rows, hd = k_pages.shape
+    if rows != PAGE or v_pages.shape != (pages, kv, hd, PAGE):
+        raise ValueError(f"{what}: page shapes {tuple(k_pages.shape)}, {tuple(v_pages.shape)} do not match")
+    if hd not in (64, 128):
+        raise ValueError(f"{what} takes head_dim 64 or 128, got {hd}")
+    if (k_scale.shape != (pages, kv) or v_scale.shape != (pages, kv)
+            or not k_scale.dtype == v_scale.dtype == torch.float32):
+        raise ValueError(f"{what}: scales must be ({pages}, {kv}) fp32, got {tuple(k_scale.shape)} "
+                         f"{k_scale.dtype}, {tuple(v_scale.shape)} {v_scale.dtype}")
+    if pages == 0 or kv == 0:
+        raise ValueError(f"{what}: a cache of no pages or heads")
+    kps, khs, k2, k3 = k_pages.stride()
+    vps, vhs, v2, v3 = v_pages.stride()
+    if (k2, k3) != (hd, 1) or (v2, v3) != (PAGE, 1):
+        raise ValueError(f"{what}: a page's head must be contiguous")
+    if (block_table.dim() != 2 or block_table.shape[0] < B or block_table.shape[1] == 0
+            or block_table.dtype != torch.int32 or block_table.stride(1) != 1):
+        raise ValueError("block_table must be (>= B, max_pages) int32 with unit column stride")
+    if not _lib.same_device(k_pages, v_pages, k_scale, v_scale, block_table):
+        raise ValueError(f"{what}: the cache and its table are on different devices")
+    return (k_pages.data_ptr(), kps, khs, v_pages.data_ptr(), vps, vhs, k_scale.data_ptr(),
+            *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride(), pages, block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1]), kv, hd
+
+
+def _per_sequence(t, B, name, device):
+    """t (B,) int32 or int64 on the cache's device, as contiguous int64."""
+    if t.shape != (B,) or t.dtype not in _INTS:
+        raise ValueError(f"{name} must be ({B},) int32 or int64, got {tuple(t.shape)} {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.dtype == torch.int64 and (B == 1 or t.stride(0) == 1):
+        return t
+    return t.to(torch.int64).contiguous()
+
+
+def _token_rows(t):
+    """t (B, n, heads, hd) with rows as the kernels read them: unit last stride, 16-byte
+    aligned; itself or a copy."""
+    b, n, h, unit = t.stride()
+    if unit != 1 or (b | n | h) & 7 or t.data_ptr() & 15:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def write_kv_fp8(k, v, k_pages, v_pages, k_scale, v_scale, block_table, positions, lengths=None):
+    """Quantise k and v (B, n, kv_heads, head_dim) bf16 (views of any strides) into the
+    cache's pages: token i of sequence b goes to position positions[b] + i of
+    `block_table`'s (>= B, max_pages) int32 row b.  lengths (B,): only a sequence's first
+    lengths[b] tokens count (a padded batch).  positions and lengths are int32 or int64 on
+    the cache's device; the host does not read them.  Tokens whose position lies outside the
+    table, or whose entry lies outside the cache's pages, are not written; nor is any token of
+    a sequence that starts there.  Codes of positions that are not written keep their bytes
+    (of positions held before theirs: see the module's description)."""
+    _lib.require_device(k, v, k_pages, v_pages, k_scale, v_scale, block_table, positions, lengths)
+    if not (k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype == torch.bfloat16):
+        raise ValueError(f"write_kv_fp8 takes bf16 k and v (B, n, kv_heads, head_dim), got "
+                         f"{tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
+    B, n = k.shape[:2]
+    cache, kv, hd = _cache_args("write_kv_fp8", k_pages, v_pages, k_scale, v_scale, block_table, B)
+    if k.shape[2:] != (kv, hd):
+        raise ValueError(f"write_kv_fp8: tokens of {tuple(k.shape[2:])}, pages of ({kv}, {hd})")
+    if k.device != k_pages.device or v.device != k_pages.device:
+        raise ValueError(f"write_kv_fp8: tokens on {k.device}, {v.device}, the cache on {k_pages.device}")
+    positions = _per_sequence(positions, B, "positions", k_pages.device)
+    if lengths is not None:
+        lengths = _per_sequence(lengths, B, "lengths", k_pages.device)
+    if B == 0 or n == 0:
+        return
+    k, v = _token_rows(k), _token_rows(v)
+    with _lib.on_device(k_pages):
+        _lib.call("evo2_kv_fp8_write", k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
+                  *cache, positions.data_ptr(), _lib.ptr(lengths), B, n, kv, hd,
+                  _lib.stream_of(k_pages))
+
+
+def read_kv_fp8(k_pages, v_pages, k_scale, v_scale, block_table, lengths, L):
+    """The first L positions of sequences 0 .. B - 1 (B: lengths' size) as bf16 keys and
+    values (B, L, kv_heads, head_dim), the values the codes stand for exactly (the layout of
+    write_kv_fp8's tokens and, flattened, of attention.packed_attention's).  Positions from
+    lengths[b] on, and those whose entry lies outside the table or the cache's pages, are
+    zeros."""
+    _lib.require_device(k_pages, v_pages, k_scale, v_scale, block_table, lengths)
+    B, L = lengths.shape[0] if lengths.dim() else -1, int(L)
+    cache, kv, hd = _cache_args("read_kv_fp8", k_pages, v_pages, k_scale, v_scale, block_table, B)
+    lengths = _per_sequence(lengths, B, "lengths", k_pages.device)
+    if L < 0:
+        raise ValueError(f"read_kv_fp8 takes L >= 0, got {L}")
+    k = torch.empty(B, L, kv, hd, dtype=torch.bfloat16, device=k_pages.device)
+    v = torch.empty_like(k)
+    if B and L:
+        with _lib.on_device(k_pages):
+            _lib.call("evo2_kv_fp8_read", *cache, lengths.data_ptr(), k.data_ptr(), v.data_ptr(), B, L,
+                      kv, hd, _lib.stream_of(k_pages))
+    return k, v
+
+
+def workspace_fp8(B, heads, kv_heads, head_dim, max_pages, device, n=1):
+    """A workspace for paged_decode_attention_fp8 on up to B sequences of n tokens (allocate
+    once, outside graph capture; calls that may run at once take one each)."""
+    need = max((_lib.workspace_bytes("evo2_decode_attention_fp8_workspace_bytes", b, n, heads,
+                                     kv_heads, head_dim, max_pages) for b in range(1, B + 1)), default=0)
+    return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+
+
+def paged_decode_attention_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, positions, scale,
+                               work=None, shared_pages=0):
+    """Attention of q (B, heads, head_dim), or n tokens of each sequence (B, n, heads,
+    head_dim), bf16, over the cache; heads a multiple of kv_heads (query head h reads key
+    head h // (heads // kv_heads)).  positions (B,): token i of sequence b attends to
+    positions 0 .. positions[b] + i of block_table's (>= B, max_pages) int32 row b (those
+    past the table do not exist).  Returns bf16 of q's shape: the exact softmax over the
+    values the codes stand for (fp32 scores and sums, the probabilities to ~16 bits).
+
+    The kernel never reads through a table entry outside [0, pages): its positions are left
+    out of the softmax (a token with none left gets zeros).  shared_pages: the first
+    shared_pages entries of every row name the same pages (attention.shared_prefix_pages
+    finds them on the host), which are then read once for 32 query rows of any sequences.
+    Bytes of positions that a sequence does not attend to may be anything; a NaN value at a
+    position that some of a launch's rows attend to (later tokens of the sequence, or longer
+    sequences on shared pages) can reach the others in its block of 64."""
+    _lib.require_device(q, k_pages, v_pages, k_scale, v_scale, block_table, positions, work)
+    if q.dim() not in (3, 4) or q.dtype != torch.bfloat16:
+        raise ValueError(f"paged_decode_attention_fp8 takes bf16 q (B, [n,] heads, head_dim), got "
+                         f"{tuple(q.shape)} {q.dtype}")
+    q4 = q.unsqueeze(1) if q.dim() == 3 else q
+    B, n, heads, hd = q4.shape
+    cache, kv, phd = _cache_args("paged_decode_attention_fp8", k_pages, v_pages, k_scale, v_scale,
+                                 block_table, B)
+    if hd != phd or heads == 0 or heads % kv:
+        raise ValueError(f"paged_decode_attention_fp8: q {tuple(q.shape)} does not match pages "
+                         f"{tuple(k_pages.shape)}")
+    if q.device != k_pages.device:
+        raise ValueError(f"paged_decode_attention_fp8: q on {q.device}, the cache on {k_pages.device}")
+    positions = _per_sequence(positions, B, "positions", k_pages.device)
+    scale = float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"paged_decode_attention_fp8 takes a positive scale, got {scale}")
+    shared_pages = int(shared_pages)
+    if not 0 <= shared_pages <= block_table.shape[1]:
+        raise ValueError(f"shared_pages {shared_pages} of a table of {block_table.shape[1]} columns")
+    if work is not None and (not work.is_contiguous() or work.device != q.device):
+        raise ValueError("work must be a contiguous tensor on q's device")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if B == 0 or n == 0:
+        return out
+    o4 = out.unsqueeze(1) if q.dim() == 3 else out
+    q4 = _token_rows(q4)
+    max_pages = block_table.shape[1]
+    with _lib.on_device(q):
+        if work is None:
+            need = _lib.workspace_bytes("evo2_decode_attention_fp8_workspace_bytes", B, n, heads, kv, hd,
+                                        max_pages)
+            if need:
+                work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _lib.call("evo2_paged_decode_attention_fp8", q4.data_ptr(), *q4.stride()[:3], *cache, shared_pages,
+                  positions.data_ptr(), _lib.ptr(work),
+                  0 if work is None else work.numel() * work.element_size(), o4.data_ptr(),
+                  *o4.stride()[:3], B, n, heads, kv, hd, scale, _lib.stream_of(q))
+    return out
+
+
+class Fp8KVCache:
+    """One attention layer's 8-bit KV pages and their scales; page 0 is never handed out."""
+
+    def __init__(self, num_pages, heads, head_dim, device):
+        self.k = torch.zeros(num_pages, heads, PAGE, head_dim, dtype=torch.uint8, device=device).view(_F8)
+        self.v = torch.zeros(num_pages, heads, head_dim, PAGE, dtype=torch.uint8, device=device).view(_F8)
+        self.k_scale = torch.ones(num_pages, heads, dtype=torch.float32, device=device)
+        self.v_scale = torch.ones(num_pages, heads, dtype=torch.float32, device=device)
+
+    @property
+    def tensors(self):
+        """The tensors as write_kv_fp8 and the other operators take them."""
+        return self.k, self.v, self.k_scale, self.v_scale
+
+    def append(self, k, v, block_table, positions):
+        """k, v (B, heads, head_dim): the entries of sequence b at positions[b]."""
+        write_kv_fp8(k[:, None], v[:, None], *self.tensors, block_table, positions)
+
+    def write_prompt(self, k, v, block_table):
+        """k, v (B, heads, L, head_dim): positions 0..L-1 of sequences 0..B-1."""
+        zero = torch.zeros(k.shape[0], dtype=torch.int64, device=k.device)
+        write_kv_fp8(k.transpose(1, 2), v.transpose(1, 2), *self.tensors, block_table, zero)
+
+    def dense(self, block_table, B, L):
+        """The first L positions of sequences 0..B-1 as contiguous bf16 caches (keys
+        (B, heads, head_dim, L), values (B, heads, L, head_dim))."""
+        lengths = torch.full((B,), L, dtype=torch.int64, device=self.k.device)
+        k, v = read_kv_fp8(*self.tensors, block_table, lengths, L)
+        return k.permute(0, 2, 3, 1).contiguous(), v.transpose(1, 2).contiguous()
+
+
+def rotary_prefill_fp8(qkv, cache, block_table, inv_freq, factor, nseq, L):
+    """attention.rotary_prefill on an Fp8KVCache: the same operands of prefill attention (of
+    the values before they are quantised); k and v are quantised into `cache`'s pages by a
+    launch of their own."""
+    _lib.require_device(qkv, cache.k, cache.v, inv_freq)
+    nh, hd = cache.k.shape[1], cache.k.shape[3]
+    qkv, inv_freq = _rotary_rows(qkv, nh, hd, inv_freq)
+    if qkv.shape[0] != nseq * L:
+        raise ValueError(f"qkv must have {nseq * L} rows, got {qkv.shape[0]}")
+    block_table = _page_table(block_table, nseq, cache.k.shape[0], qkv.device)
+    Lv = -(-L // 128) * 128
+    q = torch.empty(nseq, nh, L, hd, dtype=qkv.dtype, device=qkv.device)
+    k = torch.empty_like(q)
+    vt = torch.empty(nseq, nh, hd, Lv, dtype=qkv.dtype, device=qkv.device)
+    _lib.call("evo2_rotary_prefill", _lib.ptr(qkv), qkv.stride(0), _lib.ptr(inv_freq), float(factor),
+              _lib.ptr(q), _lib.ptr(k), _lib.ptr(vt), Lv, None, 0, 0, 0, None, 0, 0, 0, 0,
+              _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], nseq, nh, hd, L,
+              _lib.stream_of(qkv))
+    v = qkv[:, 2 * nh * hd:].view(nseq, L, nh, hd)
+    zero = torch.zeros(nseq, dtype=torch.int64, device=qkv.device)
+    write_kv_fp8(k.transpose(1, 2), v, *cache.tensors, block_table, zero)
+    return q, k, vt
+
+
+def rotary_decode_fp8(qkv, cache, block_table, positions, inv_freq, factor):
+    """attention.rotary_decode on an Fp8KVCache, in one launch: qkv (B, 3 * heads *
+    head_dim) bf16 rows (q | k | v) at positions (B,); returns q (B, heads, head_dim)
+    rotated; k and v are quantised into `cache`'s pages as write_kv_fp8 does."""
+    _lib.require_device(qkv, cache.k, cache.v, block_table, positions, inv_freq)
+    nh, hd = cache.k.shape[1], cache.k.shape[3]
+    qkv, inv_freq = _rotary_rows(qkv, nh, hd, inv_freq)
+    B = qkv.shape[0]
+    table = _page_table(block_table, B, cache.k.shape[0], qkv.device)
+    args, _, _ = _cache_args("rotary_decode_fp8", *cache.tensors, table, B)
+    positions = _per_sequence(positions, B, "positions", qkv.device)
+    q = torch.empty(B, nh, hd, dtype=qkv.dtype, device=qkv.device)
+    _lib.call("evo2_rotary_decode_fp8", _lib.ptr(qkv), qkv.stride(0), _lib.ptr(inv_freq), float(factor),
+              _lib.ptr(q), *args, _lib.ptr(positions), B, nh, hd, _lib.stream_of(qkv))
+    return q
+
+
+__all__ = ["Fp8KVCache", "write_kv_fp8", "read_kv_fp8", "paged_decode_attention_fp8", "workspace_fp8",
+           "rotary_prefill_fp8", "rotary_decode_fp8"]

@@ -1,0 +1,79 @@
+"""The next token from the logits (csrc/sample.hip): temperature, top-k, top-p and min-p, and
+the draw from given uniform numbers, behind the decoder's head (model.py:343-348).
+"""
+
+import torch
+
+from . import _lib
+
+
+def _setting(x, name, B, device, dtype):
+    """(address or None, number) of a setting: a tensor (B,) on `device`, or one number
+    for all rows; and the tensor, to be kept until the launch."""
+    if not torch.is_tensor(x):
+        return None, x, None
+    if x.shape != (B,):
+        raise ValueError(f"{name} must be one number or ({B},), got {tuple(x.shape)}")
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, the logits on {device}")
+    if dtype is torch.int32 and x.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be int32 or int64, got {x.dtype}")
+    if dtype is torch.float32 and not x.is_floating_point():
+        raise ValueError(f"{name} must be floating-point numbers, got {x.dtype}")
+    if x.dtype != dtype:
+        if x.dtype == torch.int64:
+            x = x.clamp(0, 2 ** 31 - 1)
+        x = x.to(dtype)
+    if x.stride(0) != 1:
+        x = x.contiguous()
+    return x.data_ptr(), 0, x
+
+
+def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The next token of each row: logits (B, V) bf16 or fp32 (rows of any stride),
+    uniforms (B,) fp32 numbers of [0, 1) -> (B,) int64.  temperature, top_k, top_p and min_p
+    are one number each or (B,) tensors on the logits' device (the host does not read those);
+    they are taken as fp32 and int32.
+
+    The tokens stand in the order of their logits, equal ones the lowest index first.
+    top_k > 0 keeps the first top_k; top_p < 1 the shortest front of those whose
+    probabilities (softmax(logits / temperature), of what top_k kept) reach top_p, at least
+    the first token; min_p > 0 those with at least min_p (at most 1) times the largest
+    probability.  The token is the first, in the vocabulary's order, at which the running sum
+    of what is kept passes uniforms times its total; numbers outside [0, 1) draw the first or
+    the last token kept.  temperature <= 0 (or NaN) and top_k 1 take the first token.  -inf and NaN logits are
+    never drawn (a row of nothing else gives -1); beside +inf no finite one is.  Weights are
+    summed as whole numbers (steps of 2^-49 of the largest, of 2^-61 V for V over 4096), so
+    a result does not depend on timing."""
+    _lib.require_device(logits, uniforms)
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"sample_tokens takes bf16 or fp32 logits (B, V), got {tuple(logits.shape)} "
+                         f"{logits.dtype}")
+    B, V = logits.shape
+    if not 0 < V <= 1 << 24:
+        raise ValueError(f"sample_tokens takes 1 to 2^24 logits a row, got {V}")
+    if uniforms.shape != (B,) or uniforms.dtype != torch.float32 or uniforms.device != logits.device:
+        raise ValueError(f"uniforms must be ({B},) fp32 on {logits.device}, got {tuple(uniforms.shape)} "
+                         f"{uniforms.dtype} on {uniforms.device}")
+    dev, f32 = logits.device, torch.float32
+    t, t1, keep_t = _setting(temperature, "temperature", B, dev, f32)
+    k, k1, keep_k = _setting(top_k, "top_k", B, dev, torch.int32)
+    p, p1, keep_p = _setting(top_p, "top_p", B, dev, f32)
+    m, m1, keep_m = _setting(min_p, "min_p", B, dev, f32)
+    out = torch.empty(B, dtype=torch.int64, device=dev)
+    if B == 0:
+        return out
+    if logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    if uniforms.stride(0) != 1:
+        uniforms = uniforms.contiguous()
+    with _lib.on_device(logits):
+        n = _lib.workspace_bytes("evo2_sample_workspace_bytes", B, V)
+        work = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        _lib.call("evo2_sample", logits.data_ptr(), logits.dtype == f32, logits.stride(0),
+                  uniforms.data_ptr(), t, t1, k, k1, p, p1, m, m1, _lib.ptr(work), n, out.data_ptr(), B,
+                  V, _lib.stream_of(logits))
+    return out
+
+
+__all__ = ["sample_tokens"]

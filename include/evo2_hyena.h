@@ -412,6 +412,95 @@ int evo2_iir_verify_gated(const void *zf, int64_t zs, const float *log_poles, in
                           void *stream);
 
 /*
+ * The 8-bit KV cache: e4m3 codes in pages of 16 positions with one power of two a (page,
+ * key head) as their scale, value = code * scale.  The cache's arguments, in all of its
+ * entry points:
+ *   k_pages (pages, heads, 16, head_dim), v_pages (pages, heads, head_dim, 16) bytes, the
+ *   last two dimensions contiguous; page and head strides in bytes, multiples of 16, at
+ *   least 16 * head_dim between heads; 16-byte aligned; head_dim 64 or 128
+ *   k_scale, v_scale (pages, heads) fp32, page and head strides in elements
+ *   table (B, max_pages) int32, row stride st, on the device: position l of sequence b is
+ *   in page table[b][l / 16]; entries outside [0, num_pages) are neither read nor written
+ *   through
+ *
+ * evo2_kv_fp8_write: k, v (B, n, heads, head_dim) bf16, strides in elements, unit last
+ * stride, rows 16-byte aligned, to positions positions[b] + i of sequence b for i <
+ * lengths[b] (NULL: n); positions, lengths (B,) int64.  e of a page's scale 2^e is the
+ * smallest of [-110, 119] with which no finite magnitude of its tokens is over 448 codes;
+ * a page written to behind positions that it holds keeps its e, or raises it and
+ * re-encodes those.  Round to nearest even; infinities and NaN become NaN; with e = 119
+ * larger values saturate.  Bytes of other positions stay as they are.
+ *
+ * evo2_kv_fp8_read: k, v (B, L, heads, head_dim) bf16 contiguous, 16-byte aligned: the
+ * values of positions below lengths[b] (int64), zeros from there on and where the table
+ * has no page.
+ *
+ * evo2_rotary_decode_fp8: evo2_rotary_decode with this cache (qkv rows q | k | v of heads *
+ * head_dim each; the same q bits, and the k, v of evo2_kv_fp8_write on its values).
+ */
+int evo2_kv_fp8_write(const void *k, int64_t kb, int64_t kt, int64_t kh, const void *v, int64_t vb,
+                      int64_t vt, int64_t vh, void *k_pages, int64_t kps, int64_t khs, void *v_pages,
+                      int64_t vps, int64_t vhs, float *k_scale, int64_t ksp, int64_t ksh,
+                      float *v_scale, int64_t vsp, int64_t vsh, int64_t num_pages,
+                      const int32_t *table, int64_t st, int64_t max_pages, const int64_t *positions,
+                      const int64_t *lengths, int64_t B, int64_t n, int64_t heads, int64_t head_dim,
+                      void *stream);
+int evo2_kv_fp8_read(const void *k_pages, int64_t kps, int64_t khs, const void *v_pages, int64_t vps,
+                     int64_t vhs, const float *k_scale, int64_t ksp, int64_t ksh,
+                     const float *v_scale, int64_t vsp, int64_t vsh, int64_t num_pages,
+                     const int32_t *table, int64_t st, int64_t max_pages, const int64_t *lengths,
+                     void *k, void *v, int64_t B, int64_t L, int64_t heads, int64_t head_dim,
+                     void *stream);
+int evo2_rotary_decode_fp8(const void *qkv, int64_t sqkv, const float *inv_freq, float factor, void *q,
+                           void *k_pages, int64_t kps, int64_t khs, void *v_pages, int64_t vps,
+                           int64_t vhs, float *k_scale, int64_t ksp, int64_t ksh, float *v_scale,
+                           int64_t vsp, int64_t vsh, int64_t num_pages, const int32_t *table,
+                           int64_t st, int64_t max_pages, const int64_t *positions, int64_t B,
+                           int64_t heads, int64_t head_dim, void *stream);
+
+/*
+ * Decode attention over the 8-bit cache (its arguments as above, heads: kv_heads): token i
+ * of sequence b attends to positions 0 .. positions[b] + i,
+ *   out[b, i, h] = sum_l softmax_l(scale q . k_l) v_l, keys and values of head
+ *   h / (heads / kv_heads)
+ *   q (B, n, heads, head_dim) bf16, strides in elements (multiples of 8), 16-byte aligned;
+ *   out the same shape, strides multiples of 4, 8-byte aligned; positions (B,) int64
+ *   shared_pages: the first entries of every table row that name the same pages
+ *   workspace: _workspace_bytes(B, n, heads, kv_heads, head_dim, max_pages) bytes (0: none),
+ *   8-byte aligned
+ * heads a multiple of kv_heads, scale > 0, B * n at most 65535.  Positions of entries
+ * outside the pages are left out; a token with none left gives zeros.
+ */
+int64_t evo2_decode_attention_fp8_workspace_bytes(int64_t B, int64_t n, int64_t heads, int64_t kv_heads,
+                                                  int64_t head_dim, int64_t max_pages);
+int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_t qt, int64_t qh,
+                                    const void *k_pages, int64_t kps, int64_t khs, const void *v_pages,
+                                    int64_t vps, int64_t vhs, const float *k_scale, int64_t ksp,
+                                    int64_t ksh, const float *v_scale, int64_t vsp, int64_t vsh,
+                                    int64_t num_pages, const int32_t *table, int64_t st,
+                                    int64_t max_pages, int64_t shared_pages, const int64_t *positions,
+                                    void *workspace, int64_t workspace_bytes, void *out, int64_t ob,
+                                    int64_t ot, int64_t oh, int64_t B, int64_t n, int64_t heads,
+                                    int64_t kv_heads, int64_t head_dim, float scale, void *stream);
+
+/*
+ * The next token of each row of logits z (B, V), bf16 (fp32 = 0) or fp32, row stride sz,
+ * from uniform numbers u (B,): w_i = exp((z_i - max z) / T); in the order (z descending,
+ * index ascending) top-k keeps the first k (k <= 0: all), top-p the shortest front of
+ * those with p of their weight (p >= 1: all), min-p those with w_i >= m; the token is the
+ * first index at which the running sum of what is kept passes u times its total.  T <= 0
+ * or k = 1: the first of the largest.  -inf and NaN are never drawn; a row of nothing else
+ * gives -1.  temperature, top_k, top_p, min_p (B,) by row, or NULL: t1, k1, p1, m1.
+ *   tokens (B,) int64; V up to 2^24; workspace of _workspace_bytes(B, V) bytes, 16-byte
+ *   aligned (0: none)
+ */
+int64_t evo2_sample_workspace_bytes(int64_t B, int64_t V);
+int evo2_sample(const void *logits, int32_t fp32, int64_t sz, const float *u, const float *temperature,
+                float t1, const int32_t *top_k, int64_t k1, const float *top_p, float p1,
+                const float *min_p, float m1, void *workspace, int64_t workspace_bytes,
+                int64_t *tokens, int64_t B, int64_t V, void *stream);
+
+/*
  * Causal self-attention of packed sequences and its backward pass: sequence s takes
  * rows cu[s] .. cu[s + 1] - 1 of T, query head h reads key head h / (heads / kv):
  *   p_ij = softmax_{j <= i in the sequence}(scale q_i . k_j), o = p v
