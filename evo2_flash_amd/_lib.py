@@ -358,7 +358,7 @@ SIGNATURES.update({
         *_KV_FP8, _c_p,                           # positions
         _c_i64, _c_i64, _c_i64, _c_p,             # B, heads, head_dim, stream
     ],
-    "evo2_decode_attention_fp8_workspace_bytes": [_c_i64] * 6,
+    "evo2_decode_attention_fp8_workspace_bytes": [_c_i64] * 7,
     "evo2_paged_decode_attention_fp8": [
         _c_p, _c_i64, _c_i64, _c_i64,             # q + strides
         *_KV_FP8, _c_i64, _c_p,                   # shared_pages, positions

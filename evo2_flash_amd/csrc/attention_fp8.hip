@@ -10,7 +10,7 @@
 //
 // Split over the context: a workgroup takes one chunk of positions of one key head for up
 // to 16 query rows (a sequence's tokens x the head's group; on pages that all sequences
-// share, up to 32 rows of any sequences), and writes (o, max, sum) for each; a second
+// share, up to 32 rows of any sequences, those chunks apart from the ones behind), and writes (o, max, sum) for each; a second
 // launch joins the chunks.  Contexts of one chunk are written out at once.  Each of the
 // four waves takes the chunk's blocks of 64 positions in turn, with a running maximum and
 // sum, on v_mfma_f32_16x16x32_bf16:
@@ -33,26 +33,25 @@ struct AttnFp8Args {
   KvPages c;
   const bf16_t *q; int64_t qb, qt, qh;  // (B, n, heads, hd)
   const int64_t *pos;                   // (B,) of token 0
-  float *part;                          // (B * n * heads, nchunk, hd + 2): o, max, sum
+  float *part;                          // (B * n * heads, nchunk, hd): o of a chunk
+  float2 *ml;                           // (B * n * heads, nchunk): its max (log2 units), sum
   bf16_t *out; int64_t ob, ot, oh;
   float scale;
-  int B, n, heads, group, kv;           // group: query heads to a key head
-  int chunk, nchunk;                    // positions a chunk; chunks of the table
+  uint32_t B, n, heads, group, kv;      // group: query heads to a key head
+  int shared, schunk, snum;             // positions of the shared pages; a chunk of them; chunks
+  int chunk, nchunk;                    // a chunk of the positions behind; all chunks
 };
 
 constexpr int AF_T = 256, AF_NW = AF_T / 64;
-constexpr int AF_BLK = 64;                    // positions a wave takes at once
-constexpr int AF_CHUNK = 2048;                // most positions a chunk
-constexpr int AF_PAGES = AF_CHUNK / KV_PAGE;
+constexpr int AF_BLK = 64;  // positions a wave takes at once
 
 // Query row r of a key head: rows run over (sequence, token, head of the group).
 struct AttnRow {
   int b, i, j;
 };
-__device__ __forceinline__ AttnRow attn_row(const AttnFp8Args &p, int64_t r) {
-  const int per = p.n * p.group;
-  const int b = static_cast<int>(r / per), in = static_cast<int>(r - static_cast<int64_t>(b) * per);
-  return AttnRow{b, in / p.group, in % p.group};
+__device__ __forceinline__ AttnRow attn_row(const AttnFp8Args &p, uint32_t r) {  // (B * n below 2^16: r fits)
+  const uint32_t bi = r / p.group, b = p.n == 1 ? bi : bi / p.n;
+  return AttnRow{static_cast<int>(b), static_cast<int>(bi - b * p.n), static_cast<int>(r - bi * p.group)};
 }
 __device__ __forceinline__ int row_len(const AttnFp8Args &p, const AttnRow &a) {
   const int64_t first = p.pos[a.b], all = p.c.max_pages * KV_PAGE;
@@ -60,39 +59,59 @@ __device__ __forceinline__ int row_len(const AttnFp8Args &p, const AttnRow &a) {
   return static_cast<int>(min(max(min(first, all) + a.i + 1, int64_t(0)), all));
 }
 
-// Chunks c_first .. c_first + c_count - 1.  tiles: row tiles a (chunk, key head) has, per
-// sequence (SHARED false) or in all (true).  Workgroups w of one XCD (w mod 8) take the
-// tiles of a (chunk, head) one after the other, so its codes come from that XCD's L2.
+// The value of the lane next to this one in its pair (lane ^ 1).
+__device__ __forceinline__ uint32_t other_of_pair(uint32_t v) {
+  return __builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true);
+}
+
+// Chunks of the shared pages (SHARED: a chunk and key head, a unit, to a workgroup, whose
+// waves take its blocks in turn and meet in LDS), or of the positions behind them (a unit to
+// a wave; heads run fastest, so a workgroup's waves walk the same pages side by side, and
+// no wave waits for another: 64 sequences of 8192 positions 664 us, with a unit to a
+// workgroup 672).  tiles: row tiles that a unit has, per sequence or (SHARED) in all.  The
+// workgroups of one XCD (w mod 8) take the tiles of a unit one after the other, so its
+// codes come from that XCD's L2 after the first.
 template <int HD, int NQT, bool SHARED>
-__global__ __launch_bounds__(AF_T, NQT == 2 ? 1 : 2) void attn_fp8_kernel(AttnFp8Args p, int c_first, int c_count, int tiles) {
-  constexpr int KS = HD / 32;      // k-steps of a score
-  constexpr int KH = HD / 64;      // 16-byte loads a position and lane
-  constexpr int ET = HD / 16;      // dim tiles
+__global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32_t tiles) {
+  constexpr int KS = HD / 32;           // k-steps of a score
+  constexpr int KH = HD / 64;           // 16-byte loads a position and lane
+  constexpr int ET = HD / 16;           // dim tiles
+  constexpr int EG = NQT == 2 ? 2 : 4;  // of them at once
   constexpr int ROWS = 16 * NQT;
-  __shared__ int32_t pages[AF_PAGES];
-  __shared__ float sk[AF_PAGES], sv[AF_PAGES];
-  __shared__ float wm[AF_NW][ROWS], wl[AF_NW][ROWS];
-  __shared__ float4 wo[AF_NW][ROWS][HD / 4 + 1];  // a wave's o (a row's padding parts the banks)
-  const int w = blockIdx.x, j8 = w >> 3;
-  const int64_t pair = static_cast<int64_t>(j8 / tiles) * 8 + (w & 7);
-  const int tile = j8 % tiles;
-  const int h = static_cast<int>(pair % p.kv);
-  const int64_t rest = pair / p.kv;
-  const int c = c_first + static_cast<int>(rest % c_count);
-  const int64_t seq = rest / c_count;
-  if (seq >= (SHARED ? 1 : p.B)) return;  // uniform: the grid's padding
-  const int64_t per = static_cast<int64_t>(p.n) * p.group;
-  const int64_t r0 = (SHARED ? 0 : seq * per) + static_cast<int64_t>(ROWS) * tile;
-  const int nrow = static_cast<int>(min(static_cast<int64_t>(ROWS), (SHARED ? p.B * per : (seq + 1) * per) - r0));
+  constexpr int STEP = SHARED ? AF_NW : 1;  // blocks from one of this wave's to the next
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int l0 = c * p.chunk;
+  // (all below 2^32, as the grid is: one 32-bit division each)
+  const uint32_t w = blockIdx.x, j8 = w >> 3, tile = j8 % tiles;
+  const uint32_t group = (j8 / tiles) * 8 + (w & 7), unit = SHARED ? group : group * AF_NW + wave;
+  const uint32_t rest = unit / p.kv;
+  const int h = static_cast<int>(unit - rest * p.kv);
+  const uint32_t c_count = SHARED ? p.snum : p.nchunk - p.snum;
+  const int64_t seq = rest / c_count;
+  if (seq >= (SHARED ? 1 : p.B)) return;  // the grid's padding
+  const int ci = static_cast<int>(rest % c_count), c = SHARED ? ci : p.snum + ci;
+  const uint32_t per = p.n * p.group, r0 = (SHARED ? 0 : seq * per) + ROWS * tile;
+  const int nrow = static_cast<int>(min(static_cast<uint32_t>(ROWS), (SHARED ? p.B * per : (seq + 1) * per) - r0));
+  const int64_t all = p.c.max_pages * KV_PAGE;
+  const int l0 = SHARED ? ci * p.schunk : p.shared + ci * p.chunk;  // the chunk is [l0, l2)
+  const int l2 = static_cast<int>(SHARED ? min(static_cast<int64_t>(l0) + p.schunk, static_cast<int64_t>(p.shared))
+                                         : min(static_cast<int64_t>(l0) + p.chunk, all));
+  // pages of a block: lane (n, g) reads keys of page n / 4 and values of page g
+  const int32_t *row = p.c.table + (SHARED ? 0 : seq) * p.c.st;
+  auto page_of = [&](int blk, int k) __attribute__((always_inline)) {
+    const int l = l0 + AF_BLK * blk + KV_PAGE * k;
+    int32_t pg = -1;
+    if (l < l2) pg = row[l / KV_PAGE];
+    return pg >= 0 && pg < p.c.num_pages ? pg : -1;  // -1: left out
+  };
+  const int first = SHARED ? wave : 0;
+  int32_t kpg = page_of(first, n >> 2), vpg = page_of(first, g);
   // ends of this lane's rows, of the positions any row attends to and that all do
-  int l1[NQT], l1max = l0, l1min = l0 + p.chunk;
+  int l1[NQT], l1max = l0, l1min = l2;
 #pragma unroll
   for (int nt = 0; nt < NQT; ++nt) {
     const bool live = 16 * nt + n < nrow;
-    l1[nt] = live ? min(l0 + p.chunk, row_len(p, attn_row(p, r0 + 16 * nt + n))) : l0;
+    l1[nt] = live ? min(l2, row_len(p, attn_row(p, r0 + 16 * nt + n))) : l0;
     l1max = max(l1max, l1[nt]);
     if (live) l1min = min(l1min, l1[nt]);
   }
@@ -104,23 +123,6 @@ __global__ __launch_bounds__(AF_T, NQT == 2 ? 1 : 2) void attn_fp8_kernel(AttnFp
   l1max = __builtin_amdgcn_readfirstlane(l1max);
   l1min = __builtin_amdgcn_readfirstlane(l1min);
   if (l0 >= l1max && p.nchunk > 1) return;  // the join does not ask for this chunk
-  // the chunk's pages below l1max (-1: left out) and their scales
-  const int32_t *row = p.c.table + (SHARED ? 0 : seq) * p.c.st;
-  for (int i = t; i < p.chunk / KV_PAGE; i += AF_T) {
-    int32_t pg = -1;
-    float a = 0.0f, b = 0.0f;
-    if (l0 + KV_PAGE * i < l1max) {
-      pg = row[l0 / KV_PAGE + i];
-      if (pg < 0 || pg >= p.c.num_pages) pg = -1;
-    }
-    if (pg >= 0) {
-      a = kv_pow2(kv_held(p.c.ks[pg * p.c.ksp + h * p.c.ksh]));
-      b = kv_pow2(kv_held(p.c.vs[pg * p.c.vsp + h * p.c.vsh]));
-    }
-    pages[i] = pg;
-    sk[i] = a;
-    sv[i] = b;
-  }
   // Q as the B operand: k-slot (g, j) of k-step 2 hf + u is dim 64 hf + 16 g + 8 u + j
   abf16x8_t qop[KS][NQT];
 #pragma unroll
@@ -135,7 +137,6 @@ __global__ __launch_bounds__(AF_T, NQT == 2 ? 1 : 2) void attn_fp8_kernel(AttnFp
       qop[ks][nt] = __builtin_bit_cast(abf16x8_t, x);
     }
   }
-  __syncthreads();
 
   float mrun[NQT], lrun[NQT];
   af32x4_t acc[ET][NQT];  // o^T: dims 16 e + 4 g + i in lane (n, g)
@@ -147,21 +148,33 @@ __global__ __launch_bounds__(AF_T, NQT == 2 ? 1 : 2) void attn_fp8_kernel(AttnFp
     for (int e = 0; e < ET; ++e) acc[e][nt] = af32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   const int nblk = (l1max - l0 + AF_BLK - 1) / AF_BLK;
-  // (a page left out reads page 0: its scores are masked, its values set to zero)
+  // Loads of a block: its pages' scales, keys and values (a page left out reads page 0: its
+  // scores are masked, its values set to zero).  Read once a launch, so with the
+  // non-temporal hint (64 sequences of 8192 positions: 757 -> 714 us).  A key tile's 16 rows
+  // of 128 bytes come as whole lines: eight lanes take a row, those of pair (m, m ^ 1) the
+  // row of one of them in each of two loads, and exchange the halves when they read them
+  // (half lines cost 3% of the stream).
   au32x4_t kr[4][KH], vr[ET];
-  auto kload = [&](int blk) __attribute__((always_inline)) {
-    const int64_t pg = max(pages[4 * blk + (n >> 2)], 0);
-    const uint8_t *a = p.c.k + pg * p.c.kp + h * p.c.kh + (n & 3) * HD + 16 * g;
+  float ksc, vsc;
+  const bool odd = n & 1;
+  auto kload = [&](int32_t pg) __attribute__((always_inline)) {
+    const int64_t at = max(pg, 0);
+    ksc = p.c.ks[at * p.c.ksp + h * p.c.ksh];
+    const uint8_t *a = p.c.k + at * p.c.kp + h * p.c.kh + 16 * g;
+    if constexpr (HD == 128) a += (n & 2) * HD + 64 * (n & 1);
+    else a += (n & 3) * HD;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int hf = 0; hf < KH; ++hf) kr[tt][hf] = *reinterpret_cast<const au32x4_t *>(a + 4 * tt * HD + 64 * hf);
+      for (int hf = 0; hf < KH; ++hf)
+        kr[tt][hf] = __builtin_nontemporal_load(reinterpret_cast<const au32x4_t *>(a + (4 * tt + hf) * HD));
   };
-  auto vload = [&](int blk) __attribute__((always_inline)) {
-    const int64_t pg = max(pages[4 * blk + g], 0);
-    const uint8_t *a = p.c.v + pg * p.c.vp + h * p.c.vh + 16 * n;
+  auto vload = [&](int32_t pg) __attribute__((always_inline)) {
+    const int64_t at = max(pg, 0);
+    vsc = p.c.vs[at * p.c.vsp + h * p.c.vsh];
+    const uint8_t *a = p.c.v + at * p.c.vp + h * p.c.vh + 16 * n;
 #pragma unroll
-    for (int e = 0; e < ET; ++e) vr[e] = *reinterpret_cast<const au32x4_t *>(a + 256 * e);
+    for (int e = 0; e < ET; ++e) vr[e] = __builtin_nontemporal_load(reinterpret_cast<const au32x4_t *>(a + 256 * e));
   };
   // eight codes (two dwords) as a bf16 operand
   auto operand = [&](uint32_t a, uint32_t b, float s) __attribute__((always_inline)) {
@@ -169,45 +182,73 @@ __global__ __launch_bounds__(AF_T, NQT == 2 ? 1 : 2) void attn_fp8_kernel(AttnFp
     return __builtin_bit_cast(abf16x8_t, o);
   };
   const float c2 = p.scale * 1.4426950408889634f;  // scores in log2 units
-  auto block = [&](int blk, auto mask_c) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_c)::value;
+  int32_t knext = -1, vnext = -1;                  // the next block's pages
+  if (first < nblk) {
+    kload(kpg);
+    vload(vpg);
+    knext = page_of(first + STEP, n >> 2);
+    vnext = page_of(first + STEP, g);
+  }
+  for (int blk = first; blk < nblk; blk += STEP) {
     const int lb = l0 + AF_BLK * blk;
-    const bool more = blk + AF_NW < nblk;  // uniform
+    // whole (uniform): every row attends to all of it and its pages are in the cache
+    const bool whole = lb + AF_BLK <= l1min && !__any(vpg < 0);
+    const bool more = blk + STEP < nblk;  // uniform
     af32x4_t s[4][NQT];
     {
-      const float ksc = sk[4 * blk + (n >> 2)];
+      const float sc = kv_pow2(kv_held(ksc));
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
+      for (int t0 = 0; t0 < 4; t0 += 2) {  // two tiles at once: independent sums for the matrix cores
 #pragma unroll
-        for (int nt = 0; nt < NQT; ++nt) s[tt][nt] = af32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int tt = t0; tt < t0 + 2; ++tt) {
+          if constexpr (HD == 128) {  // whole rows into their lanes
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const au32x4_t x = kr[tt][ks / 2];
-          const abf16x8_t a = operand(x[2 * (ks % 2)], x[2 * (ks % 2) + 1], ksc);
+            for (int d = 0; d < 4; ++d) {
+              const uint32_t a = kr[tt][0][d], b = kr[tt][1][d], ao = other_of_pair(a), bo = other_of_pair(b);
+              kr[tt][0][d] = odd ? bo : a;
+              kr[tt][1][d] = odd ? b : ao;
+            }
+          }
 #pragma unroll
-          for (int nt = 0; nt < NQT; ++nt)
-            s[tt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qop[ks][nt], s[tt][nt], 0, 0, 0);
+          for (int nt = 0; nt < NQT; ++nt) s[tt][nt] = af32x4_t{0.f, 0.f, 0.f, 0.f};
         }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int tt = t0; tt < t0 + 2; ++tt) {
+            const au32x4_t x = kr[tt][ks / 2];
+            const abf16x8_t a = operand(x[2 * (ks % 2)], x[2 * (ks % 2) + 1], sc);
+#pragma unroll
+            for (int nt = 0; nt < NQT; ++nt)
+              s[tt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qop[ks][nt], s[tt][nt], 0, 0, 0);
+          }
+        __builtin_amdgcn_sched_barrier(0);  // (operands of all tiles at once would take their registers)
       }
     }
-    if (more) kload(blk + AF_NW);
+    if (more) {
+      kload(knext);
+      knext = page_of(blk + 2 * STEP, n >> 2);
+    }
     // s[tt][nt][i]: position lb + 16 g + 4 tt + i (page g of the block), row 16 nt + n
-    const bool held = !MASK || pages[4 * blk + g] >= 0;
+    if (!whole) {
+#pragma unroll
+      for (int nt = 0; nt < NQT; ++nt)
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (vpg < 0 || lb + 16 * g + 4 * tt + i >= l1[nt]) s[tt][nt][i] = -INFINITY;
+    }
 #pragma unroll
     for (int nt = 0; nt < NQT; ++nt) {
       float bm = -INFINITY;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = s[tt][nt][i] * c2;
-          if constexpr (MASK) v = held && lb + 16 * g + 4 * tt + i < l1[nt] ? v : -INFINITY;
-          s[tt][nt][i] = v;
-          bm = fmaxf(bm, v);
-        }
+        for (int i = 0; i < 4; ++i) bm = fmaxf(bm, s[tt][nt][i]);
       bm = fmaxf(bm, __shfl_xor(bm, 16));
       bm = fmaxf(bm, __shfl_xor(bm, 32));
-      const float mn = fmaxf(mrun[nt], bm);
+      const float mn = fmaxf(mrun[nt], bm * c2);  // (c2 > 0)
       const float msub = mn == -INFINITY ? 0.0f : mn;  // nothing but masks so far
       const float alpha = __builtin_amdgcn_exp2f(mrun[nt] - msub);
       float ls = 0.0f;
@@ -215,7 +256,7 @@ __global__ __launch_bounds__(AF_T, NQT == 2 ? 1 : 2) void attn_fp8_kernel(AttnFp
       for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float pe = __builtin_amdgcn_exp2f(s[tt][nt][i] - msub);
+          const float pe = __builtin_amdgcn_exp2f(fmaf(s[tt][nt][i], c2, -msub));
           s[tt][nt][i] = pe;
           ls += pe;
         }
@@ -226,9 +267,8 @@ __global__ __launch_bounds__(AF_T, NQT == 2 ? 1 : 2) void attn_fp8_kernel(AttnFp
         for (int e = 0; e < ET; ++e) acc[e][nt] *= alpha;
       }
     }
-    const float vsc = sv[4 * blk + g];
-    if constexpr (MASK) {  // bytes that no query attends to (of any content) become zeros
-      const int live = held ? min(max(l1max - lb - 16 * g, 0), KV_PAGE) : 0;
+    if (!whole) {  // bytes that no query attends to (of any content) become zeros
+      const int live = vpg >= 0 ? min(max(l1max - lb - 16 * g, 0), KV_PAGE) : 0;
       au32x4_t keep;
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
@@ -238,6 +278,7 @@ __global__ __launch_bounds__(AF_T, NQT == 2 ? 1 : 2) void attn_fp8_kernel(AttnFp
 #pragma unroll
       for (int e = 0; e < ET; ++e) vr[e] &= keep;
     }
+    const float sc = kv_pow2(kv_held(vsc));
 #pragma unroll
     for (int u = 0; u < 2; ++u) {  // k-step u: positions 8 u .. 8 u + 7 of page g
       abf16x8_t ph[NQT], pl[NQT];
@@ -254,130 +295,212 @@ __global__ __launch_bounds__(AF_T, NQT == 2 ? 1 : 2) void attn_fp8_kernel(AttnFp
         pl[nt] = __builtin_bit_cast(abf16x8_t, lo);
       }
 #pragma unroll
-      for (int e = 0; e < ET; ++e) {
-        const abf16x8_t a = operand(vr[e][2 * u], vr[e][2 * u + 1], vsc);
+      for (int e0 = 0; e0 < ET; e0 += EG) {
+        abf16x8_t a[EG];
+#pragma unroll
+        for (int e = 0; e < EG; ++e) a[e] = operand(vr[e0 + e][2 * u], vr[e0 + e][2 * u + 1], sc);
 #pragma unroll
         for (int nt = 0; nt < NQT; ++nt) {
-          acc[e][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, ph[nt], acc[e][nt], 0, 0, 0);
-          acc[e][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pl[nt], acc[e][nt], 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < EG; ++e)
+            acc[e0 + e][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[e], ph[nt], acc[e0 + e][nt], 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < EG; ++e)
+            acc[e0 + e][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[e], pl[nt], acc[e0 + e][nt], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (more) vload(blk + AF_NW);
-  };
-  if (wave < nblk) {
-    kload(wave);
-    vload(wave);
-  }
-  for (int blk = wave; blk < nblk; blk += AF_NW) {
-    // whole: every row attends to all of it and its pages are in the cache
-    const int end = l0 + AF_BLK * (blk + 1);
-    const bool whole = end <= l1min && !__any(pages[4 * blk + g] < 0);
-    if (whole) block(blk, std::false_type{});
-    else block(blk, std::true_type{});
+    if (more) {
+      vload(vnext);
+      vpg = vnext;
+      vnext = page_of(blk + 2 * STEP, g);
+    }
   }
 
-  // the waves' (max, sum, o) meet
+  // a row's max and sum, in all lanes (n, .) of it
 #pragma unroll
   for (int nt = 0; nt < NQT; ++nt) {
-    float l = lrun[nt];
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    const int r = 16 * nt + n;
-    if (g == 0) {
-      wm[wave][r] = mrun[nt];
-      wl[wave][r] = l;
-    }
-#pragma unroll
-    for (int e = 0; e < ET; ++e)
-      wo[wave][r][4 * e + g] = make_float4(acc[e][nt][0], acc[e][nt][1], acc[e][nt][2], acc[e][nt][3]);
+    lrun[nt] += __shfl_xor(lrun[nt], 16);
+    lrun[nt] += __shfl_xor(lrun[nt], 32);
   }
-  __syncthreads();
-  for (int x = t; x < nrow * (HD / 4); x += AF_T) {
-    const int r = x / (HD / 4), d4 = x % (HD / 4);
-    float M = wm[0][r];
-#pragma unroll
-    for (int k = 1; k < AF_NW; ++k) M = fmaxf(M, wm[k][r]);
-    float tot = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int k = 0; k < AF_NW; ++k) {
-      const float f = wm[k][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[k][r] - M);
-      const float4 a = wo[k][r][d4];
-      tot = fmaf(f, wl[k][r], tot);
-      o.x = fmaf(f, a.x, o.x); o.y = fmaf(f, a.y, o.y); o.z = fmaf(f, a.z, o.z); o.w = fmaf(f, a.w, o.w);
-    }
+  // dims d .. d + 3 of row r: to the output (one chunk) or to the chunk's part
+  auto store = [&](int r, int d, af32x4_t o, float m, float l) __attribute__((always_inline)) {
     const AttnRow a = attn_row(p, r0 + r);
     const int64_t head = static_cast<int64_t>(h) * p.group + a.j;
     if (p.nchunk == 1) {
-      const float inv = tot != 0.0f ? 1.0f / tot : 0.0f;  // (a NaN sum stays NaN)
-      uint2 y = make_uint2(pack_bf(o.x * inv, o.y * inv), pack_bf(o.z * inv, o.w * inv));
-      *reinterpret_cast<uint2 *>(p.out + a.b * p.ob + a.i * p.ot + head * p.oh + 4 * d4) = y;
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // (a NaN sum stays NaN)
+      *reinterpret_cast<uint2 *>(p.out + a.b * p.ob + a.i * p.ot + head * p.oh + d) =
+          make_uint2(pack_bf(o[0] * inv, o[1] * inv), pack_bf(o[2] * inv, o[3] * inv));
     } else {
-      float *part = p.part + (((static_cast<int64_t>(a.b) * p.n + a.i) * p.heads + head) * p.nchunk + c) * (HD + 2);
-      *reinterpret_cast<float2 *>(part + 4 * d4) = make_float2(o.x, o.y);
-      *reinterpret_cast<float2 *>(part + 4 * d4 + 2) = make_float2(o.z, o.w);
-      if (d4 == 0) *reinterpret_cast<float2 *>(part + HD) = make_float2(M, tot);
+      const int64_t at = ((static_cast<int64_t>(a.b) * p.n + a.i) * p.heads + head) * p.nchunk + c;
+      *reinterpret_cast<af32x4_t *>(p.part + at * HD + d) = o;
+      if (d == 0) p.ml[at] = make_float2(m, l);
+    }
+  };
+  if constexpr (!SHARED) {
+#pragma unroll
+    for (int nt = 0; nt < NQT; ++nt)
+      if (16 * nt + n < nrow) {
+#pragma unroll
+        for (int e = 0; e < ET; ++e) store(16 * nt + n, 16 * e + 4 * g, acc[e][nt], mrun[nt], lrun[nt]);
+      }
+  } else {  // the waves' (max, sum, o) meet
+    __shared__ float wm[AF_NW][ROWS], wl[AF_NW][ROWS];
+    __shared__ af32x4_t wo[AF_NW][ROWS][HD / 4 + 1];  // (a row's padding parts the banks)
+#pragma unroll
+    for (int nt = 0; nt < NQT; ++nt) {
+      const int r = 16 * nt + n;
+      if (g == 0) {
+        wm[wave][r] = mrun[nt];
+        wl[wave][r] = lrun[nt];
+      }
+#pragma unroll
+      for (int e = 0; e < ET; ++e) wo[wave][r][4 * e + g] = acc[e][nt];
+    }
+    __syncthreads();
+    for (int x = t; x < nrow * (HD / 4); x += AF_T) {
+      const int r = x / (HD / 4), d4 = x % (HD / 4);
+      float M = wm[0][r];
+#pragma unroll
+      for (int k = 1; k < AF_NW; ++k) M = fmaxf(M, wm[k][r]);
+      float tot = 0.0f;
+      af32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < AF_NW; ++k) {
+        const float f = wm[k][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[k][r] - M);
+        tot = fmaf(f, wl[k][r], tot);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] = fmaf(f, wo[k][r][d4][d], o[d]);
+      }
+      store(r, 4 * d4, o, M, tot);
     }
   }
 }
 
-// Joins a query row's chunks: HD lanes, in chunk order.
+// Joins a query row's chunks, in a fixed order: weights 2^(max - all's max) of up to JN
+// chunks at a time in LDS, then wave w sums chunks w, w + 4, ..
+constexpr int JN = 256;
+
 template <int HD>
-__global__ __launch_bounds__(HD) void attn_fp8_join_kernel(AttnFp8Args p) {
-  const int d = threadIdx.x, head = blockIdx.x;
-  const int bi = blockIdx.y, b = bi / p.n, i = bi % p.n;
-  const int nc = (row_len(p, AttnRow{b, i, 0}) + p.chunk - 1) / p.chunk;
-  const float *part = p.part + (static_cast<int64_t>(bi) * p.heads + head) * p.nchunk * (HD + 2);
+__global__ __launch_bounds__(AF_T) void attn_fp8_join_kernel(AttnFp8Args p) {
+  constexpr int DL = HD / 64;  // dims a lane
+  __shared__ float f[JN], red[AF_NW], tots[AF_NW], os[AF_NW][HD];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, head = blockIdx.x;
+  const int bi = blockIdx.y, b = bi / static_cast<int>(p.n), i = bi % static_cast<int>(p.n);
+  const int len = row_len(p, AttnRow{b, i, 0});
+  // chunks that reach below len: of the shared pages, and behind them
+  const int nc = len <= p.shared ? (len + p.schunk - 1) / max(p.schunk, 1)
+                                 : p.snum + (len - p.shared + p.chunk - 1) / p.chunk;
+  const int64_t at = (static_cast<int64_t>(bi) * p.heads + head) * p.nchunk;
   float M = -INFINITY;
-#pragma unroll 8
-  for (int c = 0; c < nc; ++c) M = fmaxf(M, part[c * (HD + 2) + HD]);
-  float tot = 0.0f, o = 0.0f;
-#pragma unroll 8
-  for (int c = 0; c < nc; ++c) {
-    const float mc = part[c * (HD + 2) + HD];
-    const float f = mc == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc - M);
-    tot = fmaf(f, part[c * (HD + 2) + HD + 1], tot);
-    o = fmaf(f, part[c * (HD + 2) + d], o);
+  for (int c = t; c < nc; c += AF_T) M = fmaxf(M, p.ml[at + c].x);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+  if (lane == 0) red[wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float tot = 0.0f, o[DL] = {};
+  for (int c0 = 0; c0 < nc; c0 += JN) {
+    __syncthreads();
+    if (c0 + t < nc) {
+      const float2 ml = p.ml[at + c0 + t];
+      const float x = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+      f[t] = x;
+      tot = fmaf(x, ml.y, tot);
+    }
+    __syncthreads();
+    const int n = min(JN, nc - c0);
+#pragma unroll 4
+    for (int c = wave; c < n; c += AF_NW) {
+      const float x = f[c];
+      const float *part = p.part + (at + c0 + c) * HD + DL * lane;
+      if constexpr (DL == 2) {
+        const float2 v = *reinterpret_cast<const float2 *>(part);
+        o[0] = fmaf(x, v.x, o[0]);
+        o[1] = fmaf(x, v.y, o[1]);
+      } else {
+        o[0] = fmaf(x, part[0], o[0]);
+      }
+    }
   }
-  p.out[static_cast<int64_t>(b) * p.ob + i * p.ot + head * p.oh + d] = f2bf(tot != 0.0f ? o / tot : 0.0f);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) tot += __shfl_xor(tot, d);
+  if (lane == 0) tots[wave] = tot;
+#pragma unroll
+  for (int d = 0; d < DL; ++d) os[wave][DL * lane + d] = o[d];
+  __syncthreads();
+  if (t < HD) {
+    const float sum = (tots[0] + tots[1]) + (tots[2] + tots[3]);
+    const float v = (os[0][t] + os[1][t]) + (os[2][t] + os[3][t]);
+    p.out[static_cast<int64_t>(b) * p.ob + i * p.ot + head * p.oh + t] = f2bf(sum != 0.0f ? v / sum : 0.0f);
+  }
 }
 
-// Positions a chunk takes: as many workgroups as keep the card's loads in flight
-// (AF_GROUPS), in chunks of 256 (a block for each wave) to AF_CHUNK positions.
-constexpr int64_t AF_GROUPS = 1024;
+// Positions of a chunk (a multiple of `step`, at most `most`) for L positions of `units`
+// (sequence, key head, row tile)s, `slots` chunks at once on the card.  Costs in positions
+// of a chunk's own walk: its start and end are as long as AF_START of them, and each chunk
+// costs the join AF_JOIN; the walk's time is between that of whole rounds of equal chunks
+// and that of evenly spread work with half a chunk's tail, the mean is taken.  (64 sequences
+// of 8192 positions, 32 heads: chunks of 4352 665 us, 2048 672, 1024 683, 512 704.)
+constexpr int64_t AF_START = 128, AF_JOIN = 8;
 
-static int chunk_for(int64_t B, int64_t n, int64_t heads, int64_t kv, int64_t max_pages) {
-  const int64_t L = max_pages * KV_PAGE, rows = n * (heads / kv);
-  const int64_t units = B * kv * cdiv(rows, 16);
-  const int64_t want = cdiv(AF_GROUPS, units);  // chunks a unit
-  const int64_t chunk = cdiv(cdiv(L, want), 256) * 256;
-  return static_cast<int>(chunk < AF_CHUNK ? chunk : AF_CHUNK);
+static int chunk_for(int64_t L, int64_t units, int64_t slots, int64_t step, int64_t most) {
+  int64_t best = 0, best_cost = 0;
+  for (int64_t nc = 1, chunk = 0; chunk != step; nc += nc < 8 ? 1 : nc / 4) {
+    chunk = cdiv(cdiv(L, nc), step) * step;
+    if (chunk > most) continue;
+    const int64_t num = cdiv(L, chunk);
+    const int64_t rounds = cdiv(units * num, slots) * (chunk + AF_START);
+    const int64_t even = units * (L + num * AF_START) / slots + chunk / 2;
+    const int64_t cost = rounds + (units * num > slots ? even : rounds) + AF_JOIN * num;
+    if (!best || cost < best_cost) {
+      best = chunk;
+      best_cost = cost;
+    }
+  }
+  return static_cast<int>(best);
+}
+
+// The split of a call: shared positions, and chunks of them and of those behind.
+struct AttnSplit {
+  int shared, schunk, snum, chunk, nchunk;
+};
+static AttnSplit split_for(int64_t B, int64_t n, int64_t heads, int64_t kv, int64_t max_pages, int64_t shared_pages) {
+  const int64_t L = max_pages * KV_PAGE, shared = shared_pages * KV_PAGE, rows = n * (heads / kv);
+  AttnSplit s{static_cast<int>(shared), 0, 0, AF_BLK, 0};
+  if (shared) {  // of one length for all: as long as gives two workgroups a CU
+    s.schunk = chunk_for(shared, kv * cdiv(B * rows, 32), 512, AF_BLK * AF_NW, int64_t(1) << 30);
+    s.snum = static_cast<int>(cdiv(shared, s.schunk));
+  }
+  if (L > shared)  // lengths differ: a long chunk would be the launch's tail
+    s.chunk = chunk_for(L - shared, B * kv * cdiv(rows, 16), 2048, AF_BLK, 8192);
+  s.nchunk = s.snum + static_cast<int>(cdiv(L - shared, s.chunk));
+  return s;
 }
 
 template <int HD>
-static int launch_fp8(const AttnFp8Args &a, int shared_chunks, hipStream_t st) {
-  const int64_t per = static_cast<int64_t>(a.n) * a.group;
-  const int64_t own = a.nchunk - shared_chunks;
+static int launch_fp8(const AttnFp8Args &a, hipStream_t st) {
+  const int64_t per = static_cast<int64_t>(a.n) * a.group, own = a.nchunk - a.snum;
   const int64_t tiles0 = cdiv(a.B * per, 32), tiles1 = cdiv(per, 16);
-  const int64_t wgs0 = cdiv(static_cast<int64_t>(shared_chunks) * a.kv, 8) * 8 * tiles0;
-  const int64_t wgs1 = cdiv(own * a.kv * a.B, 8) * 8 * tiles1;
+  const int64_t wgs0 = cdiv(static_cast<int64_t>(a.snum) * a.kv, 8) * 8 * tiles0;
+  const int64_t wgs1 = cdiv(own * a.kv * a.B, 8 * AF_NW) * 8 * tiles1;
   if (!grid_fits(wgs0, AF_T) || !grid_fits(wgs1, AF_T) || static_cast<int64_t>(a.B) * a.n > 65535)
     return fail(EVO2_ERR_UNSUPPORTED, "paged_decode_attention_fp8: more workgroups than a launch takes");
-  if (shared_chunks > 0) {
-    hipLaunchKernelGGL((attn_fp8_kernel<HD, 2, true>), dim3(static_cast<unsigned>(wgs0)), dim3(AF_T), 0, st, a, 0,
-                       shared_chunks, static_cast<int>(tiles0));
+  if (wgs0) {
+    hipLaunchKernelGGL((attn_fp8_kernel<HD, 2, true>), dim3(static_cast<unsigned>(wgs0)), dim3(AF_T), 0, st, a,
+                       static_cast<uint32_t>(tiles0));
     const int rc = check_launch("paged_decode_attention_fp8 shared chunks");
     if (rc) return rc;
   }
-  if (own > 0) {
+  if (wgs1) {
     hipLaunchKernelGGL((attn_fp8_kernel<HD, 1, false>), dim3(static_cast<unsigned>(wgs1)), dim3(AF_T), 0, st, a,
-                       shared_chunks, static_cast<int>(own), static_cast<int>(tiles1));
+                       static_cast<uint32_t>(tiles1));
     const int rc = check_launch("paged_decode_attention_fp8 chunks");
     if (rc) return rc;
   }
   if (a.nchunk == 1) return EVO2_OK;
-  hipLaunchKernelGGL(attn_fp8_join_kernel<HD>, dim3(a.heads, static_cast<unsigned>(a.B * a.n)), dim3(HD), 0, st, a);
+  hipLaunchKernelGGL(attn_fp8_join_kernel<HD>, dim3(a.heads, static_cast<unsigned>(a.B * a.n)), dim3(AF_T), 0, st, a);
   return check_launch("paged_decode_attention_fp8 join");
 }
 
@@ -386,11 +509,13 @@ static int launch_fp8(const AttnFp8Args &a, int shared_chunks, hipStream_t st) {
 using namespace evo2;
 
 extern "C" int64_t evo2_decode_attention_fp8_workspace_bytes(int64_t B, int64_t n, int64_t heads, int64_t kv_heads,
-                                                             int64_t head_dim, int64_t max_pages) {
+                                                             int64_t head_dim, int64_t max_pages,
+                                                             int64_t shared_pages) {
   if (B <= 0 || n <= 0 || kv_heads <= 0 || heads < kv_heads || heads % kv_heads || head_dim <= 0 || max_pages <= 0 ||
-      B > 65535 || n > 65535 || heads > 65535 || head_dim > 65535 || max_pages > (int64_t(1) << 26))
+      B > 65535 || n > 65535 || heads > 65535 || head_dim > 65535 || max_pages > (int64_t(1) << 26) ||
+      shared_pages < 0 || shared_pages > max_pages)
     return 0;
-  const int64_t nchunk = cdiv(max_pages * KV_PAGE, chunk_for(B, n, heads, kv_heads, max_pages));
+  const int64_t nchunk = split_for(B, n, heads, kv_heads, max_pages, shared_pages).nchunk;
   return nchunk == 1 ? 0 : B * n * heads * nchunk * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
@@ -417,18 +542,21 @@ extern "C" int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_
   const int rc = kv_check(c, kv_heads, head_dim, "paged_decode_attention_fp8");
   if (rc) return rc;
   if (!q || !positions || !out) return fail(EVO2_ERR_INVALID, "paged_decode_attention_fp8: null pointer argument");
-  const int64_t need = evo2_decode_attention_fp8_workspace_bytes(B, n, heads, kv_heads, head_dim, max_pages);
+  const int64_t need = evo2_decode_attention_fp8_workspace_bytes(B, n, heads, kv_heads, head_dim, max_pages,
+                                                                 shared_pages);
   if (workspace_bytes < need || (need > 0 && !workspace))
     return fail(EVO2_ERR_INVALID, "paged_decode_attention_fp8: workspace too small");
   if (reinterpret_cast<uintptr_t>(q) % 16 || qb % 8 || qt % 8 || qh % 8 || reinterpret_cast<uintptr_t>(out) % 8 ||
-      ob % 4 || ot % 4 || oh % 4 || reinterpret_cast<uintptr_t>(workspace) % 8)
+      ob % 4 || ot % 4 || oh % 4 || reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(EVO2_ERR_UNSUPPORTED, "paged_decode_attention_fp8: rows must be 16-byte aligned");
-  const int chunk = chunk_for(B, n, heads, kv_heads, max_pages);
-  const AttnFp8Args a{c, static_cast<const bf16_t *>(q), qb, qt, qh, positions, static_cast<float *>(workspace),
-                      static_cast<bf16_t *>(out), ob, ot, oh, scale, static_cast<int>(B), static_cast<int>(n),
-                      static_cast<int>(heads), static_cast<int>(heads / kv_heads), static_cast<int>(kv_heads), chunk,
-                      static_cast<int>(cdiv(max_pages * KV_PAGE, chunk))};
-  const int shared_chunks = static_cast<int>(shared_pages * KV_PAGE / chunk);
+  const AttnSplit sp = split_for(B, n, heads, kv_heads, max_pages, shared_pages);
+  float *part = static_cast<float *>(workspace);
+  const AttnFp8Args a{c, static_cast<const bf16_t *>(q), qb, qt, qh, positions, part,
+                      part ? reinterpret_cast<float2 *>(part + B * n * heads * sp.nchunk * head_dim) : nullptr,
+                      static_cast<bf16_t *>(out), ob, ot, oh, scale, static_cast<uint32_t>(B), static_cast<uint32_t>(n),
+                      static_cast<uint32_t>(heads), static_cast<uint32_t>(heads / kv_heads),
+                      static_cast<uint32_t>(kv_heads),
+                      sp.shared, sp.schunk, sp.snum, sp.chunk, sp.nchunk};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return head_dim == 64 ? launch_fp8<64>(a, shared_chunks, s) : launch_fp8<128>(a, shared_chunks, s);
+  return head_dim == 64 ? launch_fp8<64>(a, s) : launch_fp8<128>(a, s);
 }

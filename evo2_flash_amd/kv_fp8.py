@@ -28,55 +28,77 @@ _F8 = torch.float8_e4m3fn
 _INTS = (torch.int32, torch.int64)
 
 
+# The checks below run for every call of a decode step, which waits for the host: each of a
+# tensor's properties is asked for once (attention of one sequence 20 -> 14 us a call).
 def _cache_args(what, k_pages, v_pages, k_scale, v_scale, block_table, B):
     """Checks of the cache's tensors and the table; the C entries' arguments from the key
-    pages to the table's columns, and (kv_heads, head_dim)."""
-    if not (k_pages.dim() == v_pages.dim() == 4 and k_pages.dtype == v_pages.dtype == _F8):
+    pages to the table's columns, and (kv_heads, head_dim, device index)."""
+    dev = k_pages.get_device()
+    if not (dev >= 0 and dev == v_pages.get_device() == k_scale.get_device() == v_scale.get_device()
+            == block_table.get_device()):
+        _lib.require_device(k_pages, v_pages, k_scale, v_scale, block_table)
+        raise ValueError(f"{what}: the cache and its table are on different devices")
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[2] != PAGE or k_pages.dtype != _F8 or v_pages.dtype != _F8:
         raise ValueError(f"{what} takes float8_e4m3fn pages (pages, kv_heads, {PAGE}, head_dim) and "
-                         f"(pages, kv_heads, head_dim, {PAGE})")
-    pages, kv, rows, hd = k_pages.shape
-    if rows != PAGE or v_pages.shape != (pages, kv, hd, PAGE):
-        raise ValueError(f"{what}: page shapes {tuple(k_pages.shape)}, {tuple(v_pages.shape)} do not match")
-    if hd not in (64, 128):
+                         f"(pages, kv_heads, head_dim, {PAGE}), got {tuple(shape)} {k_pages.dtype}, "
+                         f"{tuple(v_pages.shape)} {v_pages.dtype}")
+    pages, kv, _, hd = shape
+    if v_pages.shape != (pages, kv, hd, PAGE):
+        raise ValueError(f"{what}: page shapes {tuple(shape)}, {tuple(v_pages.shape)} do not match")
+    if hd != 128 and hd != 64:
         raise ValueError(f"{what} takes head_dim 64 or 128, got {hd}")
-    if (k_scale.shape != (pages, kv) or v_scale.shape != (pages, kv)
-            or not k_scale.dtype == v_scale.dtype == torch.float32):
+    if (k_scale.shape != (pages, kv) or v_scale.shape != (pages, kv) or k_scale.dtype != torch.float32
+            or v_scale.dtype != torch.float32):
         raise ValueError(f"{what}: scales must be ({pages}, {kv}) fp32, got {tuple(k_scale.shape)} "
                          f"{k_scale.dtype}, {tuple(v_scale.shape)} {v_scale.dtype}")
     if pages == 0 or kv == 0:
         raise ValueError(f"{what}: a cache of no pages or heads")
     kps, khs, k2, k3 = k_pages.stride()
     vps, vhs, v2, v3 = v_pages.stride()
-    if (k2, k3) != (hd, 1) or (v2, v3) != (PAGE, 1):
+    if k2 != hd or k3 != 1 or v2 != PAGE or v3 != 1:
         raise ValueError(f"{what}: a page's head must be contiguous")
-    if (block_table.dim() != 2 or block_table.shape[0] < B or block_table.shape[1] == 0
-            or block_table.dtype != torch.int32 or block_table.stride(1) != 1):
-        raise ValueError("block_table must be (>= B, max_pages) int32 with unit column stride")
-    if not _lib.same_device(k_pages, v_pages, k_scale, v_scale, block_table):
-        raise ValueError(f"{what}: the cache and its table are on different devices")
+    table = block_table.shape
+    if len(table) != 2 or table[0] < B or table[1] == 0 or block_table.dtype != torch.int32:
+        raise ValueError(f"block_table must be (>= {B}, max_pages) int32, got {tuple(table)} "
+                         f"{block_table.dtype}")
+    row, unit = block_table.stride()
+    if unit != 1 and table[1] != 1:
+        raise ValueError("block_table must have unit column stride")
     return (k_pages.data_ptr(), kps, khs, v_pages.data_ptr(), vps, vhs, k_scale.data_ptr(),
-            *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride(), pages, block_table.data_ptr(),
-            block_table.stride(0), block_table.shape[1]), kv, hd
+            *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride(), pages, block_table.data_ptr(), row,
+            table[1]), kv, hd, dev
 
 
-def _per_sequence(t, B, name, device):
+def _on(dev, what, *tensors):
+    """Refuse tensors that are not on the cache's device `dev`."""
+    for t in tensors:
+        if t.get_device() != dev:
+            _lib.require_device(t)
+            raise ValueError(f"{what}: a tensor on {t.device}, the cache on cuda:{dev}")
+
+
+def _per_sequence(t, B, name, dev):
     """t (B,) int32 or int64 on the cache's device, as contiguous int64."""
     if t.shape != (B,) or t.dtype not in _INTS:
         raise ValueError(f"{name} must be ({B},) int32 or int64, got {tuple(t.shape)} {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
-    if t.dtype == torch.int64 and (B == 1 or t.stride(0) == 1):
+    if t.get_device() != dev:
+        _on(dev, name, t)
+    if t.dtype == torch.int64 and (B <= 1 or t.stride(0) == 1):
         return t
     return t.to(torch.int64).contiguous()
 
 
 def _token_rows(t):
     """t (B, n, heads, hd) with rows as the kernels read them: unit last stride, 16-byte
-    aligned; itself or a copy."""
+    aligned; (itself or a copy, address, batch, token and head stride)."""
     b, n, h, unit = t.stride()
-    if unit != 1 or (b | n | h) & 7 or t.data_ptr() & 15:
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    at = t.data_ptr()
+    if unit != 1 or (b | n | h) & 7 or at & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        b, n, h, _ = t.stride()
+        at = t.data_ptr()
+    return t, at, b, n, h
 
 
 def write_kv_fp8(k, v, k_pages, v_pages, k_scale, v_scale, block_table, positions, lengths=None):
@@ -88,26 +110,25 @@ def write_kv_fp8(k, v, k_pages, v_pages, k_scale, v_scale, block_table, position
     table, or whose entry lies outside the cache's pages, are not written; nor is any token of
     a sequence that starts there.  Codes of positions that are not written keep their bytes
     (of positions held before theirs: see the module's description)."""
-    _lib.require_device(k, v, k_pages, v_pages, k_scale, v_scale, block_table, positions, lengths)
-    if not (k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype == torch.bfloat16):
+    shape, bf = k.shape, torch.bfloat16
+    if len(shape) != 4 or v.shape != shape or k.dtype != bf or v.dtype != bf:
         raise ValueError(f"write_kv_fp8 takes bf16 k and v (B, n, kv_heads, head_dim), got "
-                         f"{tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
-    B, n = k.shape[:2]
-    cache, kv, hd = _cache_args("write_kv_fp8", k_pages, v_pages, k_scale, v_scale, block_table, B)
-    if k.shape[2:] != (kv, hd):
-        raise ValueError(f"write_kv_fp8: tokens of {tuple(k.shape[2:])}, pages of ({kv}, {hd})")
-    if k.device != k_pages.device or v.device != k_pages.device:
-        raise ValueError(f"write_kv_fp8: tokens on {k.device}, {v.device}, the cache on {k_pages.device}")
-    positions = _per_sequence(positions, B, "positions", k_pages.device)
+                         f"{tuple(shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
+    B, n, heads, width = shape
+    cache, kv, hd, dev = _cache_args("write_kv_fp8", k_pages, v_pages, k_scale, v_scale, block_table, B)
+    if heads != kv or width != hd:
+        raise ValueError(f"write_kv_fp8: tokens of ({heads}, {width}), pages of ({kv}, {hd})")
+    _on(dev, "write_kv_fp8", k, v)
+    positions = _per_sequence(positions, B, "positions", dev)
     if lengths is not None:
-        lengths = _per_sequence(lengths, B, "lengths", k_pages.device)
+        lengths = _per_sequence(lengths, B, "lengths", dev)
     if B == 0 or n == 0:
         return
-    k, v = _token_rows(k), _token_rows(v)
+    k, *krow = _token_rows(k)
+    v, *vrow = _token_rows(v)
     with _lib.on_device(k_pages):
-        _lib.call("evo2_kv_fp8_write", k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
-                  *cache, positions.data_ptr(), _lib.ptr(lengths), B, n, kv, hd,
-                  _lib.stream_of(k_pages))
+        _lib.call("evo2_kv_fp8_write", *krow, *vrow, *cache, positions.data_ptr(), _lib.ptr(lengths), B,
+                  n, kv, hd, _lib.stream_of(k_pages))
 
 
 def read_kv_fp8(k_pages, v_pages, k_scale, v_scale, block_table, lengths, L):
@@ -116,13 +137,12 @@ def read_kv_fp8(k_pages, v_pages, k_scale, v_scale, block_table, lengths, L):
     write_kv_fp8's tokens and, flattened, of attention.packed_attention's).  Positions from
     lengths[b] on, and those whose entry lies outside the table or the cache's pages, are
     zeros."""
-    _lib.require_device(k_pages, v_pages, k_scale, v_scale, block_table, lengths)
     B, L = lengths.shape[0] if lengths.dim() else -1, int(L)
-    cache, kv, hd = _cache_args("read_kv_fp8", k_pages, v_pages, k_scale, v_scale, block_table, B)
-    lengths = _per_sequence(lengths, B, "lengths", k_pages.device)
+    cache, kv, hd, dev = _cache_args("read_kv_fp8", k_pages, v_pages, k_scale, v_scale, block_table, B)
+    lengths = _per_sequence(lengths, B, "lengths", dev)
     if L < 0:
         raise ValueError(f"read_kv_fp8 takes L >= 0, got {L}")
-    k = torch.empty(B, L, kv, hd, dtype=torch.bfloat16, device=k_pages.device)
+    k = torch.empty((B, L, kv, hd), dtype=torch.bfloat16, device=k_pages.device)
     v = torch.empty_like(k)
     if B and L:
         with _lib.on_device(k_pages):
@@ -131,11 +151,13 @@ def read_kv_fp8(k_pages, v_pages, k_scale, v_scale, block_table, lengths, L):
     return k, v
 
 
-def workspace_fp8(B, heads, kv_heads, head_dim, max_pages, device, n=1):
-    """A workspace for paged_decode_attention_fp8 on up to B sequences of n tokens (allocate
-    once, outside graph capture; calls that may run at once take one each)."""
+def workspace_fp8(B, heads, kv_heads, head_dim, max_pages, device, n=1, shared_pages=0):
+    """A workspace for paged_decode_attention_fp8 on up to B sequences of n tokens, with and
+    without the shared pages (allocate once, outside graph capture; calls that may run at
+    once take one each)."""
     need = max((_lib.workspace_bytes("evo2_decode_attention_fp8_workspace_bytes", b, n, heads,
-                                     kv_heads, head_dim, max_pages) for b in range(1, B + 1)), default=0)
+                                     kv_heads, head_dim, max_pages, s)
+                for b in range(1, B + 1) for s in {0, int(shared_pages)}), default=0)
     return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
 
 
@@ -155,44 +177,52 @@ def paged_decode_attention_fp8(q, k_pages, v_pages, k_scale, v_scale, block_tabl
     Bytes of positions that a sequence does not attend to may be anything; a NaN value at a
     position that some of a launch's rows attend to (later tokens of the sequence, or longer
     sequences on shared pages) can reach the others in its block of 64."""
-    _lib.require_device(q, k_pages, v_pages, k_scale, v_scale, block_table, positions, work)
-    if q.dim() not in (3, 4) or q.dtype != torch.bfloat16:
+    shape = q.shape
+    if len(shape) == 3:
+        (B, heads, width), n = shape, 1
+    elif len(shape) == 4:
+        B, n, heads, width = shape
+    if not 3 <= len(shape) <= 4 or q.dtype != torch.bfloat16:
         raise ValueError(f"paged_decode_attention_fp8 takes bf16 q (B, [n,] heads, head_dim), got "
-                         f"{tuple(q.shape)} {q.dtype}")
-    q4 = q.unsqueeze(1) if q.dim() == 3 else q
-    B, n, heads, hd = q4.shape
-    cache, kv, phd = _cache_args("paged_decode_attention_fp8", k_pages, v_pages, k_scale, v_scale,
-                                 block_table, B)
-    if hd != phd or heads == 0 or heads % kv:
-        raise ValueError(f"paged_decode_attention_fp8: q {tuple(q.shape)} does not match pages "
+                         f"{tuple(shape)} {q.dtype}")
+    cache, kv, hd, dev = _cache_args("paged_decode_attention_fp8", k_pages, v_pages, k_scale, v_scale,
+                                     block_table, B)
+    if width != hd or heads == 0 or heads % kv:
+        raise ValueError(f"paged_decode_attention_fp8: q {tuple(shape)} does not match pages "
                          f"{tuple(k_pages.shape)}")
-    if q.device != k_pages.device:
-        raise ValueError(f"paged_decode_attention_fp8: q on {q.device}, the cache on {k_pages.device}")
-    positions = _per_sequence(positions, B, "positions", k_pages.device)
-    scale = float(scale)
+    _on(dev, "paged_decode_attention_fp8", q)
+    positions = _per_sequence(positions, B, "positions", dev)
+    scale, shared_pages, max_pages = float(scale), int(shared_pages), cache[-1]
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"paged_decode_attention_fp8 takes a positive scale, got {scale}")
-    shared_pages = int(shared_pages)
-    if not 0 <= shared_pages <= block_table.shape[1]:
-        raise ValueError(f"shared_pages {shared_pages} of a table of {block_table.shape[1]} columns")
-    if work is not None and (not work.is_contiguous() or work.device != q.device):
-        raise ValueError("work must be a contiguous tensor on q's device")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if not 0 <= shared_pages <= max_pages:
+        raise ValueError(f"shared_pages {shared_pages} of a table of {max_pages} columns")
+    if work is not None and (not work.is_contiguous() or work.get_device() != dev):
+        raise ValueError("work must be a contiguous tensor on the cache's device")
+    out = torch.empty(shape, dtype=q.dtype, device=q.device)
     if B == 0 or n == 0:
         return out
-    o4 = out.unsqueeze(1) if q.dim() == 3 else out
-    q4 = _token_rows(q4)
-    max_pages = block_table.shape[1]
+    if len(shape) == 3:
+        b, h, unit = q.stride()
+        at = q.data_ptr()
+        if unit != 1 or (b | h) & 7 or at & 15:
+            q = q.clone(memory_format=torch.contiguous_format)
+            b, h, _ = q.stride()
+            at = q.data_ptr()
+        row = at, b, 0, h
+    else:
+        q, *row = _token_rows(q)
     with _lib.on_device(q):
         if work is None:
-            need = _lib.workspace_bytes("evo2_decode_attention_fp8_workspace_bytes", B, n, heads, kv, hd,
-                                        max_pages)
-            if need:
-                work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _lib.call("evo2_paged_decode_attention_fp8", q4.data_ptr(), *q4.stride()[:3], *cache, shared_pages,
-                  positions.data_ptr(), _lib.ptr(work),
-                  0 if work is None else work.numel() * work.element_size(), o4.data_ptr(),
-                  *o4.stride()[:3], B, n, heads, kv, hd, scale, _lib.stream_of(q))
+            bytes = _lib.workspace_bytes("evo2_decode_attention_fp8_workspace_bytes", B, n, heads, kv, hd,
+                                         max_pages, shared_pages)
+            if bytes:
+                work = torch.empty(bytes, dtype=torch.uint8, device=q.device)
+        else:
+            bytes = work.numel() * work.element_size()
+        _lib.call("evo2_paged_decode_attention_fp8", *row, *cache, shared_pages, positions.data_ptr(),
+                  _lib.ptr(work), bytes, out.data_ptr(), n * heads * hd, heads * hd, hd, B, n, heads, kv, hd,
+                  scale, _lib.stream_of(q))
     return out
 
 
@@ -260,8 +290,9 @@ def rotary_decode_fp8(qkv, cache, block_table, positions, inv_freq, factor):
     qkv, inv_freq = _rotary_rows(qkv, nh, hd, inv_freq)
     B = qkv.shape[0]
     table = _page_table(block_table, B, cache.k.shape[0], qkv.device)
-    args, _, _ = _cache_args("rotary_decode_fp8", *cache.tensors, table, B)
-    positions = _per_sequence(positions, B, "positions", qkv.device)
+    args, _, _, dev = _cache_args("rotary_decode_fp8", *cache.tensors, table, B)
+    _on(dev, "rotary_decode_fp8", qkv, inv_freq)
+    positions = _per_sequence(positions, B, "positions", dev)
     q = torch.empty(B, nh, hd, dtype=qkv.dtype, device=qkv.device)
     _lib.call("evo2_rotary_decode_fp8", _lib.ptr(qkv), qkv.stride(0), _lib.ptr(inv_freq), float(factor),
               _lib.ptr(q), *args, _lib.ptr(positions), B, nh, hd, _lib.stream_of(qkv))

@@ -7,24 +7,27 @@ import torch
 from . import _lib
 
 
-def _setting(x, name, B, device, dtype):
-    """(address or None, number) of a setting: a tensor (B,) on `device`, or one number
+_TYPES = (torch.bfloat16, torch.float32)
+
+
+def _setting(x, name, B, dev, dtype):
+    """(address or None, number) of a setting: a tensor (B,) on device `dev`, or one number
     for all rows; and the tensor, to be kept until the launch."""
-    if not torch.is_tensor(x):
+    if not isinstance(x, torch.Tensor):
         return None, x, None
     if x.shape != (B,):
         raise ValueError(f"{name} must be one number or ({B},), got {tuple(x.shape)}")
-    if x.device != device:
-        raise ValueError(f"{name} is on {x.device}, the logits on {device}")
-    if dtype is torch.int32 and x.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name} must be int32 or int64, got {x.dtype}")
-    if dtype is torch.float32 and not x.is_floating_point():
-        raise ValueError(f"{name} must be floating-point numbers, got {x.dtype}")
+    if x.get_device() != dev:
+        raise ValueError(f"{name} is on {x.device}, the logits on cuda:{dev}")
     if x.dtype != dtype:
-        if x.dtype == torch.int64:
+        if dtype is torch.int32:
+            if x.dtype != torch.int64:
+                raise ValueError(f"{name} must be int32 or int64, got {x.dtype}")
             x = x.clamp(0, 2 ** 31 - 1)
+        elif not x.is_floating_point():
+            raise ValueError(f"{name} must be floating-point numbers, got {x.dtype}")
         x = x.to(dtype)
-    if x.stride(0) != 1:
+    if B > 1 and x.stride(0) != 1:
         x = x.contiguous()
     return x.data_ptr(), 0, x
 
@@ -45,34 +48,35 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     never drawn (a row of nothing else gives -1); beside +inf no finite one is.  Weights are
     summed as whole numbers (steps of 2^-49 of the largest, of 2^-61 V for V over 4096), so
     a result does not depend on timing."""
-    _lib.require_device(logits, uniforms)
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"sample_tokens takes bf16 or fp32 logits (B, V), got {tuple(logits.shape)} "
-                         f"{logits.dtype}")
-    B, V = logits.shape
+    shape, dtype, dev = logits.shape, logits.dtype, logits.get_device()
+    if dev < 0 or uniforms.get_device() != dev:
+        _lib.require_device(logits, uniforms)
+        raise ValueError(f"uniforms are on {uniforms.device}, the logits on {logits.device}")
+    if len(shape) != 2 or dtype not in _TYPES:
+        raise ValueError(f"sample_tokens takes bf16 or fp32 logits (B, V), got {tuple(shape)} {dtype}")
+    B, V = shape
     if not 0 < V <= 1 << 24:
         raise ValueError(f"sample_tokens takes 1 to 2^24 logits a row, got {V}")
-    if uniforms.shape != (B,) or uniforms.dtype != torch.float32 or uniforms.device != logits.device:
-        raise ValueError(f"uniforms must be ({B},) fp32 on {logits.device}, got {tuple(uniforms.shape)} "
-                         f"{uniforms.dtype} on {uniforms.device}")
-    dev, f32 = logits.device, torch.float32
-    t, t1, keep_t = _setting(temperature, "temperature", B, dev, f32)
+    if uniforms.shape != (B,) or uniforms.dtype != torch.float32:
+        raise ValueError(f"uniforms must be ({B},) fp32, got {tuple(uniforms.shape)} {uniforms.dtype}")
+    t, t1, keep_t = _setting(temperature, "temperature", B, dev, torch.float32)
     k, k1, keep_k = _setting(top_k, "top_k", B, dev, torch.int32)
-    p, p1, keep_p = _setting(top_p, "top_p", B, dev, f32)
-    m, m1, keep_m = _setting(min_p, "min_p", B, dev, f32)
-    out = torch.empty(B, dtype=torch.int64, device=dev)
+    p, p1, keep_p = _setting(top_p, "top_p", B, dev, torch.float32)
+    m, m1, keep_m = _setting(min_p, "min_p", B, dev, torch.float32)
+    out = torch.empty(B, dtype=torch.int64, device=logits.device)
     if B == 0:
         return out
-    if logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
+    row, unit = logits.stride()
+    if unit != 1 or (row < V and B > 1):
         logits = logits.contiguous()
-    if uniforms.stride(0) != 1:
+        row = logits.stride(0)
+    if B > 1 and uniforms.stride(0) != 1:
         uniforms = uniforms.contiguous()
     with _lib.on_device(logits):
-        n = _lib.workspace_bytes("evo2_sample_workspace_bytes", B, V)
-        work = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _lib.call("evo2_sample", logits.data_ptr(), logits.dtype == f32, logits.stride(0),
-                  uniforms.data_ptr(), t, t1, k, k1, p, p1, m, m1, _lib.ptr(work), n, out.data_ptr(), B,
-                  V, _lib.stream_of(logits))
+        bytes = _lib.workspace_bytes("evo2_sample_workspace_bytes", B, V)
+        work = torch.empty(bytes, dtype=torch.uint8, device=logits.device) if bytes else None
+        _lib.call("evo2_sample", logits.data_ptr(), dtype == torch.float32, row, uniforms.data_ptr(), t, t1,
+                  k, k1, p, p1, m, m1, _lib.ptr(work), bytes, out.data_ptr(), B, V, _lib.stream_of(logits))
     return out
 
 

@@ -466,13 +466,14 @@ int evo2_rotary_decode_fp8(const void *qkv, int64_t sqkv, const float *inv_freq,
  *   q (B, n, heads, head_dim) bf16, strides in elements (multiples of 8), 16-byte aligned;
  *   out the same shape, strides multiples of 4, 8-byte aligned; positions (B,) int64
  *   shared_pages: the first entries of every table row that name the same pages
- *   workspace: _workspace_bytes(B, n, heads, kv_heads, head_dim, max_pages) bytes (0: none),
- *   8-byte aligned
+ *   workspace: _workspace_bytes(B, n, heads, kv_heads, head_dim, max_pages, shared_pages)
+ *   bytes (0: none), 16-byte aligned
  * heads a multiple of kv_heads, scale > 0, B * n at most 65535.  Positions of entries
  * outside the pages are left out; a token with none left gives zeros.
  */
 int64_t evo2_decode_attention_fp8_workspace_bytes(int64_t B, int64_t n, int64_t heads, int64_t kv_heads,
-                                                  int64_t head_dim, int64_t max_pages);
+                                                  int64_t head_dim, int64_t max_pages,
+                                                  int64_t shared_pages);
 int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_t qt, int64_t qh,
                                     const void *k_pages, int64_t kps, int64_t khs, const void *v_pages,
                                     int64_t vps, int64_t vhs, const float *k_scale, int64_t ksp,
