@@ -45,6 +45,7 @@ struct SampleArgs {
 // A row's settings.
 struct SampleRow {
   double c;       // log2(e) / T: y = (z - max) c
+  float c4;       // 4 c, at most the largest number
   double ymin;    // log2(m), -inf without min-p
   float top_p;
   int64_t top_k;  // 0: all
@@ -58,6 +59,7 @@ __device__ __forceinline__ SampleRow row_of(const SampleArgs &p, int b) {
   r.top_k = k > 0 && k < p.V ? k : 0;
   r.first = !(t > 0.0f) || k == 1;
   r.c = 1.4426950408889634 / static_cast<double>(fminf(t, 3.0e38f));  // (any infinite T is flat)
+  r.c4 = static_cast<float>(fmin(4.0 * r.c, 3.0e38));
   r.ymin = m > 0.0f ? log2(static_cast<double>(fminf(m, 1.0f))) : -INFINITY;
   return r;
 }
@@ -68,6 +70,8 @@ __device__ __forceinline__ uint32_t key_of(float z) {
   const uint32_t b = __float_as_uint(z + 0.0f);  // -0 is 0
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+constexpr uint32_t LEAST_KEY = 0x00800000u;  // of the lowest finite value
+
 // The value of a key (not 0); +inf as a number far above all others.
 __device__ __forceinline__ double value_of(uint32_t key) {
   const float z = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
@@ -104,23 +108,23 @@ __device__ __forceinline__ uint64_t weight_of(double y, int shift) {
 }
 
 // ---------------------------------------------------------------- within a wave
-// The value of the lane that DPP control CTRL names, 0 where there is none or the row is
-// not of MASK.
-template <int CTRL, int MASK = 0xF>
-__device__ __forceinline__ uint32_t dpp(uint32_t v) {
-  return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, MASK, 0xF, false);
+// The value (4 or 8 bytes) of the lane that DPP control CTRL names, 0 where there is none or
+// the row is not of MASK.
+template <int CTRL, int MASK = 0xF, typename U>
+__device__ __forceinline__ U dpp(U v) {
+  auto word = [](uint32_t x) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, MASK, 0xF, false));
+  };
+  if constexpr (sizeof(U) == 4) return word(v);
+  else return static_cast<U>(word(static_cast<uint32_t>(v >> 32))) << 32 | word(static_cast<uint32_t>(v));
 }
-template <int CTRL, int MASK = 0xF>
-__device__ __forceinline__ uint64_t dpp(uint64_t v) {
-  return static_cast<uint64_t>(dpp<CTRL, MASK>(static_cast<uint32_t>(v >> 32))) << 32 |
-         dpp<CTRL, MASK>(static_cast<uint32_t>(v));
-}
-__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
-  return __builtin_amdgcn_readlane(static_cast<int>(v), lane);
-}
-__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
-  return static_cast<uint64_t>(lane_value(static_cast<uint32_t>(v >> 32), lane)) << 32 |
-         lane_value(static_cast<uint32_t>(v), lane);
+template <typename U>
+__device__ __forceinline__ U lane_value(U v, int lane) {
+  auto word = [&](uint32_t x) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
+  };
+  if constexpr (sizeof(U) == 4) return word(v);
+  else return static_cast<U>(word(static_cast<uint32_t>(v >> 32))) << 32 | word(static_cast<uint32_t>(v));
 }
 template <typename U>
 __device__ __forceinline__ U wave_scan(U v) {  // inclusive
@@ -168,16 +172,74 @@ __device__ __forceinline__ uint32_t ties_of(uint64_t need, uint64_t above, uint6
   return static_cast<uint32_t>(min(n, uint64_t(0xffffffff)));
 }
 
+constexpr int BINS = 256;
+
+// The bin of hist (from the top down) in which its running sum reaches `need`, and the sum
+// before it; BINS where all of them do not reach it.  One wave.
+template <typename U>
+__device__ __forceinline__ uint32_t bin_reaching(const U *hist, U need, int lane, U &above) {
+  U h[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum += h[i] = hist[4 * lane + i];
+  const U run = wave_scan(sum);
+  const uint64_t hit = __ballot(run >= need);
+  if (!hit) return BINS;
+  const int l = __ffsll(static_cast<long long>(hit)) - 1;
+  U a = run - sum;
+  uint32_t bin = 4 * lane;
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (bin == static_cast<uint32_t>(4 * lane + i) && a + h[i] < need) {
+      a += h[i];
+      ++bin;
+    }
+  above = lane_value(a, l);
+  return lane_value(bin, l);
+}
+
+// A key's bits that differ between keys of T: all, or the upper half of a bf16's.
+template <typename T>
+constexpr int LOW = std::is_same_v<T, float> ? 0 : 16;
+template <typename T>
+__device__ __forceinline__ uint32_t whole_key(uint32_t high) {
+  if constexpr (LOW<T> == 0) return high;
+  else return high << LOW<T> | (high >> (31 - LOW<T>) ? 0u : (1u << LOW<T>) - 1);
+}
+
+// A search goes a byte of the keys at a time, from the highest in which any differ: pass i
+// counts the keys that share what is found so far, by their next `width` bits from `sh` up.
+struct Digits {
+  uint32_t prefix;  // bits found, in place (of keys without their LOW bits)
+  int top, sh;      // bits below top are not found yet; this pass finds those from sh up
+  __device__ __forceinline__ Digits(uint32_t kmax, uint32_t kmin) {
+    top = kmax == kmin ? 0 : 32 - __clz(kmax ^ kmin);
+    prefix = top == 32 ? 0 : kmax >> top << top;
+    sh = max(top - 8, 0);
+  }
+  __device__ __forceinline__ bool has(uint32_t k) const { return (top == 32 ? 0 : k >> top << top) == prefix; }
+  __device__ __forceinline__ uint32_t bin(uint32_t k) const {
+    return BINS - 1 - ((k >> sh) & ((1u << (top - sh)) - 1));
+  }
+  // the bin of this pass is found; false after the last pass
+  __device__ __forceinline__ bool next(uint32_t bin) {
+    prefix |= (BINS - 1 - bin) << sh;
+    if (sh == 0) return false;
+    top = sh;
+    sh = max(sh - 8, 0);
+    return true;
+  }
+};
+
 // ---------------------------------------------------------------- rows of up to 64 E logits
-// A wave takes a row, lane l logits E l .. E l + E - 1.  Top-k by bisection between the
-// least and the largest key, in turn at the mean of the two values (few steps for logits
-// as a head gives them) and at the middle of their keys (at most 32 for any); it ends
-// where exactly k keys are not below the probe.  Top-p likewise by the weights' sums, until
-// one token is left between the bounds.  8 rows of 512: see the launch below.
+// A wave takes a row, lane l logits E l .. E l + E - 1.  The cuts are found a byte at a
+// time from histograms of the wave's own in LDS (nothing but this wave's order of LDS
+// operations parts their steps).  Bisection with counts by ballots took 2 to 6 us of a
+// call, this SEARCH_K; with sums for top-p 5 us, this SEARCH_P.
 template <typename T, int E>
 __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
-  const int lane = threadIdx.x & 63;
-  const int b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  __shared__ __attribute__((aligned(16))) unsigned long long hists[4][BINS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);
   if (b >= B) return;
   const T *z = static_cast<const T *>(p.z) + b * p.sz;
   uint32_t key[E], top = 0;
@@ -186,9 +248,9 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
     const int i = E * lane + e;
     key[e] = i < p.V ? key_of(logit(z, i)) : 0;
   }
+  const SampleRow r = row_of(p, b);
 #pragma unroll
   for (int e = 0; e < E; ++e) top = max(top, key[e]);
-  const SampleRow r = row_of(p, b);
   const uint32_t kmax = wave_max(top);
   if (kmax == 0) {
     if (lane == 0) p.out[b] = -1;
@@ -203,53 +265,57 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
     if (lane == l) p.out[b] = E * l + at;
     return;
   }
-  auto count = [&](uint32_t t) __attribute__((always_inline)) {  // keys not below t
-    uint32_t n = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) n += __popcll(__ballot(key[e] >= t));
-    return n;
-  };
-  // a probe in (lo, hi), lo + 1 < hi
-  auto probe = [&](uint32_t lo, uint32_t hi, int step) __attribute__((always_inline)) {
-    uint32_t mid = lo + (hi - lo) / 2;
-    if (step & 1) {
-      const float a = static_cast<float>(0.5 * (value_of(lo) + value_of(hi - 1)));
-      mid = min(max(key_of(a), lo + 1), hi - 1);
-    }
-    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(mid));
-  };
   // What is kept: keys over `cut`, and the first `tie` that equal it.
-  uint32_t cut = 0, tie = 0, least = kmax;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (key[e]) least = min(least, key[e]);
-  least = ~wave_max(~least);
-  const uint32_t valid = count(1);
-  if (r.top_k && r.top_k < valid) {
-    const uint32_t k = static_cast<uint32_t>(r.top_k);
-    uint32_t lo = least, hi = kmax + 1, over = 0;  // count(lo) >= k > count(hi) = over
-    for (int step = 1; hi - lo > 1; ++step) {
-      const uint32_t mid = probe(lo, hi, step), n = count(mid);
-      if (n == k) {  // none of the next lower value
-        lo = mid - 1;
-        over = k;
-        break;
-      }
-      if (n > k) lo = mid;
-      else hi = mid, over = n;
-    }
-    cut = lo;
-    tie = k - over;
-  }
-  const double kv = value_of(kmax);
-  uint64_t w[E];
+  uint32_t cut = 0, tie = 0, least = kmax, valid = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const double y = (value_of(key[e] ? key[e] : kmax) - kv) * r.c;
-    w[e] = weight_of(y, p.shift);
-    if (key[e] < max(cut, 1u)) w[e] = 0;
+    if (key[e]) least = min(least, key[e]);
+    valid += __popcll(__ballot(key[e] != 0));
   }
-  // ranks of the tokens that equal the cut, in the vocabulary's order
+  least = ~wave_max(~least);
+  // The key at which the sum of x over the keys from the top reaches `need` (<= all of it),
+  // and the sum above it.
+  auto search = [&](auto *hist, auto x, auto need, uint32_t kmin, uint32_t &found, auto &above) __attribute__((always_inline)) {
+    using U = std::remove_reference_t<decltype(*hist)>;
+    Digits d(kmax >> LOW<T>, kmin >> LOW<T>);
+    U over = 0;
+    for (;;) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) hist[4 * lane + i] = 0;
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t k = key[e] >> LOW<T>;
+        if (key[e] && x(e) && d.has(k)) atomicAdd(&hist[d.bin(k)], x(e));
+      }
+      __builtin_amdgcn_wave_barrier();
+      U a = 0;
+      const uint32_t bin = min(bin_reaching<U>(hist, need - over, lane, a), static_cast<uint32_t>(BINS - 1));
+      over += a;
+      if (!d.next(bin)) break;
+    }
+    found = whole_key<T>(d.prefix);
+    above = over;
+  };
+  if (r.top_k && r.top_k < valid) {
+    uint32_t over;
+    search(reinterpret_cast<uint32_t *>(hists[wave]), [](int) { return 1u; }, static_cast<uint32_t>(r.top_k), least, cut, over);
+    tie = static_cast<uint32_t>(r.top_k) - over;
+  }
+  const double kv = value_of(kmax);
+  unsigned long long w[E];
+  uint32_t fine = 0;  // bit e: min-p keeps it
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool in = key[e] && key[e] >= cut;
+    w[e] = 0;
+    if (__any(in)) {  // uniform
+      const double y = (value_of(in ? key[e] : kmax) - kv) * r.c;
+      if (in) w[e] = weight_of(y, p.shift);
+      if (y >= r.ymin) fine |= 1u << e;
+    }
+  }
+  // of the tokens that equal the cut, those behind the first `tie` in the vocabulary's order
   auto drop_ties = [&]() __attribute__((always_inline)) {
     uint32_t n = 0;
 #pragma unroll
@@ -260,34 +326,16 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
       if (key[e] == cut && rank++ >= tie) w[e] = 0;
   };
   if (cut) drop_ties();
-  auto mass = [&](uint32_t t) __attribute__((always_inline)) {  // weight of keys not below t
-    uint64_t s = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += key[e] >= t ? w[e] : 0;
-    return wave_sum(s);
-  };
   if (r.top_p < 1.0f) {
-    const uint64_t need = need_of(r.top_p, mass(1));
-    uint32_t lo = max(cut, least), hi = kmax + 1;  // mass(lo) >= need > mass(hi) = above
-    uint32_t nlo = count(lo), nhi = 0;
-    uint64_t above = 0;
-    for (int step = 1; hi - lo > 1; ++step) {
-      if (nlo - nhi == 1) {  // one token of [lo, hi): its key is the cut
-        uint32_t at = 0;
+    unsigned long long sum = 0, above;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (key[e] >= lo && key[e] < hi) at = key[e];
-        lo = wave_max(at);
-        break;
-      }
-      const uint32_t mid = probe(lo, hi, step);
-      const uint64_t s = mass(mid);
-      if (s >= need) lo = mid, nlo = count(mid);
-      else hi = mid, nhi = count(mid), above = s;
-    }
-    const uint32_t most = ties_of(need, above, weight_of((value_of(lo) - kv) * r.c, p.shift));
-    tie = lo == cut ? min(tie, most) : most;
-    cut = lo;
+    for (int e = 0; e < E; ++e) sum += w[e];
+    const unsigned long long need = need_of(r.top_p, wave_sum(sum));
+    uint32_t at;
+    search(hists[wave], [&](int e) { return w[e]; }, need, max(cut, least), at, above);
+    const uint32_t most = ties_of(need, above, weight_of((value_of(at) - kv) * r.c, p.shift));
+    tie = at == cut ? min(tie, most) : most;
+    cut = at;
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (key[e] < cut) w[e] = 0;
@@ -296,8 +344,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
   uint64_t sum = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const double y = (value_of(key[e] ? key[e] : kmax) - kv) * r.c;
-    if (!(y >= r.ymin)) w[e] = 0;
+    if (!(fine >> e & 1)) w[e] = 0;
     sum += w[e];
   }
   const uint64_t upto = wave_scan(sum), target = target_of(p.u[b], lane_value(upto, 63));
@@ -315,39 +362,40 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
 }
 
 // ---------------------------------------------------------------- longer rows
-// Slices of SL logits.  sample_slice_kernel: a slice's largest logit, and a histogram of
-// its tokens and weights over BINS bins of a quarter of a power of two in weight, from its
-// largest down (the last bin takes all below).  Bins lie on one grid for all slices of a
-// row, floor(4 z c), and weights are 2^(S + z c - R) with a whole R of the slice's own, so
-// that histograms of slices add up by shifts.  sample_join_kernel: a row's histogram, the
-// bins in which the cuts lie.  sample_list_kernel: the keys of the slices' tokens in those
-// bins, in the vocabulary's order (top-k: all down to its cut; else the one to three bins of
-// top-p's and min-p's).  sample_draw_kernel: the exact cut among them, a byte at a time
-// from histograms, the slices' sums, and the token in the slice that the draw falls into.
+// Slices of SL logits.  sample_slice_kernel: a slice's largest logit, and a histogram over
+// BINS bins of a quarter of a power of two in weight, from its largest down (the last bin
+// takes all below), of its tokens in rows with top-k, else of its weights.  Bins lie on one
+// grid for all slices of a row, floor(4 z c), and weights are 2^(S + z c - R) with a whole R
+// of the slice's own, so that histograms of slices add up by shifts.  sample_join_kernel:
+// a row's histogram, and the bin in which the cut lies.  sample_list_kernel: the keys of the
+// slices' tokens in that bin (top-k: in all down to it), in the vocabulary's order.
+// sample_draw_kernel: the exact cut among them, a byte at a time from histograms, the
+// slices' sums, and the token in the slice that the draw falls into.
 constexpr int SL_T = 512, SL_E = 8, SL = SL_T * SL_E, SL_W = SL_T / 64;
-constexpr int BINS = 256;
+constexpr int MAX_S = 256;  // slices of the longest row, 2^20 logits
 
 struct SliceInfo {
   double top;           // its largest logit
-  uint64_t total;       // its weight, in its own units
+  uint64_t total;       // its weight, in its own units (rows without top-k)
   uint64_t base;        // weight in bins over the listed ones, in the row's units
   uint32_t key, at;     // largest key (0: no token) and its first index
   uint32_t listed, pad;
 };
 struct RowInfo {
   double top;           // the row's largest logit
-  uint64_t total;       // its weight
+  uint64_t total;       // its weight (without top-k)
   uint64_t over;        // of it in bins over the listed ones
-  int32_t mode;         // 0: drawn already, 1: nothing is cut, 2: bins lo .. hi are listed
-  int32_t lo, hi;
+  uint32_t least;       // min-p keeps keys from here on
+  int32_t mode;         // 0: drawn already, 1: nothing is listed, 2: bins from lo on are
+  int32_t lo;
+  uint32_t from, upto;  // their keys: from .. upto - 1
   uint32_t pad;
 };
 
 struct SampleWork {
   SliceInfo *slice;     // (B, S)
   RowInfo *row;         // (B,)
-  uint64_t *mass;       // (B, S, BINS)
-  uint32_t *count;      // (B, S, BINS)
+  uint64_t *hist;       // (B, S, BINS)
   uint32_t *list;       // (B, S * SL)
   int S;
 };
@@ -359,11 +407,15 @@ struct SampleRef {
   __device__ __forceinline__ uint64_t weight(double z, int shift) const {
     return weight_of(fma(z - top, c, phi), shift);
   }
-  __device__ __forceinline__ double y(double z) const { return (z - top) * c; }  // of the largest weight
 };
-__device__ __forceinline__ double grid_of(double z, double c) { return floor(z * (4.0 * c)); }
-__device__ __forceinline__ int bin_of(double top_grid, double z, double c) {
-  return static_cast<int>(fmin(top_grid - grid_of(z, c), static_cast<double>(BINS - 1)));
+// floor(4 z c), where that is past 2^29 the same for all (as a whole number, so that
+// differences add up).  c4: 4 c, finite.
+__device__ __forceinline__ int grid_of(uint32_t key, float c4) {
+  const float z = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+  return static_cast<int>(floorf(fminf(fmaxf(z * c4, -536870912.0f), 536870912.0f)));
+}
+__device__ __forceinline__ int bin_of(int top_grid, uint32_t key, float c4) {
+  return min(top_grid - grid_of(key, c4), BINS - 1);
 }
 
 // Thread t's keys of slice s: logits SL s + SL_E t .. + SL_E - 1.
@@ -392,58 +444,48 @@ __device__ __forceinline__ void slice_keys(const SampleArgs &p, int b, int s, in
 
 template <typename T>
 __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, SampleWork w) {
-  __shared__ unsigned long long mass[BINS];
-  __shared__ uint32_t count[BINS], red[SL_W];
+  __shared__ unsigned long long hist[BINS];
+  __shared__ unsigned long long sums[SL_W];
+  __shared__ uint32_t red[SL_W], red2[SL_W];
   const int s = blockIdx.x, b = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
   uint32_t key[SL_E], top = 0, at = 0;
   slice_keys<T>(p, b, s, t, key);
   const SampleRow r = row_of(p, b);
+  for (int i = t; i < BINS; i += SL_T) hist[i] = 0;
 #pragma unroll
   for (int e = 0; e < SL_E; ++e) top = max(top, key[e]);
   const uint32_t wtop = wave_max(top);
-  if (lane == 0) red[wave] = wtop;
-  for (int i = t; i < BINS; i += SL_T) mass[i] = 0, count[i] = 0;
+#pragma unroll
+  for (int e = 0; e < SL_E; ++e)  // the first of the largest, as ~index
+    if (key[e] == wtop) at = max(at, ~static_cast<uint32_t>(SL * s + SL_E * t + e));
+  at = wave_max(at);
+  if (lane == 0) red[wave] = wtop, red2[wave] = at;
   __syncthreads();
   uint32_t kmax = 0;
 #pragma unroll
   for (int i = 0; i < SL_W; ++i) kmax = max(kmax, red[i]);
-  SliceInfo &info = w.slice[static_cast<int64_t>(b) * w.S + s];
-  const int64_t h = (static_cast<int64_t>(b) * w.S + s) * BINS;
-  uint64_t total = 0;
   if (kmax && !r.first) {  // uniform
-    const double z0 = value_of(kmax);
-    const SampleRef ref(z0, r.c);
-    const double g0 = grid_of(z0, r.c);
+    const SampleRef ref(value_of(kmax), r.c);
+    const int g0 = grid_of(kmax, r.c4);
 #pragma unroll
     for (int e = 0; e < SL_E; ++e) {
       if (key[e] == 0) continue;
-      const double z = value_of(key[e]);
-      const uint64_t x = ref.weight(z, p.shift);
-      const int bin = bin_of(g0, z, r.c);
-      atomicAdd(&count[bin], 1u);
-      if (x) atomicAdd(&mass[bin], static_cast<unsigned long long>(x));
+      // (top-k: tokens; their weights are summed from the list)
+      const uint64_t x = r.top_k ? 1 : ref.weight(value_of(key[e]), p.shift);
+      if (x) atomicAdd(&hist[bin_of(g0, key[e], r.c4)], static_cast<unsigned long long>(x));
     }
   }
-#pragma unroll
-  for (int e = 0; e < SL_E; ++e)  // the first of the largest, as ~index
-    if (key[e] == kmax) at = max(at, ~static_cast<uint32_t>(SL * s + SL_E * t + e));
-  at = wave_max(at);
   __syncthreads();
-  if (t < BINS) {
-    w.mass[h + t] = total = mass[t];
-    w.count[h + t] = count[t];
-  }
+  const int64_t h = (static_cast<int64_t>(b) * w.S + s) * BINS;
+  unsigned long long total = 0;
+  if (t < BINS) w.hist[h + t] = total = hist[t];
   total = wave_sum(total);
-  __syncthreads();
-  if (lane == 0) {
-    red[wave] = at;
-    mass[wave] = total;
-  }
+  if (lane == 0) sums[wave] = total;
   __syncthreads();
   if (t == 0) {
-    for (int i = 0; i < SL_W; ++i) at = max(at, red[i]);
-    total = 0;
-    for (int i = 0; i < SL_W; ++i) total += mass[i];
+    at = 0, total = 0;
+    for (int i = 0; i < SL_W; ++i) at = red[i] == kmax ? max(at, red2[i]) : at, total += sums[i];
+    SliceInfo &info = w.slice[static_cast<int64_t>(b) * w.S + s];
     info.top = kmax ? value_of(kmax) : 0.0;
     info.total = total;
     info.key = kmax;
@@ -451,111 +493,109 @@ __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, Sample
   }
 }
 
-// The bin of hist (BINS, from the top down) in which its running sum reaches `need`, and
-// the sum before it; BINS where all of them do not reach it.  One wave.
-__device__ __forceinline__ int bin_reaching(const unsigned long long *hist, uint64_t need, int lane, uint64_t &above) {
-  uint64_t h[4], sum = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) sum += h[i] = hist[4 * lane + i];
-  const uint64_t run = wave_scan(sum);
-  const uint64_t hit = __ballot(run >= need);
-  if (!hit) return BINS;
-  const int l = __ffsll(static_cast<long long>(hit)) - 1;
-  uint64_t a = run - sum;
-  uint32_t bin = 4 * lane;
-#pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (bin == static_cast<uint32_t>(4 * lane + i) && a + h[i] < need) {
-      a += h[i];
-      ++bin;
-    }
-  above = lane_value(a, l);
-  return lane_value(bin, l);
-}
-
-constexpr int SJ_T = 1024, SJ_G = SJ_T / BINS;  // groups of threads take slices in turn
+constexpr int SJ_T = 1024, SJ_G = SJ_T / BINS, SJ_E = 8;  // groups of threads take slices in turn
 
 __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleWork w) {
-  __shared__ unsigned long long mass[BINS], count[BINS];
-  __shared__ uint32_t red[SJ_T / 64], red2[SJ_T / 64];
-  __shared__ int by[BINS], off[BINS];
-  const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, bin = t % BINS;
+  __shared__ unsigned long long hist[BINS];
+  __shared__ uint32_t red[MAX_S / 64], red2[MAX_S / 64];
+  __shared__ int by[MAX_S], off[MAX_S];
+  const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, bin = t % BINS, first = t / BINS;
   const SliceInfo *slice = w.slice + static_cast<int64_t>(b) * w.S;
+  const uint64_t *h = w.hist + static_cast<int64_t>(b) * w.S * BINS + bin;
+  // (all that does not depend on the row's largest is on its way at once)
+  unsigned long long x[SJ_E];
+#pragma unroll
+  for (int i = 0; i < SJ_E; ++i) x[i] = first + SJ_G * i < w.S ? h[(first + SJ_G * i) * BINS] : 0;
+  uint32_t key = 0, at = 0;
+  double top = 0.0;
+  if (t < w.S) key = slice[t].key, at = ~slice[t].at, top = slice[t].top;
   const SampleRow r = row_of(p, b);
   RowInfo &row = w.row[b];
-  if (t < BINS) mass[t] = 0, count[t] = 0;
-  uint32_t km = 0, at = 0;
-  for (int s = t; s < w.S; s += SJ_T) {
-    const uint32_t k = slice[s].key, first = ~slice[s].at;
-    at = k > km ? first : k == km ? max(at, first) : at;
-    km = max(km, k);
+  if (t < BINS) hist[t] = 0;
+  if (t < MAX_S) {
+    const uint32_t k = wave_max(key), a = wave_max(key == k ? at : 0);
+    if (lane == 0) red[wave] = k, red2[wave] = a;
   }
-  uint32_t kmax = wave_max(km);
-  at = wave_max(km == kmax ? at : 0);
-  if (lane == 0) red[wave] = kmax, red2[wave] = at;
   __syncthreads();
-  for (int i = 0; i < SJ_T / 64; ++i) kmax = max(kmax, red[i]);
+  uint32_t kmax = 0;
+#pragma unroll
+  for (int i = 0; i < MAX_S / 64; ++i) kmax = max(kmax, red[i]);
   if (t == 0) {  // the first of the largest; the draw writes over it
     at = 0;
-    for (int i = 0; i < SJ_T / 64; ++i) at = red[i] == kmax ? max(at, red2[i]) : at;
+    for (int i = 0; i < MAX_S / 64; ++i) at = red[i] == kmax ? max(at, red2[i]) : at;
     p.out[b] = kmax ? static_cast<int64_t>(~at) : -1;
     if (kmax == 0 || r.first) row.mode = 0;
   }
   if (kmax == 0 || r.first) return;  // uniform
   const SampleRef ref(value_of(kmax), r.c);
-  const double g0 = grid_of(ref.top, r.c);
-  for (int s0 = 0; s0 < w.S; s0 += BINS) {
-    const int n = min(w.S - s0, BINS);
-    __syncthreads();
-    if (t < n) {  // slice's units are 2^-by of the row's, its bins `off` below the row's
-      const bool live = slice[s0 + t].key != 0;
-      const double top = slice[s0 + t].top;
-      by[t] = live ? static_cast<int>(fmin(ref.r - ceil(top * r.c), 63.0)) : -1;
-      off[t] = static_cast<int>(fmin(g0 - grid_of(top, r.c), static_cast<double>(BINS - 1)));
-    }
-    __syncthreads();
-    const int64_t h = (static_cast<int64_t>(b) * w.S + s0) * BINS + bin;
-#pragma unroll 8
-    for (int s = t / BINS; s < n; s += SJ_G) {
-      const uint64_t x = w.mass[h + s * BINS];
-      const uint32_t c = w.count[h + s * BINS];
-      if (by[s] < 0) continue;
-      if (c) atomicAdd(&count[min(bin + off[s], BINS - 1)], static_cast<unsigned long long>(c));
-      if (x) atomicAdd(&mass[min(bin + off[s], BINS - 1)], static_cast<unsigned long long>(x >> by[s]));
-    }
+  const int g0 = grid_of(kmax, r.c4);
+  if (t < w.S) {  // a slice's units are 2^-by of the row's, its bins `off` below the row's
+    by[t] = key ? r.top_k ? 0 : static_cast<int>(fmin(ref.r - ceil(top * r.c), 63.0)) : -1;
+    off[t] = key ? min(g0 - grid_of(key, r.c4), BINS - 1) : 0;
   }
   __syncthreads();
-  if (wave) return;
-  uint64_t total = 0, tokens = 0;
+  auto add = [&](int s, unsigned long long v) __attribute__((always_inline)) {
+    if (by[s] >= 0 && v) atomicAdd(&hist[min(bin + off[s], BINS - 1)], v >> by[s]);
+  };
 #pragma unroll
-  for (int i = 0; i < 4; ++i) total += mass[4 * lane + i], tokens += count[4 * lane + i];
+  for (int i = 0; i < SJ_E; ++i)
+    if (first + SJ_G * i < w.S) add(first + SJ_G * i, x[i]);
+#pragma unroll 4
+  for (int s = first + SJ_G * SJ_E; s < w.S; s += SJ_G) add(s, h[s * BINS]);
+  __syncthreads();
+  if (wave) return;
+  unsigned long long total = 0, before = 0, over = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) total += hist[4 * lane + i];
   total = wave_sum(total);
-  tokens = wave_sum(tokens);
-  int lo = BINS, hi = -1;
-  uint64_t before = 0;
-  if (r.top_k && static_cast<uint64_t>(r.top_k) < tokens) {
-    lo = 0;
-    hi = bin_reaching(count, r.top_k, lane, before);
+  // The least key of which `is` holds, as it does for all larger ones up to the largest: 64
+  // probes at a time.
+  auto least_key = [&](auto is) __attribute__((always_inline)) {
+    uint32_t below = 0, found = kmax;  // below < the key <= found
+    while (found - below > 1) {
+      const uint32_t step = (found - below - 1) / 64 + 1, k = min(below + step * (lane + 1), found);
+      const uint64_t yes = __ballot(k >= LEAST_KEY && is(k));  // (lane 63's k is `found`)
+      const int l = __ffsll(static_cast<long long>(yes)) - 1;
+      found = lane_value(k, l);
+      if (l) below = lane_value(k, l - 1);
+    }
+    return found;
+  };
+  auto within = [&](int most) __attribute__((always_inline)) {
+    return least_key([&](uint32_t k) __attribute__((always_inline)) { return bin_of(g0, k, r.c4) <= most; });
+  };
+  uint32_t least = 1;
+  if (r.ymin > -INFINITY)
+    least = least_key([&](uint32_t k) __attribute__((always_inline)) { return (value_of(k) - ref.top) * r.c >= r.ymin; });
+  int lo = 0, hi = -1;
+  uint32_t from = 0, upto = ~0u;
+  if (r.top_k) {
+    hi = min(bin_reaching<unsigned long long>(hist, r.top_k, lane, before), static_cast<uint32_t>(BINS - 1));
+    from = within(hi);
   } else {
-    if (r.top_p < 1.0f) lo = hi = bin_reaching(mass, need_of(r.top_p, total), lane, before);
-    if (r.ymin > -INFINITY) {  // the value with this weight, to a bin either way
-      const int at = bin_of(g0, ref.top + r.ymin / r.c, r.c);
-      const int a = max(at - 1, 0), z = min(at + 1, BINS - 1);
-      if (hi < 0 || z < lo) lo = a, hi = z;
-      else if (a <= hi) lo = min(lo, a), hi = max(hi, z);
+    if (r.top_p < 1.0f) hi = bin_reaching<unsigned long long>(hist, need_of(r.top_p, total), lane, before);
+    if (least > 1) {
+      const int at = bin_of(g0, least, r.c4);
+      hi = hi < 0 ? at : min(hi, at);
+    }
+    if (hi >= 0) {  // the one bin, of it what min-p keeps
+      lo = hi;
+      from = max(within(hi), least);
+      if (lo > 0) upto = within(lo - 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) over += 4 * lane + i < lo ? hist[4 * lane + i] : 0;
+      over = wave_sum(over);
     }
   }
-  uint64_t over = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) over += 4 * lane + i < lo ? mass[4 * lane + i] : 0;
-  over = wave_sum(over);
   if (lane == 0) {
     row.top = ref.top;
     row.total = total;
     row.over = over;
+    row.least = least;
     row.mode = hi < 0 ? 1 : 2;
     row.lo = lo;
-    row.hi = hi;
+    row.from = from;
+    row.upto = upto;
   }
 }
 
@@ -567,23 +607,21 @@ __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleW
   const RowInfo row = w.row[b];
   if (row.mode != 2) return;  // uniform
   SliceInfo &info = w.slice[static_cast<int64_t>(b) * w.S + s];
-  const SampleRow r = row_of(p, b);
   uint32_t key[SL_E], n = 0;
   slice_keys<T>(p, b, s, t, key);
-  const double g0 = grid_of(row.top, r.c);
 #pragma unroll
   for (int e = 0; e < SL_E; ++e) {
-    const int bin = key[e] ? bin_of(g0, value_of(key[e]), r.c) : BINS;
-    if (bin < row.lo || bin > row.hi) key[e] = 0;  // (hi is below BINS)
+    if (key[e] < row.from || key[e] >= row.upto) key[e] = 0;
     n += key[e] != 0;
   }
-  // weight in bins over the listed ones
+  // weight in bins over the listed ones (none with top-k)
   uint64_t x = 0;
-  if (t < BINS && info.key) {
+  if (row.lo > 0 && t < BINS && info.key) {
+    const SampleRow r = row_of(p, b);
     const SampleRef ref(row.top, r.c), own(info.top, r.c);
     const int by = static_cast<int>(fmin(ref.r - own.r, 63.0));
-    const int off = static_cast<int>(fmin(g0 - grid_of(own.top, r.c), static_cast<double>(BINS - 1)));
-    if (min(t + off, BINS - 1) < row.lo) x = w.mass[(static_cast<int64_t>(b) * w.S + s) * BINS + t] >> by;
+    const int off = grid_of(key_of(static_cast<float>(row.top)), r.c4) - grid_of(info.key, r.c4);
+    if (min(t + min(off, BINS - 1), BINS - 1) < row.lo) x = w.hist[(static_cast<int64_t>(b) * w.S + s) * BINS + t] >> by;
   }
   x = wave_sum(x);
   const uint32_t run = wave_scan(n);
@@ -605,28 +643,31 @@ __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleW
   }
 }
 
-constexpr int SD_LDS = 8192;    // listed keys kept in LDS
-constexpr int SD_S = 4096;      // most slices: 2^24 logits
+constexpr int SD_LDS = 8192;  // listed keys kept in LDS
 
 template <typename T>
 __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleWork w) {
-  __shared__ uint32_t keys[SD_LDS], start[SD_S + 1];
-  __shared__ unsigned long long hist[BINS];
-  __shared__ uint64_t wred[SL_W];
-  __shared__ uint32_t red[SL_W], red2[SL_W];
-  __shared__ uint64_t found_above, before_slice;
-  __shared__ uint32_t found, tie_before;
+  __shared__ uint32_t keys[SD_LDS], start[MAX_S + 1], tied[MAX_S];
+  __shared__ unsigned long long sums[MAX_S];
+  __shared__ unsigned long long hist[3][BINS];
+  __shared__ uint64_t wred[SL_W], before_slice;
+  __shared__ uint32_t red[SL_W], red2[SL_W], tie_before;
   __shared__ int pick;
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const RowInfo row = w.row[b];
   if (row.mode == 0) return;  // uniform
-  SliceInfo *slice = w.slice + static_cast<int64_t>(b) * w.S;
+  const SliceInfo *slice = w.slice + static_cast<int64_t>(b) * w.S;
   const SampleRow r = row_of(p, b);
   const SampleRef ref(row.top, r.c);
-  const double g0 = grid_of(row.top, r.c);
   const uint32_t *list = w.list + static_cast<int64_t>(b) * w.S * SL;
   const bool cuts = row.mode == 2;
-  // start[s]: listed keys before slice s
+  // a slice's weight apart from ties at the cut: here that in bins over the listed ones, or
+  // all where nothing is listed; start[s]: listed keys before slice s
+  if (t < w.S) {
+    tied[t] = 0;
+    sums[t] = cuts ? slice[t].base
+                   : slice[t].key ? slice[t].total >> static_cast<int>(fmin(ref.r - ceil(slice[t].top * r.c), 63.0)) : 0;
+  }
   uint32_t listed = 0;
   if (cuts) {
     if (wave == 0) {
@@ -641,15 +682,18 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
     listed = start[w.S];
   }
   const bool fits = listed <= SD_LDS;
-  // listed key i, wherever its slice left it
-  auto fetch = [&](uint32_t i) __attribute__((always_inline)) {
+  auto slice_of = [&](uint32_t i) __attribute__((always_inline)) {  // of listed key i
     int lo = 0, hi = w.S;  // start[lo] <= i < start[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
       if (start[mid] <= i) lo = mid;
       else hi = mid;
     }
-    return list[static_cast<int64_t>(lo) * SL + (i - start[lo])];
+    return lo;
+  };
+  auto fetch = [&](uint32_t i) __attribute__((always_inline)) {
+    const int s = slice_of(i);
+    return list[static_cast<int64_t>(s) * SL + (i - start[s])];
   };
   uint32_t kmin = ~0u, kmx = 0;
   for (uint32_t i = t; i < listed; i += SL_T) {
@@ -661,6 +705,7 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   kmin = ~wave_max(~kmin);
   if (lane == 0) red[wave] = kmx, red2[wave] = kmin;
   if (t == 0) pick = 0, tie_before = 0, before_slice = 0;
+  for (int i = t; i < BINS; i += SL_T) hist[0][i] = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < SL_W; ++i) kmx = max(kmx, red[i]), kmin = min(kmin, red2[i]);
@@ -674,52 +719,43 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   uint32_t cut = 0, tie = 0;
   // The key at which sum(of(key)) over the listed keys over the cut, from the top, reaches
   // `need`, and the sum above it; false where they do not.  `extra`: of the keys at the cut.
+  // Histograms in turn, one pass clearing the next one's (whose last readers met before
+  // this pass), every wave reading the pass's: one meeting a pass.
+  int turn = 0;
   auto search = [&](auto of, uint64_t need, uint64_t extra, uint32_t &key, uint64_t &above) __attribute__((always_inline)) {
-    const int bits = kmx == kmin ? 0 : 32 - __clz(kmx ^ kmin);
-    uint32_t prefix = bits == 32 ? 0 : kmx >> bits << bits;
-    uint64_t over = 0;
-    for (int sh = max(bits - 8, 0), top = bits; top > 0 || sh == 0; top = sh, sh = max(sh - 8, 0)) {
-      const int width = top - sh;  // bits found now (none where all keys are equal)
-      for (int i = t; i < BINS; i += SL_T) hist[i] = 0;
-      __syncthreads();
-      auto add = [&](uint32_t k, uint64_t x) __attribute__((always_inline)) {
-        const uint32_t high = top >= 32 ? 0 : k >> top << top;
-        if (high == prefix) atomicAdd(&hist[BINS - 1 - ((k >> sh) & ((1u << width) - 1))], static_cast<unsigned long long>(x));
-      };
+    Digits d(kmx >> LOW<T>, kmin >> LOW<T>);
+    unsigned long long over = 0;
+    bool found = true;
+    do {
+      unsigned long long *now = hist[turn], *next = hist[turn == 2 ? 0 : turn + 1];
+      turn = turn == 2 ? 0 : turn + 1;
+      for (int i = t; i < BINS; i += SL_T) next[i] = 0;
       each([&](uint32_t k) __attribute__((always_inline)) {
-        if (k > cut) add(k, of(k));
+        if (k > cut && d.has(k >> LOW<T>)) atomicAdd(&now[d.bin(k >> LOW<T>)], static_cast<unsigned long long>(of(k)));
       });
-      if (t == 0 && extra) add(cut, extra);
+      if (t == 0 && extra && d.has(cut >> LOW<T>)) atomicAdd(&now[d.bin(cut >> LOW<T>)], static_cast<unsigned long long>(extra));
       __syncthreads();
-      if (wave == 0) {
-        uint64_t a = 0;
-        const int bin = bin_reaching(hist, need - over, lane, a);
-        if (lane == 0) found = bin, found_above = a;
-      }
-      __syncthreads();
-      const uint32_t bin = found;
-      const uint64_t a = found_above;
-      __syncthreads();
-      if (bin == BINS) return false;  // uniform
-      prefix |= (BINS - 1 - bin) << sh;
+      unsigned long long a = 0;
+      const uint32_t bin = bin_reaching<unsigned long long>(now, need - over, lane, a);
+      found = bin < BINS;  // uniform
       over += a;
-      if (sh == 0) break;
-    }
-    key = prefix;
+      if (!found || !d.next(bin)) break;
+    } while (true);
+    key = whole_key<T>(d.prefix);
     above = over;
-    return true;
+    return found;
   };
   if (cuts && listed) {
     uint32_t key;
     uint64_t above;
-    if (r.top_k && row.lo == 0 && search([](uint32_t) { return uint64_t(1); }, r.top_k, 0, key, above)) {
+    if (r.top_k && search([](uint32_t) { return uint64_t(1); }, r.top_k, 0, key, above)) {
       cut = key;
       tie = static_cast<uint32_t>(r.top_k - above);
     }
     if (r.top_p < 1.0f) {
       const uint64_t extra = cut ? tie * weight(cut) : 0;
       uint64_t total = row.total;
-      if (cut) {  // of what top-k kept
+      if (r.top_k) {  // of what top-k kept
         uint64_t x = 0;
         each([&](uint32_t k) __attribute__((always_inline)) { x += k > cut ? weight(k) : 0; });
         x = wave_sum(x);
@@ -738,53 +774,34 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
       }
     }
   }
-  // A token's weight in the draw, apart from ties at the cut; of tokens in bins over the
-  // listed ones, and of listed ones
-  const double zc = cut ? value_of(cut) : 0.0;
-  const uint64_t wc = cut && ref.y(zc) >= r.ymin ? weight(cut) : 0;
-  auto kept = [&](uint32_t k) __attribute__((always_inline)) -> uint64_t {
-    if (k <= cut || !(ref.y(value_of(k)) >= r.ymin)) return 0;
-    return weight(k);
-  };
-  // the slices' sums, a wave to a slice: into base (its weight apart from ties) and listed
-  // (its ties)
-  for (int s = wave; s < w.S; s += SL_W) {
-    SliceInfo &info = slice[s];
-    uint64_t x = 0;
-    uint32_t n = 0;
-    if (cuts) {
-      const uint32_t i0 = start[s], i1 = start[s + 1];
-      for (uint32_t i = i0 + lane; i < i1; i += 64) {
-        const uint32_t k = fits ? keys[i] : list[static_cast<int64_t>(s) * SL + (i - i0)];
-        x += kept(k);
-        n += cut && k == cut;
-      }
-      x = wave_sum(x) + info.base;
-      n = wave_sum(n);
-    } else if (info.key) {
-      x = info.total >> static_cast<int>(fmin(ref.r - ceil(info.top * r.c), 63.0));
-    }
-    if (lane == 0) info.base = x, info.listed = n;
+  // A token's weight in the draw, apart from ties at the cut; the slices' sums of it
+  const uint64_t wc = cut >= row.least ? weight(cut) : 0;
+  auto kept = [&](uint32_t k) __attribute__((always_inline)) { return k > cut && k >= row.least ? weight(k) : 0; };
+  for (uint32_t i = t; i < listed; i += SL_T) {
+    const int s = slice_of(i);
+    const uint32_t k = fits ? keys[i] : fetch(i);
+    const uint64_t x = kept(k);
+    if (x) atomicAdd(&sums[s], static_cast<unsigned long long>(x));
+    if (cut && k == cut) atomicAdd(&tied[s], 1u);
   }
   __syncthreads();
   // the slice that the draw falls into
   if (wave == 0) {
-    uint64_t total = 0;
+    uint64_t all = 0;
     uint32_t nt = 0;
     for (int s0 = 0; s0 < w.S; s0 += 64) {
       const int s = s0 + lane;
-      const uint32_t n = s < w.S ? slice[s].listed : 0, run = wave_scan(n) + nt;
-      const uint64_t x = s < w.S ? slice[s].base + (min(run, tie) - min(run - n, tie)) * wc : 0;
-      total += wave_sum(x);
+      const uint32_t n = s < w.S ? tied[s] : 0, run = wave_scan(n) + nt;
+      all += wave_sum(s < w.S ? sums[s] + (min(run, tie) - min(run - n, tie)) * wc : 0);
       nt = lane_value(run, 63);
     }
-    const uint64_t target = total ? target_of(p.u[b], total) : 0;
+    const uint64_t target = all ? target_of(p.u[b], all) : 0;
     uint64_t sum = 0;
     nt = 0;
     for (int s0 = 0; s0 < w.S; s0 += 64) {
       const int s = s0 + lane;
-      const uint32_t n = s < w.S ? slice[s].listed : 0, run = wave_scan(n) + nt;
-      const uint64_t x = s < w.S ? slice[s].base + (min(run, tie) - min(run - n, tie)) * wc : 0;
+      const uint32_t n = s < w.S ? tied[s] : 0, run = wave_scan(n) + nt;
+      const uint64_t x = s < w.S ? sums[s] + (min(run, tie) - min(run - n, tie)) * wc : 0;
       const uint64_t upto = wave_scan(x) + sum;
       const uint64_t hit = __ballot(upto > target);
       if (hit) {
@@ -813,7 +830,7 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
     x[e] = 0;
     if (key[e] == 0) continue;
     if (cut && key[e] == cut) x[e] = rank++ < tie ? wc : 0;
-    else if (!cuts || bin_of(g0, value_of(key[e]), r.c) <= row.hi) x[e] = kept(key[e]);
+    else if (key[e] >= row.from) x[e] = kept(key[e]);
     mine += x[e];
   }
   const uint64_t wrun = wave_scan(mine);
@@ -841,21 +858,20 @@ static int64_t align16(int64_t n) { return (n + 15) & ~int64_t(15); }
 
 // Offsets of the parts of a workspace; the last is its size.
 struct SampleParts {
-  int64_t slice, row, mass, count, list, bytes;
+  int64_t row, hist, list, bytes;
 };
 static SampleParts parts_of(int64_t B, int64_t V) {
   const int64_t S = cdiv(V, SL);
   SampleParts q;
-  q.slice = 0;
   q.row = align16(B * S * static_cast<int64_t>(sizeof(SliceInfo)));
-  q.mass = q.row + align16(B * static_cast<int64_t>(sizeof(RowInfo)));
-  q.count = q.mass + B * S * BINS * 8;
-  q.list = q.count + B * S * BINS * 4;
+  q.hist = q.row + align16(B * static_cast<int64_t>(sizeof(RowInfo)));
+  q.list = q.hist + B * S * BINS * 8;
   q.bytes = q.list + B * S * SL * 4;
   return q;
 }
 
 constexpr int64_t SAMPLE_WAVE = 1024;  // logits of a row that a wave takes
+constexpr int64_t SAMPLE_MOST = static_cast<int64_t>(MAX_S) * SL;
 
 template <typename T>
 static int launch_sample(const SampleArgs &a, int64_t B, char *ws, bool listed, hipStream_t st) {
@@ -868,9 +884,9 @@ static int launch_sample(const SampleArgs &a, int64_t B, char *ws, bool listed, 
     return check_launch("sample");
   }
   const SampleParts q = parts_of(B, a.V);
-  const SampleWork w{reinterpret_cast<SliceInfo *>(ws + q.slice), reinterpret_cast<RowInfo *>(ws + q.row),
-                     reinterpret_cast<uint64_t *>(ws + q.mass), reinterpret_cast<uint32_t *>(ws + q.count),
-                     reinterpret_cast<uint32_t *>(ws + q.list), static_cast<int>(cdiv(a.V, SL))};
+  const SampleWork w{reinterpret_cast<SliceInfo *>(ws), reinterpret_cast<RowInfo *>(ws + q.row),
+                     reinterpret_cast<uint64_t *>(ws + q.hist), reinterpret_cast<uint32_t *>(ws + q.list),
+                     static_cast<int>(cdiv(a.V, SL))};
   const dim3 grid(static_cast<unsigned>(w.S), static_cast<unsigned>(B));
   hipLaunchKernelGGL(sample_slice_kernel<T>, grid, dim3(SL_T), 0, st, a, w);
   int rc = check_launch("sample slices");
@@ -890,7 +906,7 @@ static int launch_sample(const SampleArgs &a, int64_t B, char *ws, bool listed, 
 using namespace evo2;
 
 extern "C" int64_t evo2_sample_workspace_bytes(int64_t B, int64_t V) {
-  if (B <= 0 || V <= SAMPLE_WAVE || V > (1 << 24) || B > 65535) return 0;
+  if (B <= 0 || V <= SAMPLE_WAVE || V > SAMPLE_MOST || B > 65535) return 0;
   return parts_of(B, V).bytes;
 }
 
@@ -898,7 +914,7 @@ extern "C" int evo2_sample(const void *logits, int32_t fp32, int64_t sz, const f
                            float t1, const int32_t *top_k, int64_t k1, const float *top_p, float p1,
                            const float *min_p, float m1, void *workspace, int64_t workspace_bytes, int64_t *tokens,
                            int64_t B, int64_t V, void *stream) {
-  if (B < 0 || V <= 0 || V > (1 << 24))
+  if (B < 0 || V <= 0 || V > SAMPLE_MOST)
     return fail(EVO2_ERR_INVALID, "sample: bad sizes B=%lld V=%lld", (long long)B, (long long)V);
   if (B == 0) return EVO2_OK;
   if (!logits || !u || !tokens) return fail(EVO2_ERR_INVALID, "sample: null pointer argument");

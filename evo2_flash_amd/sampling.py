@@ -55,8 +55,8 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     if len(shape) != 2 or dtype not in _TYPES:
         raise ValueError(f"sample_tokens takes bf16 or fp32 logits (B, V), got {tuple(shape)} {dtype}")
     B, V = shape
-    if not 0 < V <= 1 << 24:
-        raise ValueError(f"sample_tokens takes 1 to 2^24 logits a row, got {V}")
+    if not 0 < V <= 1 << 20:
+        raise ValueError(f"sample_tokens takes 1 to 2^20 logits a row, got {V}")
     if uniforms.shape != (B,) or uniforms.dtype != torch.float32:
         raise ValueError(f"uniforms must be ({B},) fp32, got {tuple(uniforms.shape)} {uniforms.dtype}")
     t, t1, keep_t = _setting(temperature, "temperature", B, dev, torch.float32)

@@ -492,7 +492,7 @@ int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_t qt, int64
  * first index at which the running sum of what is kept passes u times its total.  T <= 0
  * or k = 1: the first of the largest.  -inf and NaN are never drawn; a row of nothing else
  * gives -1.  temperature, top_k, top_p, min_p (B,) by row, or NULL: t1, k1, p1, m1.
- *   tokens (B,) int64; V up to 2^24; workspace of _workspace_bytes(B, V) bytes, 16-byte
+ *   tokens (B,) int64; V up to 2^20; workspace of _workspace_bytes(B, V) bytes, 16-byte
  *   aligned (0: none)
  */
 int64_t evo2_sample_workspace_bytes(int64_t B, int64_t V);
