@@ -34,10 +34,12 @@ def _cache_args(what, k_pages, v_pages, k_scale, v_scale, block_table, B):
     """Checks of the cache's tensors and the table; the C entries' arguments from the key
     pages to the table's columns, and (kv_heads, head_dim, device index)."""
     dev = k_pages.get_device()
-    if not (dev >= 0 and dev == v_pages.get_device() == k_scale.get_device() == v_scale.get_device()
-            == block_table.get_device()):
+    same = (dev == v_pages.get_device() == k_scale.get_device() == v_scale.get_device()
+            == block_table.get_device())
+    if dev < 0 or not same:
         _lib.require_device(k_pages, v_pages, k_scale, v_scale, block_table)
-        raise ValueError(f"{what}: the cache and its table are on different devices")
+        if not same:
+            raise ValueError(f"{what}: the cache and its table are on different devices")
     shape = k_pages.shape
     if len(shape) != 4 or shape[2] != PAGE or k_pages.dtype != _F8 or v_pages.dtype != _F8:
         raise ValueError(f"{what} takes float8_e4m3fn pages (pages, kv_heads, {PAGE}, head_dim) and "
@@ -239,6 +241,24 @@ class Fp8KVCache:
     def tensors(self):
         """The tensors as write_kv_fp8 and the other operators take them."""
         return self.k, self.v, self.k_scale, self.v_scale
+
+    def clear(self):
+        """Zeros in every page, as a new cache has."""
+        for t in (self.k, self.v):
+            t.view(torch.uint8).zero_()
+        self.k_scale.fill_(1.0)
+        self.v_scale.fill_(1.0)
+
+    def fill(self, values):
+        """Every page's 16 tokens: values(pages, 16, heads, head_dim) makes keys and values
+        for some pages at a time."""
+        pages, heads, _, hd = self.k.shape
+        step = max(1, min(65535, (1 << 27) // (PAGE * heads * hd)))
+        for at in range(0, pages, step):
+            n = min(step, pages - at)
+            table = torch.arange(at, at + n, dtype=torch.int32, device=self.k.device).view(n, 1)
+            k, v = (values(n, PAGE, heads, hd).to(torch.bfloat16) for _ in range(2))
+            write_kv_fp8(k, v, *self.tensors, table, torch.zeros(n, dtype=torch.int64, device=k.device))
 
     def append(self, k, v, block_table, positions):
         """k, v (B, heads, head_dim): the entries of sequence b at positions[b]."""

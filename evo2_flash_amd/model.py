@@ -31,6 +31,10 @@ norm and the head, on features of the layers below that stay as they are: packed
 attention, the gated product and the cross entropy run on this build's kernels in both
 directions, the projections on the library's, the norms and the rotary in torch.
 
+With kv_dtype float8_e4m3fn the attention layers keep their KV pages in 8 bits
+(kv_fp8.py): half the bytes that decode attention reads.  generate draws tokens one
+step at a time (sampling.py).
+
 Weights are random, seeded, in the benchmark's distributions.
 """
 
@@ -41,11 +45,14 @@ from .attention import (PAGE, PagedKVCache, causal_prefill_attention, check_bloc
                         packed_attention, paged_decode_attention, prefill_attention_rows,
                         rotary_decode, rotary_prefill, shared_prefix_pages,
                         workspace as attention_workspace)
+from .kv_fp8 import (Fp8KVCache, paged_decode_attention_fp8, rotary_decode_fp8, rotary_prefill_fp8,
+                     workspace_fp8)
 from .linear import gated, gated_linear, linear, plain
 from .loss import linear_cross_entropy
 from .metadata import build_metadata
 from .mixers import Linear, load_mixer_params, make_mixer, set_forward_context
 from .norm import Evo2RMSNorm
+from .sampling import sample_tokens
 from .state import HyenaStatePool, get_mamba_state_copy_func
 from .synthetic import mixer_params
 
@@ -123,11 +130,14 @@ def rotary_neox(x, positions, inv_freq, factor):
 
 class Evo2Attention(nn.Module):
     """qkv_proj, rotary, KV written to the layer's pages, softmax attention
-    over the sequence's positions, o_proj with bias (model.py:104-153)."""
+    over the sequence's positions, o_proj with bias (model.py:104-153).  kv_dtype: the
+    pages' type, bfloat16 or float8_e4m3fn (with a scale a page and head)."""
 
     def __init__(self, config, num_pages, max_pages, max_batch, rope_theta=10000.0,
-                 rope_factor=1.0, device=None):
+                 rope_factor=1.0, device=None, kv_dtype=torch.bfloat16, shared_pages=0):
         super().__init__()
+        if kv_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"kv_dtype must be bfloat16 or float8_e4m3fn, got {kv_dtype}")
         h = config.hidden_size
         self.heads = config.num_attention_heads
         self.hd = h // self.heads
@@ -136,10 +146,15 @@ class Evo2Attention(nn.Module):
         self.rope_factor = float(rope_factor)
         self.register_buffer("inv_freq", 1.0 / rope_theta ** (
             torch.arange(0, self.hd, 2, device=device, dtype=torch.float32) / self.hd))
-        self.cache = PagedKVCache(num_pages, self.heads, self.hd, device)
-        self.shared_pages = 0  # leading block-table entries every sequence shares
-        self._attn_ws = attention_workspace(max_batch, self.heads, self.hd, max_pages * PAGE,
-                                            device)
+        self.shared_pages = shared_pages  # leading block-table entries every sequence shares
+        if kv_dtype == torch.bfloat16:
+            self.cache = PagedKVCache(num_pages, self.heads, self.hd, device)
+            self._attn_ws = attention_workspace(max_batch, self.heads, self.hd, max_pages * PAGE,
+                                                device)
+        else:
+            self.cache = Fp8KVCache(num_pages, self.heads, self.hd, device)
+            self._attn_ws = workspace_fp8(max_batch, self.heads, self.heads, self.hd, max_pages,
+                                          device, shared_pages=shared_pages)
 
     def _rotated(self, qkv, positions):
         q, k, v = qkv.view(qkv.shape[0], 3, self.heads, self.hd).unbind(1)
@@ -150,11 +165,18 @@ class Evo2Attention(nn.Module):
         """x (B, H): one token per sequence at `positions` (B,)."""
         B = x.shape[0]
         qkv, _ = self.qkv_proj(x)
-        q = rotary_decode(qkv, self.cache, block_table, positions, self.inv_freq,
-                          self.rope_factor)
-        out = paged_decode_attention(q, self.cache.k, self.cache.v, block_table,
-                                     positions, self.hd ** -0.5, self._attn_ws,
-                                     shared_pages=self.shared_pages)  # (B, nh, hd)
+        if isinstance(self.cache, Fp8KVCache):
+            q = rotary_decode_fp8(qkv, self.cache, block_table, positions, self.inv_freq,
+                                  self.rope_factor)
+            out = paged_decode_attention_fp8(q, *self.cache.tensors, block_table, positions,
+                                             self.hd ** -0.5, self._attn_ws,
+                                             shared_pages=self.shared_pages)
+        else:
+            q = rotary_decode(qkv, self.cache, block_table, positions, self.inv_freq,
+                              self.rope_factor)
+            out = paged_decode_attention(q, self.cache.k, self.cache.v, block_table,
+                                         positions, self.hd ** -0.5, self._attn_ws,
+                                         shared_pages=self.shared_pages)  # (B, nh, hd)
         o, _ = self.o_proj(out.reshape(B, self.heads * self.hd))
         return o
 
@@ -166,8 +188,10 @@ class Evo2Attention(nn.Module):
         # or autocast), in the kernels' type, grid and device
         if (self.hd == 128 and nseq <= 65535 and plain(qkv)
                 and qkv.get_device() == torch.cuda.current_device()):
-            q, k, vt = rotary_prefill(qkv, self.cache, block_table, self.inv_freq,
-                                      self.rope_factor, nseq, L)
+            rotary = (rotary_prefill_fp8 if isinstance(self.cache, Fp8KVCache)
+                      else rotary_prefill)
+            q, k, vt = rotary(qkv, self.cache, block_table, self.inv_freq, self.rope_factor, nseq,
+                              L)
             out = torch.empty(nseq, L, self.heads, self.hd, dtype=qkv.dtype, device=qkv.device)
             prefill_attention_rows(q, k, vt, self.hd ** -0.5, out.transpose(1, 2))
             o, _ = self.o_proj(out.view(nseq * L, self.heads * self.hd))
@@ -257,7 +281,7 @@ class Evo2DecodeModel(nn.Module):
         return get_mamba_state_copy_func()
 
     def __init__(self, config, max_batch, max_ctx, device, rope_theta=10000.0, rope_factor=1.0,
-                 name="evo2", page_seed=0, shared_prefix=0):
+                 name="evo2", page_seed=0, shared_prefix=0, kv_dtype=torch.bfloat16):
         super().__init__()
         self.config = config
         h = config.hidden_size
@@ -288,8 +312,7 @@ class Evo2DecodeModel(nn.Module):
         for i in range(config.num_hidden_layers):
             if config.layer_kind(i) == "attn":
                 mixer = Evo2Attention(config, num_pages, self.max_pages, max_batch, rope_theta,
-                                      rope_factor, device)
-                mixer.shared_pages = shared_pages
+                                      rope_factor, device, kv_dtype, shared_pages)
             else:
                 mixer = make_mixer(config, i, prefix=f"{name}.layers.{i}.mixer", device=device)
                 pool = HyenaStatePool(max_batch + 1, h, device)
@@ -319,7 +342,13 @@ class Evo2DecodeModel(nn.Module):
                 for mod in (a.qkv_proj, a.o_proj):
                     mod.weight.data.copy_(torch.randn(mod.weight.shape, generator=g, device=dev) * 0.02)
                 a.o_proj.bias.data.copy_(torch.randn(a.o_proj.bias.shape, generator=g, device=dev) * 0.02)
-                if kv_scale:
+                if isinstance(a.cache, Fp8KVCache):
+                    if kv_scale:
+                        a.cache.fill(lambda *shape: torch.randn(shape, generator=g, device=dev)
+                                     * kv_scale)
+                    else:
+                        a.cache.clear()
+                elif kv_scale:
                     a.cache.k.copy_(torch.randn(a.cache.k.shape, generator=g, device=dev) * kv_scale)
                     a.cache.v.copy_(torch.randn(a.cache.v.shape, generator=g, device=dev) * kv_scale)
                 else:
@@ -450,6 +479,33 @@ class Evo2DecodeModel(nn.Module):
                 x = layer(positions, x, tokens, table)
         h = self.norm(x)
         return linear(h, self.embed)
+
+    @torch.no_grad()
+    def generate(self, prompts, num_tokens, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                 uniforms=None, generator=None, chunk_seqs=8):
+        """Continue prompts (B, L) by num_tokens tokens each: prefill, then one decode step a
+        token; every token is drawn by sampling.sample_tokens with these settings (numbers, or
+        (B,) tensors) from a row of `uniforms` (num_tokens, B) fp32, by default drawn from
+        `generator` (its device's, or the model's default one).  Returns the tokens
+        (B, num_tokens).  Overwrites the states and KV pages of sequences 0..B-1."""
+        B, L = prompts.shape
+        if L + num_tokens > self.max_pages * PAGE + 1:
+            raise ValueError(f"{L} + {num_tokens} tokens exceed the model's {self.max_pages * PAGE} "
+                             f"positions")
+        dev = prompts.device
+        if uniforms is None:
+            uniforms = torch.rand(num_tokens, B, generator=generator,
+                                  device=dev if generator is None else generator.device).to(dev)
+        elif uniforms.shape != (num_tokens, B):
+            raise ValueError(f"uniforms must be ({num_tokens}, {B}), got {tuple(uniforms.shape)}")
+        out = torch.empty(B, num_tokens, dtype=torch.int64, device=dev)
+        positions = torch.full((B,), L - 1, dtype=torch.int64, device=dev)
+        for i in range(num_tokens):
+            logits = (self.prefill(prompts, chunk_seqs) if i == 0
+                      else self.decode_step(out[:, i - 1].contiguous(), positions))
+            out[:, i] = sample_tokens(logits, uniforms[i], temperature, top_k, top_p, min_p)
+            positions += 1
+        return out
 
     def hyena_params(self, i):
         """{parameter name: tensor} of Hyena layer i (checkpoint names)."""

@@ -49,9 +49,11 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     summed as whole numbers (steps of 2^-49 of the largest, of 2^-61 V for V over 4096), so
     a result does not depend on timing."""
     shape, dtype, dev = logits.shape, logits.dtype, logits.get_device()
-    if dev < 0 or uniforms.get_device() != dev:
+    same = uniforms.get_device() == dev
+    if dev < 0 or not same:
         _lib.require_device(logits, uniforms)
-        raise ValueError(f"uniforms are on {uniforms.device}, the logits on {logits.device}")
+        if not same:
+            raise ValueError(f"uniforms are on {uniforms.device}, the logits on {logits.device}")
     if len(shape) != 2 or dtype not in _TYPES:
         raise ValueError(f"sample_tokens takes bf16 or fp32 logits (B, V), got {tuple(shape)} {dtype}")
     B, V = shape
