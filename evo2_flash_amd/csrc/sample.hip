@@ -46,21 +46,21 @@ struct SampleArgs {
 struct SampleRow {
   double c;       // log2(e) / T: y = (z - max) c
   float c4;       // 4 c, at most the largest number
-  double ymin;    // log2(m), -inf without min-p
+  float min_p;
   float top_p;
   int64_t top_k;  // 0: all
   bool first;     // the first of the largest
 };
 __device__ __forceinline__ SampleRow row_of(const SampleArgs &p, int b) {
   SampleRow r;
-  const float t = p.t ? p.t[b] : p.t1, m = p.m ? p.m[b] : p.m1;
+  const float t = p.t ? p.t[b] : p.t1;
+  r.min_p = p.m ? p.m[b] : p.m1;
   r.top_p = p.p ? p.p[b] : p.p1;
   const int64_t k = p.k ? p.k[b] : p.k1;
   r.top_k = k > 0 && k < p.V ? k : 0;
   r.first = !(t > 0.0f) || k == 1;
   r.c = 1.4426950408889634 / static_cast<double>(fminf(t, 3.0e38f));  // (any infinite T is flat)
   r.c4 = static_cast<float>(fmin(4.0 * r.c, 3.0e38));
-  r.ymin = m > 0.0f ? log2(static_cast<double>(fminf(m, 1.0f))) : -INFINITY;
   return r;
 }
 
@@ -72,9 +72,12 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 }
 constexpr uint32_t LEAST_KEY = 0x00800000u;  // of the lowest finite value
 
-// The value of a key (not 0); +inf as a number far above all others.
+// The value of a key (not 0), and as a double with +inf a number far above all others.
+__device__ __forceinline__ float float_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
 __device__ __forceinline__ double value_of(uint32_t key) {
-  const float z = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+  const float z = float_of(key);
   return z < INFINITY ? static_cast<double>(z) : 1e200;
 }
 
@@ -233,8 +236,7 @@ struct Digits {
 // ---------------------------------------------------------------- rows of up to 64 E logits
 // A wave takes a row, lane l logits E l .. E l + E - 1.  The cuts are found a byte at a
 // time from histograms of the wave's own in LDS (nothing but this wave's order of LDS
-// operations parts their steps).  Bisection with counts by ballots took 2 to 6 us of a
-// call, this SEARCH_K; with sums for top-p 5 us, this SEARCH_P.
+// operations parts their steps).
 template <typename T, int E>
 __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
   __shared__ __attribute__((aligned(16))) unsigned long long hists[4][BINS];
@@ -273,38 +275,82 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
     valid += __popcll(__ballot(key[e] != 0));
   }
   least = ~wave_max(~least);
-  // The key at which the sum of x over the keys from the top reaches `need` (<= all of it),
-  // and the sum above it.
-  auto search = [&](auto *hist, auto x, auto need, uint32_t kmin, uint32_t &found, auto &above) __attribute__((always_inline)) {
+  // The key at which the sum of x over the keys of [kmin, kmax] from the top reaches `need`
+  // (<= all of it), and the sum above it.  First over BINS equal steps of value, `span`
+  // down from the largest (the last bin takes all below): most often a token or a few are
+  // left, which are taken one value after the other; else those left a byte at a time.
+  auto search = [&](auto *hist, auto x, auto need, uint32_t kmin, float span, uint32_t &found, auto &above) __attribute__((always_inline)) {
     using U = std::remove_reference_t<decltype(*hist)>;
-    Digits d(kmax >> LOW<T>, kmin >> LOW<T>);
-    U over = 0;
-    for (;;) {
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) hist[4 * lane + i] = 0;
       __builtin_amdgcn_wave_barrier();
+    };
+    const float vmax = float_of(kmax), step = BINS / fminf(vmax - float_of(kmin), span);
+    uint32_t bins[E];
+    clear();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      bins[e] = static_cast<uint32_t>(fminf((vmax - float_of(key[e])) * step, BINS - 1.0f));
+      if (key[e] < kmin) bins[e] = BINS;
+      if (key[e] >= kmin && x(e)) atomicAdd(&hist[bins[e]], x(e));
+    }
+    __builtin_amdgcn_wave_barrier();
+    U over = 0;
+    const uint32_t bin = min(bin_reaching<U>(hist, need, lane, over), static_cast<uint32_t>(BINS - 1));
+    uint32_t left = 0, hi = 0, lo = ~0u;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      left += __popcll(__ballot(bins[e] == bin));
+      if (bins[e] == bin) hi = max(hi, key[e]), lo = min(lo, key[e]);
+    }
+    hi = wave_max(hi);
+    if (left <= 8) {
+      for (;;) {
+        U here = 0;
+        uint32_t next = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          here += key[e] == hi ? x(e) : 0;
+          if (bins[e] == bin && key[e] < hi) next = max(next, key[e]);
+        }
+        here = wave_sum(here);
+        next = wave_max(next);
+        if (over + here >= need || !next) break;  // (the bin's sum reaches it)
+        over += here;
+        hi = next;
+      }
+      found = hi;
+      above = over;
+      return;
+    }
+    lo = ~wave_max(~lo);
+    Digits d(hi >> LOW<T>, lo >> LOW<T>);
+    for (;;) {
+      clear();
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const uint32_t k = key[e] >> LOW<T>;
-        if (key[e] && x(e) && d.has(k)) atomicAdd(&hist[d.bin(k)], x(e));
+        if (bins[e] == bin && x(e) && d.has(k)) atomicAdd(&hist[d.bin(k)], x(e));
       }
       __builtin_amdgcn_wave_barrier();
       U a = 0;
-      const uint32_t bin = min(bin_reaching<U>(hist, need - over, lane, a), static_cast<uint32_t>(BINS - 1));
+      const uint32_t digit = min(bin_reaching<U>(hist, need - over, lane, a), static_cast<uint32_t>(BINS - 1));
       over += a;
-      if (!d.next(bin)) break;
+      if (!d.next(digit)) break;
     }
     found = whole_key<T>(d.prefix);
     above = over;
   };
+  // (weights below 2^-49 are 0)
+  const float span = static_cast<float>(fmin(50.0 / r.c, 3.0e38));
   if (r.top_k && r.top_k < valid) {
     uint32_t over;
-    search(reinterpret_cast<uint32_t *>(hists[wave]), [](int) { return 1u; }, static_cast<uint32_t>(r.top_k), least, cut, over);
+    search(reinterpret_cast<uint32_t *>(hists[wave]), [](int) { return 1u; }, static_cast<uint32_t>(r.top_k), least, span, cut, over);
     tie = static_cast<uint32_t>(r.top_k) - over;
   }
   const double kv = value_of(kmax);
   unsigned long long w[E];
-  uint32_t fine = 0;  // bit e: min-p keeps it
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const bool in = key[e] && key[e] >= cut;
@@ -312,7 +358,6 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
     if (__any(in)) {  // uniform
       const double y = (value_of(in ? key[e] : kmax) - kv) * r.c;
       if (in) w[e] = weight_of(y, p.shift);
-      if (y >= r.ymin) fine |= 1u << e;
     }
   }
   // of the tokens that equal the cut, those behind the first `tie` in the vocabulary's order
@@ -332,7 +377,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
     for (int e = 0; e < E; ++e) sum += w[e];
     const unsigned long long need = need_of(r.top_p, wave_sum(sum));
     uint32_t at;
-    search(hists[wave], [&](int e) { return w[e]; }, need, max(cut, least), at, above);
+    search(hists[wave], [&](int e) { return w[e]; }, need, max(cut, least), span, at, above);
     const uint32_t most = ties_of(need, above, weight_of((value_of(at) - kv) * r.c, p.shift));
     tie = at == cut ? min(tie, most) : most;
     cut = at;
@@ -341,10 +386,12 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
       if (key[e] < cut) w[e] = 0;
     drop_ties();
   }
+  const uint64_t one = uint64_t(1) << p.shift;  // the largest weight
+  const uint64_t least_w = r.min_p > 0.0f ? r.min_p < 1.0f ? part_of(r.min_p, one, true) : one : 0;
   uint64_t sum = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if (!(fine >> e & 1)) w[e] = 0;
+    if (w[e] < least_w) w[e] = 0;
     sum += w[e];
   }
   const uint64_t upto = wave_scan(sum), target = target_of(p.u[b], lane_value(upto, 63));
@@ -411,8 +458,7 @@ struct SampleRef {
 // floor(4 z c), where that is past 2^29 the same for all (as a whole number, so that
 // differences add up).  c4: 4 c, finite.
 __device__ __forceinline__ int grid_of(uint32_t key, float c4) {
-  const float z = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-  return static_cast<int>(floorf(fminf(fmaxf(z * c4, -536870912.0f), 536870912.0f)));
+  return static_cast<int>(floorf(fminf(fmaxf(float_of(key) * c4, -536870912.0f), 536870912.0f)));
 }
 __device__ __forceinline__ int bin_of(int top_grid, uint32_t key, float c4) {
   return min(top_grid - grid_of(key, c4), BINS - 1);
@@ -565,8 +611,10 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
     return least_key([&](uint32_t k) __attribute__((always_inline)) { return bin_of(g0, k, r.c4) <= most; });
   };
   uint32_t least = 1;
-  if (r.ymin > -INFINITY)
-    least = least_key([&](uint32_t k) __attribute__((always_inline)) { return (value_of(k) - ref.top) * r.c >= r.ymin; });
+  if (r.min_p > 0.0f) {
+    const double ymin = log2(static_cast<double>(fminf(r.min_p, 1.0f)));
+    least = least_key([&](uint32_t k) __attribute__((always_inline)) { return (value_of(k) - ref.top) * r.c >= ymin; });
+  }
   int lo = 0, hi = -1;
   uint32_t from = 0, upto = ~0u;
   if (r.top_k) {
