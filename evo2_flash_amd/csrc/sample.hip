@@ -76,9 +76,9 @@ constexpr uint32_t LEAST_KEY = 0x00800000u;  // of the lowest finite value
 __device__ __forceinline__ float float_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+__device__ __forceinline__ double wide_of(float z) { return z < INFINITY ? static_cast<double>(z) : 1e200; }
 __device__ __forceinline__ double value_of(uint32_t key) {
-  const float z = float_of(key);
-  return z < INFINITY ? static_cast<double>(z) : 1e200;
+  return wide_of(float_of(key));
 }
 
 template <typename T>
@@ -457,19 +457,16 @@ struct SampleRef {
 };
 // floor(4 z c), where that is past 2^29 the same for all (as a whole number, so that
 // differences add up).  c4: 4 c, finite.
-__device__ __forceinline__ int grid_of(uint32_t key, float c4) {
-  return static_cast<int>(floorf(fminf(fmaxf(float_of(key) * c4, -536870912.0f), 536870912.0f)));
+__device__ __forceinline__ int grid_of(float z, float c4) {
+  return static_cast<int>(floorf(fminf(fmaxf(z * c4, -536870912.0f), 536870912.0f)));
 }
-__device__ __forceinline__ int bin_of(int top_grid, uint32_t key, float c4) {
-  return min(top_grid - grid_of(key, c4), BINS - 1);
-}
+__device__ __forceinline__ int bin_of(int top_grid, float z, float c4) { return min(top_grid - grid_of(z, c4), BINS - 1); }
 
-// Thread t's keys of slice s: logits SL s + SL_E t .. + SL_E - 1.
+// Thread t's logits of slice s: SL s + SL_E t .. + SL_E - 1 (-inf past the row).
 template <typename T>
-__device__ __forceinline__ void slice_keys(const SampleArgs &p, int b, int s, int t, uint32_t (&key)[SL_E]) {
+__device__ __forceinline__ void slice_values(const SampleArgs &p, int b, int s, int t, float (&x)[SL_E]) {
   const T *z = static_cast<const T *>(p.z) + b * p.sz;
   const int i0 = SL * s + SL_E * t;
-  float x[SL_E];
   if (i0 + SL_E <= p.V && reinterpret_cast<uintptr_t>(z + i0) % 16 == 0) {
     if constexpr (std::is_same_v<T, float>) {
       const float4 a = *reinterpret_cast<const float4 *>(z + i0), c = *reinterpret_cast<const float4 *>(z + i0 + 4);
@@ -484,8 +481,6 @@ __device__ __forceinline__ void slice_keys(const SampleArgs &p, int b, int s, in
 #pragma unroll
     for (int e = 0; e < SL_E; ++e) x[e] = i0 + e < p.V ? logit(z, i0 + e) : -INFINITY;
   }
-#pragma unroll
-  for (int e = 0; e < SL_E; ++e) key[e] = key_of(x[e]);
 }
 
 template <typename T>
@@ -494,16 +489,18 @@ __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, Sample
   __shared__ unsigned long long sums[SL_W];
   __shared__ uint32_t red[SL_W], red2[SL_W];
   const int s = blockIdx.x, b = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  uint32_t key[SL_E], top = 0, at = 0;
-  slice_keys<T>(p, b, s, t, key);
+  float z[SL_E], top = -INFINITY;
+  uint32_t at = 0;
+  slice_values<T>(p, b, s, t, z);
   const SampleRow r = row_of(p, b);
   for (int i = t; i < BINS; i += SL_T) hist[i] = 0;
 #pragma unroll
-  for (int e = 0; e < SL_E; ++e) top = max(top, key[e]);
-  const uint32_t wtop = wave_max(top);
+  for (int e = 0; e < SL_E; ++e) top = fmaxf(top, z[e]);  // (of a NaN and a number the number)
+  const uint32_t wtop = wave_max(key_of(top));
+  const float ztop = float_of(wtop);
 #pragma unroll
-  for (int e = 0; e < SL_E; ++e)  // the first of the largest, as ~index
-    if (key[e] == wtop) at = max(at, ~static_cast<uint32_t>(SL * s + SL_E * t + e));
+  for (int e = SL_E - 1; e >= 0; --e)  // the first of the largest, as ~index
+    if (z[e] == ztop) at = ~static_cast<uint32_t>(SL * s + SL_E * t + e);
   at = wave_max(at);
   if (lane == 0) red[wave] = wtop, red2[wave] = at;
   __syncthreads();
@@ -512,13 +509,18 @@ __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, Sample
   for (int i = 0; i < SL_W; ++i) kmax = max(kmax, red[i]);
   if (kmax && !r.first) {  // uniform
     const SampleRef ref(value_of(kmax), r.c);
-    const int g0 = grid_of(kmax, r.c4);
+    const int g0 = grid_of(float_of(kmax), r.c4);
+    if (r.top_k) {  // uniform: tokens; their weights are summed from the list
+      uint32_t *count = reinterpret_cast<uint32_t *>(hist);
 #pragma unroll
-    for (int e = 0; e < SL_E; ++e) {
-      if (key[e] == 0) continue;
-      // (top-k: tokens; their weights are summed from the list)
-      const uint64_t x = r.top_k ? 1 : ref.weight(value_of(key[e]), p.shift);
-      if (x) atomicAdd(&hist[bin_of(g0, key[e], r.c4)], static_cast<unsigned long long>(x));
+      for (int e = 0; e < SL_E; ++e)
+        if (z[e] > -INFINITY) atomicAdd(&count[2 * bin_of(g0, z[e], r.c4)], 1u);
+    } else {
+#pragma unroll
+      for (int e = 0; e < SL_E; ++e) {
+        const uint64_t x = z[e] > -INFINITY ? ref.weight(wide_of(z[e]), p.shift) : 0;
+        if (x) atomicAdd(&hist[bin_of(g0, z[e], r.c4)], static_cast<unsigned long long>(x));
+      }
     }
   }
   __syncthreads();
@@ -574,10 +576,10 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
   }
   if (kmax == 0 || r.first) return;  // uniform
   const SampleRef ref(value_of(kmax), r.c);
-  const int g0 = grid_of(kmax, r.c4);
+  const int g0 = grid_of(float_of(kmax), r.c4);
   if (t < w.S) {  // a slice's units are 2^-by of the row's, its bins `off` below the row's
     by[t] = key ? r.top_k ? 0 : static_cast<int>(fmin(ref.r - ceil(top * r.c), 63.0)) : -1;
-    off[t] = key ? min(g0 - grid_of(key, r.c4), BINS - 1) : 0;
+    off[t] = key ? min(g0 - grid_of(float_of(key), r.c4), BINS - 1) : 0;
   }
   __syncthreads();
   auto add = [&](int s, unsigned long long v) __attribute__((always_inline)) {
@@ -608,7 +610,7 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
     return found;
   };
   auto within = [&](int most) __attribute__((always_inline)) {
-    return least_key([&](uint32_t k) __attribute__((always_inline)) { return bin_of(g0, k, r.c4) <= most; });
+    return least_key([&](uint32_t k) __attribute__((always_inline)) { return bin_of(g0, float_of(k), r.c4) <= most; });
   };
   uint32_t least = 1;
   if (r.min_p > 0.0f) {
@@ -623,7 +625,7 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
   } else {
     if (r.top_p < 1.0f) hi = bin_reaching<unsigned long long>(hist, need_of(r.top_p, total), lane, before);
     if (least > 1) {
-      const int at = bin_of(g0, least, r.c4);
+      const int at = bin_of(g0, float_of(least), r.c4);
       hi = hi < 0 ? at : min(hi, at);
     }
     if (hi >= 0) {  // the one bin, of it what min-p keeps
@@ -655,20 +657,21 @@ __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleW
   const RowInfo row = w.row[b];
   if (row.mode != 2) return;  // uniform
   SliceInfo &info = w.slice[static_cast<int64_t>(b) * w.S + s];
-  uint32_t key[SL_E], n = 0;
-  slice_keys<T>(p, b, s, t, key);
+  float z[SL_E];
+  uint32_t n = 0, in = 0;
+  slice_values<T>(p, b, s, t, z);
+  const float from = float_of(row.from), upto = row.upto == ~0u ? NAN : float_of(row.upto);
 #pragma unroll
-  for (int e = 0; e < SL_E; ++e) {
-    if (key[e] < row.from || key[e] >= row.upto) key[e] = 0;
-    n += key[e] != 0;
-  }
+  for (int e = 0; e < SL_E; ++e)
+    if (z[e] >= from && !(z[e] >= upto)) in |= 1u << e;  // (none of a NaN; all below no bound)
+  n = __popc(in);
   // weight in bins over the listed ones (none with top-k)
   uint64_t x = 0;
   if (row.lo > 0 && t < BINS && info.key) {
     const SampleRow r = row_of(p, b);
     const SampleRef ref(row.top, r.c), own(info.top, r.c);
     const int by = static_cast<int>(fmin(ref.r - own.r, 63.0));
-    const int off = grid_of(key_of(static_cast<float>(row.top)), r.c4) - grid_of(info.key, r.c4);
+    const int off = grid_of(static_cast<float>(row.top), r.c4) - grid_of(float_of(info.key), r.c4);
     if (min(t + min(off, BINS - 1), BINS - 1) < row.lo) x = w.hist[(static_cast<int64_t>(b) * w.S + s) * BINS + t] >> by;
   }
   x = wave_sum(x);
@@ -681,7 +684,7 @@ __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleW
   uint32_t *list = w.list + (static_cast<int64_t>(b) * w.S + s) * SL;
 #pragma unroll
   for (int e = 0; e < SL_E; ++e)
-    if (key[e]) list[at++] = key[e];
+    if (in >> e & 1) list[at++] = key_of(z[e]);
   if (t == 0) {
     uint32_t all = 0;
     uint64_t sum = 0;
@@ -865,7 +868,10 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   // the token: thread t has logits SL_E t .. of the slice
   uint32_t key[SL_E], n = 0;
   uint64_t x[SL_E], mine = 0;
-  slice_keys<T>(p, b, pick, t, key);
+  float z[SL_E];
+  slice_values<T>(p, b, pick, t, z);
+#pragma unroll
+  for (int e = 0; e < SL_E; ++e) key[e] = key_of(z[e]);
 #pragma unroll
   for (int e = 0; e < SL_E; ++e) n += cut && key[e] == cut;
   const uint32_t trun = wave_scan(n);
