@@ -107,11 +107,13 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
   const int first = SHARED ? wave : 0;
   int32_t kpg = page_of(first, n >> 2), vpg = page_of(first, g);
   // ends of this lane's rows, of the positions any row attends to and that all do
+  AttnRow rows[NQT];  // (slots past the last row repeat it, with no positions)
   int l1[NQT], l1max = l0, l1min = l2;
 #pragma unroll
   for (int nt = 0; nt < NQT; ++nt) {
     const bool live = 16 * nt + n < nrow;
-    l1[nt] = live ? min(l2, row_len(p, attn_row(p, r0 + 16 * nt + n))) : l0;
+    rows[nt] = attn_row(p, r0 + min(16 * nt + n, nrow - 1));
+    l1[nt] = live ? min(l2, row_len(p, rows[nt])) : l0;
     l1max = max(l1max, l1[nt]);
     if (live) l1min = min(l1min, l1[nt]);
   }
@@ -127,15 +129,12 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
   abf16x8_t qop[KS][NQT];
 #pragma unroll
   for (int nt = 0; nt < NQT; ++nt) {
-    const bool live = 16 * nt + n < nrow;
-    const AttnRow a = attn_row(p, live ? r0 + 16 * nt + n : r0);
+    const AttnRow a = rows[nt];
     const bf16_t *qr = p.q + a.b * p.qb + a.i * p.qt + (static_cast<int64_t>(h) * p.group + a.j) * p.qh + 16 * g;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      au32x4_t x = *reinterpret_cast<const au32x4_t *>(qr + 64 * (ks / 2) + 8 * (ks % 2));
-      if (!live) x = au32x4_t{0, 0, 0, 0};
-      qop[ks][nt] = __builtin_bit_cast(abf16x8_t, x);
-    }
+    for (int ks = 0; ks < KS; ++ks)
+      qop[ks][nt] = __builtin_bit_cast(
+          abf16x8_t, *reinterpret_cast<const au32x4_t *>(qr + 64 * (ks / 2) + 8 * (ks % 2)));
   }
 
   float mrun[NQT], lrun[NQT];
@@ -324,27 +323,35 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
     lrun[nt] += __shfl_xor(lrun[nt], 16);
     lrun[nt] += __shfl_xor(lrun[nt], 32);
   }
-  // dims d .. d + 3 of row r: to the output (one chunk) or to the chunk's part
-  auto store = [&](int r, int d, af32x4_t o, float m, float l) __attribute__((always_inline)) {
-    const AttnRow a = attn_row(p, r0 + r);
-    const int64_t head = static_cast<int64_t>(h) * p.group + a.j;
-    if (p.nchunk == 1) {
-      const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // (a NaN sum stays NaN)
-      *reinterpret_cast<uint2 *>(p.out + a.b * p.ob + a.i * p.ot + head * p.oh + d) =
-          make_uint2(pack_bf(o[0] * inv, o[1] * inv), pack_bf(o[2] * inv, o[3] * inv));
-    } else {
-      const int64_t at = ((static_cast<int64_t>(a.b) * p.n + a.i) * p.heads + head) * p.nchunk + c;
-      *reinterpret_cast<af32x4_t *>(p.part + at * HD + d) = o;
-      if (d == 0) p.ml[at] = make_float2(m, l);
-    }
+  // where a row's dims go: the output (one chunk), or the chunk's part
+  auto out_of = [&](const AttnRow &a) __attribute__((always_inline)) {
+    return p.out + a.b * p.ob + a.i * p.ot + (static_cast<int64_t>(h) * p.group + a.j) * p.oh;
   };
+  auto part_of = [&](const AttnRow &a) __attribute__((always_inline)) {
+    const int64_t bi = static_cast<int64_t>(a.b) * p.n + a.i;
+    return (bi * p.heads + static_cast<int64_t>(h) * p.group + a.j) * p.nchunk + c;
+  };
+  auto put = [&](bf16_t *to, af32x4_t o, float inv) __attribute__((always_inline)) {
+    *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf(o[0] * inv, o[1] * inv), pack_bf(o[2] * inv, o[3] * inv));
+  };
+  auto inverse = [](float l) __attribute__((always_inline)) { return l != 0.0f ? 1.0f / l : 0.0f; };  // (NaN stays NaN)
   if constexpr (!SHARED) {
 #pragma unroll
-    for (int nt = 0; nt < NQT; ++nt)
-      if (16 * nt + n < nrow) {
+    for (int nt = 0; nt < NQT; ++nt) {
+      if (16 * nt + n >= nrow) continue;
+      if (p.nchunk == 1) {
+        bf16_t *to = out_of(rows[nt]) + 4 * g;
+        const float inv = inverse(lrun[nt]);
 #pragma unroll
-        for (int e = 0; e < ET; ++e) store(16 * nt + n, 16 * e + 4 * g, acc[e][nt], mrun[nt], lrun[nt]);
+        for (int e = 0; e < ET; ++e) put(to + 16 * e, acc[e][nt], inv);
+      } else {
+        const int64_t at = part_of(rows[nt]);
+        float *to = p.part + at * HD + 4 * g;
+#pragma unroll
+        for (int e = 0; e < ET; ++e) *reinterpret_cast<af32x4_t *>(to + 16 * e) = acc[e][nt];
+        if (g == 0) p.ml[at] = make_float2(mrun[nt], lrun[nt]);
       }
+    }
   } else {  // the waves' (max, sum, o) meet
     __shared__ float wm[AF_NW][ROWS], wl[AF_NW][ROWS];
     __shared__ af32x4_t wo[AF_NW][ROWS][HD / 4 + 1];  // (a row's padding parts the banks)
@@ -373,7 +380,14 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] = fmaf(f, wo[k][r][d4][d], o[d]);
       }
-      store(r, 4 * d4, o, M, tot);
+      const AttnRow a = attn_row(p, r0 + r);
+      if (p.nchunk == 1) {
+        put(out_of(a) + 4 * d4, o, inverse(tot));
+      } else {
+        const int64_t at = part_of(a);
+        *reinterpret_cast<af32x4_t *>(p.part + at * HD + 4 * d4) = o;
+        if (d4 == 0) p.ml[at] = make_float2(M, tot);
+      }
     }
   }
 }
