@@ -59,6 +59,10 @@ __device__ __forceinline__ int row_len(const AttnFp8Args &p, const AttnRow &a) {
   return static_cast<int>(min(max(min(first, all) + a.i + 1, int64_t(0)), all));
 }
 
+// The first k bytes of a dword; and the sign bits of the bytes that are NaN codes.
+__device__ __forceinline__ uint32_t low_bytes(int k) { return k <= 0 ? 0u : k >= 4 ? 0xffffffffu : (1u << (8 * k)) - 1; }
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // The value of the lane next to this one in its pair (lane ^ 1).
 __device__ __forceinline__ uint32_t other_of_pair(uint32_t v) {
   return __builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true);
@@ -126,6 +130,8 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
   l1min = __builtin_amdgcn_readfirstlane(l1min);
   if (l0 >= l1max && p.nchunk > 1) return;  // the join does not ask for this chunk
   // Q as the B operand: k-slot (g, j) of k-step 2 hf + u is dim 64 hf + 16 g + 8 u + j
+  // (SHARED: in LDS, for the registers that two row tiles need)
+  __shared__ abf16x8_t qs[SHARED ? KS : 1][SHARED ? NQT : 1][64];
   abf16x8_t qop[KS][NQT];
 #pragma unroll
   for (int nt = 0; nt < NQT; ++nt) {
@@ -135,6 +141,16 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
     for (int ks = 0; ks < KS; ++ks)
       qop[ks][nt] = __builtin_bit_cast(
           abf16x8_t, *reinterpret_cast<const au32x4_t *>(qr + 64 * (ks / 2) + 8 * (ks % 2)));
+  }
+
+  if constexpr (SHARED) {
+    if (wave == 0) {
+#pragma unroll
+      for (int nt = 0; nt < NQT; ++nt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qs[ks][nt][lane] = qop[ks][nt];
+    }
+    __syncthreads();
   }
 
   float mrun[NQT], lrun[NQT];
@@ -190,6 +206,8 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
   }
   for (int blk = first; blk < nblk; blk += STEP) {
     const int lb = l0 + AF_BLK * blk;
+    int at = lane;  // (not known to be the same in every round: the reads stay where they are)
+    if constexpr (SHARED) asm volatile("" : "+v"(at));
     // whole (uniform): every row attends to all of it and its pages are in the cache
     const bool whole = lb + AF_BLK <= l1min && !__any(vpg < 0);
     const bool more = blk + STEP < nblk;  // uniform
@@ -218,8 +236,10 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
             const au32x4_t x = kr[tt][ks / 2];
             const abf16x8_t a = operand(x[2 * (ks % 2)], x[2 * (ks % 2) + 1], sc);
 #pragma unroll
-            for (int nt = 0; nt < NQT; ++nt)
-              s[tt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qop[ks][nt], s[tt][nt], 0, 0, 0);
+            for (int nt = 0; nt < NQT; ++nt) {
+              const abf16x8_t q = SHARED ? qs[SHARED ? ks : 0][SHARED ? nt : 0][at] : qop[ks][nt];
+              s[tt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q, s[tt][nt], 0, 0, 0);
+            }
           }
         __builtin_amdgcn_sched_barrier(0);  // (operands of all tiles at once would take their registers)
       }
@@ -266,16 +286,46 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
         for (int e = 0; e < ET; ++e) acc[e][nt] *= alpha;
       }
     }
-    if (!whole) {  // bytes that no query attends to (of any content) become zeros
-      const int live = vpg >= 0 ? min(max(l1max - lb - 16 * g, 0), KV_PAGE) : 0;
-      au32x4_t keep;
+    if (!whole) {
+      // bytes that no row attends to (of any content) become zeros, and so do NaN codes that
+      // not all rows attend to: a weight of 0 would carry them into the others
+      const int lp = lb + 16 * g;
+      const int live = vpg >= 0 ? min(max(l1max - lp, 0), KV_PAGE) : 0, every = min(max(l1min - lp, 0), live);
+      au32x4_t keep, some;
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        const int k = live - 4 * d;
-        keep[d] = k <= 0 ? 0u : k >= 4 ? 0xffffffffu : (1u << (8 * k)) - 1;
+        keep[d] = low_bytes(live - 4 * d);
+        some[d] = keep[d] & ~low_bytes(every - 4 * d);
       }
+      uint32_t nans = 0;
 #pragma unroll
-      for (int e = 0; e < ET; ++e) vr[e] &= keep;
+      for (int e = 0; e < ET; ++e) {
+        vr[e] &= keep;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) nans |= nan_bytes(vr[e][d]) & some[d];
+      }
+      if (__any(nans)) {
+        // the rows that attend to a dim's first such position get a NaN there themselves
+#pragma unroll
+        for (int e = 0; e < ET; ++e) {
+          int nan = 0x7fffffff;  // of dim 16 e + n
+#pragma unroll
+          for (int d = 3; d >= 0; --d) {
+            const uint32_t bad = nan_bytes(vr[e][d]) & some[d];
+            if (bad) nan = lp + 4 * d + (__ffs(bad) - 1) / 8;
+            vr[e][d] &= ~((bad >> 7) * 0xffu);
+          }
+          nan = min(nan, __shfl_xor(nan, 16));
+          nan = min(nan, __shfl_xor(nan, 32));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int first = __shfl(nan, 4 * g + i);  // of acc's dim 16 e + 4 g + i
+#pragma unroll
+            for (int nt = 0; nt < NQT; ++nt)
+              if (first < l1[nt]) acc[e][nt][i] = NAN;
+          }
+        }
+      }
     }
     const float sc = kv_pow2(kv_held(vsc));
 #pragma unroll
@@ -493,6 +543,10 @@ static AttnSplit split_for(int64_t B, int64_t n, int64_t heads, int64_t kv, int6
   return s;
 }
 
+static int64_t bytes_of(const AttnSplit &s, int64_t rows, int64_t hd) {  // parts, max and sum
+  return s.nchunk == 1 ? 0 : rows * s.nchunk * (hd + 2) * static_cast<int64_t>(sizeof(float));
+}
+
 template <int HD>
 static int launch_fp8(const AttnFp8Args &a, hipStream_t st) {
   const int64_t per = static_cast<int64_t>(a.n) * a.group, own = a.nchunk - a.snum;
@@ -529,8 +583,7 @@ extern "C" int64_t evo2_decode_attention_fp8_workspace_bytes(int64_t B, int64_t 
       B > 65535 || n > 65535 || heads > 65535 || head_dim > 65535 || max_pages > (int64_t(1) << 26) ||
       shared_pages < 0 || shared_pages > max_pages)
     return 0;
-  const int64_t nchunk = split_for(B, n, heads, kv_heads, max_pages, shared_pages).nchunk;
-  return nchunk == 1 ? 0 : B * n * heads * nchunk * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+  return bytes_of(split_for(B, n, heads, kv_heads, max_pages, shared_pages), B * n * heads, head_dim);
 }
 
 extern "C" int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_t qt, int64_t qh, const void *k_pages,
@@ -556,14 +609,13 @@ extern "C" int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_
   const int rc = kv_check(c, kv_heads, head_dim, "paged_decode_attention_fp8");
   if (rc) return rc;
   if (!q || !positions || !out) return fail(EVO2_ERR_INVALID, "paged_decode_attention_fp8: null pointer argument");
-  const int64_t need = evo2_decode_attention_fp8_workspace_bytes(B, n, heads, kv_heads, head_dim, max_pages,
-                                                                 shared_pages);
+  const AttnSplit sp = split_for(B, n, heads, kv_heads, max_pages, shared_pages);
+  const int64_t need = bytes_of(sp, B * n * heads, head_dim);
   if (workspace_bytes < need || (need > 0 && !workspace))
     return fail(EVO2_ERR_INVALID, "paged_decode_attention_fp8: workspace too small");
   if (reinterpret_cast<uintptr_t>(q) % 16 || qb % 8 || qt % 8 || qh % 8 || reinterpret_cast<uintptr_t>(out) % 8 ||
       ob % 4 || ot % 4 || oh % 4 || reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(EVO2_ERR_UNSUPPORTED, "paged_decode_attention_fp8: rows must be 16-byte aligned");
-  const AttnSplit sp = split_for(B, n, heads, kv_heads, max_pages, shared_pages);
   float *part = static_cast<float *>(workspace);
   const AttnFp8Args a{c, static_cast<const bf16_t *>(q), qb, qt, qh, positions, part,
                       part ? reinterpret_cast<float2 *>(part + B * n * heads * sp.nchunk * head_dim) : nullptr,

@@ -176,9 +176,8 @@ def paged_decode_attention_fp8(q, k_pages, v_pages, k_scale, v_scale, block_tabl
     out of the softmax (a token with none left gets zeros).  shared_pages: the first
     shared_pages entries of every row name the same pages (attention.shared_prefix_pages
     finds them on the host), which are then read once for 32 query rows of any sequences.
-    Bytes of positions that a sequence does not attend to may be anything; a NaN value at a
-    position that some of a launch's rows attend to (later tokens of the sequence, or longer
-    sequences on shared pages) can reach the others in its block of 64."""
+    Bytes of positions that a token does not attend to may be anything.  No gradients are
+    recorded."""
     shape = q.shape
     if len(shape) == 3:
         (B, heads, width), n = shape, 1
@@ -291,10 +290,11 @@ def rotary_prefill_fp8(qkv, cache, block_table, inv_freq, factor, nseq, L):
     q = torch.empty(nseq, nh, L, hd, dtype=qkv.dtype, device=qkv.device)
     k = torch.empty_like(q)
     vt = torch.empty(nseq, nh, hd, Lv, dtype=qkv.dtype, device=qkv.device)
-    _lib.call("evo2_rotary_prefill", _lib.ptr(qkv), qkv.stride(0), _lib.ptr(inv_freq), float(factor),
-              _lib.ptr(q), _lib.ptr(k), _lib.ptr(vt), Lv, None, 0, 0, 0, None, 0, 0, 0, 0,
-              _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], nseq, nh, hd, L,
-              _lib.stream_of(qkv))
+    with _lib.on_device(qkv):
+        _lib.call("evo2_rotary_prefill", _lib.ptr(qkv), qkv.stride(0), _lib.ptr(inv_freq), float(factor),
+                  _lib.ptr(q), _lib.ptr(k), _lib.ptr(vt), Lv, None, 0, 0, 0, None, 0, 0, 0, 0,
+                  _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], nseq, nh, hd, L,
+                  _lib.stream_of(qkv))
     v = qkv[:, 2 * nh * hd:].view(nseq, L, nh, hd)
     zero = torch.zeros(nseq, dtype=torch.int64, device=qkv.device)
     write_kv_fp8(k.transpose(1, 2), v, *cache.tensors, block_table, zero)
@@ -314,8 +314,9 @@ def rotary_decode_fp8(qkv, cache, block_table, positions, inv_freq, factor):
     _on(dev, "rotary_decode_fp8", qkv, inv_freq)
     positions = _per_sequence(positions, B, "positions", dev)
     q = torch.empty(B, nh, hd, dtype=qkv.dtype, device=qkv.device)
-    _lib.call("evo2_rotary_decode_fp8", _lib.ptr(qkv), qkv.stride(0), _lib.ptr(inv_freq), float(factor),
-              _lib.ptr(q), *args, _lib.ptr(positions), B, nh, hd, _lib.stream_of(qkv))
+    with _lib.on_device(qkv):
+        _lib.call("evo2_rotary_decode_fp8", _lib.ptr(qkv), qkv.stride(0), _lib.ptr(inv_freq), float(factor),
+                  _lib.ptr(q), *args, _lib.ptr(positions), B, nh, hd, _lib.stream_of(qkv))
     return q
 
 

@@ -117,6 +117,33 @@ def test_nan_and_infinite_values_that_are_attended_to():
     assert nan[1, 0, 0].all() and nan[1].sum() == 64      # a key's whole head
 
 
+@pytest.mark.parametrize("hd,shared", [(64, 0), (128, 0), (64, 4), (128, 4)])
+def test_nan_values_reach_the_tokens_that_attend_to_them(hd, shared):
+    """Later tokens of a sequence, or sequences that end further on in shared pages, attend to
+    NaN codes that the others do not: theirs alone are NaN, in those dims alone."""
+    n, lens = (5, [28, 1, 62]) if not shared else (1, [20, 70, 33, 64, 40])
+    q, cache, table, pos = _case(lens, n, 4, 2, hd, 93, shared=shared)
+    v8 = cache[1].view(torch.uint8)
+    bad = [(0, 30, 0, 3), (0, 31, 1, 60), (1, 2, 0, 9), (2, 64, 1, 17)] if not shared else [
+        (0, 25, 0, 3), (0, 39, 0, 40), (0, 63, 1, 5), (0, 19, 1, 33)]
+    for b, l, j, d in bad:
+        v8[int(table[b, l // PAGE]), j, d, l % PAGE] = 0x7F if d % 2 else 0xFF
+    out = paged_decode_attention_fp8(q.to(DEV), *cache, table.to(DEV), torch.tensor(pos, device=DEV), 0.125,
+                                     shared_pages=shared).cpu()
+    want = torch.zeros(out.shape, dtype=torch.bool)
+    for b, l, j, d in bad:
+        for s in (range(len(lens)) if shared else [b]):
+            for i in range(n):
+                if l <= pos[s] + i:
+                    want[s, i, 2 * j:2 * j + 2, d] = True
+    assert torch.equal(torch.isnan(out), want)
+    for b, l, j, d in bad:
+        v8[int(table[b, l // PAGE]), j, d, l % PAGE] = 0
+    clean = paged_decode_attention_fp8(q.to(DEV), *cache, table.to(DEV), torch.tensor(pos, device=DEV), 0.125,
+                                       shared_pages=shared).cpu()
+    assert torch.equal(out[~want], clean[~want])
+
+
 def test_strides_workspace_and_streams():
     q, cache, table, pos = _case([300, 1000, 17], 2, 8, 4, 128, 92)
     d = (table.to(DEV), torch.tensor(pos, dtype=torch.int32, device=DEV), 0.09)
