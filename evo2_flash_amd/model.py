@@ -487,8 +487,11 @@ class Evo2DecodeModel(nn.Module):
         token; every token is drawn by sampling.sample_tokens with these settings (numbers, or
         (B,) tensors) from a row of `uniforms` (num_tokens, B) fp32, by default drawn from
         `generator` (its device's, or the model's default one).  Returns the tokens
-        (B, num_tokens).  Overwrites the states and KV pages of sequences 0..B-1."""
+        (B, num_tokens).  Overwrites the states and KV pages of sequences 0..B-1.  (Where a
+        row's logits are all NaN the token is -1, and the sequence goes on with token 0.)"""
         B, L = prompts.shape
+        if L < 1:
+            raise ValueError("prompts have at least one token")
         if L + num_tokens > self.max_pages * PAGE + 1:
             raise ValueError(f"{L} + {num_tokens} tokens exceed the model's {self.max_pages * PAGE} "
                              f"positions")
@@ -502,7 +505,7 @@ class Evo2DecodeModel(nn.Module):
         positions = torch.full((B,), L - 1, dtype=torch.int64, device=dev)
         for i in range(num_tokens):
             logits = (self.prefill(prompts, chunk_seqs) if i == 0
-                      else self.decode_step(out[:, i - 1].contiguous(), positions))
+                      else self.decode_step(out[:, i - 1].clamp(min=0), positions))
             out[:, i] = sample_tokens(logits, uniforms[i], temperature, top_k, top_p, min_p)
             positions += 1
         return out

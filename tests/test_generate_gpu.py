@@ -108,6 +108,15 @@ def test_generate_draws_from_the_steps_logits(H, heads, kv_dtype):
         model.generate(prompts, 96 - 29 + 2)
     with pytest.raises(ValueError, match="uniforms"):
         model.generate(prompts, 3, uniforms=u)
+    with pytest.raises(ValueError, match="at least one"):
+        model.generate(prompts[:, :0], 3)
+
+
+def test_rows_of_nan_logits_draw_no_token():
+    model = _model(256, 4, F8)
+    model.norm.weight.data.fill_(float("nan"))
+    got = model.generate(torch.ones(2, 9, dtype=torch.int64, device=DEV), 3)
+    assert got.tolist() == [[-1] * 3] * 2
 
 
 @pytest.mark.parametrize("H,heads", SHAPES)
