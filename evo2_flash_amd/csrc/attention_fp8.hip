@@ -8,12 +8,12 @@
 // outside [0, num_pages) is never dereferenced: its positions are left out of the softmax
 // (a query with none left gets zeros).
 //
-// Split over the context: a workgroup takes one chunk of positions of one key head for up
-// to 16 query rows (a sequence's tokens x the head's group; on pages that all sequences
-// share, up to 32 rows of any sequences, those chunks apart from the ones behind), and writes (o, max, sum) for each; a second
-// launch joins the chunks.  Contexts of one chunk are written out at once.  Each of the
-// four waves takes the chunk's blocks of 64 positions in turn, with a running maximum and
-// sum, on v_mfma_f32_16x16x32_bf16:
+// Split over the context: a wave takes one chunk of positions of one key head for up to 16
+// query rows (a sequence's tokens x the head's group); on pages that all sequences share, a
+// workgroup takes a chunk for up to 32 rows of any sequences, its four waves the chunk's
+// blocks in turn.  (o, max, sum) go to a workspace and a last launch joins the chunks;
+// contexts of one chunk are written out at once.  A wave walks blocks of 64 positions with a
+// running maximum and sum, on v_mfma_f32_16x16x32_bf16:
 //  * scores S^T = K Q^T in four tiles; tile t's row m is position 4 t + m % 4 of page
 //    m / 4, so that lane (n, g) ends with the 16 scores of page g for query row n.  A
 //    lane's 16-byte load is 16 dims of one position: the A operands of two k-steps;
@@ -606,7 +606,7 @@ extern "C" int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_
   const KvPages c{static_cast<uint8_t *>(const_cast<void *>(k_pages)), kps, khs,
                   static_cast<uint8_t *>(const_cast<void *>(v_pages)), vps, vhs, const_cast<float *>(k_scale), ksp,
                   ksh, const_cast<float *>(v_scale), vsp, vsh, num_pages, table, st, max_pages};
-  const int rc = kv_check(c, kv_heads, head_dim, "paged_decode_attention_fp8");
+  const int rc = kv_check(c, kv_heads, head_dim, false, "paged_decode_attention_fp8");
   if (rc) return rc;
   if (!q || !positions || !out) return fail(EVO2_ERR_INVALID, "paged_decode_attention_fp8: null pointer argument");
   const AttnSplit sp = split_for(B, n, heads, kv_heads, max_pages, shared_pages);

@@ -83,8 +83,15 @@ struct KvPages {
   int64_t max_pages;                     // its columns
 };
 
-// Whether the pages are as the kernels address them; the status of a refusal.
-inline int kv_check(const KvPages &c, int64_t heads, int64_t hd, const char *what) {
+// Whether no two (page, head)s' `size` elements overlap.
+inline bool kv_apart(int64_t pages, int64_t sp, int64_t heads, int64_t sh, int64_t size) {
+  if (pages == 1 || heads == 1) return pages == 1 ? heads == 1 || sh >= size : sp >= size;
+  return sp > sh ? sh >= size && (sp - size) / sh >= heads - 1 : sp >= size && (sh - size) / sp >= pages - 1;
+}
+
+// Whether the pages are as the kernels address them (and, for writes, lie apart); the status
+// of a refusal.
+inline int kv_check(const KvPages &c, int64_t heads, int64_t hd, bool writes, const char *what) {
   if (hd != 64 && hd != 128)
     return fail(EVO2_ERR_UNSUPPORTED, "%s: head_dim %lld (64 or 128)", what, (long long)hd);
   if (!c.k || !c.v || !c.ks || !c.vs || !c.table) return fail(EVO2_ERR_INVALID, "%s: null pointer argument", what);
@@ -94,6 +101,10 @@ inline int kv_check(const KvPages &c, int64_t heads, int64_t hd, const char *wha
   const uintptr_t at = reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v);
   if (at % 16 || c.kp % 16 || c.kh % 16 || c.vp % 16 || c.vh % 16 || c.kh < 16 * hd || c.vh < 16 * hd)
     return fail(EVO2_ERR_UNSUPPORTED, "%s: page strides or alignment not supported", what);
+  const int64_t P = c.num_pages;
+  if (writes && !(kv_apart(P, c.kp, heads, c.kh, 16 * hd) && kv_apart(P, c.vp, heads, c.vh, 16 * hd) &&
+                  kv_apart(P, c.ksp, heads, c.ksh, 1) && kv_apart(P, c.vsp, heads, c.vsh, 1)))
+    return fail(EVO2_ERR_UNSUPPORTED, "%s: pages or scales overlap", what);
   return EVO2_OK;
 }
 

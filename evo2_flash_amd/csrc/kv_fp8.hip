@@ -331,7 +331,7 @@ extern "C" int evo2_kv_fp8_write(const void *k, int64_t kb, int64_t kt, int64_t 
   const KvPages c{static_cast<uint8_t *>(k_pages), kps, khs, static_cast<uint8_t *>(v_pages), vps, vhs, k_scale, ksp,
                   ksh, v_scale, vsp, vsh, num_pages, table, st, max_pages};
   if (B == 0 || n == 0) return EVO2_OK;
-  int rc = kv_check(c, heads, head_dim, "kv_fp8_write");
+  int rc = kv_check(c, heads, head_dim, true, "kv_fp8_write");
   if (rc) return rc;
   if (!k || !v || !positions) return fail(EVO2_ERR_INVALID, "kv_fp8_write: null pointer argument");
   const uintptr_t at = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
@@ -363,7 +363,7 @@ extern "C" int evo2_kv_fp8_read(const void *k_pages, int64_t kps, int64_t khs, c
                   static_cast<uint8_t *>(const_cast<void *>(v_pages)), vps, vhs, const_cast<float *>(k_scale), ksp,
                   ksh, const_cast<float *>(v_scale), vsp, vsh, num_pages, table, st, max_pages};
   if (B == 0 || L == 0) return EVO2_OK;
-  int rc = kv_check(c, heads, head_dim, "kv_fp8_read");
+  int rc = kv_check(c, heads, head_dim, false, "kv_fp8_read");
   if (rc) return rc;
   if (!k || !v || !lengths) return fail(EVO2_ERR_INVALID, "kv_fp8_read: null pointer argument");
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16)
@@ -390,7 +390,7 @@ extern "C" int evo2_rotary_decode_fp8(const void *qkv, int64_t sqkv, const float
   const KvPages c{static_cast<uint8_t *>(k_pages), kps, khs, static_cast<uint8_t *>(v_pages), vps, vhs, k_scale, ksp,
                   ksh, v_scale, vsp, vsh, num_pages, table, st, max_pages};
   if (B == 0) return EVO2_OK;
-  int rc = kv_check(c, heads, head_dim, "rotary_decode_fp8");
+  int rc = kv_check(c, heads, head_dim, true, "rotary_decode_fp8");
   if (rc) return rc;
   if (!qkv || !inv_freq || !q || !positions)
     return fail(EVO2_ERR_INVALID, "rotary_decode_fp8: null pointer argument");

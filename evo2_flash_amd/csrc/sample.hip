@@ -18,8 +18,8 @@
 // decide no draw that 64-bit floating point would settle.  2^y is a polynomial in 64 bits
 // whose scaling and rounding to a whole number are one FMA.
 //
-// Rows of up to 1024 logits: a wave each, the logits in its registers, the cuts by
-// bisection (sample_wave_kernel).  Longer rows: four launches over slices of 4096 logits
+// Rows of up to 1024 logits: a wave each, the logits in its registers, the cuts from
+// histograms of its own in LDS (sample_wave_kernel).  Longer rows: four launches over slices of 4096 logits
 // (sample_slice_kernel and the ones after it), which read the logits once from memory.
 #include <type_traits>
 
@@ -175,6 +175,13 @@ __device__ __forceinline__ uint32_t ties_of(uint64_t need, uint64_t above, uint6
   return static_cast<uint32_t>(min(n, uint64_t(0xffffffff)));
 }
 
+// LDS operations of a wave before and after it stay in order (they run in order; the
+// compiler knows words and double words of one array for different memory).
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 constexpr int BINS = 256;
 
 // The bin of hist (from the top down) in which its running sum reaches `need`, and the sum
@@ -234,9 +241,10 @@ struct Digits {
 };
 
 // ---------------------------------------------------------------- rows of up to 64 E logits
-// A wave takes a row, lane l logits E l .. E l + E - 1.  The cuts are found a byte at a
-// time from histograms of the wave's own in LDS (nothing but this wave's order of LDS
-// operations parts their steps).
+// A wave takes a row, lane l logits E l .. E l + E - 1.  The cuts are found from histograms
+// of the wave's own in LDS (nothing but this wave's order of LDS operations parts their
+// steps).  Bound by the chain of searches, not by its reads: 8 rows of 512 bf16 logits with
+// top-k 4 5.2 us, 777 rows of 509 fp32 ones with all three cuts 9.3 us, a wave each.
 template <typename T, int E>
 __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
   __shared__ __attribute__((aligned(16))) unsigned long long hists[4][BINS];
@@ -282,9 +290,10 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
   auto search = [&](auto *hist, auto x, auto need, uint32_t kmin, float span, uint32_t &found, auto &above) __attribute__((always_inline)) {
     using U = std::remove_reference_t<decltype(*hist)>;
     auto clear = [&]() __attribute__((always_inline)) {
+      wave_order();
 #pragma unroll
       for (int i = 0; i < 4; ++i) hist[4 * lane + i] = 0;
-      __builtin_amdgcn_wave_barrier();
+      wave_order();
     };
     const float vmax = float_of(kmax), step = BINS / fminf(vmax - float_of(kmin), span);
     uint32_t bins[E];
@@ -295,7 +304,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
       if (key[e] < kmin) bins[e] = BINS;
       if (key[e] >= kmin && x(e)) atomicAdd(&hist[bins[e]], x(e));
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
     U over = 0;
     const uint32_t bin = min(bin_reaching<U>(hist, need, lane, over), static_cast<uint32_t>(BINS - 1));
     uint32_t left = 0, hi = 0, lo = ~0u;
@@ -333,7 +342,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
         const uint32_t k = key[e] >> LOW<T>;
         if (bins[e] == bin && x(e) && d.has(k)) atomicAdd(&hist[d.bin(k)], x(e));
       }
-      __builtin_amdgcn_wave_barrier();
+      wave_order();
       U a = 0;
       const uint32_t digit = min(bin_reaching<U>(hist, need - over, lane, a), static_cast<uint32_t>(BINS - 1));
       over += a;

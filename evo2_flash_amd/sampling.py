@@ -2,6 +2,8 @@
 the draw from given uniform numbers, behind the decoder's head (model.py:343-348).
 """
 
+from operator import index
+
 import torch
 
 from . import _lib
@@ -14,7 +16,7 @@ def _setting(x, name, B, dev, dtype):
     """(address or None, number) of a setting: a tensor (B,) on device `dev`, or one number
     for all rows; and the tensor, to be kept until the launch."""
     if not isinstance(x, torch.Tensor):
-        return None, x, None
+        return None, min(max(index(x), 0), 2 ** 31 - 1) if dtype is torch.int32 else float(x), None
     if x.shape != (B,):
         raise ValueError(f"{name} must be one number or ({B},), got {tuple(x.shape)}")
     if x.get_device() != dev:
@@ -44,10 +46,10 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     the first token; min_p > 0 those with at least min_p (at most 1) times the largest
     probability.  The token is the first, in the vocabulary's order, at which the running sum
     of what is kept passes uniforms times its total; numbers outside [0, 1) draw the first or
-    the last token kept.  temperature <= 0 (or NaN) and top_k 1 take the first token.  -inf and NaN logits are
-    never drawn (a row of nothing else gives -1); beside +inf no finite one is.  Weights are
-    summed as whole numbers (steps of 2^-49 of the largest, of 2^-61 V for V over 4096), so
-    a result does not depend on timing."""
+    the last token kept.  temperature <= 0 (or NaN) and top_k 1 take the first token.  -inf and
+    NaN logits are never drawn (a row of nothing else gives -1); beside +inf no finite one
+    is.  Weights are summed as whole numbers, in steps of 2^-49 of the largest (V over 8192:
+    of 2^-62 V, V rounded up to a power of two), so a result does not depend on timing."""
     shape, dtype, dev = logits.shape, logits.dtype, logits.get_device()
     same = uniforms.get_device() == dev
     if dev < 0 or not same:

@@ -69,8 +69,8 @@ def attention_exact(q, k, v, ks, vs, table, positions, scale):
     B, n, heads, hd = q.shape
     P, kv = ks.shape
     group = heads // kv
-    out, mass, worst = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(2)), None, 0.0
-    out, mass = out
+    out, mass = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(2))
+    worst = 0.0
     for b in range(B):
         for i in range(n):
             L = min(max(int(positions[b]) + i + 1, 0), table.shape[1] * PAGE)

@@ -164,8 +164,8 @@ INVALID, UNSUPPORTED = 1, 2
 def test_c_entries_check_before_a_launch():
     lib, n, at = _lib.lib(), None, 4096  # (an aligned address that is never read)
 
-    def cache(k=at, v=at, ks=at, khs=2048, vps=4096, pages=8, table=at, cols=4):
-        return (k, 4096, khs, v, vps, 2048, ks, 2, 1, at, 2, 1, pages, table, cols, cols)
+    def cache(k=at, v=at, ks=at, kps=4096, khs=2048, vps=4096, ksp=2, ksh=1, pages=8, table=at, cols=4):
+        return (k, kps, khs, v, vps, 2048, ks, ksp, ksh, at, 2, 1, pages, table, cols, cols)
 
     def write(B=2, n_=3, heads=2, hd=128, q=at, st=256, lens=n, pos=at, **kw):
         return lib.evo2_kv_fp8_write(q, 3 * st, st, 128, at, 3 * st, st, 128, *cache(**kw), pos, lens, B, n_, heads, hd, n)
@@ -190,6 +190,11 @@ def test_c_entries_check_before_a_launch():
         assert call(pages=0) == INVALID and call(cols=0) == INVALID and call(cols=(1 << 26) + 1) == INVALID
         assert call(k=at + 8) == UNSUPPORTED and call(khs=2040) == UNSUPPORTED
         assert call(khs=1024) == UNSUPPORTED and call(vps=4104) == UNSUPPORTED
+    for call in (write, rotary):  # pages and scales that lie over one another are not written
+        assert call(kps=0) == UNSUPPORTED and call(kps=2048) == UNSUPPORTED and call(kps=4080) == UNSUPPORTED
+        assert call(vps=0) == UNSUPPORTED and call(ksp=0) == UNSUPPORTED and call(ksp=1) == UNSUPPORTED
+        assert call(ksh=0) == UNSUPPORTED and b"overlap" in lib.evo2_last_error()
+        assert call(kps=4096, khs=4096) == UNSUPPORTED and call(kps=2048, khs=7 * 2048) == UNSUPPORTED
     assert write(n_=0) == 0 and write(n_=-1) == INVALID and write(n_=1 << 31) == INVALID
     assert write(q=n) == INVALID and write(pos=n) == INVALID and write(q=at + 8) == UNSUPPORTED
     assert write(st=252) == UNSUPPORTED and write(B=65536) == UNSUPPORTED and write(heads=0) == INVALID
@@ -262,6 +267,11 @@ def test_shapes_of_a_call_reach_the_kernel(monkeypatch):
     name, a = calls.pop()
     assert len(a) == len(_lib.SIGNATURES[name]) and a[0] == z.data_ptr() and a[2] == 20
     assert a[5] == 1.0 and a[6] and a[-3:-1] == (4, 9)
+    for k, want in ((1 << 70, 2 ** 31 - 1), (-(1 << 70), 0), (True, 1)):
+        sample_tokens(z, U, top_k=k)
+        assert calls.pop()[1][7] == want
+    with pytest.raises(TypeError):
+        sample_tokens(z, U, top_k=2.5)
 
 
 def test_models_take_two_page_types():

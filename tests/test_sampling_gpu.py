@@ -1,6 +1,6 @@
 """sample_tokens against a plain 64-bit form on the host: the same token everywhere.  (The
-kernel's weights are whole numbers of 2^-49 of the largest, 2^-61 V over 4096 tokens; the
-reference's are 64-bit; a draw where these would differ lies within some 1e-12 of a border
+kernel's weights are whole numbers of 2^-49 of the largest, over 8192 tokens of 2^-62 V with V
+rounded up to a power of two; the reference's are 64-bit; a draw where these would differ lies within some 1e-12 of a border
 and does not occur among the seeds here.)"""
 
 import math
@@ -64,6 +64,21 @@ def test_settings(V, dtype):
     for n, (t, k, p, m) in enumerate(SETTINGS):
         z = (torch.randn(5, V, generator=g) * 3).to(dtype)
         _check(z, torch.rand(5, generator=g), t, k, p, m)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_longest_rows(dtype):
+    V = 1 << 20
+    g = torch.Generator().manual_seed(8)
+    z = (torch.randn(1, V, generator=g) * 2).to(dtype)
+    for t, k, p, m in ((1.0, 0, 1.0, 0.0), (0.9, 70000, 0.8, 0.01)):
+        _check(z, torch.rand(1, generator=g), t, k, p, m)
+
+
+def test_many_rows():
+    g = torch.Generator().manual_seed(9)
+    z = torch.randn(70001, 3, generator=g)
+    _check(z, torch.rand(70001, generator=g), 0.8, 2, 0.9)
 
 
 def test_settings_by_row():
