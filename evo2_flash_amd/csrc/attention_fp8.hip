@@ -10,9 +10,10 @@
 //
 // Split over the context: a wave takes one chunk of positions of one key head for up to 16
 // query rows (a sequence's tokens x the head's group); on pages that all sequences share, a
-// workgroup takes a chunk for up to 32 rows of any sequences, its four waves the chunk's
-// blocks in turn.  (o, max, sum) go to a workspace and a last launch joins the chunks;
-// contexts of one chunk are written out at once.  A wave walks blocks of 64 positions with a
+// workgroup takes a chunk for up to 32 rows of any sequences, its waves the chunk's blocks in
+// turn.  (o, max, sum) go to a workspace and a last launch joins the chunks.  Contexts of one
+// chunk are written out at once; short ones, or those of as many (sequence, head)s as CUs,
+// are one chunk of a workgroup (split_for).  A wave walks blocks of 64 positions with a
 // running maximum and sum, on v_mfma_f32_16x16x32_bf16:
 //  * scores S^T = K Q^T in four tiles; tile t's row m is position 4 t + m % 4 of page
 //    m / 4, so that lane (n, g) ends with the 16 scores of page g for query row n.  A
@@ -68,26 +69,35 @@ __device__ __forceinline__ uint32_t other_of_pair(uint32_t v) {
   return __builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true);
 }
 
-// Chunks of the shared pages (SHARED: a chunk and key head, a unit, to a workgroup, whose
-// waves take its blocks in turn and meet in LDS), or of the positions behind them (a unit to
-// a wave; heads run fastest, so a workgroup's waves walk the same pages side by side, and
-// no wave waits for another: 64 sequences of 8192 positions 664 us, with a unit to a
-// workgroup 672).  tiles: row tiles that a unit has, per sequence or (SHARED) in all.  The
-// workgroups of one XCD (w mod 8) take the tiles of a unit one after the other, so its
-// codes come from that XCD's L2 after the first.
-template <int HD, int NQT, bool SHARED>
-__global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32_t tiles) {
+// What takes a unit, a chunk of one key head of a sequence or of the shared pages:
+//  * BY_WAVE: a wave; heads run fastest, so a workgroup's waves walk the same pages side by
+//    side, and no wave waits for another (64 sequences of 8192 positions 664 us, with a unit
+//    to a workgroup 672);
+//  * BY_GROUP: a workgroup, whose eight waves take its blocks in turn and meet in LDS, for
+//    contexts of one chunk;
+//  * SHARED_BY_GROUP: a workgroup of four waves, on the shared pages.
+// tiles: row tiles that a unit has, per sequence or (shared) in all.  The workgroups of one
+// XCD (w mod 8) take the tiles of a unit one after the other, so its codes come from that
+// XCD's L2 after the first.
+enum AttnBy { BY_WAVE, BY_GROUP, SHARED_BY_GROUP };
+template <AttnBy BY>
+constexpr int AF_WAVES = BY == BY_GROUP ? 8 : AF_NW;  // of a workgroup
+
+template <int HD, int NQT, AttnBy BY>
+__global__ __launch_bounds__(64 * AF_WAVES<BY>, BY == BY_GROUP ? 1 : 2) void attn_fp8_kernel(AttnFp8Args p, uint32_t tiles) {
+  constexpr bool SHARED = BY == SHARED_BY_GROUP;
+  constexpr int NW = AF_WAVES<BY>;
   constexpr int KS = HD / 32;           // k-steps of a score
   constexpr int KH = HD / 64;           // 16-byte loads a position and lane
   constexpr int ET = HD / 16;           // dim tiles
   constexpr int EG = NQT == 2 ? 2 : 4;  // of them at once
   constexpr int ROWS = 16 * NQT;
-  constexpr int STEP = SHARED ? AF_NW : 1;  // blocks from one of this wave's to the next
+  constexpr int STEP = BY == BY_WAVE ? 1 : NW;  // blocks from one of this wave's to the next
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int n = lane & 15, g = lane >> 4;
   // (all below 2^32, as the grid is: one 32-bit division each)
   const uint32_t w = blockIdx.x, j8 = w >> 3, tile = j8 % tiles;
-  const uint32_t group = (j8 / tiles) * 8 + (w & 7), unit = SHARED ? group : group * AF_NW + wave;
+  const uint32_t group = (j8 / tiles) * 8 + (w & 7), unit = BY == BY_WAVE ? group * NW + wave : group;
   const uint32_t rest = unit / p.kv;
   const int h = static_cast<int>(unit - rest * p.kv);
   const uint32_t c_count = SHARED ? p.snum : p.nchunk - p.snum;
@@ -108,7 +118,7 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
     if (l < l2) pg = row[l / KV_PAGE];
     return pg >= 0 && pg < p.c.num_pages ? pg : -1;  // -1: left out
   };
-  const int first = SHARED ? wave : 0;
+  const int first = BY == BY_WAVE ? 0 : wave;
   int32_t kpg = page_of(first, n >> 2), vpg = page_of(first, g);
   // ends of this lane's rows, of the positions any row attends to and that all do
   AttnRow rows[NQT];  // (slots past the last row repeat it, with no positions)
@@ -385,7 +395,7 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
     *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf(o[0] * inv, o[1] * inv), pack_bf(o[2] * inv, o[3] * inv));
   };
   auto inverse = [](float l) __attribute__((always_inline)) { return l != 0.0f ? 1.0f / l : 0.0f; };  // (NaN stays NaN)
-  if constexpr (!SHARED) {
+  if constexpr (BY == BY_WAVE) {
 #pragma unroll
     for (int nt = 0; nt < NQT; ++nt) {
       if (16 * nt + n >= nrow) continue;
@@ -403,8 +413,8 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
       }
     }
   } else {  // the waves' (max, sum, o) meet
-    __shared__ float wm[AF_NW][ROWS], wl[AF_NW][ROWS];
-    __shared__ af32x4_t wo[AF_NW][ROWS][HD / 4 + 1];  // (a row's padding parts the banks)
+    __shared__ float wm[NW][ROWS], wl[NW][ROWS];
+    __shared__ af32x4_t wo[NW][ROWS][HD / 4 + 1];  // (a row's padding parts the banks)
 #pragma unroll
     for (int nt = 0; nt < NQT; ++nt) {
       const int r = 16 * nt + n;
@@ -416,15 +426,15 @@ __global__ __launch_bounds__(AF_T, 2) void attn_fp8_kernel(AttnFp8Args p, uint32
       for (int e = 0; e < ET; ++e) wo[wave][r][4 * e + g] = acc[e][nt];
     }
     __syncthreads();
-    for (int x = t; x < nrow * (HD / 4); x += AF_T) {
+    for (int x = t; x < nrow * (HD / 4); x += 64 * NW) {
       const int r = x / (HD / 4), d4 = x % (HD / 4);
       float M = wm[0][r];
 #pragma unroll
-      for (int k = 1; k < AF_NW; ++k) M = fmaxf(M, wm[k][r]);
+      for (int k = 1; k < NW; ++k) M = fmaxf(M, wm[k][r]);
       float tot = 0.0f;
       af32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < AF_NW; ++k) {
+      for (int k = 0; k < NW; ++k) {
         const float f = wm[k][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[k][r] - M);
         tot = fmaf(f, wl[k][r], tot);
 #pragma unroll
@@ -509,36 +519,59 @@ __global__ __launch_bounds__(AF_T) void attn_fp8_join_kernel(AttnFp8Args p) {
 // of 8192 positions, 32 heads: chunks of 4352 665 us, 2048 672, 1024 683, 512 704.)
 constexpr int64_t AF_START = 128, AF_JOIN = 8;
 
-static int chunk_for(int64_t L, int64_t units, int64_t slots, int64_t step, int64_t most) {
+// num chunks of a unit, `walked` positions of all units.
+static int64_t cost_of(int64_t chunk, int64_t num, int64_t units, int64_t walked, int64_t slots) {
+  const int64_t rounds = cdiv(units * num, slots) * (chunk + AF_START);
+  const int64_t even = (walked + units * num * AF_START) / slots + chunk / 2;
+  return rounds + (units * num > slots ? even : rounds);
+}
+
+static int chunk_for(int64_t L, int64_t units, int64_t slots, int64_t step, int64_t most, int64_t *least = nullptr) {
   int64_t best = 0, best_cost = 0;
   for (int64_t nc = 1, chunk = 0; chunk != step; nc += nc < 8 ? 1 : nc / 4) {
     chunk = cdiv(cdiv(L, nc), step) * step;
     if (chunk > most) continue;
     const int64_t num = cdiv(L, chunk);
-    const int64_t rounds = cdiv(units * num, slots) * (chunk + AF_START);
-    const int64_t even = units * (L + num * AF_START) / slots + chunk / 2;
-    const int64_t cost = rounds + (units * num > slots ? even : rounds) + AF_JOIN * num;
+    const int64_t cost = cost_of(chunk, num, units, units * L, slots) + AF_JOIN * num;
     if (!best || cost < best_cost) {
       best = chunk;
       best_cost = cost;
     }
   }
+  if (least) *least = best_cost;
   return static_cast<int>(best);
 }
+
+// A workgroup alone may take this much longer (the join's launch), up to this many positions
+// a wave (lengths differ: the longest sequence is the launch's tail).  Passes of a graph,
+// a workgroup against chunks and their join, heads of 128: 8 sequences of 256 positions of 32
+// heads 6.9 against 9.4 us, of 8192 86 against 89, one of 784 10.4 against 10.4 (by itself,
+// where the host launches, 14.5 against 17.6), one of 2048 15 against 11; 8 of up to 8192,
+// one as long, 70 against 66.
+constexpr int64_t AF_SAVED = 64, AF_ALONE = 2048;
 
 // The split of a call: shared positions, and chunks of them and of those behind.
 struct AttnSplit {
   int shared, schunk, snum, chunk, nchunk;
+  bool group;  // a workgroup takes all of a sequence's positions: no join
 };
 static AttnSplit split_for(int64_t B, int64_t n, int64_t heads, int64_t kv, int64_t max_pages, int64_t shared_pages) {
   const int64_t L = max_pages * KV_PAGE, shared = shared_pages * KV_PAGE, rows = n * (heads / kv);
-  AttnSplit s{static_cast<int>(shared), 0, 0, AF_BLK, 0};
+  AttnSplit s{static_cast<int>(shared), 0, 0, AF_BLK, 0, false};
   if (shared) {  // of one length for all: as long as gives two workgroups a CU
     s.schunk = chunk_for(shared, kv * cdiv(B * rows, 32), 512, AF_BLK * AF_NW, int64_t(1) << 30);
     s.snum = static_cast<int>(cdiv(shared, s.schunk));
   }
-  if (L > shared)  // lengths differ: a long chunk would be the launch's tail
-    s.chunk = chunk_for(L - shared, B * kv * cdiv(rows, 16), 2048, AF_BLK, 8192);
+  if (L > shared) {  // lengths differ: a long chunk would be the launch's tail
+    const int64_t units = B * kv * cdiv(rows, 16);
+    int64_t cost;
+    s.chunk = chunk_for(L - shared, units, 2048, AF_BLK, 8192, &cost);
+    // Without a join, a workgroup to all of a sequence's positions: where eight waves take
+    // them as fast as chunks would be taken (short contexts, or as many workgroups as CUs).
+    const int64_t c = cdiv(L, AF_BLK * AF_WAVES<BY_GROUP>) * AF_BLK;
+    s.group = shared == 0 && s.chunk < L && c <= AF_ALONE && cost_of(c, 1, units, units * c, 256) <= cost + AF_SAVED;
+    if (s.group) s.chunk = static_cast<int>(L);
+  }
   s.nchunk = s.snum + static_cast<int>(cdiv(L - shared, s.chunk));
   return s;
 }
@@ -548,22 +581,26 @@ static int64_t bytes_of(const AttnSplit &s, int64_t rows, int64_t hd) {  // part
 }
 
 template <int HD>
-static int launch_fp8(const AttnFp8Args &a, hipStream_t st) {
+static int launch_fp8(const AttnFp8Args &a, bool group, hipStream_t st) {
   const int64_t per = static_cast<int64_t>(a.n) * a.group, own = a.nchunk - a.snum;
   const int64_t tiles0 = cdiv(a.B * per, 32), tiles1 = cdiv(per, 16);
   const int64_t wgs0 = cdiv(static_cast<int64_t>(a.snum) * a.kv, 8) * 8 * tiles0;
-  const int64_t wgs1 = cdiv(own * a.kv * a.B, 8 * AF_NW) * 8 * tiles1;
-  if (!grid_fits(wgs0, AF_T) || !grid_fits(wgs1, AF_T) || static_cast<int64_t>(a.B) * a.n > 65535)
+  const int64_t wgs1 = cdiv(own * a.kv * a.B, group ? 8 : 8 * AF_NW) * 8 * tiles1;
+  if (!grid_fits(wgs0, AF_T) || !grid_fits(wgs1, group ? 64 * AF_WAVES<BY_GROUP> : AF_T) || static_cast<int64_t>(a.B) * a.n > 65535)
     return fail(EVO2_ERR_UNSUPPORTED, "paged_decode_attention_fp8: more workgroups than a launch takes");
   if (wgs0) {
-    hipLaunchKernelGGL((attn_fp8_kernel<HD, 2, true>), dim3(static_cast<unsigned>(wgs0)), dim3(AF_T), 0, st, a,
+    hipLaunchKernelGGL((attn_fp8_kernel<HD, 2, SHARED_BY_GROUP>), dim3(static_cast<unsigned>(wgs0)), dim3(AF_T), 0, st, a,
                        static_cast<uint32_t>(tiles0));
     const int rc = check_launch("paged_decode_attention_fp8 shared chunks");
     if (rc) return rc;
   }
   if (wgs1) {
-    hipLaunchKernelGGL((attn_fp8_kernel<HD, 1, false>), dim3(static_cast<unsigned>(wgs1)), dim3(AF_T), 0, st, a,
-                       static_cast<uint32_t>(tiles1));
+    if (group)
+      hipLaunchKernelGGL((attn_fp8_kernel<HD, 1, BY_GROUP>), dim3(static_cast<unsigned>(wgs1)),
+                         dim3(64 * AF_WAVES<BY_GROUP>), 0, st, a, static_cast<uint32_t>(tiles1));
+    else
+      hipLaunchKernelGGL((attn_fp8_kernel<HD, 1, BY_WAVE>), dim3(static_cast<unsigned>(wgs1)), dim3(AF_T), 0, st, a,
+                         static_cast<uint32_t>(tiles1));
     const int rc = check_launch("paged_decode_attention_fp8 chunks");
     if (rc) return rc;
   }
@@ -624,5 +661,5 @@ extern "C" int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_
                       static_cast<uint32_t>(kv_heads),
                       sp.shared, sp.schunk, sp.snum, sp.chunk, sp.nchunk};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return head_dim == 64 ? launch_fp8<64>(a, s) : launch_fp8<128>(a, s);
+  return head_dim == 64 ? launch_fp8<64>(a, sp.group, s) : launch_fp8<128>(a, sp.group, s);
 }

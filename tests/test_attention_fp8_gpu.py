@@ -76,6 +76,28 @@ def test_tables_longer_than_the_sequences(cols):
     _check(out, q, cache, table, pos, 0.1)
 
 
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_chunks_of_waves(shape):
+    """A table too long for a workgroup to a sequence: the same calls in joined chunks."""
+    lens, n, heads, kv, hd = SHAPES[shape]
+    q, cache, table, pos = _case(lens, n, heads, kv, hd, shape, cols=2100)
+    work = workspace_fp8(len(lens), heads, kv, hd, 2100, DEV, n=n)
+    assert work.numel() > 16
+    out = paged_decode_attention_fp8(q.to(DEV), *cache, table.to(DEV), torch.tensor(pos, device=DEV), hd ** -0.5, work=work)
+    _check(out, q, cache, table, pos, hd ** -0.5)
+
+
+@pytest.mark.parametrize("B,kv,hd", [(64, 4, 128), (37, 7, 64), (1, 1, 64), (2, 128, 128)])
+def test_a_workgroup_to_a_sequence(B, kv, hd):
+    """Around as many workgroups as CUs, ragged lengths, none of a workspace needed."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 700, (B,), generator=g).tolist()
+    q, cache, table, pos = _case(lens, 1, kv, kv, hd, 60 + B)
+    out = paged_decode_attention_fp8(q.to(DEV), *cache, table.to(DEV), torch.tensor(pos, device=DEV), hd ** -0.5,
+                                     work=torch.empty(0, device=DEV) if B in (1, 2, 64) else None)
+    _check(out, q, cache, table, pos, hd ** -0.5)
+
+
 @pytest.mark.parametrize("B,shared,n,heads,kv,hd", [(3, 17, 1, 4, 4, 128), (33, 40, 1, 2, 2, 64),
                                                     (5, 129, 2, 8, 2, 128), (40, 64, 1, 2, 1, 128)])
 def test_shared_pages(B, shared, n, heads, kv, hd):
@@ -117,12 +139,12 @@ def test_nan_and_infinite_values_that_are_attended_to():
     assert nan[1, 0, 0].all() and nan[1].sum() == 64      # a key's whole head
 
 
-@pytest.mark.parametrize("hd,shared", [(64, 0), (128, 0), (64, 4), (128, 4)])
-def test_nan_values_reach_the_tokens_that_attend_to_them(hd, shared):
+@pytest.mark.parametrize("hd,shared,cols", [(64, 0, 0), (128, 0, 0), (64, 4, 0), (128, 4, 0), (64, 0, 2100), (128, 0, 2100)])
+def test_nan_values_reach_the_tokens_that_attend_to_them(hd, shared, cols):
     """Later tokens of a sequence, or sequences that end further on in shared pages, attend to
     NaN codes that the others do not: theirs alone are NaN, in those dims alone."""
     n, lens = (5, [28, 1, 62]) if not shared else (1, [20, 70, 33, 64, 40])
-    q, cache, table, pos = _case(lens, n, 4, 2, hd, 93, shared=shared)
+    q, cache, table, pos = _case(lens, n, 4, 2, hd, 93, shared=shared, cols=cols)
     v8 = cache[1].view(torch.uint8)
     bad = [(0, 30, 0, 3), (0, 31, 1, 60), (1, 2, 0, 9), (2, 64, 1, 17)] if not shared else [
         (0, 25, 0, 3), (0, 39, 0, 40), (0, 63, 1, 5), (0, 19, 1, 33)]
@@ -144,8 +166,9 @@ def test_nan_values_reach_the_tokens_that_attend_to_them(hd, shared):
     assert torch.equal(out[~want], clean[~want])
 
 
-def test_strides_workspace_and_streams():
-    q, cache, table, pos = _case([300, 1000, 17], 2, 8, 4, 128, 92)
+@pytest.mark.parametrize("cols", [0, 2100])
+def test_strides_workspace_and_streams(cols):
+    q, cache, table, pos = _case([300, 1000, 17], 2, 8, 4, 128, 92, cols=cols)
     d = (table.to(DEV), torch.tensor(pos, dtype=torch.int32, device=DEV), 0.09)
     want = paged_decode_attention_fp8(q.to(DEV), *cache, *d)
     wide = torch.zeros(3, 2, 8, 200, dtype=BF, device=DEV)
@@ -189,15 +212,17 @@ def test_pages_past_32_bit_offsets():
                        paged_decode_attention_fp8(q, *near.tensors, table, pos, 0.1))
 
 
-def test_decode_step_in_a_graph():
+@pytest.mark.parametrize("cols", [4, 2100])
+def test_decode_step_in_a_graph(cols):
     """Write and attention of a step captured once; each replay against eager calls on
     another cache, with eager work between."""
     B, heads, hd = 3, 4, 64
-    table = (torch.arange(12) + 1).view(B, 4).to(torch.int32).to(DEV)
+    table = torch.zeros(B, cols, dtype=torch.int32, device=DEV)
+    table[:, :4] = (torch.arange(12, device=DEV) + 1).view(B, 4)
     a, b = Fp8KVCache(13, heads, hd, DEV), Fp8KVCache(13, heads, hd, DEV)
     k, v, q = (torch.zeros(B, heads, hd, dtype=BF, device=DEV) for _ in range(3))
     pos = torch.zeros(B, dtype=torch.int64, device=DEV)
-    work = workspace_fp8(B, heads, heads, hd, 4, DEV)
+    work = workspace_fp8(B, heads, heads, hd, cols, DEV)
 
     def step(cache):
         cache.append(k, v, table, pos)

@@ -231,6 +231,10 @@ def test_workspaces():
         assert 0 <= bytes <= rows * (-(-pages * 16 // 64) + 1) * (hd + 2) * 4
         assert bytes % (rows * (hd + 2) * 4) == 0
     assert need(4, 1, 4, 4, 128, 4, 0) == 0  # one chunk: written out at once
+    # a workgroup to a sequence: short, or as many as CUs; not of long ones, or behind shared pages
+    assert need(64, 1, 4, 4, 128, 44, 0) == 0 and need(37, 1, 7, 7, 64, 44, 0) > 0 == need(2, 1, 128, 128, 128, 44, 0) == 0
+    assert need(8, 1, 32, 32, 128, 1024, 0) == 0 < need(8, 1, 32, 32, 128, 1025, 0)
+    assert need(1, 1, 32, 32, 128, 128, 0) > 0 and need(4, 1, 4, 4, 128, 60, 20) > 0
     assert need(0, 1, 4, 4, 128, 4, 0) == 0 and need(4, 1, 4, 3, 128, 4, 0) == 0 and need(4, 1, 4, 4, 128, 4, 5) == 0
     assert lib.evo2_sample_workspace_bytes(64, 1024) == 0
     ws = lib.evo2_sample_workspace_bytes(64, 131072)
