@@ -171,8 +171,14 @@ __device__ __forceinline__ uint64_t need_of(float p, uint64_t total) {
 }
 // Tokens of one value (weight w) that a front takes whose sum before them is `above`.
 __device__ __forceinline__ uint32_t ties_of(uint64_t need, uint64_t above, uint64_t w) {
-  const uint64_t n = w ? (need - above + w - 1) / w : 0xffffffffull;
-  return static_cast<uint32_t>(min(n, uint64_t(0xffffffff)));
+  const uint64_t a = need - above;
+  if (w == 0 || a >> 31 >= w) return 0xffffffffu;
+  // (the quotient, below 2^31, in 64-bit floating point: off by one at most)
+  uint64_t n = static_cast<uint32_t>(static_cast<double>(a) / static_cast<double>(w));
+  n -= n > 0 && n * w >= a;
+  n += n * w < a;
+  n += n * w < a;
+  return static_cast<uint32_t>(n);
 }
 
 // LDS operations of a wave before and after it stay in order (they run in order; the
@@ -703,21 +709,26 @@ __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleW
   }
 }
 
-constexpr int SD_LDS = 8192;  // listed keys kept in LDS
+constexpr int SD_LDS = 4096;  // listed keys kept in LDS, with their weights and slices
 
 template <typename T>
 __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleWork w) {
   __shared__ uint32_t keys[SD_LDS], start[MAX_S + 1], tied[MAX_S];
-  __shared__ unsigned long long sums[MAX_S];
+  __shared__ unsigned long long wts[SD_LDS], sums[MAX_S];
+  __shared__ uint8_t of_slice[SD_LDS];
   __shared__ unsigned long long hist[3][BINS];
   __shared__ uint64_t wred[SL_W], before_slice;
   __shared__ uint32_t red[SL_W], red2[SL_W], tie_before;
   __shared__ int pick;
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const RowInfo row = w.row[b];
-  if (row.mode == 0) return;  // uniform
+  // (what does not depend on the row's state is on its way with it)
   const SliceInfo *slice = w.slice + static_cast<int64_t>(b) * w.S;
+  const RowInfo row = w.row[b];
   const SampleRow r = row_of(p, b);
+  const float u = p.u[b];
+  SliceInfo mine{};
+  if (t < w.S) mine = slice[t];
+  if (row.mode == 0) return;  // uniform
   const SampleRef ref(row.top, r.c);
   const uint32_t *list = w.list + static_cast<int64_t>(b) * w.S * SL;
   const bool cuts = row.mode == 2;
@@ -725,19 +736,17 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   // all where nothing is listed; start[s]: listed keys before slice s
   if (t < w.S) {
     tied[t] = 0;
-    sums[t] = cuts ? slice[t].base
-                   : slice[t].key ? slice[t].total >> static_cast<int>(fmin(ref.r - ceil(slice[t].top * r.c), 63.0)) : 0;
+    sums[t] = cuts ? mine.base
+                   : mine.key ? mine.total >> static_cast<int>(fmin(ref.r - ceil(mine.top * r.c), 63.0)) : 0;
   }
   uint32_t listed = 0;
   if (cuts) {
-    if (wave == 0) {
-      for (int s0 = 0; s0 < w.S; s0 += 64) {
-        const uint32_t n = s0 + lane < w.S ? slice[s0 + lane].listed : 0, run = wave_scan(n) + listed;
-        if (s0 + lane < w.S) start[s0 + lane + 1] = run;
-        listed = lane_value(run, 63);
-      }
-      if (lane == 0) start[0] = 0;
-    }
+    const uint32_t run = wave_scan(t < w.S ? mine.listed : 0);
+    if (lane == 63) red[wave] = run;
+    if (t == 0) start[0] = 0;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) listed += red[i];
+    if (t < w.S) start[t + 1] = listed + run;
     __syncthreads();
     listed = start[w.S];
   }
@@ -751,15 +760,32 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
     }
     return lo;
   };
-  auto fetch = [&](uint32_t i) __attribute__((always_inline)) {
-    const int s = slice_of(i);
+  auto fetch = [&](uint32_t i, int s) __attribute__((always_inline)) {
     return list[static_cast<int64_t>(s) * SL + (i - start[s])];
   };
+  // a wave takes every SL_W-th slice, four of them at once (loads of the lists' own entries
+  // behind their last as well)
   uint32_t kmin = ~0u, kmx = 0;
-  for (uint32_t i = t; i < listed; i += SL_T) {
-    const uint32_t k = fetch(i);
-    if (fits) keys[i] = k;
-    kmin = min(kmin, k), kmx = max(kmx, k);
+  if (listed) {  // uniform
+#pragma unroll 1
+    for (int s0 = wave; s0 < w.S; s0 += 4 * SL_W) {
+      uint32_t k[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = list[static_cast<int64_t>(min(s0 + SL_W * i, w.S - 1)) * SL + lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + SL_W * i;
+        if (s >= w.S) break;  // uniform
+        const uint32_t end = start[s + 1];
+        uint32_t at = start[s] + lane, key = k[i];
+        while (at < end) {
+          if (fits) keys[at] = key, of_slice[at] = static_cast<uint8_t>(s);
+          kmin = min(kmin, key), kmx = max(kmx, key);
+          at += 64;
+          if (at < end) key = fetch(at, s);
+        }
+      }
+    }
   }
   kmx = wave_max(kmx);
   kmin = ~wave_max(~kmin);
@@ -767,154 +793,178 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   if (t == 0) pick = 0, tie_before = 0, before_slice = 0;
   for (int i = t; i < BINS; i += SL_T) hist[0][i] = 0;
   __syncthreads();
-#pragma unroll
   for (int i = 0; i < SL_W; ++i) kmx = max(kmx, red[i]), kmin = min(kmin, red2[i]);
-  // f(key) for all listed keys
-  auto each = [&](auto f) __attribute__((always_inline)) {
-    for (uint32_t i = t; i < listed; i += SL_T) f(fits ? keys[i] : fetch(i));
-  };
   auto weight = [&](uint32_t k) __attribute__((always_inline)) { return ref.weight(value_of(k), p.shift); };
+  // f(i, key) for all listed keys
+  auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (uint32_t i = t; i < listed; i += SL_T) f(i, fits ? keys[i] : fetch(i, slice_of(i)));
+  };
 
-  // What is kept of the listed: keys over `cut`, and the first `tie` that equal it.
+  // What is kept of the listed: keys over `cut`, and the first `tie` that equal it, each of
+  // weight `wc`.
   uint32_t cut = 0, tie = 0;
-  // The key at which sum(of(key)) over the listed keys over the cut, from the top, reaches
-  // `need`, and the sum above it; false where they do not.  `extra`: of the keys at the cut.
+  uint64_t wc = 0;
   // Histograms in turn, one pass clearing the next one's (whose last readers met before
   // this pass), every wave reading the pass's: one meeting a pass.
   int turn = 0;
-  auto search = [&](auto of, uint64_t need, uint64_t extra, uint32_t &key, uint64_t &above) __attribute__((always_inline)) {
-    Digits d(kmx >> LOW<T>, kmin >> LOW<T>);
-    unsigned long long over = 0;
-    bool found = true;
-    do {
-      unsigned long long *now = hist[turn], *next = hist[turn == 2 ? 0 : turn + 1];
-      turn = turn == 2 ? 0 : turn + 1;
-      for (int i = t; i < BINS; i += SL_T) next[i] = 0;
-      each([&](uint32_t k) __attribute__((always_inline)) {
-        if (k > cut && d.has(k >> LOW<T>)) atomicAdd(&now[d.bin(k >> LOW<T>)], static_cast<unsigned long long>(of(k)));
-      });
-      if (t == 0 && extra && d.has(cut >> LOW<T>)) atomicAdd(&now[d.bin(cut >> LOW<T>)], static_cast<unsigned long long>(extra));
-      __syncthreads();
-      unsigned long long a = 0;
-      const uint32_t bin = bin_reaching<unsigned long long>(now, need - over, lane, a);
-      found = bin < BINS;  // uniform
-      over += a;
-      if (!found || !d.next(bin)) break;
-    } while (true);
-    key = whole_key<T>(d.prefix);
-    above = over;
-    return found;
-  };
   if (cuts && listed) {
-    uint32_t key;
-    uint64_t above;
-    if (r.top_k && search([](uint32_t) { return uint64_t(1); }, r.top_k, 0, key, above)) {
+#pragma unroll 1
+    for (int by_weight = r.top_k ? 0 : 1; by_weight < 2; ++by_weight) {  // top-k, top-p
+      uint64_t need = r.top_k, extra = 0;  // extra: of the keys at the cut
+      if (by_weight) {
+        uint64_t x = 0;  // over the cut
+        each([&](uint32_t i, uint32_t k) __attribute__((always_inline)) {
+          const uint64_t v = k > cut ? weight(k) : 0;
+          if (fits) wts[i] = v;
+          x += v;
+        });
+        if (!(r.top_p < 1.0f)) break;
+        uint64_t total = row.total;
+        extra = tie * wc;
+        if (r.top_k) {  // of what top-k kept
+          x = wave_sum(x);
+          if (lane == 0) wred[wave] = x;
+          __syncthreads();
+          total = extra;
+          for (int i = 0; i < SL_W; ++i) total += wred[i];
+        }
+        need = need_of(r.top_p, total);
+        if (need <= row.over) break;
+        need -= row.over;
+      }
+      // the key at which the sum over the listed keys over the cut, from the top, reaches
+      // `need`, and the sum above it
+      Digits d(kmx >> LOW<T>, kmin >> LOW<T>);
+      unsigned long long above = 0;
+      bool found;
+      do {
+        unsigned long long *now = hist[turn], *next = hist[turn == 2 ? 0 : turn + 1];
+        turn = turn == 2 ? 0 : turn + 1;
+        for (int i = t; i < BINS; i += SL_T) next[i] = 0;
+        each([&](uint32_t i, uint32_t k) __attribute__((always_inline)) {
+          if (k > cut && d.has(k >> LOW<T>))
+            atomicAdd(&now[d.bin(k >> LOW<T>)], by_weight ? fits ? wts[i] : static_cast<unsigned long long>(weight(k)) : 1ull);
+        });
+        if (t == 0 && extra && d.has(cut >> LOW<T>)) atomicAdd(&now[d.bin(cut >> LOW<T>)], static_cast<unsigned long long>(extra));
+        __syncthreads();
+        unsigned long long a = 0;
+        const uint32_t bin = bin_reaching<unsigned long long>(now, need - above, lane, a);
+        found = bin < BINS;  // uniform
+        above += a;
+        if (!found || !d.next(bin)) break;
+      } while (true);
+      if (!found) continue;  // all of them
+      const uint32_t key = whole_key<T>(d.prefix);
+      const uint64_t wk = weight(key);
+      const uint32_t most = ties_of(need, above, by_weight ? wk : 1);
+      tie = key == cut ? min(tie, most) : most;
       cut = key;
-      tie = static_cast<uint32_t>(r.top_k - above);
-    }
-    if (r.top_p < 1.0f) {
-      const uint64_t extra = cut ? tie * weight(cut) : 0;
-      uint64_t total = row.total;
-      if (r.top_k) {  // of what top-k kept
-        uint64_t x = 0;
-        each([&](uint32_t k) __attribute__((always_inline)) { x += k > cut ? weight(k) : 0; });
-        x = wave_sum(x);
-        if (lane == 0) wred[wave] = x;
-        __syncthreads();
-        total = extra;
-        for (int i = 0; i < SL_W; ++i) total += wred[i];
-        __syncthreads();
-      }
-      const uint64_t need = need_of(r.top_p, total);
-      if (need > row.over &&
-          search([&](uint32_t k) __attribute__((always_inline)) { return weight(k); }, need - row.over, extra, key, above)) {
-        const uint32_t most = ties_of(need - row.over, above, weight(key));
-        tie = key == cut ? min(tie, most) : most;
-        cut = key;
-      }
+      wc = wk;
     }
   }
-  // A token's weight in the draw, apart from ties at the cut; the slices' sums of it
-  const uint64_t wc = cut >= row.least ? weight(cut) : 0;
-  auto kept = [&](uint32_t k) __attribute__((always_inline)) { return k > cut && k >= row.least ? weight(k) : 0; };
-  for (uint32_t i = t; i < listed; i += SL_T) {
-    const int s = slice_of(i);
-    const uint32_t k = fits ? keys[i] : fetch(i);
-    const uint64_t x = kept(k);
+  // A token's weight in the draw: over the cut and from `least` on its own, at the cut for
+  // the first `tie` wc.  The slices' sums
+  if (cut < row.least) wc = 0;
+  each([&](uint32_t i, uint32_t k) __attribute__((always_inline)) {
+    const int s = fits ? of_slice[i] : slice_of(i);
+    const uint64_t x = k > cut && k >= row.least ? fits ? wts[i] : static_cast<unsigned long long>(weight(k)) : 0;
     if (x) atomicAdd(&sums[s], static_cast<unsigned long long>(x));
     if (cut && k == cut) atomicAdd(&tied[s], 1u);
-  }
+  });
   __syncthreads();
   // the slice that the draw falls into
   if (wave == 0) {
     uint64_t all = 0;
     uint32_t nt = 0;
-    for (int s0 = 0; s0 < w.S; s0 += 64) {
+#pragma unroll 1
+    for (int s0 = 0; s0 < w.S; s0 += 64) {  // sums up to a slice's end, ties before it
       const int s = s0 + lane;
       const uint32_t n = s < w.S ? tied[s] : 0, run = wave_scan(n) + nt;
-      all += wave_sum(s < w.S ? sums[s] + (min(run, tie) - min(run - n, tie)) * wc : 0);
+      const uint64_t upto =
+          wave_scan(s < w.S ? sums[s] + (min(run, tie) - min(run - n, tie)) * wc : 0) + all;
+      if (s < w.S) sums[s] = upto, tied[s] = run - n;
       nt = lane_value(run, 63);
+      all = lane_value(upto, 63);
     }
-    const uint64_t target = all ? target_of(p.u[b], all) : 0;
-    uint64_t sum = 0;
-    nt = 0;
+    wave_order();
+    const uint64_t target = all ? target_of(u, all) : 0;
+#pragma unroll 1
     for (int s0 = 0; s0 < w.S; s0 += 64) {
       const int s = s0 + lane;
-      const uint32_t n = s < w.S ? tied[s] : 0, run = wave_scan(n) + nt;
-      const uint64_t x = s < w.S ? sums[s] + (min(run, tie) - min(run - n, tie)) * wc : 0;
-      const uint64_t upto = wave_scan(x) + sum;
-      const uint64_t hit = __ballot(upto > target);
+      const uint64_t hit = __ballot(s < w.S && sums[s] > target);
       if (hit) {
-        const int l = __ffsll(static_cast<long long>(hit)) - 1;
-        if (lane == l) pick = s, before_slice = target - (upto - x), tie_before = run - n;
+        if (lane == __ffsll(static_cast<long long>(hit)) - 1)
+          pick = s, before_slice = target - (s ? sums[s - 1] : 0), tie_before = tied[s];
         break;
       }
-      sum = lane_value(upto, 63);
-      nt = lane_value(run, 63);
     }
   }
   __syncthreads();
-  // the token: thread t has logits SL_E t .. of the slice
-  uint32_t key[SL_E], n = 0;
-  uint64_t x[SL_E], mine = 0;
+  // the token: thread t has logits SL_E t .. of the slice, of which those that are kept
+  // (most often a few hundred) go to LDS in their order, for a weight a thread
+  float *vals = reinterpret_cast<float *>(wts);
+  uint16_t *ids = reinterpret_cast<uint16_t *>(keys);
+  static_assert(SL * sizeof(float) <= sizeof(wts) && SL * sizeof(uint16_t) <= sizeof(keys), "");
+  const float at_cut = cut ? float_of(cut) : NAN, over = cut ? at_cut : -INFINITY;
+  const uint32_t least = max(row.from, row.least);
+  const float from = least > LEAST_KEY ? float_of(least) : -INFINITY;
   float z[SL_E];
   slice_values<T>(p, b, pick, t, z);
+  uint32_t n = 0;  // kept, and in the upper half those at the cut
 #pragma unroll
-  for (int e = 0; e < SL_E; ++e) key[e] = key_of(z[e]);
-#pragma unroll
-  for (int e = 0; e < SL_E; ++e) n += cut && key[e] == cut;
-  const uint32_t trun = wave_scan(n);
-  if (lane == 63) red[wave] = trun;
+  for (int e = 0; e < SL_E; ++e) n += z[e] == at_cut ? 0x10001u : z[e] > over && z[e] >= from ? 1u : 0u;
+  uint32_t run = wave_scan(n);
+  if (lane == 63) red[wave] = run;
   __syncthreads();
-  uint32_t rank = trun - n + tie_before;
-  for (int i = 0; i < wave; ++i) rank += red[i];
+  uint32_t entries = 0;
+  run -= n;
+  for (int i = 0; i < SL_W; ++i) {
+    if (i < wave) run += red[i];
+    entries += red[i] & 0xffffu;
+  }
+  uint32_t rank = tie_before + (run >> 16), to = run & 0xffffu;
 #pragma unroll
   for (int e = 0; e < SL_E; ++e) {
-    x[e] = 0;
-    if (key[e] == 0) continue;
-    if (cut && key[e] == cut) x[e] = rank++ < tie ? wc : 0;
-    else if (key[e] >= row.from) x[e] = kept(key[e]);
-    mine += x[e];
-  }
-  const uint64_t wrun = wave_scan(mine);
-  if (lane == 63) wred[wave] = wrun;
-  __syncthreads();
-  uint64_t run = wrun - mine, all = 0;
-  for (int i = 0; i < SL_W; ++i) {
-    if (i < wave) run += wred[i];
-    all += wred[i];
-  }
-  // (sums of slices in other units were shifted: the last token's end may lie a few steps off)
-  const uint64_t target = min(before_slice, all ? all - 1 : 0);
-  if (mine && run <= target && target < run + mine) {
-    int at = 0;
-    for (int e = 0; e < SL_E; ++e) {
-      run += x[e];
-      if (run > target) break;
-      at = e + 1;
+    const bool tied_here = z[e] == at_cut;
+    if (tied_here || (z[e] > over && z[e] >= from)) {
+      vals[to] = tied_here && rank >= tie ? -INFINITY : z[e];  // (no weight)
+      ids[to++] = static_cast<uint16_t>(SL_E * t + e);
+      rank += tied_here;
     }
-    p.out[b] = static_cast<int64_t>(SL) * pick + SL_E * t + at;
   }
+  __syncthreads();
+  // (sums of slices in other units were shifted: the last token's end may lie a few steps
+  // off, then it is the last one of any weight)
+  uint64_t before = 0;
+  uint32_t last = 0;
+#pragma unroll 1
+  for (uint32_t c = 0; c < entries; c += SL_T) {
+    const uint32_t i = c + t;
+    const float v = i < entries ? vals[i] : -INFINITY;
+    uint64_t x = 0;
+    if (v > -INFINITY) x = v == at_cut ? wc : ref.weight(wide_of(v), p.shift);
+    if (x) last = i + 1;
+    const uint64_t sum = wave_scan(x);
+    if (lane == 63) wred[wave] = sum;
+    __syncthreads();
+    uint64_t upto = before + sum;
+    for (int k = 0; k < SL_W; ++k) {
+      if (k < wave) upto += wred[k];
+      before += wred[k];
+    }
+    if (before > before_slice) {  // uniform
+      if (upto > before_slice && upto - x <= before_slice) p.out[b] = static_cast<int64_t>(SL) * pick + ids[i];
+      return;
+    }
+    __syncthreads();
+  }
+  const uint32_t wlast = wave_max(last);
+  if (lane == 0) red2[wave] = wlast;
+  __syncthreads();
+  uint32_t at = 0;
+  for (int k = 0; k < SL_W; ++k) at = max(at, red2[k]);
+  if (t == 0 && at) p.out[b] = static_cast<int64_t>(SL) * pick + ids[at - 1];
 }
 
 static int64_t align16(int64_t n) { return (n + 15) & ~int64_t(15); }
