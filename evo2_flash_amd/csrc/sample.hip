@@ -19,8 +19,9 @@
 // whose scaling and rounding to a whole number are one FMA.
 //
 // Rows of up to 1024 logits: a wave each, the logits in its registers, the cuts from
-// histograms of its own in LDS (sample_wave_kernel).  Longer rows: four launches over slices of 4096 logits
-// (sample_slice_kernel and the ones after it), which read the logits once from memory.
+// histograms of its own in LDS (sample_wave_kernel).  Longer rows: four launches over slices of 4096 or
+// 8192 logits (sample_slice_kernel and the ones after it), which read the logits once from
+// memory.
 #include <type_traits>
 
 #include "common.h"
@@ -85,6 +86,28 @@ template <typename T>
 __device__ __forceinline__ float logit(const T *z, int i) {
   if constexpr (std::is_same_v<T, float>) return z[i];
   else return bf2f(z[i]);
+}
+
+// Logits i0 .. i0 + E - 1 of a row of V (-inf past it): 16-byte loads at any alignment that
+// elements have.
+template <typename T, int E>
+__device__ __forceinline__ void logits_of(const T *z, int i0, int V, float (&x)[E]) {
+  constexpr int PER = 16 / sizeof(T);
+  if (i0 + E <= V) {
+#pragma unroll
+    for (int g = 0; g < E; g += PER) {
+      uint32_t d[4] = {};
+      __builtin_memcpy(d, z + i0 + g, sizeof(T) * (E < PER ? E : PER));
+#pragma unroll
+      for (int e = 0; e < (E < PER ? E / (PER / 4) : 4); ++e) {
+        if constexpr (std::is_same_v<T, float>) x[g + e] = __uint_as_float(d[e]);
+        else x[g + 2 * e] = lo_bf(d[e]), x[g + 2 * e + 1] = hi_bf(d[e]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = i0 + e < V ? logit(z, i0 + e) : -INFINITY;
+  }
 }
 
 // round(2^(S + y)) for y <= 0, S <= 51: 2^f of the fraction by its series (ln 2)^k / k!
@@ -250,20 +273,18 @@ struct Digits {
 // A wave takes a row, lane l logits E l .. E l + E - 1.  The cuts are found from histograms
 // of the wave's own in LDS (nothing but this wave's order of LDS operations parts their
 // steps).  Bound by the chain of searches, not by its reads: 8 rows of 512 bf16 logits with
-// top-k 4 5.2 us, 777 rows of 509 fp32 ones with all three cuts 9.3 us, a wave each.
+// top-k 4 4.7 us, 777 rows of 509 fp32 ones with all three cuts 8.9 us, a wave each.
 template <typename T, int E>
 __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
   __shared__ __attribute__((aligned(16))) unsigned long long hists[4][BINS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);
   if (b >= B) return;
-  const T *z = static_cast<const T *>(p.z) + b * p.sz;
+  float z[E];
+  logits_of<T, E>(static_cast<const T *>(p.z) + b * p.sz, E * lane, p.V, z);
   uint32_t key[E], top = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = E * lane + e;
-    key[e] = i < p.V ? key_of(logit(z, i)) : 0;
-  }
+  for (int e = 0; e < E; ++e) key[e] = key_of(z[e]);
   const SampleRow r = row_of(p, b);
 #pragma unroll
   for (int e = 0; e < E; ++e) top = max(top, key[e]);
@@ -424,7 +445,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
 }
 
 // ---------------------------------------------------------------- longer rows
-// Slices of SL logits.  sample_slice_kernel: a slice's largest logit, and a histogram over
+// Slices of SL_T * E logits, E a thread.  sample_slice_kernel: a slice's largest logit, and a histogram over
 // BINS bins of a quarter of a power of two in weight, from its largest down (the last bin
 // takes all below), of its tokens in rows with top-k, else of its weights.  Bins lie on one
 // grid for all slices of a row, floor(4 z c), and weights are 2^(S + z c - R) with a whole R
@@ -432,8 +453,12 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
 // a row's histogram, and the bin in which the cut lies.  sample_list_kernel: the keys of the
 // slices' tokens in that bin (top-k: in all down to it), in the vocabulary's order.
 // sample_draw_kernel: the exact cut among them, a byte at a time from histograms, the
-// slices' sums, and the token in the slice that the draw falls into.
-constexpr int SL_T = 512, SL_E = 8, SL = SL_T * SL_E, SL_W = SL_T / 64;
+// slices' sums, and the token in the slice that the draw falls into.  Bound by latency, each
+// launch by the one before: one row of 131072 fp32 logits with top-p 5.1, 5.4, 4.1 and 10.4
+// us; 64 rows of bf16 ones with all three cuts 13.8, 6.5, 5.4 and 11.9.  The draw's way: the
+// rows' and slices' records 1.5 us, the lists 1.5, three passes of a search 3, the sums and
+// the slice 1.5, its tokens 2.
+constexpr int SL_T = 512, SL_W = SL_T / 64;
 constexpr int MAX_S = 256;  // slices of the longest row, 2^20 logits
 
 struct SliceInfo {
@@ -458,7 +483,7 @@ struct SampleWork {
   SliceInfo *slice;     // (B, S)
   RowInfo *row;         // (B,)
   uint64_t *hist;       // (B, S, BINS)
-  uint32_t *list;       // (B, S * SL)
+  uint32_t *list;       // (B, S * SL_T * E)
   int S;
 };
 
@@ -477,45 +502,30 @@ __device__ __forceinline__ int grid_of(float z, float c4) {
 }
 __device__ __forceinline__ int bin_of(int top_grid, float z, float c4) { return min(top_grid - grid_of(z, c4), BINS - 1); }
 
-// Thread t's logits of slice s: SL s + SL_E t .. + SL_E - 1 (-inf past the row).
-template <typename T>
-__device__ __forceinline__ void slice_values(const SampleArgs &p, int b, int s, int t, float (&x)[SL_E]) {
-  const T *z = static_cast<const T *>(p.z) + b * p.sz;
-  const int i0 = SL * s + SL_E * t;
-  if (i0 + SL_E <= p.V && reinterpret_cast<uintptr_t>(z + i0) % 16 == 0) {
-    if constexpr (std::is_same_v<T, float>) {
-      const float4 a = *reinterpret_cast<const float4 *>(z + i0), c = *reinterpret_cast<const float4 *>(z + i0 + 4);
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = c.x, x[5] = c.y, x[6] = c.z, x[7] = c.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4 *>(z + i0);
-      const uint32_t d[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[2 * e] = lo_bf(d[e]), x[2 * e + 1] = hi_bf(d[e]);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < SL_E; ++e) x[e] = i0 + e < p.V ? logit(z, i0 + e) : -INFINITY;
-  }
+// Thread t's logits of slice s.
+template <typename T, int E>
+__device__ __forceinline__ void slice_values(const SampleArgs &p, int b, int s, int t, float (&x)[E]) {
+  logits_of<T, E>(static_cast<const T *>(p.z) + b * p.sz, E * (SL_T * s + t), p.V, x);
 }
 
-template <typename T>
+template <typename T, int E>
 __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, SampleWork w) {
   __shared__ unsigned long long hist[BINS];
   __shared__ unsigned long long sums[SL_W];
   __shared__ uint32_t red[SL_W], red2[SL_W];
   const int s = blockIdx.x, b = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  float z[SL_E], top = -INFINITY;
+  float z[E], top = -INFINITY;
   uint32_t at = 0;
-  slice_values<T>(p, b, s, t, z);
+  slice_values<T, E>(p, b, s, t, z);
   const SampleRow r = row_of(p, b);
   for (int i = t; i < BINS; i += SL_T) hist[i] = 0;
 #pragma unroll
-  for (int e = 0; e < SL_E; ++e) top = fmaxf(top, z[e]);  // (of a NaN and a number the number)
+  for (int e = 0; e < E; ++e) top = fmaxf(top, z[e]);  // (of a NaN and a number the number)
   const uint32_t wtop = wave_max(key_of(top));
   const float ztop = float_of(wtop);
 #pragma unroll
-  for (int e = SL_E - 1; e >= 0; --e)  // the first of the largest, as ~index
-    if (z[e] == ztop) at = ~static_cast<uint32_t>(SL * s + SL_E * t + e);
+  for (int e = E - 1; e >= 0; --e)  // the first of the largest, as ~index
+    if (z[e] == ztop) at = ~static_cast<uint32_t>(E * (SL_T * s + t) + e);
   at = wave_max(at);
   if (lane == 0) red[wave] = wtop, red2[wave] = at;
   __syncthreads();
@@ -528,11 +538,11 @@ __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, Sample
     if (r.top_k) {  // uniform: tokens; their weights are summed from the list
       uint32_t *count = reinterpret_cast<uint32_t *>(hist);
 #pragma unroll
-      for (int e = 0; e < SL_E; ++e)
-        if (z[e] > -INFINITY) atomicAdd(&count[2 * bin_of(g0, z[e], r.c4)], 1u);
+      for (int e = 0; e < E; ++e)
+        if (z[e] > -INFINITY) atomicAdd(&count[bin_of(g0, z[e], r.c4)], 1u);
     } else {
 #pragma unroll
-      for (int e = 0; e < SL_E; ++e) {
+      for (int e = 0; e < E; ++e) {
         const uint64_t x = z[e] > -INFINITY ? ref.weight(wide_of(z[e]), p.shift) : 0;
         if (x) atomicAdd(&hist[bin_of(g0, z[e], r.c4)], static_cast<unsigned long long>(x));
       }
@@ -541,7 +551,7 @@ __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, Sample
   __syncthreads();
   const int64_t h = (static_cast<int64_t>(b) * w.S + s) * BINS;
   unsigned long long total = 0;
-  if (t < BINS) w.hist[h + t] = total = hist[t];
+  if (t < BINS) w.hist[h + t] = total = r.top_k ? reinterpret_cast<const uint32_t *>(hist)[t] : hist[t];
   total = wave_sum(total);
   if (lane == 0) sums[wave] = total;
   __syncthreads();
@@ -664,7 +674,7 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
   }
 }
 
-template <typename T>
+template <typename T, int E>
 __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleWork w) {
   __shared__ uint32_t red[SL_W];
   __shared__ uint64_t base[SL_W];
@@ -672,12 +682,12 @@ __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleW
   const RowInfo row = w.row[b];
   if (row.mode != 2) return;  // uniform
   SliceInfo &info = w.slice[static_cast<int64_t>(b) * w.S + s];
-  float z[SL_E];
+  float z[E];
   uint32_t n = 0, in = 0;
-  slice_values<T>(p, b, s, t, z);
+  slice_values<T, E>(p, b, s, t, z);
   const float from = float_of(row.from), upto = row.upto == ~0u ? NAN : float_of(row.upto);
 #pragma unroll
-  for (int e = 0; e < SL_E; ++e)
+  for (int e = 0; e < E; ++e)
     if (z[e] >= from && !(z[e] >= upto)) in |= 1u << e;  // (none of a NaN; all below no bound)
   n = __popc(in);
   // weight in bins over the listed ones (none with top-k)
@@ -696,9 +706,9 @@ __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleW
   __syncthreads();
   uint32_t at = run - n;
   for (int i = 0; i < wave; ++i) at += red[i];
-  uint32_t *list = w.list + (static_cast<int64_t>(b) * w.S + s) * SL;
+  uint32_t *list = w.list + (static_cast<int64_t>(b) * w.S + s) * (SL_T * E);
 #pragma unroll
-  for (int e = 0; e < SL_E; ++e)
+  for (int e = 0; e < E; ++e)
     if (in >> e & 1) list[at++] = key_of(z[e]);
   if (t == 0) {
     uint32_t all = 0;
@@ -711,8 +721,9 @@ __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleW
 
 constexpr int SD_LDS = 4096;  // listed keys kept in LDS, with their weights and slices
 
-template <typename T>
+template <typename T, int E>
 __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleWork w) {
+  constexpr int SL = SL_T * E;
   __shared__ uint32_t keys[SD_LDS], start[MAX_S + 1], tied[MAX_S];
   __shared__ unsigned long long wts[SD_LDS], sums[MAX_S];
   __shared__ uint8_t of_slice[SD_LDS];
@@ -901,7 +912,7 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
     }
   }
   __syncthreads();
-  // the token: thread t has logits SL_E t .. of the slice, of which those that are kept
+  // the token: thread t has logits E t .. of the slice, of which those that are kept
   // (most often a few hundred) go to LDS in their order, for a weight a thread
   float *vals = reinterpret_cast<float *>(wts);
   uint16_t *ids = reinterpret_cast<uint16_t *>(keys);
@@ -909,11 +920,11 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   const float at_cut = cut ? float_of(cut) : NAN, over = cut ? at_cut : -INFINITY;
   const uint32_t least = max(row.from, row.least);
   const float from = least > LEAST_KEY ? float_of(least) : -INFINITY;
-  float z[SL_E];
-  slice_values<T>(p, b, pick, t, z);
+  float z[E];
+  slice_values<T, E>(p, b, pick, t, z);
   uint32_t n = 0;  // kept, and in the upper half those at the cut
 #pragma unroll
-  for (int e = 0; e < SL_E; ++e) n += z[e] == at_cut ? 0x10001u : z[e] > over && z[e] >= from ? 1u : 0u;
+  for (int e = 0; e < E; ++e) n += z[e] == at_cut ? 0x10001u : z[e] > over && z[e] >= from ? 1u : 0u;
   uint32_t run = wave_scan(n);
   if (lane == 63) red[wave] = run;
   __syncthreads();
@@ -925,11 +936,11 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   }
   uint32_t rank = tie_before + (run >> 16), to = run & 0xffffu;
 #pragma unroll
-  for (int e = 0; e < SL_E; ++e) {
+  for (int e = 0; e < E; ++e) {
     const bool tied_here = z[e] == at_cut;
     if (tied_here || (z[e] > over && z[e] >= from)) {
       vals[to] = tied_here && rank >= tie ? -INFINITY : z[e];  // (no weight)
-      ids[to++] = static_cast<uint16_t>(SL_E * t + e);
+      ids[to++] = static_cast<uint16_t>(E * t + e);
       rank += tied_here;
     }
   }
@@ -969,22 +980,47 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
 
 static int64_t align16(int64_t n) { return (n + 15) & ~int64_t(15); }
 
+// Logits a thread: 8, where that is one round of workgroups (four a CU), else 16 (rows of
+// 131072 bf16 logits with top-p 0.95: 64 of them 43 us, with 8 46; 8 rows 26, with 16 29).
+static int logits_a_thread(int64_t B, int64_t V) { return B * cdiv(V, SL_T * 8) <= 1024 ? 8 : 16; }
+
 // Offsets of the parts of a workspace; the last is its size.
 struct SampleParts {
-  int64_t row, hist, list, bytes;
+  int64_t S, row, hist, list, bytes;
 };
 static SampleParts parts_of(int64_t B, int64_t V) {
-  const int64_t S = cdiv(V, SL);
+  const int64_t size = static_cast<int64_t>(SL_T) * logits_a_thread(B, V), S = cdiv(V, size);
   SampleParts q;
+  q.S = S;
   q.row = align16(B * S * static_cast<int64_t>(sizeof(SliceInfo)));
   q.hist = q.row + align16(B * static_cast<int64_t>(sizeof(RowInfo)));
   q.list = q.hist + B * S * BINS * 8;
-  q.bytes = q.list + B * S * SL * 4;
+  q.bytes = q.list + B * S * size * 4;
   return q;
 }
 
 constexpr int64_t SAMPLE_WAVE = 1024;  // logits of a row that a wave takes
-constexpr int64_t SAMPLE_MOST = static_cast<int64_t>(MAX_S) * SL;
+constexpr int64_t SAMPLE_MOST = static_cast<int64_t>(MAX_S) * SL_T * 8;
+
+template <typename T, int E>
+static int launch_slices(const SampleArgs &a, int64_t B, char *ws, bool listed, hipStream_t st) {
+  const SampleParts q = parts_of(B, a.V);
+  const SampleWork w{reinterpret_cast<SliceInfo *>(ws), reinterpret_cast<RowInfo *>(ws + q.row),
+                     reinterpret_cast<uint64_t *>(ws + q.hist), reinterpret_cast<uint32_t *>(ws + q.list),
+                     static_cast<int>(q.S)};
+  const dim3 grid(static_cast<unsigned>(w.S), static_cast<unsigned>(B));
+  hipLaunchKernelGGL((sample_slice_kernel<T, E>), grid, dim3(SL_T), 0, st, a, w);
+  int rc = check_launch("sample slices");
+  if (rc) return rc;
+  hipLaunchKernelGGL(sample_join_kernel, dim3(static_cast<unsigned>(B)), dim3(SJ_T), 0, st, a, w);
+  if ((rc = check_launch("sample join"))) return rc;
+  if (listed) {
+    hipLaunchKernelGGL((sample_list_kernel<T, E>), grid, dim3(SL_T), 0, st, a, w);
+    if ((rc = check_launch("sample list"))) return rc;
+  }
+  hipLaunchKernelGGL((sample_draw_kernel<T, E>), dim3(static_cast<unsigned>(B)), dim3(SL_T), 0, st, a, w);
+  return check_launch("sample draw");
+}
 
 template <typename T>
 static int launch_sample(const SampleArgs &a, int64_t B, char *ws, bool listed, hipStream_t st) {
@@ -996,22 +1032,7 @@ static int launch_sample(const SampleArgs &a, int64_t B, char *ws, bool listed, 
     else hipLaunchKernelGGL((sample_wave_kernel<T, 16>), grid, dim3(256), 0, st, a, n);
     return check_launch("sample");
   }
-  const SampleParts q = parts_of(B, a.V);
-  const SampleWork w{reinterpret_cast<SliceInfo *>(ws), reinterpret_cast<RowInfo *>(ws + q.row),
-                     reinterpret_cast<uint64_t *>(ws + q.hist), reinterpret_cast<uint32_t *>(ws + q.list),
-                     static_cast<int>(cdiv(a.V, SL))};
-  const dim3 grid(static_cast<unsigned>(w.S), static_cast<unsigned>(B));
-  hipLaunchKernelGGL(sample_slice_kernel<T>, grid, dim3(SL_T), 0, st, a, w);
-  int rc = check_launch("sample slices");
-  if (rc) return rc;
-  hipLaunchKernelGGL(sample_join_kernel, dim3(static_cast<unsigned>(B)), dim3(SJ_T), 0, st, a, w);
-  if ((rc = check_launch("sample join"))) return rc;
-  if (listed) {
-    hipLaunchKernelGGL(sample_list_kernel<T>, grid, dim3(SL_T), 0, st, a, w);
-    if ((rc = check_launch("sample list"))) return rc;
-  }
-  hipLaunchKernelGGL(sample_draw_kernel<T>, dim3(static_cast<unsigned>(B)), dim3(SL_T), 0, st, a, w);
-  return check_launch("sample draw");
+  return logits_a_thread(B, a.V) == 8 ? launch_slices<T, 8>(a, B, ws, listed, st) : launch_slices<T, 16>(a, B, ws, listed, st);
 }
 
 }  // namespace evo2

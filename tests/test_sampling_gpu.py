@@ -75,6 +75,21 @@ def test_the_longest_rows(dtype):
         _check(z, torch.rand(1, generator=g), t, k, p, m)
 
 
+@pytest.mark.parametrize("B,V,dtype", [(350, 8195, torch.bfloat16), (521, 4099, torch.float32)])
+def test_many_long_rows(B, V, dtype):
+    """Enough rows for slices of 8192: ordinary ones, few values, equal values, masked ones."""
+    g = torch.Generator().manual_seed(B)
+    z = torch.randn(B, V, generator=g) * 3
+    z[::7] = torch.randint(-2, 3, (len(z[::7]), V), generator=g).float()
+    z[1::9] = 0.5
+    z[2::11, : V - 5] = float("-inf")
+    z[3] = float("nan")
+    z[4, 40:50] = float("inf")
+    pick = lambda v: torch.tensor(v)[torch.randint(len(v), (B,), generator=g)]  # noqa: E731
+    _check(z.to(dtype), torch.rand(B, generator=g), pick([0.0, 0.6, 1.0, 1.7]), pick([0, 0, 1, 40, 4096, 5000]),
+           pick([0.1, 0.5, 0.95, 1.0]), pick([0.0, 0.0, 0.02, 1.0]))
+
+
 def test_many_rows():
     g = torch.Generator().manual_seed(9)
     z = torch.randn(70001, 3, generator=g)
