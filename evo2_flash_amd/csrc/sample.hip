@@ -454,9 +454,9 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
 // slices' tokens in that bin (top-k: in all down to it), in the vocabulary's order.
 // sample_draw_kernel: the exact cut among them, a byte at a time from histograms, the
 // slices' sums, and the token in the slice that the draw falls into.  Bound by latency, each
-// launch by the one before: one row of 131072 fp32 logits with top-p 5.1, 5.4, 4.1 and 10.4
-// us; 64 rows of bf16 ones with all three cuts 13.8, 6.5, 5.4 and 11.9.  The draw's way: the
-// rows' and slices' records 1.5 us, the lists 1.5, three passes of a search 3, the sums and
+// launch by the one before: one row of 131072 fp32 logits with top-p 5.0, 4.4, 4.2 and 9.9
+// us; 64 rows of bf16 ones with all three cuts 13.8, 4.9, 5.4 and 11.9.  The draw's way: the
+// rows' and slices' records 1.5 us, the lists 1.5, a search 2.5, the sums and
 // the slice 1.5, its tokens 2.
 constexpr int SL_T = 512, SL_W = SL_T / 64;
 constexpr int MAX_S = 256;  // slices of the longest row, 2^20 logits
@@ -622,25 +622,36 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
   for (int i = 0; i < 4; ++i) total += hist[4 * lane + i];
   total = wave_sum(total);
   // The least key of which `is` holds, as it does for all larger ones up to the largest: 64
-  // probes at a time.
-  auto least_key = [&](auto is) __attribute__((always_inline)) {
+  // probes at a time, the first ones next to each other around a guess (which is most often
+  // right: one round for six).
+  auto least_key = [&](float guess, auto is) __attribute__((always_inline)) {
     uint32_t below = 0, found = kmax;  // below < the key <= found
-    while (found - below > 1) {
-      const uint32_t step = (found - below - 1) / 64 + 1, k = min(below + step * (lane + 1), found);
-      const uint64_t yes = __ballot(k >= LEAST_KEY && is(k));  // (lane 63's k is `found`)
+    uint32_t step = 1, first = max(key_of(guess), LEAST_KEY + 32) - 32;
+    do {
+      const uint32_t k = min(first + step * lane, found);
+      const uint64_t yes = __ballot(k == found || (k >= LEAST_KEY && is(k)));
       const int l = __ffsll(static_cast<long long>(yes)) - 1;
-      found = lane_value(k, l);
-      if (l) below = lane_value(k, l - 1);
-    }
+      if (yes) {
+        found = lane_value(k, l);
+        if (l) below = lane_value(k, l - 1);
+      } else {
+        below = lane_value(k, 63);
+      }
+      step = (found - below - 1) / 64 + 1;
+      first = below + step;  // (then lane 63's k is `found`)
+    } while (found - below > 1);
     return found;
   };
   auto within = [&](int most) __attribute__((always_inline)) {
-    return least_key([&](uint32_t k) __attribute__((always_inline)) { return bin_of(g0, float_of(k), r.c4) <= most; });
+    return least_key(static_cast<float>((g0 - most) / static_cast<double>(r.c4)),
+                     [&](uint32_t k) __attribute__((always_inline)) { return bin_of(g0, float_of(k), r.c4) <= most; });
   };
   uint32_t least = 1;
   if (r.min_p > 0.0f) {
     const double ymin = log2(static_cast<double>(fminf(r.min_p, 1.0f)));
-    least = least_key([&](uint32_t k) __attribute__((always_inline)) { return (value_of(k) - ref.top) * r.c >= ymin; });
+    least = least_key(static_cast<float>(ref.top + ymin / r.c), [&](uint32_t k) __attribute__((always_inline)) {
+      return (value_of(k) - ref.top) * r.c >= ymin;
+    });
   }
   int lo = 0, hi = -1;
   uint32_t from = 0, upto = ~0u;
@@ -728,6 +739,8 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   __shared__ unsigned long long wts[SD_LDS], sums[MAX_S];
   __shared__ uint8_t of_slice[SD_LDS];
   __shared__ unsigned long long hist[3][BINS];
+  __shared__ unsigned long long few_w[64];
+  __shared__ uint32_t few_k[64], few[2];
   __shared__ uint64_t wred[SL_W], before_slice;
   __shared__ uint32_t red[SL_W], red2[SL_W], tie_before;
   __shared__ int pick;
@@ -801,7 +814,7 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   kmx = wave_max(kmx);
   kmin = ~wave_max(~kmin);
   if (lane == 0) red[wave] = kmx, red2[wave] = kmin;
-  if (t == 0) pick = 0, tie_before = 0, before_slice = 0;
+  if (t == 0) pick = 0, tie_before = 0, before_slice = 0, few[0] = few[1] = 0;
   for (int i = t; i < BINS; i += SL_T) hist[0][i] = 0;
   __syncthreads();
   for (int i = 0; i < SL_W; ++i) kmx = max(kmx, red[i]), kmin = min(kmin, red2[i]);
@@ -845,28 +858,73 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
         need -= row.over;
       }
       // the key at which the sum over the listed keys over the cut, from the top, reaches
-      // `need`, and the sum above it
+      // `need`, and the sum above it.  fp32 keys of more than eight differing bits first over
+      // BINS equal steps of value: few are left, which are compared with one another (10.4 ->
+      // 9.9 us); many, and bf16 keys, of which most often many are equal, a byte at a time.
       Digits d(kmx >> LOW<T>, kmin >> LOW<T>);
+      const float vmax = float_of(kmx), scale = BINS / (vmax - float_of(kmin));
+      auto step_of = [&](uint32_t k) __attribute__((always_inline)) {
+        return static_cast<uint32_t>(fminf((vmax - float_of(k)) * scale, BINS - 1.0f));  // (of a NaN the last)
+      };
       unsigned long long above = 0;
-      bool found;
-      do {
+      bool steps = LOW<T> == 0 && d.top > 8, found;
+      uint32_t at = BINS, key = 0;  // at: the step that reaches it
+      for (;;) {
         unsigned long long *now = hist[turn], *next = hist[turn == 2 ? 0 : turn + 1];
         turn = turn == 2 ? 0 : turn + 1;
         for (int i = t; i < BINS; i += SL_T) next[i] = 0;
+        auto add = [&](uint32_t k, auto x) __attribute__((always_inline)) {
+          if (steps) atomicAdd(&now[step_of(k)], static_cast<unsigned long long>(x()));
+          else if (d.has(k >> LOW<T>) && (at == BINS || step_of(k) == at))
+            atomicAdd(&now[d.bin(k >> LOW<T>)], static_cast<unsigned long long>(x()));
+        };
+        auto x_of = [&](uint32_t i, uint32_t k) __attribute__((always_inline)) {
+          return by_weight ? fits ? static_cast<uint64_t>(wts[i]) : weight(k) : 1;
+        };
         each([&](uint32_t i, uint32_t k) __attribute__((always_inline)) {
-          if (k > cut && d.has(k >> LOW<T>))
-            atomicAdd(&now[d.bin(k >> LOW<T>)], by_weight ? fits ? wts[i] : static_cast<unsigned long long>(weight(k)) : 1ull);
+          if (k > cut) add(k, [&]() __attribute__((always_inline)) { return x_of(i, k); });
         });
-        if (t == 0 && extra && d.has(cut >> LOW<T>)) atomicAdd(&now[d.bin(cut >> LOW<T>)], static_cast<unsigned long long>(extra));
+        if (t == 0 && extra) add(cut, [&]() __attribute__((always_inline)) { return extra; });
         __syncthreads();
         unsigned long long a = 0;
         const uint32_t bin = bin_reaching<unsigned long long>(now, need - above, lane, a);
         found = bin < BINS;  // uniform
         above += a;
-        if (!found || !d.next(bin)) break;
-      } while (true);
+        if (!found) break;
+        if (!steps) {
+          if (d.next(bin)) continue;
+          key = whole_key<T>(d.prefix);
+          break;
+        }
+        steps = false;
+        at = bin;
+        auto put = [&](uint32_t k, uint64_t x) __attribute__((always_inline)) {
+          const uint32_t i = atomicAdd(&few[by_weight], 1u);
+          if (i < 64) few_k[i] = k, few_w[i] = x;
+        };
+        each([&](uint32_t i, uint32_t k) __attribute__((always_inline)) {
+          if (k > cut && step_of(k) == at) put(k, x_of(i, k));
+        });
+        if (t == 0 && extra && step_of(cut) == at) put(cut, extra);
+        __syncthreads();
+        const uint32_t n = few[by_weight];
+        if (n > 64) continue;  // uniform
+        const bool in = static_cast<uint32_t>(lane) < n;
+        const uint32_t k = in ? few_k[lane] : 0;
+        const uint64_t x = in ? few_w[lane] : 0;
+        uint64_t before = above, same = 0;
+        for (uint32_t j = 0; j < n; ++j) {
+          const uint32_t kj = lane_value(k, j);
+          const uint64_t xj = lane_value(x, j);
+          before += kj > k ? xj : 0;
+          same += kj == k ? xj : 0;
+        }
+        const int l = __ffsll(static_cast<long long>(__ballot(in && before < need && need <= before + same))) - 1;
+        key = lane_value(k, l);
+        above = lane_value(before, l);
+        break;
+      }
       if (!found) continue;  // all of them
-      const uint32_t key = whole_key<T>(d.prefix);
       const uint64_t wk = weight(key);
       const uint32_t most = ties_of(need, above, by_weight ? wk : 1);
       tie = key == cut ? min(tie, most) : most;
