@@ -19,9 +19,9 @@
 // whose scaling and rounding to a whole number are one FMA.
 //
 // Rows of up to 1024 logits: a wave each, the logits in its registers, the cuts from
-// histograms of its own in LDS (sample_wave_kernel).  Longer rows: four launches over slices of 4096 or
-// 8192 logits (sample_slice_kernel and the ones after it), which read the logits once from
-// memory.
+// histograms of its own in LDS (sample_wave_kernel); of up to 8192: a workgroup each
+// (sample_group_kernel).  Longer rows: four launches over slices of 4096 or 8192 logits
+// (sample_slice_kernel and the ones after it), which read the logits once from memory.
 #include <type_traits>
 
 #include "common.h"
@@ -441,6 +441,190 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
       at = e + 1;
     }
     p.out[b] = E * l + at;
+  }
+}
+
+// ---------------------------------------------------------------- rows of up to 1024 E logits
+// The same with a workgroup to a row, thread t logits E t .. E t + E - 1: what is left of a
+// search's first pass is compared by every wave, or goes a byte at a time where it is more
+// than 64 keys.  Histograms in turn, one pass clearing the next one's (whose last readers met
+// before this pass).  Bound by the chain of searches (one row of 4096 bf16 logits with top-k
+// and top-p 14 us), where there are many rows by their weights' 64-bit arithmetic (2048 of
+// them 77 us).
+constexpr int SG_T = 1024, SG_W = SG_T / 64;
+
+template <typename T, int E>
+__global__ __launch_bounds__(SG_T) void sample_group_kernel(SampleArgs p) {
+  __shared__ unsigned long long hist[3][BINS], few_w[64];
+  __shared__ uint64_t red64[2][SG_W];
+  __shared__ uint32_t red[6][SG_W], few_k[64], few[2];
+  const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  float z[E];
+  logits_of<T, E>(static_cast<const T *>(p.z) + b * p.sz, E * t, p.V, z);
+  const SampleRow r = row_of(p, b);
+  const float u = p.u[b];
+  uint32_t key[E], top = 0, low = ~0u, valid = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    key[e] = key_of(z[e]);
+    top = max(top, key[e]);
+    if (key[e]) low = min(low, key[e]);
+    valid += __popcll(__ballot(key[e] != 0));
+  }
+  top = wave_max(top);
+  low = wave_max(~low);
+  if (lane == 0) red[0][wave] = top, red[1][wave] = low, red[2][wave] = valid;
+  if (t < BINS) hist[0][t] = 0;
+  if (t < 2) few[t] = 0;
+  __syncthreads();
+  const uint32_t kmax = wave_max(lane < SG_W ? red[0][lane] : 0), least = ~wave_max(lane < SG_W ? red[1][lane] : 0);
+  valid = wave_sum(lane < SG_W ? red[2][lane] : 0);
+  if (kmax == 0) {
+    if (t == 0) p.out[b] = -1;
+    return;
+  }
+  if (r.first) {
+    uint32_t at = 0;
+#pragma unroll
+    for (int e = E - 1; e >= 0; --e)
+      if (key[e] == kmax) at = ~static_cast<uint32_t>(E * t + e);
+    at = wave_max(at);
+    if (lane == 0) red[3][wave] = at;
+    __syncthreads();
+    at = wave_max(lane < SG_W ? red[3][lane] : 0);
+    if (t == 0) p.out[b] = static_cast<int64_t>(~at);
+    return;
+  }
+  // The workgroup's inclusive sums of v, and all of it; `by`: used once.
+  auto scan = [&](auto v, auto *by, auto &all) __attribute__((always_inline)) {
+    const auto run = wave_scan(v);
+    if (lane == 63) by[wave] = run;
+    __syncthreads();
+    const auto waves = wave_scan(lane < SG_W ? by[lane] : 0);
+    all = lane_value(waves, SG_W - 1);
+    return run + (wave ? lane_value(waves, wave - 1) : 0);
+  };
+  uint32_t cut = 0, tie = 0;
+  int turn = 0;
+  const float span = static_cast<float>(fmin(50.0 / r.c, 3.0e38));
+  auto search = [&](int which, auto x, uint64_t need, uint32_t kmin, uint32_t &found, uint64_t &above) __attribute__((always_inline)) {
+    const float vmax = float_of(kmax), step = BINS / fminf(vmax - float_of(kmin), span);
+    uint32_t bins[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      bins[e] = key[e] >= kmin ? static_cast<uint32_t>(fminf((vmax - float_of(key[e])) * step, BINS - 1.0f)) : BINS;
+    above = 0;
+    auto pass = [&](auto bin_at) __attribute__((always_inline)) {
+      unsigned long long *now = hist[turn], *next = hist[turn == 2 ? 0 : turn + 1];
+      turn = turn == 2 ? 0 : turn + 1;
+      if (t < BINS) next[t] = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t at = bin_at(e);
+        if (at < BINS && x(e)) atomicAdd(&now[at], static_cast<unsigned long long>(x(e)));
+      }
+      __syncthreads();
+      unsigned long long a = 0;
+      const uint32_t bin = min(bin_reaching<unsigned long long>(now, need - above, lane, a), static_cast<uint32_t>(BINS - 1));
+      above += a;
+      return bin;
+    };
+    const uint32_t bin = pass([&](int e) __attribute__((always_inline)) { return bins[e]; });
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (bins[e] == bin) {
+        const uint32_t i = atomicAdd(&few[which], 1u);
+        if (i < 64) few_k[i] = key[e], few_w[i] = x(e);
+      }
+    __syncthreads();
+    const uint32_t n = few[which];
+    if (n <= 64) {  // uniform
+      const bool in = static_cast<uint32_t>(lane) < n;
+      const uint32_t k = in ? few_k[lane] : 0;
+      const uint64_t w = in ? few_w[lane] : 0;
+      uint64_t before = above, same = 0;
+      for (uint32_t j = 0; j < n; ++j) {
+        const uint32_t kj = lane_value(k, j);
+        const uint64_t wj = lane_value(w, j);
+        before += kj > k ? wj : 0;
+        same += kj == k ? wj : 0;
+      }
+      const int l = __ffsll(static_cast<long long>(__ballot(in && before < need && need <= before + same))) - 1;
+      found = lane_value(k, l);
+      above = lane_value(before, l);
+      return;
+    }
+    Digits d(kmax >> LOW<T>, kmin >> LOW<T>);
+    for (;;) {
+      const uint32_t digit = pass([&](int e) __attribute__((always_inline)) {
+        const uint32_t k = key[e] >> LOW<T>;
+        return bins[e] == bin && d.has(k) ? d.bin(k) : BINS;
+      });
+      if (!d.next(digit)) break;
+    }
+    found = whole_key<T>(d.prefix);
+  };
+  if (r.top_k && r.top_k < valid) {
+    uint64_t over;
+    search(0, [](int) { return uint64_t(1); }, r.top_k, least, cut, over);
+    tie = static_cast<uint32_t>(r.top_k - over);
+  }
+  const double kv = value_of(kmax);
+  uint64_t w[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool in = key[e] && key[e] >= cut;
+    w[e] = 0;
+    if (__any(in)) {  // uniform
+      const double y = (value_of(in ? key[e] : kmax) - kv) * r.c;
+      if (in) w[e] = weight_of(y, p.shift);
+    }
+  }
+  // of the tokens that equal the cut, those behind the first `tie` in the vocabulary's order
+  auto drop_ties = [&](uint32_t *by) __attribute__((always_inline)) {
+    uint32_t n = 0, all;
+#pragma unroll
+    for (int e = 0; e < E; ++e) n += key[e] == cut;
+    uint32_t rank = scan(n, by, all) - n;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (key[e] == cut && rank++ >= tie) w[e] = 0;
+  };
+  if (cut) drop_ties(red[4]);
+  if (r.top_p < 1.0f) {
+    uint64_t sum = 0, all, above;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += w[e];
+    scan(sum, red64[0], all);
+    const uint64_t need = need_of(r.top_p, all);
+    uint32_t at;
+    search(1, [&](int e) __attribute__((always_inline)) { return w[e]; }, need, max(cut, least), at, above);
+    const uint32_t most = ties_of(need, above, weight_of((value_of(at) - kv) * r.c, p.shift));
+    tie = at == cut ? min(tie, most) : most;
+    cut = at;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (key[e] < cut) w[e] = 0;
+    drop_ties(red[5]);
+  }
+  const uint64_t one = uint64_t(1) << p.shift;  // the largest weight
+  const uint64_t least_w = r.min_p > 0.0f ? r.min_p < 1.0f ? part_of(r.min_p, one, true) : one : 0;
+  uint64_t sum = 0, all;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (w[e] < least_w) w[e] = 0;
+    sum += w[e];
+  }
+  const uint64_t upto = scan(sum, red64[1], all), target = target_of(u, all);
+  if (upto > target && upto - sum <= target) {
+    uint64_t run = upto - sum;
+    int at = 0;
+    for (int e = 0; e < E; ++e) {  // the first at which the sum passes the target
+      run += w[e];
+      if (run > target) break;
+      at = e + 1;
+    }
+    p.out[b] = E * t + at;
   }
 }
 
@@ -1058,6 +1242,10 @@ static SampleParts parts_of(int64_t B, int64_t V) {
 }
 
 constexpr int64_t SAMPLE_WAVE = 1024;  // logits of a row that a wave takes
+// Rows that a workgroup takes by itself (us, bf16 rows with top-p 0.95: one of 4096 logits 12,
+// over slices 18, 2048 of them 74, over slices 82; one of 8192 14 and 19, 512 of them 34 and
+// 32), of more logits than a wave takes.
+static bool by_group(int64_t B, int64_t V) { return V <= 4 * SG_T || (V <= 8 * SG_T && B <= 256); }
 constexpr int64_t SAMPLE_MOST = static_cast<int64_t>(MAX_S) * SL_T * 8;
 
 template <typename T, int E>
@@ -1090,6 +1278,12 @@ static int launch_sample(const SampleArgs &a, int64_t B, char *ws, bool listed, 
     else hipLaunchKernelGGL((sample_wave_kernel<T, 16>), grid, dim3(256), 0, st, a, n);
     return check_launch("sample");
   }
+  if (by_group(B, a.V)) {
+    const dim3 grid(static_cast<unsigned>(B));
+    if (a.V <= 4 * SG_T) hipLaunchKernelGGL((sample_group_kernel<T, 4>), grid, dim3(SG_T), 0, st, a);
+    else hipLaunchKernelGGL((sample_group_kernel<T, 8>), grid, dim3(SG_T), 0, st, a);
+    return check_launch("sample");
+  }
   return logits_a_thread(B, a.V) == 8 ? launch_slices<T, 8>(a, B, ws, listed, st) : launch_slices<T, 16>(a, B, ws, listed, st);
 }
 
@@ -1098,7 +1292,7 @@ static int launch_sample(const SampleArgs &a, int64_t B, char *ws, bool listed, 
 using namespace evo2;
 
 extern "C" int64_t evo2_sample_workspace_bytes(int64_t B, int64_t V) {
-  if (B <= 0 || V <= SAMPLE_WAVE || V > SAMPLE_MOST || B > 65535) return 0;
+  if (B <= 0 || by_group(B, V) || V > SAMPLE_MOST || B > 65535) return 0;
   return parts_of(B, V).bytes;
 }
 
@@ -1111,9 +1305,9 @@ extern "C" int evo2_sample(const void *logits, int32_t fp32, int64_t sz, const f
   if (B == 0) return EVO2_OK;
   if (!logits || !u || !tokens) return fail(EVO2_ERR_INVALID, "sample: null pointer argument");
   if (sz < V && B > 1) return fail(EVO2_ERR_UNSUPPORTED, "sample: rows must not overlap");
-  if (V > SAMPLE_WAVE ? B > 65535 : !grid_fits(cdiv(B, 4), 256))
+  if (!by_group(B, V) ? B > 65535 : !grid_fits(V > SAMPLE_WAVE ? B : cdiv(B, 4), V > SAMPLE_WAVE ? SG_T : 256))
     return fail(EVO2_ERR_UNSUPPORTED, "sample: more workgroups than a launch takes");
-  if (workspace_bytes < evo2_sample_workspace_bytes(B, V) || (V > SAMPLE_WAVE && !workspace) ||
+  if (workspace_bytes < evo2_sample_workspace_bytes(B, V) || (!by_group(B, V) && !workspace) ||
       reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(EVO2_ERR_INVALID, "sample: workspace too small or not 16-byte aligned");
   // S: a row's weights stay below 2^62, one below 2^52

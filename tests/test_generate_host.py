@@ -214,9 +214,9 @@ def test_c_entries_check_before_a_launch():
     assert sample(B=0) == 0 and sample(B=-1) == INVALID and sample(V=0) == INVALID
     assert sample(V=(1 << 20) + 1, sz=1 << 21) == INVALID
     assert sample(z=n) == INVALID and sample(u=n) == INVALID and sample(sz=8) == UNSUPPORTED
-    assert sample(V=5000, sz=5000, bytes=64) == INVALID and sample(V=5000, sz=5000, ws=n) == INVALID
-    assert sample(V=5000, sz=5000, ws=at + 8) == INVALID and b"workspace" in lib.evo2_last_error()
-    assert sample(V=5000, sz=5000, B=65536) == UNSUPPORTED and b"workgroups" in lib.evo2_last_error()
+    assert sample(V=9000, sz=9000, bytes=64) == INVALID and sample(V=9000, sz=9000, ws=n) == INVALID
+    assert sample(V=9000, sz=9000, ws=at + 8) == INVALID and b"workspace" in lib.evo2_last_error()
+    assert sample(V=9000, sz=9000, B=65536) == UNSUPPORTED and b"workgroups" in lib.evo2_last_error()
 
 
 def test_workspaces():
@@ -236,7 +236,9 @@ def test_workspaces():
     assert need(8, 1, 32, 32, 128, 1024, 0) == 0 < need(8, 1, 32, 32, 128, 1025, 0)
     assert need(1, 1, 32, 32, 128, 128, 0) > 0 and need(4, 1, 4, 4, 128, 60, 20) > 0
     assert need(0, 1, 4, 4, 128, 4, 0) == 0 and need(4, 1, 4, 3, 128, 4, 0) == 0 and need(4, 1, 4, 4, 128, 4, 5) == 0
-    assert lib.evo2_sample_workspace_bytes(64, 1024) == 0
+    for B, V in ((64, 1024), (70000, 4096), (256, 8192)):  # a wave or a workgroup to a row
+        assert lib.evo2_sample_workspace_bytes(B, V) == 0
+    assert lib.evo2_sample_workspace_bytes(257, 8192) > 0 < lib.evo2_sample_workspace_bytes(1, 8193)
     ws = lib.evo2_sample_workspace_bytes(64, 131072)
     assert 64 * 131072 * 4 <= ws <= 64 * 131072 * 6
     assert lib.evo2_sample_workspace_bytes(0, 131072) == 0 == lib.evo2_sample_workspace_bytes(4, (1 << 20) + 1)

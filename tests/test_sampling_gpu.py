@@ -58,7 +58,7 @@ SETTINGS = [(1.0, 0, 1.0, 0.0), (1.0, 4, 1.0, 0.0), (0.7, 0, 0.9, 0.0), (1.3, 50
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [1, 2, 63, 64, 65, 509, 512, 4096, 4097, 20011, 65537])
+@pytest.mark.parametrize("V", [1, 2, 63, 64, 65, 509, 512, 1025, 4096, 4097, 8192, 8193, 20011, 65537])
 def test_settings(V, dtype):
     g = torch.Generator().manual_seed(V)
     for n, (t, k, p, m) in enumerate(SETTINGS):
@@ -109,7 +109,7 @@ def test_settings_by_row():
 def test_equal_logits_go_by_index():
     """Ties at the cuts: few values among many tokens, -0 equal to 0."""
     g = torch.Generator().manual_seed(2)
-    for V in (40, 512, 9000):
+    for V in (40, 512, 3000, 9000):
         z = torch.randint(-2, 3, (40, V), generator=g).float()
         z[z == 0] *= torch.where(torch.rand(int((z == 0).sum()), generator=g) < 0.5, -1.0, 1.0)
         for t, k, p, m in ((1.0, 7, 1.0, 0.0), (1.0, V // 3, 1.0, 0.0), (1.0, 0, 0.37, 0.0), (1.0, V // 2, 0.61, 0.0),
@@ -122,7 +122,7 @@ def test_equal_logits_go_by_index():
         _check(same, u, 1.0, 3)
 
 
-@pytest.mark.parametrize("V", [33, 512, 6000])
+@pytest.mark.parametrize("V", [33, 512, 2000, 6000, 9500])
 def test_masked_infinite_and_nan_logits(V):
     g = torch.Generator().manual_seed(3)
     z = torch.randn(12, V, generator=g)
@@ -144,7 +144,7 @@ def test_masked_infinite_and_nan_logits(V):
 
 def test_uniforms_at_and_past_the_ends():
     g = torch.Generator().manual_seed(4)
-    for V in (100, 5000):
+    for V in (100, 5000, 9000):
         z = torch.randn(7, V, generator=g)
         z[:, 0] = z[:, -1] = float("-inf")
         u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, 7.0, -1.0, float("inf"), float("nan")])
@@ -169,7 +169,7 @@ def test_extreme_settings():
 
 def test_rows_apart_streams_and_graphs():
     g = torch.Generator().manual_seed(6)
-    for V in (500, 30000):
+    for V in (500, 4000, 30000):
         wide = torch.randn(6, V + 13, generator=g).to(DEV)
         z, u = wide[:, 5:V + 5], torch.rand(6, generator=g).to(DEV)
         want = sample_tokens(z.contiguous(), u, 0.9, 40, 0.9)
