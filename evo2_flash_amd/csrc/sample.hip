@@ -14,9 +14,12 @@
 // order (-0 as 0; -inf and NaN below all, never drawn).
 //
 // Weights are whole numbers, round(w 2^S): sums of them are exact and the same in any
-// order, also through atomics, and their steps (2^-45 of the largest at 131072 tokens)
-// decide no draw that 64-bit floating point would settle.  2^y is a polynomial in 64 bits
-// whose scaling and rounding to a whole number are one FMA.
+// order, also through atomics.  S is 49 for rows of up to 8192 tokens.  Longer rows have the
+// slices' largest in the place of the row's where they are summed whole, and the largest S
+// (of at most 49) that holds a row's sum near 2^62 where a cut parts them; joining the slices
+// drops up to a step for each of a slice's bins.  In all a running sum is off by at most
+// V 2^-48 of the total (2^-31 at 131072 tokens; u has steps of 2^-24).  2^y is a polynomial in
+// 64 bits whose scaling and rounding to a whole number are one FMA.
 //
 // Rows of up to 1024 logits: a wave each, the logits in its registers, the cuts from
 // histograms of its own in LDS (sample_wave_kernel); of up to 8192: a workgroup each
@@ -40,7 +43,7 @@ struct SampleArgs {
   const float *m; float m1;
   int64_t *out;               // (B,): the token, -1 for a row with none left
   int V;
-  int shift;                  // S
+  int shift;                  // S; of longer rows one that is safe for any of them
 };
 
 // A row's settings.
@@ -632,9 +635,11 @@ __global__ __launch_bounds__(SG_T) void sample_group_kernel(SampleArgs p) {
 // Slices of SL_T * E logits, E a thread.  sample_slice_kernel: a slice's largest logit, and a histogram over
 // BINS bins of a quarter of a power of two in weight, from its largest down (the last bin
 // takes all below), of its tokens in rows with top-k, else of its weights.  Bins lie on one
-// grid for all slices of a row, floor(4 z c), and weights are 2^(S + z c - R) with a whole R
-// of the slice's own, so that histograms of slices add up by shifts.  sample_join_kernel:
-// a row's histogram, and the bin in which the cut lies.  sample_list_kernel: the keys of the
+// grid for all slices of a row, floor(4 z c), and weights are 2^(OWN + z c - R) with a whole R
+// of the slice's own (the row's units: its R, and S for OWN), so that histograms of slices add
+// up by shifts.  A slice's sum in the row's units is that in its own, shifted once, and the
+// draw looks for the token in the slice's own units again, so that its tokens' sum reaches
+// what the slice was drawn for.  Listed tokens are in the row's.  sample_join_kernel: a row's histogram, and the bin in which the cut lies.  sample_list_kernel: the keys of the
 // slices' tokens in that bin (top-k: in all down to it), in the vocabulary's order.
 // sample_draw_kernel: the exact cut among them, a byte at a time from histograms, the
 // slices' sums, and the token in the slice that the draw falls into.  Bound by latency, each
@@ -644,11 +649,12 @@ __global__ __launch_bounds__(SG_T) void sample_group_kernel(SampleArgs p) {
 // the slice 1.5, its tokens 2.
 constexpr int SL_T = 512, SL_W = SL_T / 64;
 constexpr int MAX_S = 256;  // slices of the longest row, 2^20 logits
+constexpr int OWN = 49;     // S of a slice's own units: 8192 weights sum up to 2^62 at most
 
 struct SliceInfo {
   double top;           // its largest logit
   uint64_t total;       // its weight, in its own units (rows without top-k)
-  uint64_t base;        // weight in bins over the listed ones, in the row's units
+  uint64_t base;        // of it in bins over the listed ones
   uint32_t key, at;     // largest key (0: no token) and its first index
   uint32_t listed, pad;
 };
@@ -660,7 +666,7 @@ struct RowInfo {
   int32_t mode;         // 0: drawn already, 1: nothing is listed, 2: bins from lo on are
   int32_t lo;
   uint32_t from, upto;  // their keys: from .. upto - 1
-  uint32_t pad;
+  int32_t shift;        // S of the row's units
 };
 
 struct SampleWork {
@@ -678,7 +684,13 @@ struct SampleRef {
   __device__ __forceinline__ uint64_t weight(double z, int shift) const {
     return weight_of(fma(z - top, c, phi), shift);
   }
+  // by: the units of a row (its S: `shift`) are 2^by of those of a slice with largest logit z
+  __device__ __forceinline__ int by(double z, int shift) const {
+    return static_cast<int>(fmin(r - ceil(z * c), 4096.0)) + OWN - shift;
+  }
 };
+// A slice's sum in the row's units (a slice of by over 62 has less than one).
+__device__ __forceinline__ uint64_t in_row(uint64_t sum, int by) { return sum >> min(by, 63); }
 // floor(4 z c), where that is past 2^29 the same for all (as a whole number, so that
 // differences add up).  c4: 4 c, finite.
 __device__ __forceinline__ int grid_of(float z, float c4) {
@@ -727,7 +739,7 @@ __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, Sample
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const uint64_t x = z[e] > -INFINITY ? ref.weight(wide_of(z[e]), p.shift) : 0;
+        const uint64_t x = z[e] > -INFINITY ? ref.weight(wide_of(z[e]), OWN) : 0;
         if (x) atomicAdd(&hist[bin_of(g0, z[e], r.c4)], static_cast<unsigned long long>(x));
       }
     }
@@ -753,7 +765,7 @@ __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, Sample
 constexpr int SJ_T = 1024, SJ_G = SJ_T / BINS, SJ_E = 8;  // groups of threads take slices in turn
 
 __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleWork w) {
-  __shared__ unsigned long long hist[BINS];
+  __shared__ unsigned long long hist[BINS], totals[MAX_S / 64];
   __shared__ uint32_t red[MAX_S / 64], red2[MAX_S / 64];
   __shared__ int by[MAX_S], off[MAX_S];
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, bin = t % BINS, first = t / BINS;
@@ -764,8 +776,9 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
 #pragma unroll
   for (int i = 0; i < SJ_E; ++i) x[i] = first + SJ_G * i < w.S ? h[(first + SJ_G * i) * BINS] : 0;
   uint32_t key = 0, at = 0;
+  uint64_t own = 0;
   double top = 0.0;
-  if (t < w.S) key = slice[t].key, at = ~slice[t].at, top = slice[t].top;
+  if (t < w.S) key = slice[t].key, at = ~slice[t].at, top = slice[t].top, own = slice[t].total;
   const SampleRow r = row_of(p, b);
   RowInfo &row = w.row[b];
   if (t < BINS) hist[t] = 0;
@@ -786,13 +799,27 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
   if (kmax == 0 || r.first) return;  // uniform
   const SampleRef ref(value_of(kmax), r.c);
   const int g0 = grid_of(float_of(kmax), r.c4);
-  if (t < w.S) {  // a slice's units are 2^-by of the row's, its bins `off` below the row's
-    by[t] = key ? r.top_k ? 0 : static_cast<int>(fmin(ref.r - ceil(top * r.c), 63.0)) : -1;
-    off[t] = key ? min(g0 - grid_of(float_of(key), r.c4), BINS - 1) : 0;
+  // The row's sum in units of S = p.shift (short by less than a step a slice), which has S
+  // raised by the bits that leave it at 2^62.  A slice's bins lie `off` below the row's.
+  if (t < MAX_S) {
+    const int by0 = ref.by(top, p.shift);
+    if (t < w.S) {
+      by[t] = key ? r.top_k ? 0 : by0 : -1;
+      off[t] = key ? min(g0 - grid_of(float_of(key), r.c4), BINS - 1) : 0;
+    }
+    const uint64_t sum = wave_sum(key && !r.top_k ? in_row(own, by0) : uint64_t(0));
+    if (lane == 0) totals[wave] = sum;
   }
   __syncthreads();
+  auto raise = [&](uint64_t sum) __attribute__((always_inline)) {
+    return min(max(__clzll(static_cast<long long>(sum)) - 2, 0), OWN - p.shift);
+  };
+  uint64_t whole = MAX_S;
+#pragma unroll
+  for (int i = 0; i < MAX_S / 64; ++i) whole += totals[i];
+  int raised = r.top_k ? 0 : raise(whole);
   auto add = [&](int s, unsigned long long v) __attribute__((always_inline)) {
-    if (by[s] >= 0 && v) atomicAdd(&hist[min(bin + off[s], BINS - 1)], v >> by[s]);
+    if (by[s] >= 0 && v) atomicAdd(&hist[min(bin + off[s], BINS - 1)], static_cast<unsigned long long>(in_row(v, by[s] - raised)));
   };
 #pragma unroll
   for (int i = 0; i < SJ_E; ++i)
@@ -842,6 +869,15 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
   if (r.top_k) {
     hi = min(bin_reaching<unsigned long long>(hist, r.top_k, lane, before), static_cast<uint32_t>(BINS - 1));
     from = within(hi);
+    // for S a bound of the listed tokens' weight: one of bin i is below 2^((1 - i) / 4) of the
+    // largest, where fp32 has steps of value far below a bin's, else below the largest
+    uint64_t bound = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int down = abs(g0) < (1 << 20) ? max(4 * lane + i - 2, 0) / 4 : 0;
+      if (4 * lane + i <= hi) bound += hist[4 * lane + i] << max(p.shift - down, 0);
+    }
+    raised = raise(wave_sum(bound));
   } else {
     if (r.top_p < 1.0f) hi = bin_reaching<unsigned long long>(hist, need_of(r.top_p, total), lane, before);
     if (least > 1) {
@@ -866,6 +902,7 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
     row.lo = lo;
     row.from = from;
     row.upto = upto;
+    row.shift = p.shift + raised;
   }
 }
 
@@ -885,14 +922,12 @@ __global__ __launch_bounds__(SL_T) void sample_list_kernel(SampleArgs p, SampleW
   for (int e = 0; e < E; ++e)
     if (z[e] >= from && !(z[e] >= upto)) in |= 1u << e;  // (none of a NaN; all below no bound)
   n = __popc(in);
-  // weight in bins over the listed ones (none with top-k)
+  // weight in bins over the listed ones, in the slice's own units (none with top-k)
   uint64_t x = 0;
   if (row.lo > 0 && t < BINS && info.key) {
     const SampleRow r = row_of(p, b);
-    const SampleRef ref(row.top, r.c), own(info.top, r.c);
-    const int by = static_cast<int>(fmin(ref.r - own.r, 63.0));
     const int off = grid_of(static_cast<float>(row.top), r.c4) - grid_of(float_of(info.key), r.c4);
-    if (min(t + min(off, BINS - 1), BINS - 1) < row.lo) x = w.hist[(static_cast<int64_t>(b) * w.S + s) * BINS + t] >> by;
+    if (min(t + min(off, BINS - 1), BINS - 1) < row.lo) x = w.hist[(static_cast<int64_t>(b) * w.S + s) * BINS + t];
   }
   x = wave_sum(x);
   const uint32_t run = wave_scan(n);
@@ -944,8 +979,7 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   // all where nothing is listed; start[s]: listed keys before slice s
   if (t < w.S) {
     tied[t] = 0;
-    sums[t] = cuts ? mine.base
-                   : mine.key ? mine.total >> static_cast<int>(fmin(ref.r - ceil(mine.top * r.c), 63.0)) : 0;
+    sums[t] = mine.key ? in_row(cuts ? mine.base : mine.total, ref.by(mine.top, row.shift)) : 0;
   }
   uint32_t listed = 0;
   if (cuts) {
@@ -1002,7 +1036,7 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   for (int i = t; i < BINS; i += SL_T) hist[0][i] = 0;
   __syncthreads();
   for (int i = 0; i < SL_W; ++i) kmx = max(kmx, red[i]), kmin = min(kmin, red2[i]);
-  auto weight = [&](uint32_t k) __attribute__((always_inline)) { return ref.weight(value_of(k), p.shift); };
+  auto weight = [&](uint32_t k) __attribute__((always_inline)) { return ref.weight(value_of(k), row.shift); };
   // f(i, key) for all listed keys
   auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll 1
@@ -1162,6 +1196,7 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   const float at_cut = cut ? float_of(cut) : NAN, over = cut ? at_cut : -INFINITY;
   const uint32_t least = max(row.from, row.least);
   const float from = least > LEAST_KEY ? float_of(least) : -INFINITY;
+  const double own_top = slice[pick].top;
   float z[E];
   slice_values<T, E>(p, b, pick, t, z);
   uint32_t n = 0;  // kept, and in the upper half those at the cut
@@ -1187,8 +1222,15 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
     }
   }
   __syncthreads();
-  // (sums of slices in other units were shifted: the last token's end may lie a few steps
-  // off, then it is the last one of any weight)
+  // The slice's sum was that of its own units (of which the row's are 2^by) for the tokens over
+  // the listed ones, and of the row's for those: so are the weights here, in its own units, and
+  // their sum passes the target.  (8192 weights are at most 2^62; a listed one that rounds to
+  // any step of the row's is at most doubled by that: 2^63.)  For u >= 1 it is the slice's last
+  // token of any weight.
+  const SampleRef own(own_top, r.c);
+  const int by = min(ref.by(own_top, row.shift), 63);
+  const float over_listed = !cuts ? -INFINITY : row.upto == ~0u ? NAN : float_of(row.upto);
+  const uint64_t target = u >= 1.0f ? ~uint64_t(0) : before_slice << by;
   uint64_t before = 0;
   uint32_t last = 0;
 #pragma unroll 1
@@ -1196,7 +1238,11 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
     const uint32_t i = c + t;
     const float v = i < entries ? vals[i] : -INFINITY;
     uint64_t x = 0;
-    if (v > -INFINITY) x = v == at_cut ? wc : ref.weight(wide_of(v), p.shift);
+    if (v > -INFINITY) {
+      const bool listed = !(v >= over_listed);
+      x = v == at_cut ? wc : (listed ? ref : own).weight(wide_of(v), listed ? row.shift : OWN);
+      if (listed) x <<= by;
+    }
     if (x) last = i + 1;
     const uint64_t sum = wave_scan(x);
     if (lane == 63) wred[wave] = sum;
@@ -1206,8 +1252,8 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
       if (k < wave) upto += wred[k];
       before += wred[k];
     }
-    if (before > before_slice) {  // uniform
-      if (upto > before_slice && upto - x <= before_slice) p.out[b] = static_cast<int64_t>(SL) * pick + ids[i];
+    if (before > target) {  // uniform
+      if (upto > target && upto - x <= target) p.out[b] = static_cast<int64_t>(SL) * pick + ids[i];
       return;
     }
     __syncthreads();
@@ -1310,7 +1356,7 @@ extern "C" int evo2_sample(const void *logits, int32_t fp32, int64_t sz, const f
   if (workspace_bytes < evo2_sample_workspace_bytes(B, V) || (!by_group(B, V) && !workspace) ||
       reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(EVO2_ERR_INVALID, "sample: workspace too small or not 16-byte aligned");
-  // S: a row's weights stay below 2^62, one below 2^52
+  // S: a row's weights stay at 2^62 or below, one below 2^52
   int bits = 0;
   while ((int64_t(1) << bits) < V) ++bits;
   const SampleArgs a{logits, sz, u, temperature, t1, top_k, k1, top_p, p1, min_p, m1, tokens, static_cast<int>(V),
