@@ -308,6 +308,7 @@ class Evo2DecodeModel(nn.Module):
         shared_pages = min(sp, shared_prefix_pages(table, max_batch))
         self.block_table = table.to(device)
         self.shared_prefix = shared_prefix
+        self.kv_dtype = kv_dtype
         layers, self.pools = [], {}
         for i in range(config.num_hidden_layers):
             if config.layer_kind(i) == "attn":
@@ -375,8 +376,14 @@ class Evo2DecodeModel(nn.Module):
         groups of `chunk_seqs` sequences: fresh Hyena states (the prefill
         kernels write each sequence's final state and windows into its
         blocks) and KV pages for positions 0..L-1.  Returns the logits of the
-        last position (B, vocab)."""
+        last position (B, vocab).  With a shared prefix (prefill_shared) the
+        prompts' first shared_prefix tokens have to be the same ones, as they
+        go to the same pages; several prompts are refused where those are of
+        8 bits, whose scale and codes they would not write together."""
         L = tokens.shape[1]
+        if self.shared_prefix and tokens.shape[0] > 1 and self.kv_dtype == torch.float8_e4m3fn:
+            raise ValueError("the model's sequences share their first 8-bit pages: prefill takes "
+                             "one prompt (prefill_shared)")
         last = [x.view(n, L, -1)[:, -1] for _, n, x in self._prompts(tokens, chunk_seqs,
                                                                      self.layers)]
         h = self.norm(torch.cat(last))
@@ -466,7 +473,8 @@ class Evo2DecodeModel(nn.Module):
     def decode_step(self, tokens, positions):
         """One token for each of the first B = len(tokens) sequences at the
         given positions: returns logits (B, vocab) and advances every layer's
-        state (Hyena state blocks, KV pages)."""
+        state (Hyena state blocks, KV pages).  With a shared prefix several
+        sequences' positions lie behind it."""
         B = tokens.shape[0]
         m = getattr(self, "_meta", None)
         if m is None or m.num_decodes != B:
@@ -487,11 +495,16 @@ class Evo2DecodeModel(nn.Module):
         token; every token is drawn by sampling.sample_tokens with these settings (numbers, or
         (B,) tensors) from a row of `uniforms` (num_tokens, B) fp32, by default drawn from
         `generator` (its device's, or the model's default one).  Returns the tokens
-        (B, num_tokens).  Overwrites the states and KV pages of sequences 0..B-1.  (Where a
-        row's logits are all NaN the token is -1, and the sequence goes on with token 0.)"""
+        (B, num_tokens).  Overwrites the states and KV pages of sequences 0..B-1, so a model
+        with a shared prefix takes one prompt (the pages of several would be the same ones).
+        (Where a row's logits are all NaN the token is -1, and the sequence goes on with
+        token 0.)"""
         B, L = prompts.shape
         if L < 1:
             raise ValueError("prompts have at least one token")
+        if B > 1 and self.shared_prefix:
+            raise ValueError(f"the model's sequences share the pages of their first "
+                             f"{self.shared_prefix} positions: generate takes one prompt")
         if L + num_tokens > self.max_pages * PAGE + 1:
             raise ValueError(f"{L} + {num_tokens} tokens exceed the model's {self.max_pages * PAGE} "
                              f"positions")
