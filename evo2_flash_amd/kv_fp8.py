@@ -25,6 +25,7 @@ from . import _lib
 from .attention import PAGE, _page_table, _rotary_rows
 
 _F8 = torch.float8_e4m3fn
+_NO_SCALE = 2.0 ** -110  # of a page of zeros
 _INTS = (torch.int32, torch.int64)
 
 
@@ -229,13 +230,14 @@ def paged_decode_attention_fp8(q, k_pages, v_pages, k_scale, v_scale, block_tabl
 
 
 class Fp8KVCache:
-    """One attention layer's 8-bit KV pages and their scales; page 0 is never handed out."""
+    """One attention layer's 8-bit KV pages and their scales, zeros at first; page 0 is never
+    handed out."""
 
     def __init__(self, num_pages, heads, head_dim, device):
         self.k = torch.zeros(num_pages, heads, PAGE, head_dim, dtype=torch.uint8, device=device).view(_F8)
         self.v = torch.zeros(num_pages, heads, head_dim, PAGE, dtype=torch.uint8, device=device).view(_F8)
-        self.k_scale = torch.ones(num_pages, heads, dtype=torch.float32, device=device)
-        self.v_scale = torch.ones(num_pages, heads, dtype=torch.float32, device=device)
+        self.k_scale = torch.full((num_pages, heads), _NO_SCALE, dtype=torch.float32, device=device)
+        self.v_scale = torch.full((num_pages, heads), _NO_SCALE, dtype=torch.float32, device=device)
 
     @property
     def tensors(self):
@@ -246,8 +248,8 @@ class Fp8KVCache:
         """Zeros in every page, as a new cache has."""
         for t in (self.k, self.v):
             t.view(torch.uint8).zero_()
-        self.k_scale.fill_(1.0)
-        self.v_scale.fill_(1.0)
+        self.k_scale.fill_(_NO_SCALE)
+        self.v_scale.fill_(_NO_SCALE)
 
     def fill(self, values):
         """Every page's 16 tokens: values(pages, 16, heads, head_dim) makes keys and values
