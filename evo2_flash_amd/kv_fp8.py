@@ -156,12 +156,13 @@ def read_kv_fp8(k_pages, v_pages, k_scale, v_scale, block_table, lengths, L):
 
 
 def workspace_fp8(B, heads, kv_heads, head_dim, max_pages, device, n=1, shared_pages=0):
-    """A workspace for paged_decode_attention_fp8 on up to B sequences of n tokens, with and
-    without the shared pages (allocate once, outside graph capture; calls that may run at
-    once take one each)."""
-    need = max((_lib.workspace_bytes("evo2_decode_attention_fp8_workspace_bytes", b, n, heads,
+    """A workspace for paged_decode_attention_fp8 on up to B sequences of up to n tokens over
+    tables of max_pages columns (a table of fewer can need more), with and without the shared
+    pages (allocate once, outside graph capture; calls that may run at once take one each)."""
+    need = max((_lib.workspace_bytes("evo2_decode_attention_fp8_workspace_bytes", b, m, heads,
                                      kv_heads, head_dim, max_pages, s)
-                for b in range(1, B + 1) for s in {0, int(shared_pages)}), default=0)
+                for b in range(1, B + 1) for m in range(1, n + 1) for s in {0, int(shared_pages)}),
+               default=0)
     return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
 
 
