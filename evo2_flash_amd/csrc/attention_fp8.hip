@@ -637,7 +637,7 @@ extern "C" int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_
     return fail(EVO2_ERR_INVALID, "paged_decode_attention_fp8: bad sizes B=%lld n=%lld heads=%lld kv_heads=%lld "
                 "shared_pages=%lld", (long long)B, (long long)n, (long long)heads, (long long)kv_heads,
                 (long long)shared_pages);
-  if (!(scale > 0.0f) || scale > 3.0e38f)
+  if (!(scale > 0.0f) || !(scale * 1.4426950408889634f < INFINITY))  // (the kernel's units)
     return fail(EVO2_ERR_INVALID, "paged_decode_attention_fp8: the scale must be positive and finite");
   if (B == 0 || n == 0) return EVO2_OK;
   const KvPages c{static_cast<uint8_t *>(const_cast<void *>(k_pages)), kps, khs,

@@ -468,7 +468,7 @@ int evo2_rotary_decode_fp8(const void *qkv, int64_t sqkv, const float *inv_freq,
  *   shared_pages: the first entries of every table row that name the same pages
  *   workspace: _workspace_bytes(B, n, heads, kv_heads, head_dim, max_pages, shared_pages)
  *   bytes (0: none), 16-byte aligned
- * heads a multiple of kv_heads, scale > 0, B * n at most 65535.  Positions of entries
+ * heads a multiple of kv_heads, scale > 0 (below 2.3e38), B * n at most 65535.  Positions of entries
  * outside the pages are left out; a token with none left gives zeros.
  */
 int64_t evo2_decode_attention_fp8_workspace_bytes(int64_t B, int64_t n, int64_t heads, int64_t kv_heads,
