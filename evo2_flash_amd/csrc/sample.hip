@@ -14,12 +14,13 @@
 // order (-0 as 0; -inf and NaN below all, never drawn).
 //
 // Weights are whole numbers, round(w 2^S): sums of them are exact and the same in any
-// order, also through atomics.  S is 49 for rows of up to 8192 tokens.  Longer rows have the
-// slices' largest in the place of the row's where they are summed whole, and the largest S
-// (of at most 49) that holds a row's sum near 2^62 where a cut parts them; joining the slices
-// drops up to a step for each of a slice's bins.  In all a running sum is off by at most
-// V 2^-48 of the total (2^-31 at 131072 tokens; u has steps of 2^-24).  2^y is a polynomial in
-// 64 bits whose scaling and rounding to a whole number are one FMA.
+// order, also through atomics; tokens that are all equal are parted exactly where p and u say.  S
+// is 49 for rows of up to 8192 tokens.  Longer rows have 62 - ceil(log2 V) against each
+// slice's own largest, and where a cut goes through their values the largest S (of at most 49)
+// that leaves the row's sum at 2^62; joining the slices drops up to a step for each of a
+// slice's bins.  In all a running sum is off by at most V 2^-48 of the total (2^-31 at 131072
+// tokens; u has steps of 2^-24).  2^y is a polynomial in 64 bits whose scaling and rounding to
+// a whole number are one FMA.
 //
 // Rows of up to 1024 logits: a wave each, the logits in its registers, the cuts from
 // histograms of its own in LDS (sample_wave_kernel); of up to 8192: a workgroup each
@@ -43,7 +44,7 @@ struct SampleArgs {
   const float *m; float m1;
   int64_t *out;               // (B,): the token, -1 for a row with none left
   int V;
-  int shift;                  // S; of longer rows one that is safe for any of them
+  int shift;                  // S; of longer rows that of a slice
 };
 
 // A row's settings.
@@ -635,10 +636,10 @@ __global__ __launch_bounds__(SG_T) void sample_group_kernel(SampleArgs p) {
 // Slices of SL_T * E logits, E a thread.  sample_slice_kernel: a slice's largest logit, and a histogram over
 // BINS bins of a quarter of a power of two in weight, from its largest down (the last bin
 // takes all below), of its tokens in rows with top-k, else of its weights.  Bins lie on one
-// grid for all slices of a row, floor(4 z c), and weights are 2^(OWN + z c - R) with a whole R
-// of the slice's own (the row's units: its R, and S for OWN), so that histograms of slices add
-// up by shifts.  A slice's sum in the row's units is that in its own, shifted once, and the
-// draw looks for the token in the slice's own units again, so that its tokens' sum reaches
+// grid for all slices of a row, floor(4 z c), and weights are 2^(S + z c - R) with a whole R of
+// the slice's own (the row's units: its R, and an S of its own), so that histograms of slices
+// add up by shifts.  A slice's sum in the row's units is that in its own, shifted once, and the
+// draw looks for the token in the slice's own weights again, so that its tokens' sum reaches
 // what the slice was drawn for.  Listed tokens are in the row's.  sample_join_kernel: a row's histogram, and the bin in which the cut lies.  sample_list_kernel: the keys of the
 // slices' tokens in that bin (top-k: in all down to it), in the vocabulary's order.
 // sample_draw_kernel: the exact cut among them, a byte at a time from histograms, the
@@ -649,7 +650,7 @@ __global__ __launch_bounds__(SG_T) void sample_group_kernel(SampleArgs p) {
 // the slice 1.5, its tokens 2.
 constexpr int SL_T = 512, SL_W = SL_T / 64;
 constexpr int MAX_S = 256;  // slices of the longest row, 2^20 logits
-constexpr int OWN = 49;     // S of a slice's own units: 8192 weights sum up to 2^62 at most
+constexpr int MOST_S = 49;
 
 struct SliceInfo {
   double top;           // its largest logit
@@ -661,12 +662,12 @@ struct SliceInfo {
 struct RowInfo {
   double top;           // the row's largest logit
   uint64_t total;       // its weight (without top-k)
-  uint64_t over;        // of it in bins over the listed ones
+  uint64_t over, bin;   // of it in bins over the listed one, and in that
   uint32_t least;       // min-p keeps keys from here on
   int32_t mode;         // 0: drawn already, 1: nothing is listed, 2: bins from lo on are
   int32_t lo;
   uint32_t from, upto;  // their keys: from .. upto - 1
-  int32_t shift;        // S of the row's units
+  int32_t raised;       // S of the row's units is this much over the slices'
 };
 
 struct SampleWork {
@@ -684,13 +685,14 @@ struct SampleRef {
   __device__ __forceinline__ uint64_t weight(double z, int shift) const {
     return weight_of(fma(z - top, c, phi), shift);
   }
-  // by: the units of a row (its S: `shift`) are 2^by of those of a slice with largest logit z
-  __device__ __forceinline__ int by(double z, int shift) const {
-    return static_cast<int>(fmin(r - ceil(z * c), 4096.0)) + OWN - shift;
+  // by: the row's units are 2^by of those of a slice with largest logit z, where S is `raised`
+  // more for the row
+  __device__ __forceinline__ int by(double z, int raised) const {
+    return static_cast<int>(fmin(r - ceil(z * c), 4096.0)) - raised;
   }
 };
 // A slice's sum in the row's units (a slice of by over 62 has less than one).
-__device__ __forceinline__ uint64_t in_row(uint64_t sum, int by) { return sum >> min(by, 63); }
+__device__ __forceinline__ uint64_t in_row(uint64_t sum, int by) { return by < 0 ? sum << -by : sum >> min(by, 63); }
 // floor(4 z c), where that is past 2^29 the same for all (as a whole number, so that
 // differences add up).  c4: 4 c, finite.
 __device__ __forceinline__ int grid_of(float z, float c4) {
@@ -739,7 +741,7 @@ __global__ __launch_bounds__(SL_T) void sample_slice_kernel(SampleArgs p, Sample
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const uint64_t x = z[e] > -INFINITY ? ref.weight(wide_of(z[e]), OWN) : 0;
+        const uint64_t x = z[e] > -INFINITY ? ref.weight(wide_of(z[e]), p.shift) : 0;
         if (x) atomicAdd(&hist[bin_of(g0, z[e], r.c4)], static_cast<unsigned long long>(x));
       }
     }
@@ -799,10 +801,10 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
   if (kmax == 0 || r.first) return;  // uniform
   const SampleRef ref(value_of(kmax), r.c);
   const int g0 = grid_of(float_of(kmax), r.c4);
-  // The row's sum in units of S = p.shift (short by less than a step a slice), which has S
-  // raised by the bits that leave it at 2^62.  A slice's bins lie `off` below the row's.
+  // The row's sum in units of the slices' S (short by less than a step a slice), which is
+  // raised by the bits that leave the sum at 2^62.  A slice's bins lie `off` below the row's.
   if (t < MAX_S) {
-    const int by0 = ref.by(top, p.shift);
+    const int by0 = ref.by(top, 0);
     if (t < w.S) {
       by[t] = key ? r.top_k ? 0 : by0 : -1;
       off[t] = key ? min(g0 - grid_of(float_of(key), r.c4), BINS - 1) : 0;
@@ -812,7 +814,7 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
   }
   __syncthreads();
   auto raise = [&](uint64_t sum) __attribute__((always_inline)) {
-    return min(max(__clzll(static_cast<long long>(sum)) - 2, 0), OWN - p.shift);
+    return min(max(__clzll(static_cast<long long>(sum)) - 2, 0), MOST_S - p.shift);
   };
   uint64_t whole = MAX_S;
 #pragma unroll
@@ -865,6 +867,7 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
     });
   }
   int lo = 0, hi = -1;
+  uint64_t at_bin = 0;
   uint32_t from = 0, upto = ~0u;
   if (r.top_k) {
     hi = min(bin_reaching<unsigned long long>(hist, r.top_k, lane, before), static_cast<uint32_t>(BINS - 1));
@@ -884,9 +887,10 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
       const int at = bin_of(g0, float_of(least), r.c4);
       hi = hi < 0 ? at : min(hi, at);
     }
-    if (hi >= 0) {  // the one bin, of it what min-p keeps
+    if (hi >= 0) {  // the one bin; of it what min-p keeps, where no sum of its tokens is needed
       lo = hi;
-      from = max(within(hi), least);
+      from = r.top_p < 1.0f ? within(hi) : max(within(hi), least);
+      at_bin = hist[hi];
       if (lo > 0) upto = within(lo - 1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) over += 4 * lane + i < lo ? hist[4 * lane + i] : 0;
@@ -897,12 +901,13 @@ __global__ __launch_bounds__(SJ_T) void sample_join_kernel(SampleArgs p, SampleW
     row.top = ref.top;
     row.total = total;
     row.over = over;
+    row.bin = at_bin;
     row.least = least;
     row.mode = hi < 0 ? 1 : 2;
     row.lo = lo;
     row.from = from;
     row.upto = upto;
-    row.shift = p.shift + raised;
+    row.raised = raised;
   }
 }
 
@@ -979,7 +984,7 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   // all where nothing is listed; start[s]: listed keys before slice s
   if (t < w.S) {
     tied[t] = 0;
-    sums[t] = mine.key ? in_row(cuts ? mine.base : mine.total, ref.by(mine.top, row.shift)) : 0;
+    sums[t] = mine.key ? in_row(cuts ? mine.base : mine.total, ref.by(mine.top, row.raised)) : 0;
   }
   uint32_t listed = 0;
   if (cuts) {
@@ -1036,7 +1041,8 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
   for (int i = t; i < BINS; i += SL_T) hist[0][i] = 0;
   __syncthreads();
   for (int i = 0; i < SL_W; ++i) kmx = max(kmx, red[i]), kmin = min(kmin, red2[i]);
-  auto weight = [&](uint32_t k) __attribute__((always_inline)) { return ref.weight(value_of(k), row.shift); };
+  const int row_shift = p.shift + row.raised;
+  auto weight = [&](uint32_t k) __attribute__((always_inline)) { return ref.weight(value_of(k), row_shift); };
   // f(i, key) for all listed keys
   auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll 1
@@ -1062,15 +1068,14 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
           x += v;
         });
         if (!(r.top_p < 1.0f)) break;
-        uint64_t total = row.total;
+        // of what top-k kept, or of the row with its listed bin weighed as it is here: tokens
+        // that are all equal then have a total of so many times their weight
         extra = tie * wc;
-        if (r.top_k) {  // of what top-k kept
-          x = wave_sum(x);
-          if (lane == 0) wred[wave] = x;
-          __syncthreads();
-          total = extra;
-          for (int i = 0; i < SL_W; ++i) total += wred[i];
-        }
+        x = wave_sum(x);
+        if (lane == 0) wred[wave] = x;
+        __syncthreads();
+        uint64_t total = r.top_k ? extra : row.total - row.bin;
+        for (int i = 0; i < SL_W; ++i) total += wred[i];
         need = need_of(r.top_p, total);
         if (need <= row.over) break;
         need -= row.over;
@@ -1222,15 +1227,15 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
     }
   }
   __syncthreads();
-  // The slice's sum was that of its own units (of which the row's are 2^by) for the tokens over
-  // the listed ones, and of the row's for those: so are the weights here, in its own units, and
-  // their sum passes the target.  (8192 weights are at most 2^62; a listed one that rounds to
-  // any step of the row's is at most doubled by that: 2^63.)  For u >= 1 it is the slice's last
-  // token of any weight.
+  // The slice's sum was one of its own weights, in units of which the row's are 2^by, for the
+  // tokens over the listed ones, and of the row's weights for those: so it is here, in the
+  // finer of the two units, and passes the target.  (8192 weights of a slice are at most 2^62;
+  // a listed one that rounds to any step of the row's is at most doubled by that: 2^63.)  For
+  // u >= 1 it is the slice's last token of any weight.
   const SampleRef own(own_top, r.c);
-  const int by = min(ref.by(own_top, row.shift), 63);
+  const int by = min(ref.by(own_top, row.raised), 63), up = max(by, 0), own_up = max(-by, 0);
   const float over_listed = !cuts ? -INFINITY : row.upto == ~0u ? NAN : float_of(row.upto);
-  const uint64_t target = u >= 1.0f ? ~uint64_t(0) : before_slice << by;
+  const uint64_t target = u >= 1.0f ? ~uint64_t(0) : before_slice << up;
   uint64_t before = 0;
   uint32_t last = 0;
 #pragma unroll 1
@@ -1240,8 +1245,8 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
     uint64_t x = 0;
     if (v > -INFINITY) {
       const bool listed = !(v >= over_listed);
-      x = v == at_cut ? wc : (listed ? ref : own).weight(wide_of(v), listed ? row.shift : OWN);
-      if (listed) x <<= by;
+      x = v == at_cut ? wc : (listed ? ref : own).weight(wide_of(v), listed ? row_shift : p.shift);
+      x <<= listed ? up : own_up;
     }
     if (x) last = i + 1;
     const uint64_t sum = wave_scan(x);

@@ -48,9 +48,9 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     of what is kept passes uniforms times its total; numbers outside [0, 1) draw the first or
     the last token kept.  temperature <= 0 (or NaN) and top_k 1 take the first token.  -inf and
     NaN logits are never drawn (a row of nothing else gives -1); beside +inf no finite one
-    is.  Weights are summed as whole numbers, so a result does not depend on timing: in steps of
-    2^-49 of the largest (V over 8192: or of 2^-58 of their sum, whichever is longer), of which
-    a token below half a step may have none.  A running sum, and so the border between two
+    is.  Weights are summed as whole numbers, so a result does not depend on timing, and tokens
+    that are all equal are parted exactly.  A token of less than 2^-50 of the largest weight (V
+    over 8192: V 2^-62) may count for nothing; a running sum, and so the border between two
     tokens, is off by at most V 2^-48 of the total."""
     shape, dtype, dev = logits.shape, logits.dtype, logits.get_device()
     same = uniforms.get_device() == dev

@@ -4,12 +4,13 @@ a token of that part, and numbers of 1 and above the last token kept.
 
 The reference holds weights and running sums in 80-bit floating point.  The kernel's sums:
 
-* a token's weight is off by at most half a step, of 2^-49 of its slice's largest or, where a
-  cut goes through its values, of the row's (rows of more than 8192 tokens of like weight: of
-  2^-61 of their sum, which is less than that a token); a slice's sum loses at most a step, and
-  so does each of its 256 bins where a cut is looked for;
-* so V 2^-50 of the largest weight for the tokens, 256 V / 4096 2^-49 for the bins: a running
-  sum is off by less than E = V 2^-48 of the total.
+* a token's weight is off by at most half a step of its slice's units, 2^-62 of the largest
+  times V rounded up to a power of two: 8192 of them by V 2^-49 of the slice's largest, all by
+  V 2^-49 of the total.  Where a cut goes through its values the units are the row's, of 2^-49
+  of the largest or 2^-61 of the sum: V 2^-50 of the total for all;
+* a slice's sum loses at most a step of the row's units, and each of its 256 bins where a cut is
+  looked for: 256 V / 4096 of them;
+* so a running sum is off by less than E = V 2^-48 of the total.
 
 A number u draws a token whose part of the running sum u times the total reaches within 3 E
 (its own sum, the total and top-p's border); top-p keeps tokens whose front is below p times
@@ -95,8 +96,9 @@ def test_a_peak_over_a_flat_tail(at, depth, V, dtype):
 
 def test_the_number_next_to_one_draws_from_the_tail():
     """A tail of 2^20 - 1 tokens of e^-30.1 weighs 2^-23.4: two thirds of it lie behind
-    1 - 2^-24 of the total.  A token of it is 47 steps of 2^-49: within half a step of its
-    weight, 1.1% of those two thirds."""
+    1 - 2^-24 of the total.  Those in the peak's slice, of up to 8192 (0.8% of the row), count
+    for nothing; one in the row's units is 47 steps of 2^-49, within half a step of its weight,
+    1.1% of those two thirds."""
     V = 1 << 20
     z = _peaked(V, 30.1, 0, torch.float32)
     w = np.exp(-np.float64(z[1].abs()))
