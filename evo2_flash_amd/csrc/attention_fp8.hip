@@ -551,6 +551,12 @@ static int chunk_for(int64_t L, int64_t units, int64_t slots, int64_t step, int6
 constexpr int64_t AF_SAVED = 64, AF_ALONE = 2048;
 
 // The split of a call: shared positions, and chunks of them and of those behind.
+//
+// L is that of the table's columns: the host does not read the positions, and the workspace has
+// to hold whatever they are.  A table far longer than its sequences makes chunks that few waves
+// take (32 heads: 777 positions 10.4 us, in a table of 131072 positions 31; 8 sequences of 8192
+// 91, there 129, in one of 2^20 324).  A caller who knows a bound passes the table's first
+// columns.
 struct AttnSplit {
   int shared, schunk, snum, chunk, nchunk;
   bool group;  // a workgroup takes all of a sequence's positions: no join

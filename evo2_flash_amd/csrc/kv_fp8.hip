@@ -238,8 +238,9 @@ __global__ __launch_bounds__(64 * KV_WAVES) void kv_read_kernel(KvPages c, KvOut
 
 // The decode step between the qkv projection and the attention: neox rotary of q and k
 // (each product and sum rounded by itself, the bits of rotary_decode_kernel) and the
-// write of k and v.  A wave takes one head of one sequence, lane f dims f and f + HD / 2;
-// latency only.
+// write of k and v.  A wave takes one head of one sequence, lane f dims f and f + HD / 2.
+// Latency only: 32 heads of 128, 8 sequences 4.6-5.1 us and 64 of them 4.8-5.5 (the bytes,
+// 2.6 MB, 0.5; with bf16 pages 4.5-4.8 and 6.0).
 struct KvRotary {
   const bf16_t *qkv; int64_t sqkv;  // rows (q | k | v), each heads * HD
   const float *inv_freq;

@@ -453,8 +453,9 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs p, int B) {
 // search's first pass is compared by every wave, or goes a byte at a time where it is more
 // than 64 keys.  Histograms in turn, one pass clearing the next one's (whose last readers met
 // before this pass).  Bound by the chain of searches (one row of 4096 bf16 logits with top-k
-// and top-p 14 us), where there are many rows by their weights' 64-bit arithmetic (2048 of
-// them 77 us).
+// and top-p 11 us), where there are many rows by the instructions of it, which every wave of a
+// row runs (2048 of them 61 us, with top-p 0.95 alone 69: 1160 vector instructions a wave, some
+// 100 of them the weights' 64-bit arithmetic, are 66 of the kernel's 74 us by its counters).
 constexpr int SG_T = 1024, SG_W = SG_T / 64;
 
 template <typename T, int E>
@@ -644,8 +645,8 @@ __global__ __launch_bounds__(SG_T) void sample_group_kernel(SampleArgs p) {
 // slices' tokens in that bin (top-k: in all down to it), in the vocabulary's order.
 // sample_draw_kernel: the exact cut among them, a byte at a time from histograms, the
 // slices' sums, and the token in the slice that the draw falls into.  Bound by latency, each
-// launch by the one before: one row of 131072 fp32 logits with top-p 5.0, 4.4, 4.2 and 9.9
-// us; 64 rows of bf16 ones with all three cuts 13.8, 4.9, 5.4 and 11.9.  The draw's way: the
+// launch by the one before: one row of 131072 fp32 logits with top-p 5.0, 5.0, 4.1 and 10.8
+// us; 64 rows of bf16 ones with all three cuts 14.7, 5.2, 5.4 and 12.5.  The draw's way: the
 // rows' and slices' records 1.5 us, the lists 1.5, a search 2.5, the sums and
 // the slice 1.5, its tokens 2.
 constexpr int SL_T = 512, SL_W = SL_T / 64;
@@ -1274,7 +1275,9 @@ __global__ __launch_bounds__(SL_T) void sample_draw_kernel(SampleArgs p, SampleW
 static int64_t align16(int64_t n) { return (n + 15) & ~int64_t(15); }
 
 // Logits a thread: 8, where that is one round of workgroups (four a CU), else 16 (rows of
-// 131072 bf16 logits with top-p 0.95: 64 of them 43 us, with 8 46; 8 rows 26, with 16 29).
+// 131072 bf16 logits with top-p 0.95: 512 of them 154 us, with 8 179; 64 of them 43.5, with 8
+// 44.1, without any cut 39.1 and 34.4; 8 of them 25.3, with 16 28.8; 512 rows of 20011 51.6, with
+// 8 48.5).
 static int logits_a_thread(int64_t B, int64_t V) { return B * cdiv(V, SL_T * 8) <= 1024 ? 8 : 16; }
 
 // Offsets of the parts of a workspace; the last is its size.

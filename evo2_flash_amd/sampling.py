@@ -51,7 +51,8 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     is.  Weights are summed as whole numbers, so a result does not depend on timing, and tokens
     that are all equal are parted exactly.  A token of less than 2^-50 of the largest weight (V
     over 8192: V 2^-62) may count for nothing; a running sum, and so the border between two
-    tokens, is off by at most V 2^-48 of the total."""
+    tokens, is off by at most V 2^-48 of the total.  More than 65535 rows are refused where a
+    row has more than 4096 logits."""
     shape, dtype, dev = logits.shape, logits.dtype, logits.get_device()
     same = uniforms.get_device() == dev
     if dev < 0 or not same:

@@ -428,8 +428,9 @@ int evo2_iir_verify_gated(const void *zf, int64_t zs, const float *log_poles, in
  * lengths[b] (NULL: n); positions, lengths (B,) int64.  e of a page's scale 2^e is the
  * smallest of [-110, 119] with which no finite magnitude of its tokens is over 448 codes;
  * a page written to behind positions that it holds keeps its e, or raises it and
- * re-encodes those.  Round to nearest even; infinities and NaN become NaN; with e = 119
- * larger values saturate.  Bytes of other positions stay as they are.
+ * re-encodes those; writing over a token does not lower it.  Round to nearest even;
+ * infinities and NaN become NaN; with e = 119 larger values saturate.  Bytes of other
+ * positions stay as they are.
  *
  * evo2_kv_fp8_read: k, v (B, L, heads, head_dim) bf16 contiguous, 16-byte aligned: the
  * values of positions below lengths[b] (int64), zeros from there on and where the table
@@ -492,8 +493,8 @@ int evo2_paged_decode_attention_fp8(const void *q, int64_t qb, int64_t qt, int64
  * first index at which the running sum of what is kept passes u times its total.  T <= 0
  * or k = 1: the first of the largest.  -inf and NaN are never drawn; a row of nothing else
  * gives -1.  temperature, top_k, top_p, min_p (B,) by row, or NULL: t1, k1, p1, m1.
- *   tokens (B,) int64; V up to 2^20; workspace of _workspace_bytes(B, V) bytes, 16-byte
- *   aligned (0: none)
+ *   tokens (B,) int64; V up to 2^20 (over 4096: B up to 65535); workspace of
+ *   _workspace_bytes(B, V) bytes, 16-byte aligned (0: none)
  */
 int64_t evo2_sample_workspace_bytes(int64_t B, int64_t V);
 int evo2_sample(const void *logits, int32_t fp32, int64_t sz, const float *u, const float *temperature,
