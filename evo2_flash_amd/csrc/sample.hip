@@ -14,8 +14,8 @@
 // order (-0 as 0; -inf and NaN below all, never drawn).
 //
 // Weights are whole numbers, round(w 2^S): sums of them are exact and the same in any
-// order, also through atomics; tokens that are all equal are parted exactly where p and u say.  S
-// is 49 for rows of up to 8192 tokens.  Longer rows have 62 - ceil(log2 V) against each
+// order, also through atomics; tokens that are all equal are parted exactly where p and u say.
+// S is 49 for rows of up to 8192 tokens.  Longer rows have 62 - ceil(log2 V) against each
 // slice's own largest, and where a cut goes through their values the largest S (of at most 49)
 // that leaves the row's sum at 2^62; joining the slices drops up to a step for each of a
 // slice's bins.  In all a running sum is off by at most V 2^-48 of the total (2^-31 at 131072
@@ -641,8 +641,9 @@ __global__ __launch_bounds__(SG_T) void sample_group_kernel(SampleArgs p) {
 // the slice's own (the row's units: its R, and an S of its own), so that histograms of slices
 // add up by shifts.  A slice's sum in the row's units is that in its own, shifted once, and the
 // draw looks for the token in the slice's own weights again, so that its tokens' sum reaches
-// what the slice was drawn for.  Listed tokens are in the row's.  sample_join_kernel: a row's histogram, and the bin in which the cut lies.  sample_list_kernel: the keys of the
-// slices' tokens in that bin (top-k: in all down to it), in the vocabulary's order.
+// what the slice was drawn for.  Listed tokens are in the row's.  sample_join_kernel: a row's
+// histogram, and the bin in which the cut lies.  sample_list_kernel: the keys of the slices'
+// tokens in that bin (top-k: in all down to it), in the vocabulary's order.
 // sample_draw_kernel: the exact cut among them, a byte at a time from histograms, the
 // slices' sums, and the token in the slice that the draw falls into.  Bound by latency, each
 // launch by the one before: one row of 131072 fp32 logits with top-p 5.0, 5.0, 4.1 and 10.8
@@ -651,7 +652,7 @@ __global__ __launch_bounds__(SG_T) void sample_group_kernel(SampleArgs p) {
 // the slice 1.5, its tokens 2.
 constexpr int SL_T = 512, SL_W = SL_T / 64;
 constexpr int MAX_S = 256;  // slices of the longest row, 2^20 logits
-constexpr int MOST_S = 49;
+constexpr int MOST_S = 49;  // of a row (a slice's 8192 weights are then at most 2^62)
 
 struct SliceInfo {
   double top;           // its largest logit
